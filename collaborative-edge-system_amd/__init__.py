@@ -9,6 +9,8 @@ Import with ``importlib.import_module("collaborative-edge-system_amd")``.  Modul
 * :mod:`.layers` - RMSNorm, rotary, SiLU-gate (collab_infer/models/llama.py)
 * :mod:`.kv_cache` - head-major KV cache with the rotary of K fused into the append
   (collab_infer/models/cache.py)
+* :mod:`.paged_cache` - paged KV cache: append, attention of tokens and chunks over pages, page
+  copies, and the book of pages that sequences share and give back
 * :mod:`.partition` - splits and sequence layouts (collab_infer/parallel/partition.py)
 * :mod:`.projection` - the fused Q/K/V and gate/up projections (own gfx950 GEMM; column views,
   gate/up with the activation fused)
@@ -19,7 +21,7 @@ Import with ``importlib.import_module("collaborative-edge-system_amd")``.  Modul
   ``models.llama``, ``models.cache``) with its public names and signatures
 """
 
-from . import _native, attention, kv_cache, layers, partition, projection, sequence_parallel, workloads  # noqa: F401
+from . import _native, attention, kv_cache, layers, paged_cache, partition, projection, sequence_parallel, workloads  # noqa: F401
 from . import models, parallel  # noqa: F401
 from .attention import (  # noqa: F401
     MASK_CHUNK_ELEMENTS,
@@ -46,6 +48,15 @@ from .layers import (  # noqa: F401
     rmsnorm,
     rmsnorm_rope,
     silu_mul,
+)
+from .paged_cache import (  # noqa: F401
+    PageBook,
+    PagedKVCache,
+    PagedStep,
+    copy_pages,
+    paged_attention,
+    paged_attention_with_lse,
+    paged_kv_append,
 )
 from .partition import HeadShard, SequenceLayout, partition_heads, split_sizes  # noqa: F401
 from .projection import FusedColumnParallelLinear, fused_linear, linear, linear_gated  # noqa: F401

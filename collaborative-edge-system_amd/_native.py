@@ -129,6 +129,21 @@ _SIGNATURES = {
         ctypes.c_int,
         [_P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_int64, ctypes.c_void_p],
     ),
+    "cea_paged_kv_append": (ctypes.c_int, [_P] * 11 + [ctypes.c_void_p]),
+    "cea_paged_attention_workspace_bytes": (
+        ctypes.c_size_t,
+        [ctypes.c_int64] * 7 + [ctypes.c_int32],
+    ),
+    "cea_paged_attention": (
+        ctypes.c_int,
+        [_P] * 7 + [ctypes.c_int32, ctypes.c_double, ctypes.POINTER(ctypes.c_int32), ctypes.c_int32,
+                    _P, _P, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
+    ),
+    "cea_copy_pages": (
+        ctypes.c_int,
+        [ctypes.c_int32, _P, ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int64),
+         ctypes.c_int64, ctypes.c_void_p],
+    ),
 }
 
 _lib = None

@@ -1,0 +1,60 @@
+// Parameter block and launchers of the paged KV cache: pools of pages of `page` slots, a table of
+// page indices per batch row, and the rows' lengths, all read on the device.
+//
+// Slot j of row b is place j % page of page tables[b, j / page].  It exists while j < lengths[b]
+// (clamped to what the table holds); a page index outside the pool holds no keys.  Its position is
+// j, or what pos_pages holds there when that is given.  Nothing outside the pools is read or
+// written whatever the tables, lengths and offsets hold.
+#pragma once
+
+#include "cea_kernels.hpp"
+
+namespace cea {
+
+constexpr int kPagedMapHeads = 64;  // query heads of an explicit head map on the matrix-core kernels
+
+struct PagedParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  const int64_t* q_pos;
+  const int64_t* pos;        // [P, page] or null: position j in slot j
+  const int64_t* tables;     // [B, W]
+  const int64_t* lengths;    // [B]
+  void* out;
+  void* lse;                 // may be null
+  int64_t P;
+  int32_t B, Sq, Hq, Hkv, D, W, page;
+  int64_t qs_b, qs_s, qs_h;
+  int64_t ks_p, ks_h, ks_s;
+  int64_t vs_p, vs_h, vs_s;
+  int64_t ps_p, ps_s;
+  int64_t ts_b, ts_w, ns_b;  // tables, lengths
+  int64_t qps_b, qps_s;
+  int64_t os_b, os_s, os_h;
+  int64_t ls_b, ls_h, ls_s;
+  double scale;
+  int32_t causal;
+  int32_t in_dtype, out_dtype;
+  int32_t group;             // > 0: KV head of query head h is h / group; 0: explicit map
+};
+
+// Slots of row b: its length within what its table holds.
+__device__ __forceinline__ int64_t paged_slots(const PagedParams& p, int b) {
+  const int64_t n = p.lengths[b * p.ns_b], cap = (int64_t)p.W * p.page;
+  return n < 0 ? 0 : n < cap ? n : cap;
+}
+
+int launch_paged_generic(const PagedParams& p, const HeadMap& map, hipStream_t s);
+
+// Appends, one row of k and v per token and head; null tensors are left out.
+int launch_paged_append(const cea_tensor* k, const cea_tensor* v, const cea_tensor* pos,
+                        const cea_tensor* c, const cea_tensor* sn, const cea_tensor* tables,
+                        const cea_tensor* offsets, const cea_tensor* counts, cea_tensor* kp,
+                        cea_tensor* vp, cea_tensor* pp, hipStream_t s);
+
+// Copies pages src[i] -> dst[i] of every pool (validated by the caller).
+int launch_copy_pages(int n, const cea_tensor* pools, const int64_t* src, const int64_t* dst,
+                      int64_t m, hipStream_t s);
+
+}  // namespace cea

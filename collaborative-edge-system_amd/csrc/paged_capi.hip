@@ -1,0 +1,201 @@
+// C ABI of the paged KV cache: argument checks, the choice of kernel and the workspace layout.
+#include <string.h>
+
+#include <new>
+#include <unordered_set>
+
+#include "paged.hpp"
+
+namespace cea {
+namespace {
+
+int check_pages(const cea_tensor* kp, const cea_tensor* vp, int dt, int64_t H, int64_t D,
+                const char* what) {
+  int rc;
+  if ((rc = check_tensor(kp, "k_pages", 4, dt, true))) return rc;
+  if ((rc = check_tensor(vp, "v_pages", 4, dt, true))) return rc;
+  for (const cea_tensor* t : {kp, vp})
+    CEA_REQUIRE(t->size[0] == kp->size[0] && t->size[2] == kp->size[2] && t->size[1] == H &&
+                    t->size[3] == D,
+                CEA_EINVAL, "%s: k_pages and v_pages must be [P, %lld, page, %lld]", what,
+                (long long)H, (long long)D);
+  return CEA_OK;
+}
+
+int check_rows(const cea_tensor* tables, const cea_tensor* per_row, const char* name, int64_t B,
+               const char* what) {
+  int rc;
+  if ((rc = check_tensor(tables, "tables", 2, CEA_I64, false))) return rc;
+  CEA_REQUIRE(tables->size[0] == B, CEA_EINVAL, "%s: tables must be [B, W]", what);
+  if ((rc = check_tensor(per_row, name, 1, CEA_I64, false))) return rc;
+  CEA_REQUIRE(per_row->size[0] == B, CEA_EINVAL, "%s: %s must be [B]", what, name);
+  return CEA_OK;
+}
+
+int check_pos_pages(const cea_tensor* pp, const cea_tensor* kp, const char* what) {
+  int rc;
+  if ((rc = check_tensor(pp, "pos_pages", 2, CEA_I64, false))) return rc;
+  CEA_REQUIRE(pp->size[0] == kp->size[0] && pp->size[1] == kp->size[2], CEA_EINVAL,
+              "%s: pos_pages must be [P, page]", what);
+  return CEA_OK;
+}
+
+}  // namespace
+}  // namespace cea
+
+using namespace cea;
+
+extern "C" {
+
+int cea_paged_kv_append(const cea_tensor* k, const cea_tensor* v, const cea_tensor* pos,
+                        const cea_tensor* cos, const cea_tensor* sin, const cea_tensor* tables,
+                        const cea_tensor* offsets, const cea_tensor* counts, cea_tensor* k_pages,
+                        cea_tensor* v_pages, cea_tensor* pos_pages, void* stream) {
+  const char* what = "paged_kv_append";
+  int rc;
+  if ((rc = check_tensor(k, "k", 4, -1, true))) return rc;
+  const int dt = k->dtype;
+  CEA_REQUIRE(dt != CEA_I64, CEA_EUNSUPPORTED, "%s: unsupported dtype int64", what);
+  if ((rc = check_tensor(v, "v", 4, dt, true))) return rc;
+  const int64_t B = k->size[0], n = k->size[1], H = k->size[2], D = k->size[3];
+  for (int i = 0; i < 4; ++i)
+    CEA_REQUIRE(v->size[i] == k->size[i], CEA_EINVAL, "%s: v must match k [B,n,H,D]", what);
+  CEA_REQUIRE(D % 2 == 0, CEA_EINVAL, "%s: head size must be even", what);
+  if ((rc = check_pages(k_pages, v_pages, dt, H, D, what))) return rc;
+  if ((rc = check_rows(tables, offsets, "offsets", B, what))) return rc;
+  if (counts) {
+    if ((rc = check_tensor(counts, "counts", 1, CEA_I64, false))) return rc;
+    CEA_REQUIRE(counts->size[0] == B, CEA_EINVAL, "%s: counts must be [B]", what);
+  }
+  CEA_REQUIRE((pos == nullptr) == (pos_pages == nullptr), CEA_EINVAL,
+              "%s: give both positions and pos_pages or neither", what);
+  if (pos) {
+    if ((rc = check_tensor(pos, "positions", 2, CEA_I64, false))) return rc;
+    CEA_REQUIRE(pos->size[0] == B && pos->size[1] == n, CEA_EINVAL, "%s: positions must be [B, n]",
+                what);
+    if ((rc = check_pos_pages(pos_pages, k_pages, what))) return rc;
+  }
+  CEA_REQUIRE((cos == nullptr) == (sin == nullptr), CEA_EINVAL,
+              "%s: give both rotary tables or neither", what);
+  cea_tensor c, sn;
+  if (cos) {
+    if ((rc = check_tensor(cos, "cos", 3, dt, true))) return rc;
+    if ((rc = check_tensor(sin, "sin", 3, dt, true))) return rc;
+    for (const cea_tensor* t : {cos, sin})
+      CEA_REQUIRE((t->size[0] == B || t->size[0] == 1) && t->size[1] == n && t->size[2] == D,
+                  CEA_EINVAL, "%s: cos/sin must be [B, n, D]", what);
+    c = *cos, sn = *sin;
+    if (c.size[0] == 1) c.stride[0] = 0;  // broadcast over the batch
+    if (sn.size[0] == 1) sn.stride[0] = 0;
+  }
+  return launch_paged_append(k, v, pos, cos ? &c : nullptr, cos ? &sn : nullptr, tables, offsets,
+                             counts, k_pages, v_pages, pos_pages, (hipStream_t)stream);
+}
+
+size_t cea_paged_attention_workspace_bytes(int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int64_t D,
+                                           int64_t W, int64_t page, int32_t in_dtype) {
+  return 0;
+}
+
+int cea_paged_attention(const cea_tensor* q, const cea_tensor* k_pages, const cea_tensor* v_pages,
+                        const cea_tensor* pos_pages, const cea_tensor* tables,
+                        const cea_tensor* lengths, const cea_tensor* q_pos, int32_t causal,
+                        double scale, const int32_t* kv_map, int32_t kv_map_len, cea_tensor* out,
+                        cea_tensor* lse, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "paged_attention";
+  int rc;
+  if ((rc = check_tensor(q, "q", 4, -1, true))) return rc;
+  const int dt = q->dtype;
+  CEA_REQUIRE(dt != CEA_I64, CEA_EUNSUPPORTED, "%s: unsupported dtype int64", what);
+  const int64_t B = q->size[0], Sq = q->size[1], Hq = q->size[2], D = q->size[3];
+  CEA_REQUIRE(D >= 1, CEA_EINVAL, "%s: empty head dimension", what);
+  CEA_REQUIRE(k_pages != nullptr, CEA_EINVAL, "k_pages: missing tensor");
+  const int64_t Hkv = k_pages->ndim == 4 ? k_pages->size[1] : 0;
+  if ((rc = check_pages(k_pages, v_pages, dt, Hkv, D, what))) return rc;
+  if ((rc = check_rows(tables, lengths, "lengths", B, what))) return rc;
+  if (pos_pages && (rc = check_pos_pages(pos_pages, k_pages, what))) return rc;
+  if ((rc = check_tensor(q_pos, "q_pos", 2, CEA_I64, false))) return rc;
+  CEA_REQUIRE(q_pos->size[0] == B && q_pos->size[1] == Sq, CEA_EINVAL, "%s: q_pos must be [B, Sq]",
+              what);
+  const int acc = dt == CEA_F64 ? CEA_F64 : CEA_F32;
+  if ((rc = check_tensor(out, "out", 4, -1, true))) return rc;
+  CEA_REQUIRE(out->size[0] == B && out->size[1] == Sq && out->size[2] == Hq && out->size[3] == D,
+              CEA_EINVAL, "%s: out must be [B, Sq, Hq, D]", what);
+  CEA_REQUIRE(out->dtype == acc || out->dtype == dt, CEA_EINVAL, "%s: out must be %s or %s", what,
+              dtype_name(acc), dtype_name(dt));
+  if (lse) {
+    if ((rc = check_tensor(lse, "lse", 3, acc, false))) return rc;
+    CEA_REQUIRE(lse->size[0] == B && lse->size[1] == Hq && lse->size[2] == Sq, CEA_EINVAL,
+                "%s: lse must be [B, Hq, Sq]", what);
+  }
+  HeadMap map;
+  if ((rc = make_head_map(&map, Hq, Hkv, kv_map, kv_map_len))) return rc;
+  const int64_t page = k_pages->size[2], W = tables->size[1];
+  CEA_REQUIRE(W == 0 || page < ((int64_t)1 << 40) / W, CEA_EUNSUPPORTED, "%s: tables too wide", what);
+
+  PagedParams p;
+  memset(&p, 0, sizeof(p));
+  p.q = q->data, p.k = k_pages->data, p.v = v_pages->data;
+  p.q_pos = (const int64_t*)q_pos->data;
+  p.pos = pos_pages ? (const int64_t*)pos_pages->data : nullptr;
+  p.tables = (const int64_t*)tables->data, p.lengths = (const int64_t*)lengths->data;
+  p.out = out->data, p.lse = lse ? lse->data : nullptr;
+  p.P = k_pages->size[0];
+  p.B = (int)B, p.Sq = (int)Sq, p.Hq = (int)Hq, p.Hkv = (int)Hkv, p.D = (int)D;
+  p.W = (int)W, p.page = (int)page;
+  p.qs_b = q->stride[0], p.qs_s = q->stride[1], p.qs_h = q->stride[2];
+  p.ks_p = k_pages->stride[0], p.ks_h = k_pages->stride[1], p.ks_s = k_pages->stride[2];
+  p.vs_p = v_pages->stride[0], p.vs_h = v_pages->stride[1], p.vs_s = v_pages->stride[2];
+  if (pos_pages) p.ps_p = pos_pages->stride[0], p.ps_s = pos_pages->stride[1];
+  p.ts_b = tables->stride[0], p.ts_w = tables->stride[1], p.ns_b = lengths->stride[0];
+  p.qps_b = q_pos->stride[0], p.qps_s = q_pos->stride[1];
+  p.os_b = out->stride[0], p.os_s = out->stride[1], p.os_h = out->stride[2];
+  if (lse) p.ls_b = lse->stride[0], p.ls_h = lse->stride[1], p.ls_s = lse->stride[2];
+  p.scale = scale;
+  p.causal = causal ? 1 : 0;
+  p.in_dtype = dt, p.out_dtype = out->dtype;
+  p.group = map.group;
+  if (B == 0 || Sq == 0 || Hq == 0) return CEA_OK;
+  if (page == 0 || p.P == 0) p.W = 0, p.page = 1;  // no slots: every row is empty
+  return launch_paged_generic(p, map, (hipStream_t)stream);
+}
+
+int cea_copy_pages(int32_t n, const cea_tensor* pools, const int64_t* src, const int64_t* dst,
+                   int64_t moves, void* stream) {
+  const char* what = "copy_pages";
+  int rc;
+  CEA_REQUIRE(n >= 1 && n <= CEA_MAX_PARTS, n < 1 ? CEA_EINVAL : CEA_EUNSUPPORTED,
+              "%s: 1 to %d pools, got %d", what, CEA_MAX_PARTS, n);
+  CEA_REQUIRE(pools != nullptr && moves >= 0 && (moves == 0 || (src && dst)), CEA_EINVAL,
+              "%s: missing arguments", what);
+  for (int i = 0; i < n; ++i) {
+    if ((rc = check_tensor(&pools[i], "pool", 3, -1, true))) return rc;
+    CEA_REQUIRE(pools[i].size[1] == pools[0].size[1], CEA_EINVAL,
+                "%s: the pools differ in their number of pages", what);
+    for (int j = 0; j < 2; ++j)
+      CEA_REQUIRE(pools[i].size[j] <= 1 || pools[i].stride[j] >= pools[i].size[2], CEA_EINVAL,
+                  "%s: pages overlap", what);
+  }
+  const int64_t P = pools[0].size[1];
+  try {
+    std::unordered_set<int64_t> written;
+    written.reserve((size_t)moves);
+    for (int64_t i = 0; i < moves; ++i) {
+      CEA_REQUIRE(src[i] >= 0 && src[i] < P && dst[i] >= 0 && dst[i] < P, CEA_EINVAL,
+                  "%s: move %lld (%lld to %lld) leaves the %lld pages", what, (long long)i,
+                  (long long)src[i], (long long)dst[i], (long long)P);
+      CEA_REQUIRE(written.insert(dst[i]).second, CEA_EINVAL, "%s: page %lld is written twice", what,
+                  (long long)dst[i]);
+    }
+    for (int64_t i = 0; i < moves; ++i)
+      CEA_REQUIRE(!written.count(src[i]), CEA_EINVAL, "%s: page %lld is both read and written", what,
+                  (long long)src[i]);
+  } catch (const std::bad_alloc&) {
+    set_error("%s: out of host memory", what);
+    return CEA_ELAUNCH;
+  }
+  if (moves == 0) return CEA_OK;
+  return launch_copy_pages(n, pools, src, dst, moves, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -533,6 +533,120 @@ void kv_append(Tensor cache_k, Tensor cache_v, Tensor cache_pos, int64_t offset,
   }
 }
 
+// ---------------------------------------------------------------------------------------
+// paged KV cache
+// ---------------------------------------------------------------------------------------
+Tensor given(const c10::optional<Tensor>& t) { return t ? *t : Tensor(); }
+
+// Caches are written and read in place, so their layout is the caller's: no copies are made.
+void check_pools(const Tensor& k_pages, const Tensor& v_pages) {
+  TORCH_CHECK_VALUE(k_pages.dim() == 4 && v_pages.dim() == 4, "k_pages and v_pages must be [P, H, page, D]");
+}
+
+void paged_kv_append(Tensor k_pages, Tensor v_pages, const c10::optional<Tensor>& pos_pages_in,
+                     const Tensor& tables_in, const Tensor& offsets_in, const c10::optional<Tensor>& counts_in,
+                     const Tensor& k_in, const Tensor& v_in, const c10::optional<Tensor>& pos_in,
+                     const c10::optional<Tensor>& cos_in, const c10::optional<Tensor>& sin_in) {
+  const Tensor pp = given(pos_pages_in), counts0 = given(counts_in), pos0 = given(pos_in);
+  const Tensor cos0 = given(cos_in), sin0 = given(sin_in);
+  const at::Device dev = device_of({&k_pages, &v_pages, &pp, &tables_in, &offsets_in, &counts0, &k_in, &v_in,
+                                    &pos0, &cos0, &sin0});
+  check_pools(k_pages, v_pages);
+  TORCH_CHECK_VALUE(cos0.defined() == sin0.defined(), "give both rotary tables or neither");
+  c10::DeviceGuard guard(dev);
+  const Tensor k = inner(k_in), v = inner(v_in), tables = as_i64(tables_in), offsets = as_i64(offsets_in);
+  const Tensor counts = counts0.defined() ? as_i64(counts0) : counts0, pos = pos0.defined() ? as_i64(pos0) : pos0;
+  const Tensor cos = cos0.defined() ? inner(cos0.to(k.scalar_type())) : cos0;
+  const Tensor sin = sin0.defined() ? inner(sin0.to(k.scalar_type())) : sin0;
+  cea_tensor a[11];
+  const Tensor* t[11] = {&k, &v, &pos, &cos, &sin, &tables, &offsets, &counts, &k_pages, &v_pages, &pp};
+  cea_tensor* p[11];
+  for (int i = 0; i < 11; ++i) {
+    p[i] = nullptr;
+    if (t[i]->defined()) a[i] = arg(*t[i]), p[i] = &a[i];
+  }
+  check_rc(cea_paged_kv_append(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], p[8], p[9], p[10], stream_of(dev)),
+           "paged_kv_append");
+}
+
+std::vector<Tensor> paged_attention(const Tensor& q_in, const Tensor& k_pages, const Tensor& v_pages,
+                                    const c10::optional<Tensor>& pos_pages_in, const Tensor& tables_in,
+                                    const Tensor& lengths_in, const Tensor& q_pos_in, bool causal, double scale,
+                                    c10::optional<at::IntArrayRef> kv_map, bool with_lse) {
+  const Tensor pp = given(pos_pages_in);
+  const at::Device dev = device_of({&q_in, &k_pages, &v_pages, &pp, &tables_in, &lengths_in, &q_pos_in});
+  check_pools(k_pages, v_pages);
+  TORCH_CHECK_VALUE(q_in.dim() == 4, "q must be [B, S, H, D]");
+  TORCH_CHECK_VALUE(tables_in.dim() == 2, "tables must be [B, W]");
+  c10::DeviceGuard guard(dev);
+  const Tensor q = inner(q_in), tables = as_i64(tables_in), lengths = as_i64(lengths_in), qp = as_i64(q_pos_in);
+  const int64_t B = q.size(0), Sq = q.size(1), Hq = q.size(2), D = q.size(3);
+  const at::ScalarType acc = acc_of(q.scalar_type());
+  const auto o_opts = at::TensorOptions().device(dev).dtype(with_lse ? acc : q.scalar_type());
+  Tensor out = at::empty({B, Sq, Hq, D}, o_opts);
+  Tensor lse = with_lse ? at::empty({B, Hq, Sq}, o_opts.dtype(acc)) : Tensor();
+  const std::vector<int32_t> m = map_of(kv_map);
+  const size_t bytes = cea_paged_attention_workspace_bytes(B, Sq, Hq, k_pages.size(1), D, tables.size(1),
+                                                           k_pages.size(2), code_of(q.scalar_type()));
+  const Scratch ws = bytes ? workspace(bytes) : Scratch();
+  cea_tensor a[6] = {arg(q), arg(k_pages), arg(v_pages), arg(tables), arg(lengths), arg(qp)};
+  cea_tensor pa, o = arg(out), l;
+  if (pp.defined()) pa = arg(pp);
+  if (with_lse) l = arg(lse);
+  check_rc(cea_paged_attention(&a[0], &a[1], &a[2], pp.defined() ? &pa : nullptr, &a[3], &a[4], &a[5],
+                               causal ? 1 : 0, scale, m.empty() ? nullptr : m.data(), (int32_t)m.size(), &o,
+                               with_lse ? &l : nullptr, ws.data(), ws.size, stream_of(dev)),
+           "paged_attention");
+  if (with_lse) return {out, lse};
+  return {out};
+}
+
+// A pool tensor with its page dimension `dim` as [N, P, E]: the dimensions before it have to
+// collapse into one, those after it to be contiguous (they are copied as bytes).
+cea_tensor pool_arg(const Tensor& t, int64_t dim) {
+  cea_tensor a;
+  a.dtype = code_of(t.scalar_type());
+  TORCH_CHECK_NOT_IMPLEMENTED(a.dtype >= 0, "dtype ", t.scalar_type(), " is not supported by the kernels");
+  TORCH_CHECK_VALUE(dim >= 0 && dim < t.dim(), "copy_pages: a pool of ", t.dim(), " dimensions has no dimension ",
+                    dim);
+  int64_t e = 1, n = 1, stride = 0;
+  for (int64_t i = t.dim() - 1; i > dim; --i) {
+    TORCH_CHECK_VALUE(t.size(i) == 1 || t.stride(i) == e || t.numel() == 0, "copy_pages: a page must be contiguous");
+    e *= t.size(i);
+  }
+  for (int64_t i = dim - 1; i >= 0; --i) {
+    if (t.size(i) == 1) continue;
+    TORCH_CHECK_VALUE(n == 1 || t.stride(i) == stride * n || t.numel() == 0,
+                      "copy_pages: the dimensions before the pages must collapse");
+    if (n == 1) stride = t.stride(i);
+    n *= t.size(i);
+  }
+  a.data = t.numel() > 0 ? t.data_ptr() : nullptr;
+  a.ndim = 3;
+  for (int i = 0; i < CEA_MAX_DIMS; ++i) a.size[i] = a.stride[i] = 0;
+  a.size[0] = n, a.size[1] = t.size(dim), a.size[2] = e;
+  a.stride[0] = stride, a.stride[1] = t.stride(dim), a.stride[2] = 1;
+  return a;
+}
+
+void copy_pages(at::TensorList pools, int64_t dim, const Tensor& src_in, const Tensor& dst_in) {
+  TORCH_CHECK_VALUE(!pools.empty(), "copy_pages: need at least one pool");
+  TORCH_CHECK_VALUE(src_in.device().is_cpu() && dst_in.device().is_cpu() && src_in.dim() == 1 && dst_in.dim() == 1 &&
+                        src_in.size(0) == dst_in.size(0),
+                    "copy_pages: src and dst must be host lists of the same length");
+  TORCH_CHECK_VALUE(at::isIntegralType(src_in.scalar_type(), false) && at::isIntegralType(dst_in.scalar_type(), false),
+                    "copy_pages: page indices must be whole numbers");
+  const at::Device dev = device_of({}, pools);
+  const Tensor src = as_i64(src_in).contiguous(), dst = as_i64(dst_in).contiguous();
+  std::vector<cea_tensor> a;
+  a.reserve(pools.size());
+  for (const Tensor& t : pools) a.push_back(pool_arg(t, dim));
+  c10::DeviceGuard guard(dev);
+  check_rc(cea_copy_pages((int32_t)a.size(), a.data(), src.data_ptr<int64_t>(), dst.data_ptr<int64_t>(), src.numel(),
+                          stream_of(dev)),
+           "copy_pages");
+}
+
 }  // namespace
 
 TORCH_LIBRARY(collab_edge, m) {
@@ -562,6 +676,11 @@ TORCH_LIBRARY(collab_edge, m) {
   m.def("linear_gated(Tensor x, Tensor w_gate, Tensor w_up, Tensor? b_gate, Tensor? b_up, int act) -> Tensor");
   m.def("kv_append(Tensor(a!) cache_k, Tensor(b!) cache_v, Tensor(c!) cache_pos, int offset, Tensor k, "
         "Tensor v, Tensor pos, Tensor? cos, Tensor? sin) -> ()");
+  m.def("paged_kv_append(Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor(c!)? pos_pages, Tensor tables, "
+        "Tensor offsets, Tensor? counts, Tensor k, Tensor v, Tensor? pos, Tensor? cos, Tensor? sin) -> ()");
+  m.def("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor? pos_pages, Tensor tables, "
+        "Tensor lengths, Tensor q_pos, bool causal, float scale, int[]? kv_map, bool with_lse) -> Tensor[]");
+  m.def("copy_pages(Tensor(a!)[] pools, int dim, Tensor src, Tensor dst) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(collab_edge, CompositeExplicitAutograd, m) {
@@ -584,4 +703,7 @@ TORCH_LIBRARY_IMPL(collab_edge, CompositeExplicitAutograd, m) {
   m.impl("linear_into", linear_into);
   m.impl("linear_gated", linear_gated);
   m.impl("kv_append", kv_append);
+  m.impl("paged_kv_append", paged_kv_append);
+  m.impl("paged_attention", paged_attention);
+  m.impl("copy_pages", copy_pages);
 }

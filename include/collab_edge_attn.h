@@ -369,6 +369,54 @@ int cea_linear_gated_ws(const cea_tensor* x, const cea_tensor* w_gate, const cea
                         const cea_tensor* b_gate, const cea_tensor* b_up, cea_tensor* y,
                         int32_t act, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * The paged KV cache.  Pools k_pages, v_pages [P,H,page,D] (any strides, innermost 1) hold pages of
+ * `page` slots; slot j of batch row b is place j % page of page tables[b, j / page].  tables [B,W],
+ * lengths, offsets and counts [B] are int64 device tensors that only the device reads: a page index
+ * outside [0, P) is a page that holds nothing (no key there, and what would be written there is
+ * dropped), lengths count up to W * page slots, and nothing outside the pools is touched whatever
+ * they hold.
+ *
+ * Append: token s < counts[b] (all of them with counts NULL) of row b goes to slot offsets[b] + s: k
+ * [B,n,H,D], rotated with cos/sin [B,n,D] (both or neither; batch may be 1) in f32 (f64 for f64) and
+ * rounded once, v as it is, and its position [B,n] into pos_pages [P,page] (both or neither).  Slots
+ * outside [0, W * page) are dropped.  Two tokens must not share a slot.  The paged form of
+ * LayerKVCache.append after apply_rotary (collab_infer/models/cache.py:51-62, llama.py:80-88).
+ */
+int cea_paged_kv_append(const cea_tensor* k, const cea_tensor* v, const cea_tensor* pos,
+                        const cea_tensor* cos, const cea_tensor* sin, const cea_tensor* tables,
+                        const cea_tensor* offsets, const cea_tensor* counts, cea_tensor* k_pages,
+                        cea_tensor* v_pages, cea_tensor* pos_pages, void* stream);
+
+/*
+ * Attention of q [B,Sq,Hq,D] over the slots 0 .. lengths[b]-1 of each row's pages, by the masking
+ * rule above; the position of slot j is j, or what pos_pages [P,page] holds there when it is given.
+ * Keys that a query does not see do not reach its result, whatever their pages hold.  A chunk of new
+ * tokens is attended after its append, with lengths that include it; padding queries have q_pos -1.
+ * The paged form of attention / attention_with_lse (collab_infer/parallel/attention.py:201-239,
+ * 270-301) over a LayerKVCache view.
+ *   out [B,Sq,Hq,D] in q's dtype or the accumulation dtype; lse [B,Hq,Sq] in the latter, or NULL.
+ *   workspace: device memory of cea_paged_attention_workspace_bytes() bytes (16-byte aligned,
+ *   contents need no initialisation), not shared with a call that may run at the same time.
+ */
+size_t cea_paged_attention_workspace_bytes(int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int64_t D,
+                                           int64_t W, int64_t page, int32_t in_dtype);
+int cea_paged_attention(const cea_tensor* q, const cea_tensor* k_pages, const cea_tensor* v_pages,
+                        const cea_tensor* pos_pages, const cea_tensor* tables,
+                        const cea_tensor* lengths, const cea_tensor* q_pos, int32_t causal,
+                        double scale, const int32_t* kv_map, int32_t kv_map_len, cea_tensor* out,
+                        cea_tensor* lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Copies page src[i] to page dst[i] (host arrays of `moves` indices) in every pool: n tensors
+ * [N,P,E] of any element type with contiguous pages (N pools each, e.g. the layers' keys and values).
+ * Forks copy the page that two sequences are about to write differently, a compaction moves pages
+ * together.  No page may be written twice, or both read and written; indices outside [0, P) are
+ * refused.  A captured call copies these pages on every replay.
+ */
+int cea_copy_pages(int32_t n, const cea_tensor* pools, const int64_t* src, const int64_t* dst,
+                   int64_t moves, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,235 @@
+"""The host side of the paged KV cache: pages handed out, shared, copied on write, given back and
+compacted, and the argument checks of its entry points (no kernel runs here)."""
+
+import ctypes
+import random
+
+import pytest
+import torch
+
+from test_abi import _t
+
+
+def contents_model(book, store, moves):
+    """Applies page copies to a model of the pool's contents."""
+    for a, b in moves:
+        store[b] = list(store[a])
+
+
+def test_extend_takes_the_lowest_pages_and_fails_whole(cea):
+    book = cea.PageBook(4, 16)
+    a, b = book.new(), book.new()
+    assert book.extend([a, b], [17, 3]) == []
+    assert book.table(a) == [0, 1] and book.table(b) == [2] and book.free_pages == 1
+    with pytest.raises(RuntimeError, match="full"):
+        book.extend([a, b], [16, 14])
+    assert book.length(a) == 17 and book.length(b) == 3 and book.free_pages == 1
+    book.free(a)
+    assert book.free_pages == 3 and book.sequences() == [b]
+    with pytest.raises(ValueError):
+        book.length(a)
+
+
+def test_fork_copies_the_partial_page_on_the_first_write_only(cea):
+    book = cea.PageBook(10, 4)
+    a = book.new()
+    book.extend([a], [6])
+    c1, c2 = book.fork(a), book.fork(a)
+    assert book.table(c1) == book.table(a) and book.free_pages == 8
+    # all three write: two copies, the last holder keeps the page
+    assert book.extend([c1, a, c2], [1, 1, 1]) == [(1, 2), (1, 3)]
+    assert (book.table(c1), book.table(a), book.table(c2)) == ([0, 2], [0, 3], [0, 1])
+    assert book.extend([c1, a, c2], [1, 1, 1]) == []
+    # at a page's end nothing is copied
+    d = book.fork(a)
+    assert book.extend([a, d], [1, 1]) == []
+    book.free(a), book.free(c1), book.free(c2)
+    assert book.free_pages == 7 and book.table(d)[0] == 0
+
+
+def test_a_row_that_only_reads_copies_nothing(cea):
+    book = cea.PageBook(4, 4)
+    a = book.new()
+    book.extend([a], [2])
+    b = book.fork(a)
+    assert book.extend([a, b], [0, 0]) == []
+    assert book.table(a) == book.table(b) == [0]
+
+
+def test_truncate_gives_back_whole_pages(cea):
+    book = cea.PageBook(6, 4)
+    a = book.new()
+    book.extend([a], [11])
+    b = book.fork(a)
+    book.truncate(a, 4)
+    assert book.table(a) == [0] and book.free_pages == 3
+    book.truncate(b, 2)
+    assert book.extend([b], [1]) == [(0, 1)]  # page 0 is a's too
+    with pytest.raises(ValueError):
+        book.truncate(a, 5)
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_random_life_against_a_model(cea, seed):
+    """Sequences of token numbers: whatever is forked, freed, truncated and compacted, a sequence's
+    slots hold its own tokens, written through its table only."""
+    rng = random.Random(seed)
+    page, pages = 4, 40
+    book = cea.PageBook(pages, page)
+    store = [[None] * page for _ in range(pages)]
+    want, fresh = {}, 0
+    for step in range(300):
+        do = rng.choice(["new", "extend", "extend", "extend", "fork", "free", "truncate", "compact"])
+        seqs = book.sequences()
+        if do == "new":
+            want[book.new()] = []
+        elif do == "extend" and seqs:
+            some = rng.sample(seqs, rng.randint(1, len(seqs)))
+            counts = [rng.randint(0, 6) for _ in some]
+            free = book.free_pages
+            try:
+                moves = book.extend(some, counts)
+            except RuntimeError:
+                assert book.free_pages == free
+                continue
+            assert len({b for _, b in moves}) == len(moves)
+            assert not {a for a, _ in moves} & {b for _, b in moves}
+            contents_model(book, store, moves)
+            for s, n in zip(some, counts):
+                for _ in range(n):
+                    slot = len(want[s])
+                    store[book.table(s)[slot // page]][slot % page] = fresh
+                    want[s].append(fresh)
+                    fresh += 1
+        elif do == "fork" and seqs:
+            s = rng.choice(seqs)
+            want[book.fork(s)] = list(want[s])
+        elif do == "free" and seqs:
+            s = rng.choice(seqs)
+            book.free(s)
+            del want[s]
+        elif do == "truncate" and seqs:
+            s = rng.choice(seqs)
+            n = rng.randint(0, len(want[s]))
+            book.truncate(s, n)
+            del want[s][n:]
+        elif do == "compact":
+            moves = book.compact()
+            contents_model(book, store, moves)
+            held = {p for s in book.sequences() for p in book.table(s)}
+            assert held == set(range(len(held)))
+        for s, tokens in want.items():
+            t = book.table(s)
+            assert book.length(s) == len(tokens) and len(t) == -(-len(tokens) // page)
+            assert [store[t[i // page]][i % page] for i in range(len(tokens))] == tokens
+        held = {p for s in book.sequences() for p in book.table(s)}
+        assert book.free_pages == pages - len(held)
+
+
+def test_extend_argument_errors(cea):
+    book = cea.PageBook(4, 4)
+    a = book.new()
+    for seqs, counts in (([a, a], [1, 1]), ([a], [1, 2]), ([a], [-1]), ([7], [1])):
+        with pytest.raises(ValueError):
+            book.extend(seqs, counts)
+    with pytest.raises(ValueError):
+        cea.PageBook(0, 4)
+
+
+def _refs(*ts):
+    return [None if t is None else ctypes.byref(t) for t in ts]
+
+
+def test_c_abi_refuses_bad_arguments_without_launching(cea):
+    """(the pointers here are never dereferenced)"""
+    nat = cea._native
+    lib = nat.load_library()
+    bf16, i64, f32 = 1, 4, 0
+    q, kp, vp = _t((2, 3, 8, 64), bf16), _t((5, 2, 16, 64), bf16), _t((5, 2, 16, 64), bf16)
+    tab, n, qp = _t((2, 4), i64), _t((2,), i64), _t((2, 3), i64)
+    out, lse = _t((2, 3, 8, 64), bf16), _t((2, 8, 3), f32)
+
+    def attend(q=q, kp=kp, vp=vp, pp=None, tab=tab, n=n, qp=qp, out=out, lse=None):
+        return lib.cea_paged_attention(*_refs(q, kp, vp, pp, tab, n, qp), 1, 0.125, None, 0,
+                                       *_refs(out, lse), None, 0, None)
+
+    for bad, word in ((dict(vp=_t((5, 2, 32, 64), bf16)), "pages"), (dict(vp=_t((4, 2, 16, 64), bf16)), "pages"),
+                      (dict(tab=_t((3, 4), i64)), "tables"), (dict(tab=_t((2, 4), f32)), "tables"),
+                      (dict(n=_t((3,), i64)), "lengths"), (dict(qp=_t((2, 2), i64)), "q_pos"),
+                      (dict(pp=_t((5, 15), i64)), "pos_pages"), (dict(out=_t((2, 3, 8, 32), bf16)), "out"),
+                      (dict(lse=_t((2, 3, 8), f32)), "lse"), (dict(kp=_t((5, 3, 16, 64), bf16), vp=_t((5, 3, 16, 64), bf16)), "share"),
+                      (dict(q=_t((2, 3, 8, 64), 2)), "dtype")):
+        assert attend(**bad) == nat.EINVAL, bad
+        assert word in nat.last_error(), (bad, nat.last_error())
+    assert attend(q=_t((2, 3, 8, 64), i64)) == nat.EUNSUPPORTED
+
+    k, v, off = _t((2, 3, 2, 64), bf16), _t((2, 3, 2, 64), bf16), _t((2,), i64)
+
+    def append(k=k, v=v, pos=None, cos=None, sin=None, tab=tab, off=off, counts=None, kp=kp, vp=vp, pp=None):
+        return lib.cea_paged_kv_append(*_refs(k, v, pos, cos, sin, tab, off, counts, kp, vp, pp), None)
+
+    cs = _t((2, 3, 64), bf16)
+    odd = _t((2, 3, 2, 63), bf16)
+    for bad, word in ((dict(v=_t((2, 3, 2, 32), bf16)), "v must"), (dict(off=_t((1,), i64)), "offsets"),
+                      (dict(counts=_t((3,), i64)), "counts"), (dict(pos=qp), "both"), (dict(cos=cs), "both"),
+                      (dict(cos=_t((2, 2, 64), bf16), sin=cs), "cos/sin"), (dict(k=odd, v=odd), "even"),
+                      (dict(kp=_t((5, 3, 16, 64), bf16)), "pages")):
+        assert append(**bad) == nat.EINVAL, bad
+        assert word in nat.last_error(), (bad, nat.last_error())
+
+    pool = (nat.CeaTensor * 1)(_t((2, 6, 32), bf16))
+
+    def copy(src, dst, pools=pool, n=1):
+        arr = ctypes.c_int64 * max(1, len(src))
+        return lib.cea_copy_pages(n, pools, arr(*src), arr(*dst), len(src), None)
+
+    for src, dst, word in (([0], [6], "leaves"), ([-1], [0], "leaves"), ([0, 1], [2, 2], "twice"),
+                           ([0, 1], [1, 2], "both"), ([3], [3], "both")):
+        assert copy(src, dst) == nat.EINVAL and word in nat.last_error(), (src, dst, nat.last_error())
+    assert copy([], []) == 0
+    two = (nat.CeaTensor * 2)(_t((2, 6, 32), bf16), _t((2, 5, 32), bf16))
+    assert copy([0], [1], two, 2) == nat.EINVAL and "number of pages" in nat.last_error()
+    lapped = _t((2, 6, 32), bf16)
+    lapped.stride[1] = 16
+    assert copy([0], [1], (nat.CeaTensor * 1)(lapped)) == nat.EINVAL and "overlap" in nat.last_error()
+    assert copy([0], [1], pool, 17) == nat.EUNSUPPORTED
+
+
+def test_host_tensors_are_refused(cea):
+    k = torch.zeros(1, 1, 2, 64)
+    kp = torch.zeros(2, 2, 16, 64)
+    tab, n = torch.zeros(1, 1, dtype=torch.int64), torch.ones(1, dtype=torch.int64)
+    with pytest.raises(RuntimeError):
+        cea.paged_attention(k, kp, kp, tab, n, torch.zeros(1, 1, dtype=torch.int64))
+    with pytest.raises(RuntimeError):
+        cea.paged_kv_append(kp, kp, tab, n, k, k)
+    with pytest.raises(RuntimeError):
+        cea.copy_pages(kp, [0], [1])
+    with pytest.raises(ValueError):
+        cea.paged_kv_append(kp, kp, tab, n, k, k, pos=n.view(1, 1))
+    with pytest.raises(ValueError):
+        cea.paged_attention(k, kp.half(), kp.half(), tab, n, torch.zeros(1, 1, dtype=torch.int64))
+    with pytest.raises(ValueError):
+        cea.paged_attention(torch.zeros(1, 1, 3, 64), kp, kp, tab, n, torch.zeros(1, 1, dtype=torch.int64))
+
+
+def test_a_step_is_refused_after_its_pages_may_have_changed_hands(cea):
+    cache = cea.PagedKVCache(1, 4, 16, 2, 64, device="cpu")
+    a, b = cache.new(), cache.new()
+    step = cache.extend([a, b], [3, 20])
+    assert step.offsets.tolist() == [0, 0] and step.lengths.tolist() == [3, 20]
+    assert step.tables.tolist() == [[0, -1], [1, 2]] and step.counts.tolist() == [3, 20]
+    cache._check(step)
+    cache.free(a)
+    q = torch.zeros(2, 1, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="older"):
+        cache.attention(0, step, q, torch.zeros(2, 1, dtype=torch.int64))
+    again = cache.extend([b], 1)
+    cache.extend([b], [1], into=again)
+    assert again.offsets.tolist() == [21] and again.lengths.tolist() == [22]
+    cache._check(again)
+    with pytest.raises(ValueError, match="wide"):
+        cache.extend([b], [16], into=again)
+    with pytest.raises(ValueError, match="rows"):
+        cache.extend([], [], into=again)
+    assert cache.length(b) == 22
