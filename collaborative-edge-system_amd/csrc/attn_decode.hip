@@ -35,6 +35,7 @@
 //     out (f32 or the query dtype) and lse.
 #include "cea_kernels.hpp"
 #include "cea_lds_dma.hpp"
+#include "cea_mfma16.hpp"
 
 namespace cea {
 namespace {
@@ -46,50 +47,6 @@ constexpr int CHMAX = 1024;           // keys per chunk at most
 static_assert(CHMAX % DTHREADS == 0 && CHMAX <= 4 * DTHREADS, "one 64-bit tile mask per chunk");
 constexpr float kRescaleLog2 = 8.0f;  // lazy-rescale threshold, log2 units
 
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) s16x4* lds_s16x4_ptr;
-
-template <typename T> struct Mfma16;
-template <> struct Mfma16<bf16> {
-  typedef bf16x8 frag8;
-  static __device__ __forceinline__ f32x4 qk(frag8 a, frag8 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ f32x4 pv(s16x4 a, s16x4 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ s16x4 pack(float a, float b, float c, float d) {
-    bf16x4 v = {(bf16)a, (bf16)b, (bf16)c, (bf16)d};
-    s16x4 r;
-    __builtin_memcpy(&r, &v, 8);
-    return r;
-  }
-};
-template <> struct Mfma16<f16> {
-  typedef f16x8 frag8;
-  static __device__ __forceinline__ f32x4 qk(frag8 a, frag8 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ f32x4 pv(s16x4 a, s16x4 b, f32x4 c) {
-    f16x4 x, y;
-    __builtin_memcpy(&x, &a, 8);
-    __builtin_memcpy(&y, &b, 8);
-    return __builtin_amdgcn_mfma_f32_16x16x16f16(x, y, c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ s16x4 pack(float a, float b, float c, float d) {
-    f16x4 v = {(f16)a, (f16)b, (f16)c, (f16)d};
-    s16x4 r;
-    __builtin_memcpy(&r, &v, 8);
-    return r;
-  }
-};
-
 template <int D> struct DLayout {
   static constexpr int ROW = D * 2;                 // bytes per key row
   static constexpr int TILE_BYTES = TK * ROW;       // one K or V tile
@@ -99,27 +56,6 @@ template <int D> struct DLayout {
   static constexpr int LOADS = TILE_BYTES / 1024;   // direct loads per tensor per tile
 };
 
-__device__ __forceinline__ float max_halves(float x) {
-  const uint32_t u = __float_as_uint(x);
-  const auto sw = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  return __builtin_fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-}
-__device__ __forceinline__ float sum_halves(float x) {
-  const uint32_t u = __float_as_uint(x);
-  const auto sw = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  return __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
-}
-// the same over the lane pairs l, l ^ 16 (v_permlane16_swap: rows 0 and 1, rows 2 and 3)
-__device__ __forceinline__ float max_rows16(float x) {
-  const uint32_t u = __float_as_uint(x);
-  const auto sw = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-  return __builtin_fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-}
-__device__ __forceinline__ float sum_rows16(float x) {
-  const uint32_t u = __float_as_uint(x);
-  const auto sw = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-  return __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
-}
 // max / sum over the 64 lanes, the result in every lane, without LDS round trips: each step
 // pairs every lane with one partner (xor 1 and xor 2 by DPP quad permutes, the quads of a
 // half-row by DPP row_half_mirror, the half-rows by row_mirror, then l ^ 16 and l ^ 32 by

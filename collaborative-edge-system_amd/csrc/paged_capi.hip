@@ -1,6 +1,8 @@
 // C ABI of the paged KV cache: argument checks, the choice of kernel and the workspace layout.
+#include <math.h>
 #include <string.h>
 
+#include <algorithm>
 #include <new>
 #include <unordered_set>
 
@@ -41,6 +43,27 @@ int check_pos_pages(const cea_tensor* pp, const cea_tensor* kp, const char* what
 }
 
 }  // namespace
+
+bool paged_tiles_supported(const PagedParams& p) {
+  if (!(p.in_dtype == CEA_BF16 || p.in_dtype == CEA_F16) || !(p.D == 64 || p.D == 128)) return false;
+  if (p.page % 16 != 0 || p.W == 0) return false;
+  // slots and places in 32 bits, and page numbers by multiplication (u / m = u * ceil(2^32 / m) >> 32
+  // while u * m < 2^32, u the slot's sixteenth, m the page's)
+  const int64_t slots = (int64_t)p.W * p.page;
+  if (slots >= (int64_t)1 << 30 || slots / 16 * (p.page / 16) >= (int64_t)1 << 32) return false;
+  // exponents take |scale| * log2(e) as a factor, which has to be a normal number
+  if (!(fabs(p.scale) >= 1e-30 && fabs(p.scale) <= 1e30)) return false;
+  const int64_t s8[] = {p.qs_b, p.qs_s, p.qs_h, p.ks_p, p.ks_h, p.ks_s, p.vs_p, p.vs_h, p.vs_s};
+  for (int64_t s : s8)
+    if (s % 8) return false;
+  for (const void* d : {p.q, p.k, p.v})
+    if ((uintptr_t)d % 16) return false;
+  // a 64-row tile spans less than 2^31 bytes
+  for (int64_t s : {p.ks_s, p.vs_s})
+    if (s < p.D || s >= (int64_t)1 << 23) return false;
+  return p.pos == nullptr || p.ps_s == 1;
+}
+
 }  // namespace cea
 
 using namespace cea;
@@ -94,7 +117,13 @@ int cea_paged_kv_append(const cea_tensor* k, const cea_tensor* v, const cea_tens
 
 size_t cea_paged_attention_workspace_bytes(int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int64_t D,
                                            int64_t W, int64_t page, int32_t in_dtype) {
-  return 0;
+  if (!(in_dtype == CEA_BF16 || in_dtype == CEA_F16) || !(D == 64 || D == 128)) return 0;
+  if (B <= 0 || Sq <= 0 || Hq <= 0 || Hkv <= 0 || W <= 0 || page <= 0 || page % 16) return 0;
+  // (an explicit map takes the place of an even grouping, or there is none: room for either)
+  size_t most = paged_token_workspace_bytes(B, Sq, Hq, Hkv, 0, D, W * page);
+  if (Hq % Hkv == 0)
+    most = std::max(most, paged_token_workspace_bytes(B, Sq, Hq, Hkv, (int)(Hq / Hkv), D, W * page));
+  return most;
 }
 
 int cea_paged_attention(const cea_tensor* q, const cea_tensor* k_pages, const cea_tensor* v_pages,
@@ -157,7 +186,14 @@ int cea_paged_attention(const cea_tensor* q, const cea_tensor* k_pages, const ce
   p.group = map.group;
   if (B == 0 || Sq == 0 || Hq == 0) return CEA_OK;
   if (page == 0 || p.P == 0) p.W = 0, p.page = 1;  // no slots: every row is empty
-  return launch_paged_generic(p, map, (hipStream_t)stream);
+  hipStream_t st = (hipStream_t)stream;
+  if (paged_tiles_supported(p) && paged_token_supported(p, map)) {
+    const size_t need = paged_token_workspace_bytes(B, Sq, Hq, Hkv, map.group, D, W * page);
+    CEA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), CEA_ENOSPACE,
+                "%s: workspace of %zu bytes needed, %zu given", what, need, workspace_bytes);
+    return launch_paged_token(p, map, workspace, st);
+  }
+  return launch_paged_generic(p, map, st);
 }
 
 int cea_copy_pages(int32_t n, const cea_tensor* pools, const int64_t* src, const int64_t* dst,
