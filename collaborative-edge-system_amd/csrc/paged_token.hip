@@ -47,10 +47,17 @@ struct TokenParams {
   int32_t G, units;       // query heads of a unit, units of a row
   int32_t page16;         // page / 16
   uint32_t magic;         // ceil(2^32 / page16), for page16 > 1
-  int32_t wgs, min_run;   // workgroups, blocks of a run at least
+  int32_t wgs;            // workgroups at most
   float* partial;         // 2 x wgs parts of [rows][D + 2]: o, m, l
   uint8_t kv[kPagedMapHeads];  // explicit head map (p.group == 0)
 };
+
+// The kernel's arguments behind a pointer that the compiler knows nothing about.
+typedef const void __attribute__((address_space(4))) * kernel_args_ptr;
+__device__ __forceinline__ kernel_args_ptr opaque(kernel_args_ptr p) {
+  asm volatile("" : "+s"(p));
+  return p;
+}
 
 template <int D> struct TLayout {
   static constexpr int ROW = D * 2;
@@ -130,9 +137,21 @@ __device__ __forceinline__ LineRow row_of(const TokenParams& t, const Line& line
   return r;
 }
 
-// Blocks of a workgroup's run.
-__device__ __forceinline__ int run_of(const TokenParams& t, int total) {
-  return max((total + t.wgs - 1) / t.wgs, t.min_run);
+// The line cut into runs: the first `more` workgroups take `run + 1` blocks, the others `run`.
+struct Runs {
+  int run, more;
+  __device__ __forceinline__ int start(int wg) const { return wg * run + min(wg, more); }
+  __device__ __forceinline__ int wg_of(int at) const {  // the workgroup that takes block `at`
+    const int big = more * (run + 1);
+    return at < big ? at / (run + 1) : more + (at - big) / run;
+  }
+};
+__device__ __forceinline__ Runs runs_of(const TokenParams& t, int total) {
+  const int wgs = max(1, min(t.wgs, total));
+  Runs r;
+  r.run = total / wgs;
+  r.more = total - r.run * wgs;
+  return r;
 }
 
 template <typename O> __device__ __forceinline__ void write_out(const PagedParams& p, int b, int s, int h, int d,
@@ -146,49 +165,47 @@ template <typename T> __device__ __forceinline__ void write_row(const PagedParam
 }
 
 template <typename T, int D, bool POS, int NW, bool SPLIT, int PC>
-__global__ __launch_bounds__(NW * 64) void paged_token_kernel(const TokenParams t) {
+__global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void paged_token_kernel(const TokenParams args) {
   typedef TLayout<D> L;
   typedef typename Mfma16<T>::frag8 frag8;
   constexpr int BLK = NW * TK;
   constexpr float kPScale = std::is_same<T, f16>::value ? 128.f : 1.f;  // keeps the second piece normal
   extern __shared__ __attribute__((aligned(16))) char dsmem[];
-  __shared__ float red_m[NW][ROWS], red_l[NW][ROWS];
-  const PagedParams& p = t.p;
+  __shared__ float2 red_ml[ROWS][NW];
   const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63;
   const int row = lane & 15, grp = lane >> 4;
-  const int nrows = p.Sq * t.G;
+  const int nrows = args.p.Sq * args.G;
   const bool row_real = row < nrows;
-  const int rs = row_real ? row / t.G : 0, rg = row_real ? row - rs * t.G : 0;
+  const int rs = row_real ? row / args.G : 0, rg = row_real ? row - rs * args.G : 0;
   char* wb = dsmem + wave * L::WAVE_BYTES;
 
   // ---- this workgroup's run of blocks
   int b, unit, lo, left, blocks;
   if constexpr (SPLIT) {
-    const Line line = line_of<BLK>(t);
-    const int run = run_of(t, line.total);
-    const int64_t at64 = (int64_t)blockIdx.x * run;
-    if (at64 >= line.total) return;
-    const int at = (int)at64;
-    const LineRow r = row_of<BLK>(t, line, at, 0);
+    const Line line = line_of<BLK>(args);
+    const Runs runs = runs_of(args, line.total);
+    const int at = runs.start(blockIdx.x);
+    if (at >= line.total) return;
+    const LineRow r = row_of<BLK>(args, line, at, 0);
     b = r.b, blocks = r.blocks;
     unit = (at - r.first) / blocks;
     lo = at - r.first - unit * blocks;
-    left = min(run, line.total - at);
+    left = runs.run + (blockIdx.x < runs.more ? 1 : 0);
   } else {
-    b = blockIdx.x / t.units;
-    unit = blockIdx.x - b * t.units;
-    const int n = slots_of(p, b);
+    b = blockIdx.x / args.units;
+    unit = blockIdx.x - b * args.units;
+    const int n = slots_of(args.p, b);
     blocks = n > 0 ? (n + BLK - 1) / BLK : 1;
     lo = 0;
     left = blocks;
   }
 
-  const int cap = p.W * p.page;
-  const float scale = (float)p.scale;
+  const int cap = args.p.W * args.p.page;
+  const float scale = (float)args.p.scale;
   const float c = fabsf(scale) * 1.4426950408889634f;  // exp2 units
   const float grow_thr = kRescaleLog2 / c;
   const uint32_t flip = scale < 0.f ? 0x80008000u : 0u;
-  const uint32_t krow = (uint32_t)(p.ks_s * sizeof(T)), vrow = (uint32_t)(p.vs_s * sizeof(T));
+  const uint32_t krow = (uint32_t)(args.p.ks_s * sizeof(T)), vrow = (uint32_t)(args.p.vs_s * sizeof(T));
   uint32_t k_voff[L::LOADS], v_voff[L::LOADS];
 #pragma unroll
   for (int i = 0; i < L::LOADS; ++i) {
@@ -210,33 +227,19 @@ __global__ __launch_bounds__(NW * 64) void paged_token_kernel(const TokenParams 
 
   while (true) {
     // ---- one unit of the run, blocks [lo, hi)
+    // (the arguments are read again for every unit: kept across units they would fill the scalar
+    // registers, whose spills took 24 to 48 vector registers and a wave of the occupancy)
+    const kernel_args_ptr ap = opaque((kernel_args_ptr)__builtin_amdgcn_kernarg_segment_ptr());
+    const TokenParams& t = *(const TokenParams*)ap;
+    const PagedParams& p = t.p;
     const int hi = min(blocks, lo + left);
     const int kvh = p.group > 0 ? unit * t.G / p.group : t.kv[unit * t.G];
     const int n = slots_of(p, b);
     const scalar_i64 table = (scalar_i64)(uintptr_t)(p.tables + b * p.ts_b);
-    const int64_t qpos = p.q_pos[b * p.qps_b + rs * p.qps_s];
-    // slots [0, lim) of this lane's row are visible by slot, all rows see [0, lim_all), none beyond
-    // lim_any (with positions in the pool the slots say nothing but where the row ends)
-    int lim = n, lim_all = n, lim_any = n;
-    if (POS && p.causal && __ballot(row_real && qpos >= 0) == 0) lim_any = 0;
-    if (!POS && p.causal) {
-      lim = (int)max((int64_t)0, min(qpos + 1, (int64_t)n));
-      lim_all = row_real ? lim : n;
-      lim_any = row_real ? lim : 0;
-      if (p.Sq > 1) {
-#pragma unroll
-        for (int off = 8; off >= 1; off >>= 1) {
-          lim_all = min(lim_all, __shfl_xor(lim_all, off, 64));
-          lim_any = max(lim_any, __shfl_xor(lim_any, off, 64));
-        }
-      }
-      lim_all = uniform(lim_all), lim_any = uniform(lim_any);  // (lane 0 holds a real row)
-    }
     const char* kh = (const char*)((const T*)p.k + (int64_t)kvh * p.ks_h);
     const char* vh = (const char*)((const T*)p.v + (int64_t)kvh * p.vs_h);
 
     // this wave's tiles: slots slot0, slot0 + BLK, ... below end
-    const int end = min(hi * BLK, lim_any);
     auto page_of = [&](int slot) -> int {
       const uint32_t u = (uint32_t)slot >> 4;
       return (int)(t.page16 == 1 ? u : __umulhi(u, t.magic));
@@ -265,11 +268,15 @@ __global__ __launch_bounds__(NW * 64) void paged_token_kernel(const TokenParams 
     };
     constexpr int LPT = 2 * L::LOADS + (POS ? 1 : 0);
 
+    // (the first two tiles are on their way before the queries' positions are known: they may be read
+    // for nothing)
+    int end = min(hi * BLK, n);
     int s0 = lo * BLK + wave * TK;  // the tile being computed; s0 + BLK and s0 + 2 BLK follow
     int64_t id0 = id_of(s0), id1 = id_of(s0 + BLK), id2 = id_of(s0 + 2 * BLK);
     if (s0 < end) load_tile(s0, id0, 0);
     if (s0 + BLK < end) load_tile(s0 + BLK, id1, 1);
 
+    const int64_t qpos = p.q_pos[b * p.qps_b + rs * p.qps_s];
     // this lane's query fragments (B operand of S = K.Q^T), the sign of a negative scale folded in
     frag8 qf[D / 32];
     {
@@ -283,6 +290,26 @@ __global__ __launch_bounds__(NW * 64) void paged_token_kernel(const TokenParams 
         __builtin_memcpy(&qf[ks], &raw, 16);
       }
     }
+
+    // this lane's row sees slots [0, lim) by their number, all rows see [0, lim_all), none beyond
+    // lim_any (with positions in the pool the slots say nothing but where the row ends)
+    int lim = n, lim_all = n, lim_any = n;
+    if (POS && p.causal && __ballot(row_real && qpos >= 0) == 0) lim_any = 0;
+    if (!POS && p.causal) {
+      lim = (int)max((int64_t)0, min(qpos + 1, (int64_t)n));
+      lim_all = row_real ? lim : n;
+      lim_any = row_real ? lim : 0;
+      if (p.Sq > 1) {
+#pragma unroll
+        for (int off = 8; off >= 1; off >>= 1) {
+          lim_all = min(lim_all, __shfl_xor(lim_all, off, 64));
+          lim_any = max(lim_any, __shfl_xor(lim_any, off, 64));
+        }
+      }
+      lim_all = uniform(lim_all), lim_any = uniform(lim_any);  // (lane 0 holds a real row)
+    }
+    end = min(end, lim_any);
+    if (s0 >= end) wait_vmcnt<0>();  // no tile to wait for below, but the buffers are free after it
 
     f32x4 o[D / 16];
 #pragma unroll
@@ -402,10 +429,7 @@ __global__ __launch_bounds__(NW * 64) void paged_token_kernel(const TokenParams 
 
     // ---- join the waves.  A row's sum is 0 exactly where it saw no key (a NaN is kept).
     const float l_row = sum_halves(sum_rows16(l_run));
-    if (grp == 0) {
-      red_m[wave][row] = m_run == -__builtin_inff() ? m_run : m_run * fabsf(scale);
-      red_l[wave][row] = l_row;
-    }
+    if (grp == 0) red_ml[row][wave] = make_float2(m_run, l_row);
     float* red_o = (float*)wb;  // this wave's own buffers, no longer read as tiles
     if (row_real) {
 #pragma unroll
@@ -416,26 +440,33 @@ __global__ __launch_bounds__(NW * 64) void paged_token_kernel(const TokenParams 
     float* part = t.partial + ((int64_t)blockIdx.x * 2 + (lo == 0 ? 1 : 0)) * nrows * (D + 2);
     for (int i = tid; i < nrows * D; i += NW * 64) {
       const int r = i / D, d = i % D;
-      float M = -__builtin_inff();
+      float2 ml[NW];
+      float x[NW];
 #pragma unroll
-      for (int w = 0; w < NW; ++w) M = fmaxf(M, red_m[w][r]);
+      for (int w = 0; w < NW; ++w) {
+        ml[w] = red_ml[r][w];
+        x[w] = ((const float*)(dsmem + w * L::WAVE_BYTES))[i];
+      }
+      float M = -__builtin_inff();  // of the raw scores
+#pragma unroll
+      for (int w = 0; w < NW; ++w) M = fmaxf(M, ml[w].x);
       const float shift = M == -__builtin_inff() ? 0.f : M;
       float acc = 0.f, sum = 0.f;
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
-        const float l = red_l[w][r];
-        if (l == 0.f) continue;
-        const float wt = red_m[w][r] == -__builtin_inff() ? 1.f : expf(red_m[w][r] - shift);
-        acc = __builtin_fmaf(((const float*)(dsmem + w * L::WAVE_BYTES))[i], wt, acc);
-        sum = __builtin_fmaf(l, wt, sum);
+        // (a wave that saw nothing has zeros; one whose scores are all NaN keeps its NaN)
+        const float wt = ml[w].x == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f((ml[w].x - shift) * c);
+        acc = __builtin_fmaf(x[w], wt, acc);
+        sum = __builtin_fmaf(ml[w].y, wt, sum);
       }
       acc *= 1.f / kPScale;
+      M *= fabsf(scale);
       if (!SPLIT || all) {
         const int s = r / t.G, h = unit * t.G + r - s * t.G;
         write_row<T>(p, b, s, h, d, sum == 0.f ? 0.f : acc / sum);
         if (p.lse && d == 0)
           ((float*)p.lse)[b * p.ls_b + h * p.ls_h + s * p.ls_s] =
-              sum == 0.f ? -__builtin_inff() : shift + logf(sum);
+              sum == 0.f ? -__builtin_inff() : (M == -__builtin_inff() ? 0.f : M) + logf(sum);
       } else {
         // non-temporal: written back past the caches, they disturb the reads of other workgroups least
         __builtin_nontemporal_store(acc, part + r * (D + 2) + d);
@@ -459,77 +490,101 @@ __global__ __launch_bounds__(NW * 64) void paged_token_kernel(const TokenParams 
   }
 }
 
-// Joins the parts of the units that the runs cut, one workgroup per (row, token, query head).
+// Joins the parts of the units that the runs cut, one workgroup per (row, token, query head): every
+// wave weighs 64 parts at a time, a part a lane, and sums every fourth part's features, whose reads
+// are under way by then (one trip to memory for the lengths and one for up to 64 parts).
 template <typename T, int D, int NW>
 __global__ __launch_bounds__(256) void paged_token_join_kernel(const TokenParams t) {
   constexpr int FPL = D / 64;  // features per lane
-  __shared__ float m_s[4], l_s[4], o_s[4][D];
+  constexpr int PER = 16;      // parts of a wave among 64
+  __shared__ float o_s[4][D];
   const PagedParams& p = t.p;
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63;
   const int h = blockIdx.x % p.Hq, s = (blockIdx.x / p.Hq) % p.Sq, b = blockIdx.x / (p.Hq * p.Sq);
-  LineRow r;
   const Line line = line_of<NW * TK>(t);
-  r = row_of<NW * TK>(t, line, -1, b);
-  const int run = run_of(t, line.total), unit = h / t.G;
-  const int start = r.first + unit * r.blocks, end = start + r.blocks;
-  const int w0 = start / run, w1 = (end - 1) / run;
-  if (w0 == w1) return;  // finished by its workgroup
-  const int nrows = p.Sq * t.G, rr = s * t.G + h - unit * t.G;
-  const int64_t stride = (int64_t)nrows * (D + 2);
-  // the first part is its workgroup's last unit (slot 1), the others' first (slot 0)
-  const float* base = t.partial + rr * (D + 2);
+  const LineRow r = row_of<NW * TK>(t, line, -1, b);
+  const Runs runs = runs_of(t, line.total);
+  const int unit = h / t.G, start = r.first + unit * r.blocks;
+  const int w0 = runs.wg_of(start), n = runs.wg_of(start + r.blocks - 1) - w0 + 1;
+  if (n == 1) return;  // finished by its workgroup
+  const int nrows = p.Sq * t.G;
+  // the first part is its workgroup's last unit (slot 1), the others' their first (slot 0)
+  const int64_t stride = 2 * (int64_t)nrows * (D + 2);
+  const float* base = t.partial + w0 * stride + (int64_t)(s * t.G + h - unit * t.G) * (D + 2);
+  auto part = [&](int j) { return base + j * stride + (j == 0 ? stride / 2 : 0); };
   float m = -__builtin_inff(), l = 0.f, o[FPL] = {};
-  for (int w = w0 + wave; w <= w1; w += 4) {
-    const float* part = base + ((int64_t)w * 2 + (w == w0 ? 1 : 0)) * stride;
-    const float pm = part[D], pl = part[D + 1];
-    float x[FPL];
+  for (int j0 = 0; j0 < n; j0 += 64) {
+    float x[PER][FPL];
 #pragma unroll
-    for (int i = 0; i < FPL; ++i) x[i] = part[lane * FPL + i];
-    if (pl == 0.f) continue;
-    const float m_new = fmaxf(m, pm), shift = m_new == -__builtin_inff() ? 0.f : m_new;
-    const float a = l == 0.f || m == -__builtin_inff() ? 1.f : expf(m - shift);
-    const float e = pm == -__builtin_inff() ? 1.f : expf(pm - shift);
+    for (int k = 0; k < PER; ++k) {
+      const int j = j0 + wave + 4 * k;
+      const float* q = part(j < n ? j : 0) + lane * FPL;
+#pragma unroll
+      for (int i = 0; i < FPL; ++i) x[k][i] = q[i];
+    }
+    const float* q = part(j0 + lane < n ? j0 + lane : 0);
+    const float pm = j0 + lane < n ? q[D] : -__builtin_inff(), pl = j0 + lane < n ? q[D + 1] : 0.f;
+    float m_new = m;
+    {
+      float v = pm;
+#pragma unroll
+      for (int off = 1; off < 16; off <<= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
+      m_new = fmaxf(m, max_halves(max_rows16(v)));
+    }
+    const float shift = m_new == -__builtin_inff() ? 0.f : m_new;
+    const float a = m == -__builtin_inff() ? 1.f : expf(m - shift);
+    const float wt = pl == 0.f ? 0.f : pm == -__builtin_inff() ? 1.f : expf(pm - shift);
+    float sum = pl * wt;
+#pragma unroll
+    for (int off = 1; off < 16; off <<= 1) sum += __shfl_xor(sum, off, 64);
     m = m_new;
-    l = l * a + pl * e;
+    l = l * a + sum_halves(sum_rows16(sum));
 #pragma unroll
-    for (int i = 0; i < FPL; ++i) o[i] = o[i] * a + x[i] * e;
+    for (int i = 0; i < FPL; ++i) o[i] *= a;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wt), wave + 4 * k));
+#pragma unroll
+      for (int i = 0; i < FPL; ++i)
+        if (w != 0.f) o[i] = __builtin_fmaf(x[k][i], w, o[i]);
+    }
   }
-  if (lane == 0) m_s[wave] = m, l_s[wave] = l;
 #pragma unroll
   for (int i = 0; i < FPL; ++i) o_s[wave][lane * FPL + i] = o[i];
   __syncthreads();
   if (tid >= D) return;
-  float M = -__builtin_inff();
-#pragma unroll
-  for (int w = 0; w < 4; ++w) M = fmaxf(M, m_s[w]);
-  const float shift = M == -__builtin_inff() ? 0.f : M;
-  float acc = 0.f, sum = 0.f;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    if (l_s[w] == 0.f) continue;
-    const float wt = m_s[w] == -__builtin_inff() ? 1.f : expf(m_s[w] - shift);
-    acc = __builtin_fmaf(o_s[w][tid], wt, acc);
-    sum = __builtin_fmaf(l_s[w], wt, sum);
-  }
-  write_row<T>(p, b, s, h, tid, sum == 0.f ? 0.f : acc / sum);
+  const float acc = (o_s[0][tid] + o_s[1][tid]) + (o_s[2][tid] + o_s[3][tid]);
+  write_row<T>(p, b, s, h, tid, l == 0.f ? 0.f : acc / l);
   if (p.lse && tid == 0)
-    ((float*)p.lse)[b * p.ls_b + h * p.ls_h + s * p.ls_s] = sum == 0.f ? -__builtin_inff() : shift + logf(sum);
+    ((float*)p.lse)[b * p.ls_b + h * p.ls_h + s * p.ls_s] =
+        l == 0.f ? -__builtin_inff() : (m == -__builtin_inff() ? 0.f : m) + logf(l);
 }
 
-constexpr int NW_SPLIT = 4, NW_WHOLE = 8;
+constexpr int NW_SPLIT = 4;  // waves of a workgroup that takes a run
+
+template <typename T, int D, bool POS, int PC, int NW>
+int launch_whole(const TokenParams& t, hipStream_t st) {
+  constexpr int lds = NW * TLayout<D>::WAVE_BYTES;
+  const hipError_t e = reserve_lds<paged_token_kernel<T, D, POS, NW, false, PC>>(lds);
+  CEA_REQUIRE(e == hipSuccess, CEA_ELAUNCH, "paged_attention: cannot reserve %d bytes of LDS: %s", lds,
+              hipGetErrorString(e));
+  hipLaunchKernelGGL((paged_token_kernel<T, D, POS, NW, false, PC>), dim3((unsigned)(t.p.B * t.units)), dim3(NW * 64),
+                     lds, st, t);
+  CEA_CHECK_LAUNCH("paged_token");
+  return CEA_OK;
+}
 
 template <typename T, int D, bool POS, int PC>
 int launch_form(const TokenParams& t, bool whole, hipStream_t st) {
   typedef TLayout<D> L;
   if (whole) {
-    constexpr int lds = NW_WHOLE * L::WAVE_BYTES;
-    const hipError_t e = reserve_lds<paged_token_kernel<T, D, POS, NW_WHOLE, false, PC>>(lds);
-    CEA_REQUIRE(e == hipSuccess, CEA_ELAUNCH, "paged_attention: cannot reserve %d bytes of LDS: %s", lds,
-                hipGetErrorString(e));
-    hipLaunchKernelGGL((paged_token_kernel<T, D, POS, NW_WHOLE, false, PC>), dim3((unsigned)(t.p.B * t.units)),
-                       dim3(NW_WHOLE * 64), lds, st, t);
-    CEA_CHECK_LAUNCH("paged_token");
-    return CEA_OK;
+    // as many waves as keep all units resident at once (us, 4 / 8 / 16 waves: 4 units of 777 keys, D =
+    // 64, 14.9 / 10.3 / 9.8; 256 units of up to 1000, D = 64, 18.6 / 13.9 / 13.6; D = 128: 64 units
+    // of up to 1000 keys 21.4 / 16.4 / -, 320 26.3 / 24.5 / -, 512 of up to 700 26.6 / 28.1 / -)
+    const int64_t pairs = (int64_t)t.p.B * t.units;
+    if (D == 64 && pairs <= 256) return launch_whole<T, D, POS, PC, D == 64 ? 16 : 8>(t, st);
+    if (pairs <= (D == 64 ? 512 : 384)) return launch_whole<T, D, POS, PC, 8>(t, st);
+    return launch_whole<T, D, POS, PC, 4>(t, st);
   }
   constexpr int lds = NW_SPLIT * L::WAVE_BYTES;
   const hipError_t e = reserve_lds<paged_token_kernel<T, D, POS, NW_SPLIT, true, PC>>(lds);
@@ -553,7 +608,7 @@ template <typename T, int D> int launch_td(const TokenParams& t, bool whole, hip
 }
 
 struct TokenPlan {
-  int32_t G, units, wgs, min_run;
+  int32_t G, units, wgs;
   bool whole;
 };
 
@@ -565,6 +620,9 @@ int unit_heads(int64_t Sq, int64_t Hq, int64_t Hkv, int group) {
   return 0;
 }
 
+// Slots of a table up to which a unit is one workgroup's: the second launch costs the host 3 us, and the
+// GPU as much as the split saves (us, whole / split: 4 units of 777 keys, D = 64, 9.8 / 9.7; 4 of 1500
+// 14.1 / 9.9; D = 128: 8 of 777 12.6 / 10.8, 64 of up to 1000 16.4 / 14.8, 320 24.5 / 33.1).
 constexpr int64_t kTokenWhole = 1024;
 
 TokenPlan plan_token(int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int group, int64_t slots) {
@@ -574,8 +632,10 @@ TokenPlan plan_token(int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int group, 
   r.whole = slots <= kTokenWhole;
   const int64_t blocks = std::max<int64_t>(1, (slots + NW_SPLIT * TK - 1) / (NW_SPLIT * TK));
   const int cus = device_cus() > 0 ? device_cus() : 256;
-  r.min_run = 1;
-  r.wgs = (int32_t)std::min<int64_t>(B * r.units * blocks, 4 * cus);
+  // two workgroups per compute unit, as many as are resident at D = 128 (us, 512 / 1024: 8 rows of
+  // 100 to 4096 keys, 32/8 heads of 128, 22.7 / 27.7; one row of 30000 31.4 / 37.1; 32 rows of 1024 to
+  // 32768 346 / 348; 64 rows of 2500 to 7500, 32/4 heads of 64, 69.4 / 72.1; 16 of 500 to 2500 18.3 / 17.3)
+  r.wgs = (int32_t)std::min<int64_t>(B * r.units * blocks, 2 * cus);
   return r;
 }
 
@@ -601,7 +661,7 @@ int launch_paged_token(const PagedParams& p, const HeadMap& map, void* ws, hipSt
   const TokenPlan r = plan_token(p.B, p.Sq, p.Hq, p.Hkv, map.group, (int64_t)p.W * p.page);
   TokenParams t;
   t.p = p;
-  t.G = r.G, t.units = r.units, t.wgs = r.wgs, t.min_run = r.min_run;
+  t.G = r.G, t.units = r.units, t.wgs = r.wgs;
   t.page16 = p.page / 16;
   t.magic = t.page16 > 1 ? (uint32_t)((((uint64_t)1 << 32) + t.page16 - 1) / t.page16) : 0;
   t.partial = (float*)ws;
