@@ -51,6 +51,7 @@ FILE_FLAGS = {
     # M0 is set by the kernel's own LDS-DMA assembly; the clobber note is expected
     "attn_prefill.hip": ["-fno-honor-nans", "-Wno-inline-asm"],
     "attn_decode.hip": ["-fno-honor-nans", "-Wno-inline-asm"],
+    "paged_chunk.hip": ["-fno-honor-nans", "-Wno-inline-asm"],
     "paged_token.hip": ["-Wno-inline-asm"],
     # the layer ops round every product to the tensor dtype before the next add, as the
     # reference's separate tensor ops do: no multiply-add contraction (without this flag

@@ -49,11 +49,17 @@ __device__ __forceinline__ int64_t paged_slots(const PagedParams& p, int b) {
 // of 16 slots, rows of 16-byte vectors, contiguous positions.
 bool paged_tiles_supported(const PagedParams& p);
 
-// A few new tokens per row (at most 16 query rows of a KV head; the head map within kPagedMapHeads).
+// A few new tokens per row (at most 16 query rows of a unit; an explicit head map within kPagedMapHeads).
 bool paged_token_supported(const PagedParams& p, const HeadMap& map);
 size_t paged_token_workspace_bytes(int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int group, int64_t D,
                                    int64_t slots);
 int launch_paged_token(const PagedParams& p, const HeadMap& map, void* ws, hipStream_t s);
+
+// Any number of new tokens per row.  Scratch: tile summaries with positions in the pool, and the partial
+// results of key splits.
+bool paged_chunk_supported(const PagedParams& p, const HeadMap& map);
+size_t paged_chunk_workspace_bytes(int64_t B, int64_t Sq, int64_t Hq, int group, int64_t D, int64_t slots, bool pos);
+int launch_paged_chunk(const PagedParams& p, const HeadMap& map, void* ws, hipStream_t s);
 
 int launch_paged_generic(const PagedParams& p, const HeadMap& map, hipStream_t s);
 

@@ -120,9 +120,11 @@ size_t cea_paged_attention_workspace_bytes(int64_t B, int64_t Sq, int64_t Hq, in
   if (!(in_dtype == CEA_BF16 || in_dtype == CEA_F16) || !(D == 64 || D == 128)) return 0;
   if (B <= 0 || Sq <= 0 || Hq <= 0 || Hkv <= 0 || W <= 0 || page <= 0 || page % 16) return 0;
   // (an explicit map takes the place of an even grouping, or there is none: room for either)
-  size_t most = paged_token_workspace_bytes(B, Sq, Hq, Hkv, 0, D, W * page);
-  if (Hq % Hkv == 0)
-    most = std::max(most, paged_token_workspace_bytes(B, Sq, Hq, Hkv, (int)(Hq / Hkv), D, W * page));
+  const int64_t slots = W * page;
+  size_t most = 0;
+  for (const int group : {0, Hq % Hkv == 0 ? (int)(Hq / Hkv) : 0})
+    most = std::max({most, paged_token_workspace_bytes(B, Sq, Hq, Hkv, group, D, slots),
+                     paged_chunk_workspace_bytes(B, Sq, Hq, group, D, slots, true)});
   return most;
 }
 
@@ -187,11 +189,19 @@ int cea_paged_attention(const cea_tensor* q, const cea_tensor* k_pages, const ce
   if (B == 0 || Sq == 0 || Hq == 0) return CEA_OK;
   if (page == 0 || p.P == 0) p.W = 0, p.page = 1;  // no slots: every row is empty
   hipStream_t st = (hipStream_t)stream;
-  if (paged_tiles_supported(p) && paged_token_supported(p, map)) {
-    const size_t need = paged_token_workspace_bytes(B, Sq, Hq, Hkv, map.group, D, W * page);
-    CEA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), CEA_ENOSPACE,
-                "%s: workspace of %zu bytes needed, %zu given", what, need, workspace_bytes);
-    return launch_paged_token(p, map, workspace, st);
+  if (paged_tiles_supported(p)) {
+    // the token form while one unit holds a KV head's queries, so its keys are read once; and for single
+    // tokens of larger groups
+    const bool few = Sq == 1 || map.group <= 0 || Sq * map.group <= 16;
+    const bool token = few && paged_token_supported(p, map);
+    if (token || paged_chunk_supported(p, map)) {
+      const int64_t slots = W * page;
+      const size_t need = token ? paged_token_workspace_bytes(B, Sq, Hq, Hkv, map.group, D, slots)
+                                : paged_chunk_workspace_bytes(B, Sq, Hq, map.group, D, slots, p.pos != nullptr);
+      CEA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), CEA_ENOSPACE,
+                  "%s: workspace of %zu bytes needed, %zu given", what, need, workspace_bytes);
+      return token ? launch_paged_token(p, map, workspace, st) : launch_paged_chunk(p, map, workspace, st);
+    }
   }
   return launch_paged_generic(p, map, st);
 }

@@ -1,0 +1,796 @@
+// Attention of a chunk of new tokens over a paged KV cache on the matrix cores (bf16 / f16, head size
+// 64 or 128): chunked prefill and whole prompts.
+//
+//   out = sum_j p_j v_j / sum_j p_j,  p_j = exp(s_j - m),  s_j = scale * q.k_j,  lse = m + log sum_j p_j
+//
+// Bound by the matrix cores and the LDS reads that feed them.  The tile body is the prefill kernel's: a workgroup
+// of 8 waves holds 256 query rows of one query head (or, for short chunks, of 2, 4 or 8 heads of one KV
+// head), a wave 32 of them; S^T = K.Q^T per 64-key tile with v_mfma_f32_32x32x16 (a lane holds one
+// row's scores, so its statistics are scalars), O^T += V^T.P^T from the score registers, V
+// transposed on its way out of LDS; K and V go global -> LDS directly through a ring of 4 tiles, 3 in
+// flight; exp2 domain, the reference maximum moved only when a row's grows by 2^8.  What the pages
+// change:
+//   * a wave loads 8 rows of a tile, and pages are multiples of 16 slots, so they lie in one page:
+//     its address stays scalar, and the page index is a scalar read a step ahead of the load;
+//   * without positions in the pool slot j is position j, so the tiles that a workgroup visits are
+//     a prefix of the row and every mask is one 32-bit comparison with the query row's limit; with them a
+//     launch before this one summarises the tiles, and the workgroup lists those it needs;
+//   * lengths are known on the device alone: a launch with few query blocks is cut into key splits by
+//     the table's width, and each split takes an equal run of the tiles that the row really has;
+//   * hidden keys may hold anything.  Their scores are masked; a value that is not finite shows up as
+//     a result that is not, and the workgroup then goes over its tiles once more, carefully: such values are
+//     taken out of the products and added per row as the infinity or NaN that the visible ones make.
+//     A chunk without them pays one look at its results.
+#include <math.h>
+#include <string.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "cea_lds_dma.hpp"
+#include "paged.hpp"
+
+namespace cea {
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4_ptr;
+typedef const int64_t __attribute__((address_space(4))) * scalar_i64;  // read through the scalar cache
+
+template <typename T> struct Mfma;
+template <> struct Mfma<bf16> {
+  typedef bf16x8 frag;
+  static __device__ __forceinline__ f32x16 run(frag a, frag b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <> struct Mfma<f16> {
+  typedef f16x8 frag;
+  static __device__ __forceinline__ f32x16 run(frag a, frag b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+// bit patterns of the 16-bit types: exponent all ones (infinity; above it a NaN), and 1
+template <typename T> struct Bits16;
+template <> struct Bits16<bf16> { static constexpr uint16_t kInf = 0x7f80, kOne = 0x3f80; };
+template <> struct Bits16<f16> { static constexpr uint16_t kInf = 0x7c00, kOne = 0x3c00; };
+
+constexpr int NWAVES = 8;
+constexpr int NTHREADS = NWAVES * 64;
+constexpr int BM = NWAVES * 32;       // query rows per workgroup
+constexpr int BN = kTileKeys;         // keys per tile
+constexpr int WROWS = BN / NWAVES;    // rows of a tile that a wave loads
+constexpr int NSTAGE = 4;             // LDS ring depth
+constexpr int LIST_CAP = 2048;        // tiles listed per pass (positions in the pool)
+constexpr float kRescaleLog2 = 8.0f;
+
+struct ChunkParams {
+  PagedParams p;
+  const TileInfo* tiles;     // [B, ntiles] with positions in the pool
+  int32_t ntiles;
+  int32_t hp;                // query heads of a workgroup: 1, 2, 4, 8
+  int32_t splits;            // key splits
+  int64_t split_out, split_lse;  // elements between the splits' partial results
+  int32_t order_units, order_per_kv;  // workgroup columns that an XCD works through together
+  int32_t page16;
+  uint32_t magic;            // ceil(2^32 / page16), for page16 > 1
+  uint8_t kv[kPagedMapHeads];
+};
+
+template <int D, bool POS> struct Layout {
+  static constexpr int KROW = D * 2;
+  static constexpr int NCG = D / 8;
+  static constexpr int K_BYTES = BN * KROW;
+  static constexpr int V_BYTES = BN * KROW;
+  static constexpr int STAGE_BYTES = K_BYTES + V_BYTES + (POS ? BN * 8 : 0);
+  static constexpr int LDS_BYTES = NSTAGE * STAGE_BYTES;
+  static constexpr int KV_LOADS = K_BYTES / (NTHREADS * 16);
+  static constexpr int ROWS_PER_LOAD = 1024 / KROW;
+  static constexpr int LPT = 2 * KV_LOADS + (POS ? 1 : 0);  // loads of one wave per tile
+  static_assert(KV_LOADS * ROWS_PER_LOAD == WROWS, "a wave loads 8 rows");
+};
+
+template <int D> __device__ __forceinline__ int k_swz(int key) {
+  if constexpr (D / 8 >= 16) return key & 15;
+  else return (key >> 1) & 7;
+}
+template <int D> __device__ __forceinline__ int v_swz(int key) {
+  if constexpr (D == 128) return key & 3;
+  else return (key >> 1) & 1;
+}
+
+template <typename F>
+__device__ __forceinline__ F read_tr_frag(const char* a0, const char* a1) {
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)a0);
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)a1);
+  F f;
+  __builtin_memcpy(&f, &lo, 8);
+  __builtin_memcpy((char*)&f + 8, &hi, 8);
+  return f;
+}
+__device__ __forceinline__ float max3f(float a, float b, float c) {
+  return __builtin_fmaxf(a, __builtin_fmaxf(b, c));
+}
+__device__ __forceinline__ float max_halves(float x) {
+  const uint32_t u = __float_as_uint(x);
+  const auto sw = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __builtin_fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+}
+__device__ __forceinline__ float sum_halves(float x) {
+  const uint32_t u = __float_as_uint(x);
+  const auto sw = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+}
+__device__ __forceinline__ int wave_min_i32(int v) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) v = min(v, __shfl_xor(v, off, 64));
+  return v;
+}
+__device__ __forceinline__ int wave_max_i32(int v) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) v = max(v, __shfl_xor(v, off, 64));
+  return v;
+}
+template <int LPT> __device__ __forceinline__ void wait_tiles_ahead(int ahead) {
+  static_assert(NSTAGE == 4, "wait ladder written for 2 tiles ahead at most");
+  if (ahead >= 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LPT) : "memory");
+  else if (ahead == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LPT) : "memory");
+  else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+// Summaries of the tiles' positions, one wave per tile and row.
+__global__ __launch_bounds__(64) void paged_tile_info_kernel(const PagedParams p, int ntiles, TileInfo* out) {
+  const int t = blockIdx.x, b = blockIdx.y;
+  const int64_t n = paged_slots(p, b), j = (int64_t)t * BN + threadIdx.x;
+  int64_t pos = -1;
+  if (j < n) {
+    const int pg = (int)j / p.page, place = (int)j - pg * p.page;
+    const int64_t id = p.tables[b * p.ts_b + pg * p.ts_w];
+    if (id >= 0 && id < p.P) pos = p.pos[id * p.ps_p + place];
+  }
+  const bool valid = pos >= 0;
+  const int64_t mn = wave_min_i64(valid ? pos : INT64_MAX);
+  const int64_t mx = wave_max_i64(valid ? pos : INT64_MIN);
+  const int cnt = __builtin_popcountll(__ballot(valid));
+  if (threadIdx.x == 0) {
+    TileInfo ti;
+    ti.min_valid = mn;
+    ti.max_valid = mx;
+    ti.n_valid = cnt;
+    ti.pad[0] = ti.pad[1] = ti.pad[2] = 0;
+    out[(int64_t)b * ntiles + t] = ti;
+  }
+}
+
+// PIECES: 16-bit numbers whose sum enters the value product for a probability: one for 16-bit results
+// (p rounded once, half a step of the type, as the result's own rounding is), three of bf16 or two of f16
+// for f32 results (p to 2^-23 and better).
+template <typename T, int D, bool POS, int PIECES>
+__global__ __launch_bounds__(NTHREADS, 2) void paged_chunk_kernel(const ChunkParams c_) {
+  typedef Layout<D, POS> L;
+  typedef typename Mfma<T>::frag frag;
+  const PagedParams& p = c_.p;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ int2 tile_list[POS ? LIST_CAP : 1];  // (tile, 2-bit mode of every wave)
+  __shared__ int64_t red_max[NWAVES], red_min[NWAVES];
+  __shared__ int red_act[NWAVES], wave_cnt[NWAVES];
+  __shared__ int flags[2];  // a page that is not there; a result that is not finite
+
+  const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63;
+  const int r = lane & 31, g = lane >> 5;
+
+  // ---- work mapping over the 8 XCDs, as the prefill kernel's: KV heads are dealt to the XCDs in turn, an
+  // XCD takes as many query heads together as its L2 holds the keys of and starts the latest query
+  // blocks, which see the most, of all of them first; splits are slowest
+  const int hp_log2 = __builtin_ctz(c_.hp), hp = 1 << hp_log2;
+  const int rows_pb = BM >> hp_log2;
+  const int nqb = (p.Sq + rows_pb - 1) >> (__builtin_ctz(BM) - hp_log2);
+  const int ngroups = p.Hq >> hp_log2, units = ngroups * p.B, total = nqb * units;
+  const int nsplit = c_.splits, all = total * nsplit;
+  int blk = blockIdx.x, split = 0, qb, b, hg;
+  if (nsplit > 1) {
+    if ((all & 7) == 0) blk = (blk & 7) * (all >> 3) + (blk >> 3);
+    split = blk / total;
+    blk -= split * total;
+    const int bh = blk / nqb;
+    qb = nqb - 1 - (blk - bh * nqb);
+    b = bh / ngroups;
+    hg = bh - b * ngroups;
+  } else {
+    int unit;
+    if (nqb == 1) {
+      qb = 0;
+      unit = (units & 7) == 0 ? (blk & 7) * (units >> 3) + (blk >> 3) : blk;
+    } else if ((units & 7) == 0) {
+      const int per_xcd = units >> 3, i = blk >> 3;
+      const int set = c_.order_units == per_xcd ? 0 : i / (c_.order_units * nqb);
+      const int x = i - set * c_.order_units * nqb;
+      const int size = min(c_.order_units, per_xcd - set * c_.order_units);
+      qb = x / size;
+      const int per_kv = c_.order_per_kv;
+      const int turn = per_kv % 4 != 0 && size % 2 == 0 ? qb >> 1 : 0;
+      int u = x - qb * size;
+      if (turn != 0) u = (u + turn) % size;
+      u += set * c_.order_units;
+      if (p.group > 0 && ((p.B * p.Hkv) & 7) == 0) {
+        const int kv = per_kv == 1 ? u : u / per_kv;
+        unit = ((blk & 7) + 8 * kv) * per_kv + (u - kv * per_kv);
+      } else {
+        unit = (blk & 7) * per_xcd + u;
+      }
+    } else {
+      qb = blk / units;
+      unit = blk - qb * units;
+    }
+    qb = nqb - 1 - qb;
+    b = p.B == 1 ? 0 : unit / ngroups;
+    hg = unit - b * ngroups;
+  }
+  qb = uniform(qb), b = uniform(b), hg = uniform(hg), split = uniform(split);
+  const int waves_log2 = __builtin_ctz(NWAVES) - hp_log2;  // waves of one head
+  const int h = hg * hp + (wave >> waves_log2);
+  const int kvh = p.group > 0 ? hg * hp / p.group : c_.kv[hg * hp];
+  const int row = qb * rows_pb + (wave & ((1 << waves_log2) - 1)) * 32 + r;
+  const bool row_ok = row < p.Sq;
+  const int64_t qpos = row_ok ? p.q_pos[b * p.qps_b + (int64_t)row * p.qps_s] : -1;
+  const int n = uniform((int)paged_slots(p, b));
+  const int cap = p.W * p.page;
+  const scalar_i64 table = (scalar_i64)(uintptr_t)(p.tables + b * p.ts_b);
+
+  // ---- what the rows see: slots [0, lim) of this lane's row by their number (POS: positions to qpos)
+  const bool sees = row_ok && (!p.causal || qpos >= 0);
+  const int lim = !sees ? 0 : p.causal && !POS ? (int)min(qpos + 1, (int64_t)n) : n;
+  int lim_min = 0, lim_max = 0;  // of the wave's rows that see anything
+  if constexpr (POS) {
+    const int64_t mn = wave_min_i64(sees ? qpos : INT64_MAX), mx = wave_max_i64(sees ? qpos : INT64_MIN);
+    const bool act = __ballot(sees) != 0;
+    if (lane == 0) red_max[wave] = mx, red_min[wave] = mn, red_act[wave] = act ? 1 : 0;
+  } else {
+    lim_min = uniform(wave_min_i32(lim > 0 ? lim : INT32_MAX));
+    lim_max = uniform(wave_max_i32(lim));
+    if (lane == 0) red_max[wave] = lim_max;
+  }
+  if (tid < 2) flags[tid] = 0;
+  __syncthreads();
+  int64_t max_wg = red_max[0];
+#pragma unroll
+  for (int w = 1; w < NWAVES; ++w) max_wg = max(max_wg, red_max[w]);
+  bool any_wg = !POS;
+  if constexpr (POS)
+#pragma unroll
+    for (int w = 0; w < NWAVES; ++w) any_wg = any_wg || red_act[w] != 0;
+
+  // ---- this split's run of tiles
+  const int seen_tiles = uniform(!any_wg ? 0 : ((POS ? n : (int)max_wg) + BN - 1) / BN);
+  const int per_split = (seen_tiles + nsplit - 1) / nsplit;
+  const int t_first = min(seen_tiles, split * per_split), t_last = min(seen_tiles, t_first + per_split);
+
+  auto page_of = [&](int slot) -> int {
+    const uint32_t u = (uint32_t)slot >> 4;
+    return (int)(c_.page16 == 1 ? u : __umulhi(u, c_.magic));
+  };
+  // a page index of the run that is not one: its keys are looked up one by one below
+  if (t_first < t_last) {
+    const int pg0 = page_of(t_first * BN), pg1 = page_of(min(t_last * BN, n) - 1);
+    bool bad = false;
+    for (int pg = pg0 + tid; pg <= pg1; pg += NTHREADS) {
+      const int64_t id = p.tables[b * p.ts_b + (int64_t)pg * p.ts_w];
+      bad = bad || id < 0 || id >= p.P;
+    }
+    if (__ballot(bad) != 0 && lane == 0) flags[0] = 1;
+  }
+
+  const float scale = (float)p.scale;
+  const float c = fabsf(scale) * 1.4426950408889634f;
+  const float grow_thr = kRescaleLog2 / c;
+  const uint32_t qflip = scale < 0.f ? 0x80008000u : 0u;
+  frag qf[D / 16];
+  {
+    const T* qrow = (const T*)p.q + b * p.qs_b + (int64_t)row * p.qs_s + h * p.qs_h;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      uint4 raw = make_uint4(0, 0, 0, 0);
+      if (sees) raw = *(const uint4*)(qrow + ks * 16 + g * 8);
+      raw.x ^= qflip; raw.y ^= qflip; raw.z ^= qflip; raw.w ^= qflip;
+      __builtin_memcpy(&qf[ks], &raw, 16);
+    }
+  }
+
+  const uint32_t krow = (uint32_t)(p.ks_s * 2), vrow = (uint32_t)(p.vs_s * 2);
+  uint32_t k_voff[L::KV_LOADS], v_voff[L::KV_LOADS];
+#pragma unroll
+  for (int i = 0; i < L::KV_LOADS; ++i) {
+    const int local = i * L::ROWS_PER_LOAD + lane / L::NCG, key = wave * WROWS + local;
+    const int pg = lane % L::NCG;  // physical 16-byte group in the row
+    k_voff[i] = local * krow + ((pg ^ k_swz<D>(key)) << 4);
+    const int lgv = (((pg >> 2) ^ v_swz<D>(key)) << 2) | (pg & 3);
+    v_voff[i] = local * vrow + (lgv << 4);
+  }
+  uint32_t k_raddr[D / 16], v_raddr[D / 32];
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks) k_raddr[ks] = r * L::KROW + (((2 * ks + g) ^ k_swz<D>(r)) << 4);
+  {
+    const int src = lane & 15, grp = lane >> 4;
+    const int vr = g * 4 + (src >> 2);
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+      v_raddr[dt] = L::K_BYTES + vr * L::KROW + ((dt ^ v_swz<D>(vr)) << 6) + (16 * (grp & 1) + 4 * (src & 3)) * 2;
+  }
+  const uint32_t smem_lds = lds_addr(smem);
+  const uint32_t wave_kv = wave * (L::KV_LOADS * 1024);
+  const char* kh = (const char*)((const T*)p.k + (int64_t)kvh * p.ks_h);
+  const char* vh = (const char*)((const T*)p.v + (int64_t)kvh * p.vs_h);
+  const int64_t ks_p = p.ks_p * 2, vs_p = p.vs_p * 2;
+
+  // the page index of this wave's rows of a tile (a scalar read; the table ends with a page)
+  auto id_of = [&](int tile) -> int64_t {
+    const int slot = tile * BN + wave * WROWS;
+    return slot < cap ? table[(int64_t)page_of(slot) * p.ts_w] : -1;
+  };
+  auto load_tile = [&](int tile, int64_t id, int stage) {
+    const int slot = tile * BN + wave * WROWS;
+    const int rows = min(n - slot, WROWS);  // rows behind the row's end, and of no page, read 0
+    const bool ok = id >= 0 && id < p.P && rows > 0;
+    const int64_t at = ok ? id : 0;
+    const int place = ok ? slot - page_of(slot) * (c_.page16 * 16) : 0;
+    const i32x4 krs = make_rsrc(kh + at * ks_p + (int64_t)place * krow, ok ? (uint32_t)(rows - 1) * krow + L::KROW : 0u);
+    const i32x4 vrs = make_rsrc(vh + at * vs_p + (int64_t)place * vrow, ok ? (uint32_t)(rows - 1) * vrow + L::KROW : 0u);
+    const uint32_t st = smem_lds + stage * L::STAGE_BYTES;
+#pragma unroll
+    for (int i = 0; i < L::KV_LOADS; ++i) buffer_load_lds16_m0(krs, st + wave_kv + i * 1024, k_voff[i]);
+#pragma unroll
+    for (int i = 0; i < L::KV_LOADS; ++i) buffer_load_lds16_m0(vrs, st + L::K_BYTES + wave_kv + i * 1024, v_voff[i]);
+    if constexpr (POS) {
+      const i32x4 prs = make_rsrc(p.pos + at * p.ps_p + place, ok ? (uint32_t)rows * 8 : 0u);
+      if (lane < WROWS / 2)
+        buffer_load_lds16_m0(prs, st + L::K_BYTES + L::V_BYTES + wave * (WROWS * 8), lane * 16);
+    }
+  };
+
+  // f16 takes 2^7 p, so small probabilities stay normal numbers: with one piece through the exponent (l
+  // holds the factor too), with two as a product, which costs small scores no bits
+  constexpr bool kF16 = std::is_same<T, f16>::value;
+  constexpr float kExpShift = kF16 && PIECES == 1 ? 7.f : 0.f;
+  constexpr float kPieceScale = kF16 && PIECES > 1 ? 128.f : 1.f;
+  f32x16 oacc[D / 32];
+  float m_run, m_use, l_run;
+  auto clear = [&]() {
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) oacc[i][e] = 0.f;
+    m_run = -__builtin_inff();
+    m_use = -kExpShift;
+    l_run = 0.f;
+  };
+
+  // mode: 1 every key of the tile visible to every row of the wave that sees anything, 2 masked, 3 masked
+  // and the pages looked up
+  auto compute = [&](int stage, int slot0, int mode, auto careful) {
+    const char* sb = smem + stage * L::STAGE_BYTES;
+    f32x16 sacc[2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      frag kf[D / 16];
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) kf[ks] = *(const frag*)(sb + kb * 32 * L::KROW + k_raddr[ks]);
+      f32x16 acc = {};
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) acc = Mfma<T>::run(kf[ks], qf[ks], acc);
+      sacc[kb] = acc;
+    }
+    __builtin_amdgcn_sched_group_barrier(0x100, D / 16, 0);
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, D / 16, 0);
+    if (mode >= 2) {
+      if constexpr (POS) {
+        const char* pl = sb + L::K_BYTES + L::V_BYTES;
+        const uint64_t qlim = p.causal ? (uint64_t)qpos : (uint64_t)INT64_MAX;  // (-1 wraps past it)
+        const int left = sees ? n - slot0 : 0;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int i4 = 0; i4 < 4; ++i4) {
+            const int key0 = kb * 32 + i4 * 8 + g * 4;
+            const uint4 a = *(const uint4*)(pl + key0 * 8), a2 = *(const uint4*)(pl + key0 * 8 + 16);
+            const uint64_t kp[4] = {((uint64_t)a.y << 32) | a.x, ((uint64_t)a.w << 32) | a.z,
+                                    ((uint64_t)a2.y << 32) | a2.x, ((uint64_t)a2.w << 32) | a2.z};
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (!(key0 + j < left && kp[j] <= qlim)) sacc[kb][i4 * 4 + j] = -__builtin_inff();
+          }
+      } else {
+        const int left = lim - slot0 - g * 4;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (kb * 32 + (e >> 2) * 8 + (e & 3) >= left) sacc[kb][e] = -__builtin_inff();
+      }
+      if (mode == 3) {  // some page of the run is not there
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int i4 = 0; i4 < 4; ++i4) {
+            const int slot = slot0 + kb * 32 + i4 * 8 + g * 4;  // its four keys lie in one page
+            int64_t id = -1;
+            if (slot < cap) id = p.tables[b * p.ts_b + (int64_t)page_of(slot) * p.ts_w];
+            if (id < 0 || id >= p.P)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) sacc[kb][i4 * 4 + j] = -__builtin_inff();
+          }
+        // (drains this wave's tile loads, which its own waits do not mind)
+      }
+    }
+    float t1[11];
+#pragma unroll
+    for (int i = 0; i < 10; ++i) {
+      const int e = 3 * i;
+      t1[i] = max3f(sacc[e >> 4][e & 15], sacc[(e + 1) >> 4][(e + 1) & 15], sacc[(e + 2) >> 4][(e + 2) & 15]);
+    }
+    t1[10] = __builtin_fmaxf(sacc[1][14], sacc[1][15]);
+    const float t2a = max3f(t1[0], t1[1], t1[2]), t2b = max3f(t1[3], t1[4], t1[5]);
+    const float t2c = max3f(t1[6], t1[7], t1[8]), t2d = __builtin_fmaxf(t1[9], t1[10]);
+    float mx = __builtin_fmaxf(max3f(t2a, t2b, t2c), t2d);
+    mx = max_halves(mx);
+    const bool grow = mx > m_run + grow_thr;
+    if (__ballot(grow) != 0) {
+      const float m_new = grow ? mx : m_run;
+      const float alpha = grow ? __builtin_amdgcn_exp2f((m_run - m_new) * c) : 1.f;
+      m_run = m_new;
+      m_use = (m_run == -__builtin_inff() ? 0.f : m_run * c) - kExpShift;
+      l_run *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) oacc[dt][e] *= alpha;
+    }
+    frag pf[PIECES][4];
+    float pr[32];
+    uint32_t seen = 0, none = 0;  // visible keys of this lane, those of them with probability 0
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[kb][e], c, -m_use));
+        pr[kb * 16 + e] = x;
+        if constexpr (decltype(careful)::value) {
+          const bool vis = __float_as_uint(sacc[kb][e]) != 0xff800000u;
+          seen |= (vis ? 1u : 0u) << (kb * 16 + e);
+          none |= (vis && (__float_as_uint(x) << 1) == 0 ? 1u : 0u) << (kb * 16 + e);
+        }
+        float rest = x * kPieceScale;
+#pragma unroll
+        for (int pc = 0; pc < PIECES; ++pc) {
+          pf[pc][kb * 2 + (e >> 3)][e & 7] = (T)rest;
+          if (pc + 1 < PIECES) rest -= to_f32<T>(pf[pc][kb * 2 + (e >> 3)][e & 7]);
+        }
+      }
+#pragma unroll
+    for (int w = 16; w >= 1; w >>= 1)
+#pragma unroll
+      for (int e = 0; e < w; ++e) pr[e] += pr[e + w];
+    l_run += pr[0];
+    if constexpr (decltype(careful)::value) {
+      // values that are not finite: out of the products, then per feature the visible keys with +inf or
+      // NaN, and those with -inf or NaN, are counted by products of ones, and the sum takes an infinity of
+      // that sign (both make a NaN; a visible key of probability 0 counts for both: 0 * inf)
+      auto keys = [&](uint32_t bits, int s) {
+        u16x8 x;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = (bits >> (8 * s + j)) & 1 ? Bits16<T>::kOne : 0;
+        return __builtin_bit_cast(frag, x);
+      };
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) {
+        __builtin_amdgcn_sched_barrier(0);
+        f32x16 count[2] = {};
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          u16x8 x = __builtin_bit_cast(u16x8, read_tr_frag<frag>(sb + s * 16 * L::KROW + v_raddr[dt],
+                                                                 sb + (s * 16 + 8) * L::KROW + v_raddr[dt]));
+          u16x8 one[2], any;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const uint16_t mag = x[j] & 0x7fff;
+            any[j] = mag >= Bits16<T>::kInf ? Bits16<T>::kOne : 0;
+            one[0][j] = mag > Bits16<T>::kInf || x[j] >> 15 == 0 ? any[j] : 0;
+            one[1][j] = mag > Bits16<T>::kInf || x[j] >> 15 == 1 ? any[j] : 0;
+            if (mag >= Bits16<T>::kInf) x[j] = 0;
+          }
+#pragma unroll
+          for (int pc = 0; pc < PIECES; ++pc) oacc[dt] = Mfma<T>::run(__builtin_bit_cast(frag, x), pf[pc][s], oacc[dt]);
+#pragma unroll
+          for (int sign = 0; sign < 2; ++sign) {
+            count[sign] = Mfma<T>::run(__builtin_bit_cast(frag, one[sign]), keys(seen, s), count[sign]);
+            count[sign] = Mfma<T>::run(__builtin_bit_cast(frag, any), keys(none, s), count[sign]);
+          }
+        }
+#pragma unroll
+        for (int sign = 0; sign < 2; ++sign)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            uint32_t add = count[sign][e] > 0.f ? (sign ? 0xff800000u : 0x7f800000u) : 0x80000000u;
+            asm volatile("" : "+v"(add));  // the file is compiled as if no NaN occurred
+            oacc[dt][e] += __uint_as_float(add);
+          }
+      }
+      return;
+    }
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) {
+      frag vf[4];
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        vf[s] = read_tr_frag<frag>(sb + s * 16 * L::KROW + v_raddr[dt], sb + (s * 16 + 8) * L::KROW + v_raddr[dt]);
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int pc = 0; pc < PIECES; ++pc) oacc[dt] = Mfma<T>::run(vf[s], pf[pc][s], oacc[dt]);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x100, 8, 1);
+#pragma unroll
+    for (int j = 0; j < D / 32 - 1; ++j) {
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        __builtin_amdgcn_sched_group_barrier(0x008, PIECES, 1);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+      }
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 4 * PIECES, 1);
+  };
+
+  // ---- the stream over this run's tiles
+  auto stream = [&](auto careful) {
+    for (int base = t_first; base < t_last; base += POS ? LIST_CAP : t_last - t_first) {
+      int nt = t_last - base;
+      if constexpr (POS) {
+        const TileInfo* tinfo = c_.tiles + (int64_t)b * c_.ntiles;
+        const int span = min(LIST_CAP, nt);
+        nt = 0;
+        for (int r0 = 0; r0 < span; r0 += NTHREADS) {
+          const int t = base + r0 + tid;
+          bool need = false;
+          int modes = 0;
+          if (r0 + tid < span) {
+            const TileInfo ti = tinfo[t];
+            need = ti.n_valid > 0 && !(p.causal && max_wg < ti.min_valid);
+#pragma unroll
+            for (int w = 0; w < NWAVES; ++w) {
+              int m;
+              if (!red_act[w] || ti.n_valid == 0 || (p.causal && red_max[w] < ti.min_valid)) m = 0;
+              else if (ti.n_valid == BN && (!p.causal || ti.max_valid <= red_min[w])) m = 1;
+              else m = 2;
+              modes |= m << (2 * w);
+            }
+          }
+          const uint64_t bal = __ballot(need);
+          if (lane == 0) wave_cnt[wave] = __builtin_popcountll(bal);
+          __syncthreads();
+          int off = nt;
+          for (int w = 0; w < wave; ++w) off += wave_cnt[w];
+          int tot = nt;
+          for (int w = 0; w < NWAVES; ++w) tot += wave_cnt[w];
+          if (need)
+            tile_list[off + __builtin_amdgcn_mbcnt_hi((uint32_t)(bal >> 32),
+                                                      __builtin_amdgcn_mbcnt_lo((uint32_t)bal, 0))] = make_int2(t, modes);
+          __syncthreads();
+          nt = tot;
+        }
+        nt = uniform(nt);
+        if (nt == 0) continue;
+      }
+      auto tile_of = [&](int i) -> int {
+        if constexpr (POS) return uniform(tile_list[i].x);
+        else return base + i;
+      };
+      const int bad = uniform(flags[0]);
+      int issued = 0;
+      for (; issued < nt && issued < NSTAGE - 1; ++issued) load_tile(tile_of(issued), id_of(tile_of(issued)), issued);
+      // the tile to load next, and its page, are known a step ahead of its load
+      int t_load = issued < nt ? tile_of(issued) : base;
+      int64_t id_load = id_of(t_load);
+      int e_cur = 0;
+      if constexpr (POS) e_cur = tile_list[0].y;
+      for (int i = 0; i < nt; ++i) {
+        wait_tiles_ahead<L::LPT>(issued - i - 1);
+        barrier_no_fence();  // tile i landed for every wave; the stage of tile i-1 is free
+        if (issued < nt) {
+          load_tile(t_load, id_load, (int)((unsigned)issued % NSTAGE));
+          ++issued;
+        }
+        int tile, mode;
+        int2 e_nxt = make_int2(0, 0), l_nxt = make_int2(0, 0);
+        if constexpr (POS) {
+          tile = uniform(tile_list[i].x);
+          mode = uniform((e_cur >> (2 * wave)) & 3);
+          e_nxt = tile_list[i + 1 < nt ? i + 1 : i];
+          l_nxt = tile_list[issued < nt ? issued : 0];
+        } else {
+          tile = base + i;
+          mode = tile * BN >= lim_max ? 0 : (tile + 1) * BN <= lim_min ? 1 : 2;
+          if (issued < nt) t_load = base + issued, id_load = id_of(t_load);
+        }
+        if (bad && mode != 0) mode = 3;
+        if (mode != 0) compute((int)((unsigned)i % NSTAGE), tile * BN, mode, careful);
+        if constexpr (POS) {
+          e_cur = e_nxt.y;
+          if (issued < nt) t_load = uniform(l_nxt.x), id_load = id_of(t_load);
+        }
+      }
+      __syncthreads();  // the next pass rewrites the list and the stages
+    }
+  };
+
+  __syncthreads();  // flags[0]
+  clear();
+  stream(std::false_type());
+  {
+    uint32_t worst = 0;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) worst = max(worst, __float_as_uint(oacc[dt][e]) & 0x7fffffffu);
+    if (__ballot(sees && worst >= 0x7f800000u) != 0 && lane == 0) flags[1] = 1;
+    __syncthreads();
+    if (flags[1] != 0) {
+      clear();
+      stream(std::true_type());
+    }
+  }
+
+  // ---- epilogue.  A row's sum is 0 exactly where it saw no key (a NaN is kept).
+  if (!row_ok) return;
+  const float l_tot = sum_halves(l_run);
+  uint32_t l_bits = __float_as_uint(l_tot);
+  asm volatile("" : "+v"(l_bits));  // (compared as a float, a NaN might be taken for 0 in this file)
+  const bool empty = !sees || (l_bits << 1) == 0;
+  const float inv = empty ? 0.f : 1.f / (l_tot * kPieceScale);
+  if (p.lse && g == 0) {
+    float* lp = (float*)p.lse + split * c_.split_lse + b * p.ls_b + h * p.ls_h + (int64_t)row * p.ls_s;
+    *lp = empty ? -__builtin_inff() : (m_run * fabsf(scale) + logf(l_tot)) - kExpShift * 0.69314718055994531f;
+  }
+  const int64_t orow = split * c_.split_out + b * p.os_b + (int64_t)row * p.os_s + h * p.os_h;
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int i4 = 0; i4 < 4; ++i4) {
+      float x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = empty ? 0.f : oacc[dt][i4 * 4 + j] * inv;
+      const int64_t at = orow + dt * 32 + i4 * 8 + g * 4;
+      if (p.out_dtype == CEA_F32) {
+        *(float4*)((float*)p.out + at) = make_float4(x[0], x[1], x[2], x[3]);
+      } else {
+        const T v4[4] = {(T)x[0], (T)x[1], (T)x[2], (T)x[3]};
+        uint2 raw;
+        __builtin_memcpy(&raw, v4, 8);
+        *(uint2*)((T*)p.out + at) = raw;
+      }
+    }
+}
+
+template <typename T, int D, bool POS, int PIECES>
+int launch_form(const ChunkParams& c, hipStream_t st) {
+  const PagedParams& p = c.p;
+  const int nqb = (p.Sq + BM / c.hp - 1) / (BM / c.hp);
+  const int64_t total = (int64_t)nqb * (p.Hq / c.hp) * p.B * c.splits;
+  constexpr int lds = Layout<D, POS>::LDS_BYTES;
+  const hipError_t e = reserve_lds<paged_chunk_kernel<T, D, POS, PIECES>>(lds);
+  CEA_REQUIRE(e == hipSuccess, CEA_ELAUNCH, "paged_attention: cannot reserve %d bytes of LDS: %s", lds,
+              hipGetErrorString(e));
+  hipLaunchKernelGGL((paged_chunk_kernel<T, D, POS, PIECES>), dim3((unsigned)total), dim3(NTHREADS), lds, st, c);
+  CEA_CHECK_LAUNCH("paged_chunk");
+  return CEA_OK;
+}
+
+template <typename T, int D> int launch_td(const ChunkParams& c, bool f32, hipStream_t st) {
+  constexpr int kFull = std::is_same<T, bf16>::value ? 3 : 2;
+  if (c.p.pos) return f32 ? launch_form<T, D, true, kFull>(c, st) : launch_form<T, D, true, 1>(c, st);
+  return f32 ? launch_form<T, D, false, kFull>(c, st) : launch_form<T, D, false, 1>(c, st);
+}
+
+size_t align256(size_t x) { return (x + 255) / 256 * 256; }
+
+struct ChunkPlan {
+  int hp, splits;
+  size_t tiles, part_out, part_lse;  // bytes: summaries, one split's partial result
+};
+
+ChunkPlan plan_chunk(int64_t B, int64_t Sq, int64_t Hq, int group, int64_t D, int64_t slots, bool pos) {
+  ChunkPlan r;
+  r.hp = prefill_heads_per_wg(Sq, group);
+  r.splits = prefill_key_splits(B, Sq, Hq, slots, r.hp);
+  r.tiles = pos ? align256((size_t)B * ((slots + BN - 1) / BN) * sizeof(TileInfo)) : 0;
+  r.part_out = align256((size_t)B * Sq * Hq * D * sizeof(float));
+  r.part_lse = align256((size_t)B * Sq * Hq * sizeof(float));
+  return r;
+}
+
+}  // namespace
+
+size_t paged_chunk_workspace_bytes(int64_t B, int64_t Sq, int64_t Hq, int group, int64_t D, int64_t slots, bool pos) {
+  const ChunkPlan r = plan_chunk(B, Sq, Hq, group, D, slots, pos);
+  return r.tiles + (r.splits > 1 ? r.splits * (r.part_out + r.part_lse) : 0);
+}
+
+bool paged_chunk_supported(const PagedParams& p, const HeadMap& map) {
+  if (map.group <= 0 && (p.Hq > kPagedMapHeads || p.Hkv > 256)) return false;
+  for (int64_t s : {p.os_b, p.os_s, p.os_h})
+    if (s % 4) return false;
+  if ((uintptr_t)p.out % 16 || (p.pos && (uintptr_t)p.pos % 8)) return false;
+  return p.B < 65536 && (int64_t)p.B * p.Hq * ((p.Sq + 31) / 32) * kMaxKeySplits < ((int64_t)1 << 31);
+}
+
+int launch_paged_chunk(const PagedParams& params, const HeadMap& map, void* ws, hipStream_t st) {
+  const int64_t slots = (int64_t)params.W * params.page;
+  const PagedParams& o = params;
+  const ChunkPlan r = plan_chunk(o.B, o.Sq, o.Hq, map.group, o.D, slots, o.pos != nullptr);
+  ChunkParams c;
+  memset(&c, 0, sizeof(c));
+  c.p = o;
+  c.hp = r.hp, c.splits = r.splits;
+  c.page16 = o.page / 16;
+  c.magic = c.page16 > 1 ? (uint32_t)((((uint64_t)1 << 32) + c.page16 - 1) / c.page16) : 0;
+  for (int h = 0; h < kPagedMapHeads && h < o.Hq && map.group <= 0; ++h) c.kv[h] = (uint8_t)map.kv[h];
+  char* at = (char*)ws;
+  if (o.pos) {
+    c.tiles = (const TileInfo*)at;
+    c.ntiles = (int32_t)((slots + BN - 1) / BN);
+    hipLaunchKernelGGL(paged_tile_info_kernel, dim3((unsigned)c.ntiles, (unsigned)o.B), dim3(64), 0, st, o, c.ntiles,
+                       (TileInfo*)at);
+    CEA_CHECK_LAUNCH("paged_tile_info");
+    at += r.tiles;
+  }
+  // query heads that an XCD takes together: whole KV heads, as many as 5 MB of keys and values hold (by
+  // the table's width: the lengths are on the device), in sets of even size
+  const int64_t kv_bytes = std::max<int64_t>(slots * o.D * 4, 1);
+  const int64_t per_kv = map.group > 0 ? o.Hq / c.hp / o.Hkv : 1;
+  c.order_per_kv = (int)per_kv;
+  const int64_t heads = std::max<int64_t>(((int64_t)o.B * (o.Hq / c.hp) + 8 * per_kv - 1) / (8 * per_kv), 1);
+  const int64_t fit = std::max<int64_t>(((int64_t)5 << 20) / kv_bytes, 1);
+  const int64_t sets = (heads + fit - 1) / fit;
+  c.order_units = (int)((heads + sets - 1) / sets * per_kv);
+  if (o.B == 1 && heads == 1) c.order_units = 1;
+
+  if (r.splits > 1) {  // partial results (f32), merged below
+    c.p.out = at;
+    c.p.out_dtype = CEA_F32;
+    c.p.os_h = o.D, c.p.os_s = (int64_t)o.Hq * o.D, c.p.os_b = c.p.os_s * o.Sq;
+    c.p.lse = at + r.splits * r.part_out;
+    c.p.ls_s = 1, c.p.ls_h = o.Sq, c.p.ls_b = (int64_t)o.Hq * o.Sq;
+    c.split_out = (int64_t)(r.part_out / sizeof(float)), c.split_lse = (int64_t)(r.part_lse / sizeof(float));
+  }
+  const bool f32 = o.out_dtype == CEA_F32;
+  int rc;
+  if (o.in_dtype == CEA_BF16)
+    rc = o.D == 128 ? launch_td<bf16, 128>(c, f32, st) : launch_td<bf16, 64>(c, f32, st);
+  else
+    rc = o.D == 128 ? launch_td<f16, 128>(c, f32, st) : launch_td<f16, 64>(c, f32, st);
+  if (rc || r.splits == 1) return rc;
+  MergeParams m;
+  memset(&m, 0, sizeof(m));
+  m.n = r.splits;
+  m.B = o.B, m.Sq = o.Sq, m.H = o.Hq, m.D = o.D;
+  m.dtype = CEA_F32, m.out_dtype = o.out_dtype;
+  for (int i = 0; i < r.splits; ++i) {
+    m.outs[i] = (const float*)c.p.out + i * c.split_out;
+    m.lses[i] = (const float*)c.p.lse + i * c.split_lse;
+    m.os[i][0] = c.p.os_b, m.os[i][1] = c.p.os_s, m.os[i][2] = c.p.os_h;
+    m.ls[i][0] = c.p.ls_b, m.ls[i][1] = c.p.ls_h, m.ls[i][2] = c.p.ls_s;
+  }
+  m.out = o.out, m.lse = o.lse;
+  m.dos[0] = o.os_b, m.dos[1] = o.os_s, m.dos[2] = o.os_h;
+  m.dls[0] = o.ls_b, m.dls[1] = o.ls_h, m.dls[2] = o.ls_s;
+  return launch_merge(m, st);
+}
+
+}  // namespace cea
