@@ -11,16 +11,19 @@
 // flight; exp2 domain, the reference maximum moved only when a row's grows by 2^8.  What the pages
 // change:
 //   * a wave loads 8 rows of a tile, and pages are multiples of 16 slots, so they lie in one page:
-//     its address stays scalar, and the page index is a scalar read a step ahead of the load;
+//     its address stays scalar; the page indices of 512 tiles at a time wait in LDS (read through the
+//     scalar cache, each delayed the next tile's first product);
 //   * without positions in the pool slot j is position j, so the tiles that a workgroup visits are
-//     a prefix of the row and every mask is one 32-bit comparison with the query row's limit; with them a
-//     launch before this one summarises the tiles, and the workgroup lists those it needs;
+//     a prefix of the row and every mask is one 32-bit comparison with the query row's limit; with
+//     them a launch before this one summarises the tiles and writes the positions in 32 bits,
+//     and the workgroup lists the tiles it needs;
 //   * lengths are known on the device alone: a launch with few query blocks is cut into key splits by
 //     the table's width, and each split takes an equal run of the tiles that the row really has;
 //   * hidden keys may hold anything.  Their scores are masked; a value that is not finite shows up as
-//     a result that is not, and the workgroup then goes over its tiles once more, carefully: such values are
-//     taken out of the products and added per row as the infinity or NaN that the visible ones make.
-//     A chunk without them pays one look at its results.
+//     a result that is not, and the workgroup then goes over its tiles once more: such values are taken
+//     out of the tiles as they land, and the tiles that had some are visited again to add, per row and
+//     feature, the infinity or NaN that the visible ones make.  A chunk without them pays one look at
+//     its results.
 #include <math.h>
 #include <string.h>
 
@@ -39,7 +42,6 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4_ptr;
-typedef const int64_t __attribute__((address_space(4))) * scalar_i64;  // read through the scalar cache
 
 template <typename T> struct Mfma;
 template <> struct Mfma<bf16> {
@@ -65,12 +67,14 @@ constexpr int BM = NWAVES * 32;       // query rows per workgroup
 constexpr int BN = kTileKeys;         // keys per tile
 constexpr int WROWS = BN / NWAVES;    // rows of a tile that a wave loads
 constexpr int NSTAGE = 4;             // LDS ring depth
-constexpr int LIST_CAP = 2048;        // tiles listed per pass (positions in the pool)
+constexpr int PASS = 512;             // tiles of a pass: their page indices (and list) are in LDS
+constexpr int32_t kHidden32 = INT32_MAX;  // no key; visible positions end below it
 constexpr float kRescaleLog2 = 8.0f;
 
 struct ChunkParams {
   PagedParams p;
-  const TileInfo* tiles;     // [B, ntiles] with positions in the pool
+  const TileInfo* tiles;     // with positions in the pool: [B, ntiles] summaries (pad[0]: some position
+  const int32_t* pos32;      // does not fit 31 bits), and [B, ntiles * 64] positions, kHidden32 where no key
   int32_t ntiles;
   int32_t hp;                // query heads of a workgroup: 1, 2, 4, 8
   int32_t splits;            // key splits
@@ -86,11 +90,11 @@ template <int D, bool POS> struct Layout {
   static constexpr int NCG = D / 8;
   static constexpr int K_BYTES = BN * KROW;
   static constexpr int V_BYTES = BN * KROW;
-  static constexpr int STAGE_BYTES = K_BYTES + V_BYTES + (POS ? BN * 8 : 0);
+  static constexpr int STAGE_BYTES = K_BYTES + V_BYTES + (POS ? BN * 4 : 0);
   static constexpr int LDS_BYTES = NSTAGE * STAGE_BYTES;
   static constexpr int KV_LOADS = K_BYTES / (NTHREADS * 16);
   static constexpr int ROWS_PER_LOAD = 1024 / KROW;
-  static constexpr int LPT = 2 * KV_LOADS + (POS ? 1 : 0);  // loads of one wave per tile
+  static constexpr int LPT = 2 * KV_LOADS;  // loads of one wave per tile (wave 0: and the positions)
   static_assert(KV_LOADS * ROWS_PER_LOAD == WROWS, "a wave loads 8 rows");
 };
 
@@ -135,6 +139,17 @@ __device__ __forceinline__ int wave_max_i32(int v) {
   for (int off = 32; off >= 1; off >>= 1) v = max(v, __shfl_xor(v, off, 64));
   return v;
 }
+// A wave-uniform value in scalar registers, whatever the compiler makes of where it came from.
+template <typename X> __device__ __forceinline__ X scalar(X v) {
+  if constexpr (sizeof(X) == 4) {
+    return (X)__builtin_amdgcn_readfirstlane((int)v);
+  } else {
+    const uint64_t x = (uint64_t)v;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)x);
+    const uint32_t hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(x >> 32));
+    return (X)(((uint64_t)hi << 32) | lo);
+  }
+}
 template <int LPT> __device__ __forceinline__ void wait_tiles_ahead(int ahead) {
   static_assert(NSTAGE == 4, "wait ladder written for 2 tiles ahead at most");
   if (ahead >= 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LPT) : "memory");
@@ -142,43 +157,54 @@ template <int LPT> __device__ __forceinline__ void wait_tiles_ahead(int ahead) {
   else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-// Summaries of the tiles' positions, one wave per tile and row.
-__global__ __launch_bounds__(64) void paged_tile_info_kernel(const PagedParams p, int ntiles, TileInfo* out) {
-  const int t = blockIdx.x, b = blockIdx.y;
-  const int64_t n = paged_slots(p, b), j = (int64_t)t * BN + threadIdx.x;
-  int64_t pos = -1;
-  if (j < n) {
-    const int pg = (int)j / p.page, place = (int)j - pg * p.page;
-    const int64_t id = p.tables[b * p.ts_b + pg * p.ts_w];
-    if (id >= 0 && id < p.P) pos = p.pos[id * p.ps_p + place];
-  }
-  const bool valid = pos >= 0;
-  const int64_t mn = wave_min_i64(valid ? pos : INT64_MAX);
-  const int64_t mx = wave_max_i64(valid ? pos : INT64_MIN);
-  const int cnt = __builtin_popcountll(__ballot(valid));
-  if (threadIdx.x == 0) {
-    TileInfo ti;
-    ti.min_valid = mn;
-    ti.max_valid = mx;
-    ti.n_valid = cnt;
-    ti.pad[0] = ti.pad[1] = ti.pad[2] = 0;
-    out[(int64_t)b * ntiles + t] = ti;
+// Summaries and 32-bit positions of a row's tiles, a wave per tile; the row's length, not the table's
+// width, decides how many there are.
+__global__ __launch_bounds__(256) void paged_tile_info_kernel(const PagedParams p, int ntiles, TileInfo* out,
+                                                              int32_t* pos32) {
+  const int b = blockIdx.y, lane = threadIdx.x & 63;
+  const int n = (int)paged_slots(p, b);
+  for (int t = blockIdx.x * 4 + (threadIdx.x >> 6); t * BN < n; t += gridDim.x * 4) {
+    const int j = t * BN + lane;
+    int64_t pos = -1;
+    if (j < n) {
+      const int pg = j / p.page, place = j - pg * p.page;
+      const int64_t id = p.tables[b * p.ts_b + pg * p.ts_w];
+      if (id >= 0 && id < p.P) pos = p.pos[id * p.ps_p + place];
+    }
+    const bool valid = pos >= 0, wide = pos >= kHidden32;
+    const int64_t mn = wave_min_i64(valid ? pos : INT64_MAX);
+    const int64_t mx = wave_max_i64(valid ? pos : INT64_MIN);
+    const uint64_t some = __ballot(valid), far = __ballot(wide);
+    const int64_t at = (int64_t)b * ntiles + t;
+    pos32[at * BN + lane] = valid && !wide ? (int32_t)pos : kHidden32;
+    if (lane == 0) {
+      TileInfo ti;
+      ti.min_valid = mn;
+      ti.max_valid = mx;
+      ti.n_valid = __builtin_popcountll(some);
+      ti.pad[0] = far != 0 ? 1 : 0;
+      ti.pad[1] = ti.pad[2] = 0;
+      out[at] = ti;
+    }
   }
 }
 
 // PIECES: 16-bit numbers whose sum enters the value product for a probability: one for 16-bit results
 // (p rounded once, half a step of the type, as the result's own rounding is), three of bf16 or two of f16
 // for f32 results (p to 2^-23 and better).
+constexpr bool lean(int D, int pieces) { return false; }
 template <typename T, int D, bool POS, int PIECES>
-__global__ __launch_bounds__(NTHREADS, 2) void paged_chunk_kernel(const ChunkParams c_) {
+__global__ __launch_bounds__(NTHREADS, lean(D, PIECES) ? 4 : 2) void paged_chunk_kernel(const ChunkParams c_) {
   typedef Layout<D, POS> L;
   typedef typename Mfma<T>::frag frag;
   const PagedParams& p = c_.p;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ int2 tile_list[POS ? LIST_CAP : 1];  // (tile, 2-bit mode of every wave)
+  __shared__ int2 tile_list[POS ? PASS : 1];      // (tile, 2-bit mode of every wave)
+  __shared__ int32_t ids[PASS * BN / 16];         // page indices of the pass, -1 where none
+  __shared__ uint32_t marks[PASS / 32];           // tiles that hold a value that is not finite
   __shared__ int64_t red_max[NWAVES], red_min[NWAVES];
   __shared__ int red_act[NWAVES], wave_cnt[NWAVES];
-  __shared__ int flags[2];  // a page that is not there; a result that is not finite
+  __shared__ int flags[2];  // some page of the run is not there; some result is not finite
 
   const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63;
   const int r = lane & 31, g = lane >> 5;
@@ -237,9 +263,9 @@ __global__ __launch_bounds__(NTHREADS, 2) void paged_chunk_kernel(const ChunkPar
   const int row = qb * rows_pb + (wave & ((1 << waves_log2) - 1)) * 32 + r;
   const bool row_ok = row < p.Sq;
   const int64_t qpos = row_ok ? p.q_pos[b * p.qps_b + (int64_t)row * p.qps_s] : -1;
-  const int n = uniform((int)paged_slots(p, b));
-  const int cap = p.W * p.page;
-  const scalar_i64 table = (scalar_i64)(uintptr_t)(p.tables + b * p.ts_b);
+  const int n = scalar(uniform((int)paged_slots(p, b)));
+  const int page16 = scalar(c_.page16);
+  const uint32_t magic = scalar(c_.magic);
 
   // ---- what the rows see: slots [0, lim) of this lane's row by their number (POS: positions to qpos)
   const bool sees = row_ok && (!p.causal || qpos >= 0);
@@ -267,23 +293,13 @@ __global__ __launch_bounds__(NTHREADS, 2) void paged_chunk_kernel(const ChunkPar
   // ---- this split's run of tiles
   const int seen_tiles = uniform(!any_wg ? 0 : ((POS ? n : (int)max_wg) + BN - 1) / BN);
   const int per_split = (seen_tiles + nsplit - 1) / nsplit;
-  const int t_first = min(seen_tiles, split * per_split), t_last = min(seen_tiles, t_first + per_split);
+  const int t_first = scalar(min(seen_tiles, split * per_split));
+  const int t_last = scalar(min(seen_tiles, t_first + per_split));
 
   auto page_of = [&](int slot) -> int {
     const uint32_t u = (uint32_t)slot >> 4;
-    return (int)(c_.page16 == 1 ? u : __umulhi(u, c_.magic));
+    return (int)(page16 == 1 ? u : __umulhi(u, magic));
   };
-  // a page index of the run that is not one: its keys are looked up one by one below
-  if (t_first < t_last) {
-    const int pg0 = page_of(t_first * BN), pg1 = page_of(min(t_last * BN, n) - 1);
-    bool bad = false;
-    for (int pg = pg0 + tid; pg <= pg1; pg += NTHREADS) {
-      const int64_t id = p.tables[b * p.ts_b + (int64_t)pg * p.ts_w];
-      bad = bad || id < 0 || id >= p.P;
-    }
-    if (__ballot(bad) != 0 && lane == 0) flags[0] = 1;
-  }
-
   const float scale = (float)p.scale;
   const float c = fabsf(scale) * 1.4426950408889634f;
   const float grow_thr = kRescaleLog2 / c;
@@ -300,7 +316,7 @@ __global__ __launch_bounds__(NTHREADS, 2) void paged_chunk_kernel(const ChunkPar
     }
   }
 
-  const uint32_t krow = (uint32_t)(p.ks_s * 2), vrow = (uint32_t)(p.vs_s * 2);
+  const uint32_t krow = scalar((uint32_t)(p.ks_s * 2)), vrow = scalar((uint32_t)(p.vs_s * 2));
   uint32_t k_voff[L::KV_LOADS], v_voff[L::KV_LOADS];
 #pragma unroll
   for (int i = 0; i < L::KV_LOADS; ++i) {
@@ -322,21 +338,20 @@ __global__ __launch_bounds__(NTHREADS, 2) void paged_chunk_kernel(const ChunkPar
   }
   const uint32_t smem_lds = lds_addr(smem);
   const uint32_t wave_kv = wave * (L::KV_LOADS * 1024);
-  const char* kh = (const char*)((const T*)p.k + (int64_t)kvh * p.ks_h);
-  const char* vh = (const char*)((const T*)p.v + (int64_t)kvh * p.vs_h);
-  const int64_t ks_p = p.ks_p * 2, vs_p = p.vs_p * 2;
+  const char* kh = scalar((const char*)((const T*)p.k + (int64_t)kvh * p.ks_h));
+  const char* vh = scalar((const char*)((const T*)p.v + (int64_t)kvh * p.vs_h));
+  const int64_t ks_p = scalar(p.ks_p * 2), vs_p = scalar(p.vs_p * 2);
+  const int32_t* pos32 = POS ? scalar(c_.pos32 + (int64_t)b * c_.ntiles * BN) : nullptr;
 
-  // the page index of this wave's rows of a tile (a scalar read; the table ends with a page)
-  auto id_of = [&](int tile) -> int64_t {
-    const int slot = tile * BN + wave * WROWS;
-    return slot < cap ? table[(int64_t)page_of(slot) * p.ts_w] : -1;
-  };
-  auto load_tile = [&](int tile, int64_t id, int stage) {
+  int pg0 = 0;  // page of the pass's first slot
+  // the page index of this wave's rows of a tile (behind the row's end: the last one's)
+  auto id_of = [&](int tile) -> int { return ids[page_of(min(tile * BN + wave * WROWS, n - 1)) - pg0]; };
+  auto load_tile = [&](int tile, int id, int stage) {
     const int slot = tile * BN + wave * WROWS;
     const int rows = min(n - slot, WROWS);  // rows behind the row's end, and of no page, read 0
-    const bool ok = id >= 0 && id < p.P && rows > 0;
-    const int64_t at = ok ? id : 0;
-    const int place = ok ? slot - page_of(slot) * (c_.page16 * 16) : 0;
+    const bool ok = id >= 0 && rows > 0;
+    const int at = ok ? id : 0;
+    const int place = ok ? slot - page_of(slot) * (page16 * 16) : 0;
     const i32x4 krs = make_rsrc(kh + at * ks_p + (int64_t)place * krow, ok ? (uint32_t)(rows - 1) * krow + L::KROW : 0u);
     const i32x4 vrs = make_rsrc(vh + at * vs_p + (int64_t)place * vrow, ok ? (uint32_t)(rows - 1) * vrow + L::KROW : 0u);
     const uint32_t st = smem_lds + stage * L::STAGE_BYTES;
@@ -345,9 +360,10 @@ __global__ __launch_bounds__(NTHREADS, 2) void paged_chunk_kernel(const ChunkPar
 #pragma unroll
     for (int i = 0; i < L::KV_LOADS; ++i) buffer_load_lds16_m0(vrs, st + L::K_BYTES + wave_kv + i * 1024, v_voff[i]);
     if constexpr (POS) {
-      const i32x4 prs = make_rsrc(p.pos + at * p.ps_p + place, ok ? (uint32_t)rows * 8 : 0u);
-      if (lane < WROWS / 2)
-        buffer_load_lds16_m0(prs, st + L::K_BYTES + L::V_BYTES + wave * (WROWS * 8), lane * 16);
+      if (wave == 0) {
+        const i32x4 prs = make_rsrc(pos32 + (int64_t)tile * BN, BN * 4);
+        if (lane < BN / 4) buffer_load_lds16_m0(prs, st + L::K_BYTES + L::V_BYTES, lane * 16);
+      }
     }
   };
 
@@ -368,11 +384,11 @@ __global__ __launch_bounds__(NTHREADS, 2) void paged_chunk_kernel(const ChunkPar
     l_run = 0.f;
   };
 
-  // mode: 1 every key of the tile visible to every row of the wave that sees anything, 2 masked, 3 masked
-  // and the pages looked up
-  auto compute = [&](int stage, int slot0, int mode, auto careful) {
+  // The scores of a tile.  mode: 1 every key visible to every row of the wave that sees anything, 2 masked,
+  // 3 masked and looked up: a page of the pass that is not there, or (POS) a position beyond 31 bits.
+  const int qlim32 = !sees ? -1 : p.causal ? (int)min(qpos, (int64_t)kHidden32 - 1) : kHidden32 - 1;
+  auto scores = [&](int stage, int slot0, int mode, f32x16 (&sacc)[2]) {
     const char* sb = smem + stage * L::STAGE_BYTES;
-    f32x16 sacc[2];
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
       frag kf[D / 16];
@@ -383,29 +399,28 @@ __global__ __launch_bounds__(NTHREADS, 2) void paged_chunk_kernel(const ChunkPar
       for (int ks = 0; ks < D / 16; ++ks) acc = Mfma<T>::run(kf[ks], qf[ks], acc);
       sacc[kb] = acc;
     }
-    __builtin_amdgcn_sched_group_barrier(0x100, D / 16, 0);
+    if constexpr (!lean(D, PIECES)) {
+      __builtin_amdgcn_sched_group_barrier(0x100, D / 16, 0);
 #pragma unroll
-    for (int j = 0; j < D / 16; ++j) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      for (int j = 0; j < D / 16; ++j) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, D / 16, 0);
     }
-    __builtin_amdgcn_sched_group_barrier(0x008, D / 16, 0);
-    if (mode >= 2) {
+    if (mode == 1) return;
+    if (mode == 2) {
       if constexpr (POS) {
         const char* pl = sb + L::K_BYTES + L::V_BYTES;
-        const uint64_t qlim = p.causal ? (uint64_t)qpos : (uint64_t)INT64_MAX;  // (-1 wraps past it)
-        const int left = sees ? n - slot0 : 0;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
           for (int i4 = 0; i4 < 4; ++i4) {
-            const int key0 = kb * 32 + i4 * 8 + g * 4;
-            const uint4 a = *(const uint4*)(pl + key0 * 8), a2 = *(const uint4*)(pl + key0 * 8 + 16);
-            const uint64_t kp[4] = {((uint64_t)a.y << 32) | a.x, ((uint64_t)a.w << 32) | a.z,
-                                    ((uint64_t)a2.y << 32) | a2.x, ((uint64_t)a2.w << 32) | a2.z};
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (!(key0 + j < left && kp[j] <= qlim)) sacc[kb][i4 * 4 + j] = -__builtin_inff();
+            const int4 kp = *(const int4*)(pl + (kb * 32 + i4 * 8 + g * 4) * 4);
+            if (kp.x > qlim32) sacc[kb][i4 * 4 + 0] = -__builtin_inff();
+            if (kp.y > qlim32) sacc[kb][i4 * 4 + 1] = -__builtin_inff();
+            if (kp.z > qlim32) sacc[kb][i4 * 4 + 2] = -__builtin_inff();
+            if (kp.w > qlim32) sacc[kb][i4 * 4 + 3] = -__builtin_inff();
           }
       } else {
         const int left = lim - slot0 - g * 4;
@@ -415,21 +430,32 @@ __global__ __launch_bounds__(NTHREADS, 2) void paged_chunk_kernel(const ChunkPar
           for (int e = 0; e < 16; ++e)
             if (kb * 32 + (e >> 2) * 8 + (e & 3) >= left) sacc[kb][e] = -__builtin_inff();
       }
-      if (mode == 3) {  // some page of the run is not there
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int i4 = 0; i4 < 4; ++i4) {
-            const int slot = slot0 + kb * 32 + i4 * 8 + g * 4;  // its four keys lie in one page
-            int64_t id = -1;
-            if (slot < cap) id = p.tables[b * p.ts_b + (int64_t)page_of(slot) * p.ts_w];
-            if (id < 0 || id >= p.P)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) sacc[kb][i4 * 4 + j] = -__builtin_inff();
-          }
-        // (drains this wave's tile loads, which its own waits do not mind)
-      }
+      return;
     }
+    uint32_t hide = 0;
+#pragma unroll 1
+    for (int x = 0; x < 32; ++x) {  // (rare: the pool's positions are read in place, which waits for every load)
+      const int slot = slot0 + (x >> 4) * 32 + ((x >> 2) & 3) * 8 + g * 4 + (x & 3);
+      bool vis = slot < lim;
+      if (vis) {
+        const int pg = page_of(slot), id = ids[pg - pg0];
+        vis = id >= 0;
+        if (POS && vis) {
+          const int64_t pos = p.pos[(int64_t)id * p.ps_p + slot - pg * (page16 * 16)];
+          vis = pos >= 0 && (!p.causal || pos <= qpos);
+        }
+      }
+      hide |= (vis ? 0u : 1u) << x;
+    }
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if ((hide >> i) & 1u) sacc[i >> 4][i & 15] = -__builtin_inff();
+  };
+
+  auto compute = [&](int stage, int slot0, int mode) {
+    const char* sb = smem + stage * L::STAGE_BYTES;
+    f32x16 sacc[2];
+    scores(stage, slot0, mode, sacc);
     float t1[11];
 #pragma unroll
     for (int i = 0; i < 10; ++i) {
@@ -454,76 +480,34 @@ __global__ __launch_bounds__(NTHREADS, 2) void paged_chunk_kernel(const ChunkPar
         for (int e = 0; e < 16; ++e) oacc[dt][e] *= alpha;
     }
     frag pf[PIECES][4];
-    float pr[32];
-    uint32_t seen = 0, none = 0;  // visible keys of this lane, those of them with probability 0
+    if constexpr (lean(D, PIECES)) {
+      float sum[4] = {};
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[kb][e], c, -m_use));
-        pr[kb * 16 + e] = x;
-        if constexpr (decltype(careful)::value) {
-          const bool vis = __float_as_uint(sacc[kb][e]) != 0xff800000u;
-          seen |= (vis ? 1u : 0u) << (kb * 16 + e);
-          none |= (vis && (__float_as_uint(x) << 1) == 0 ? 1u : 0u) << (kb * 16 + e);
-        }
-        float rest = x * kPieceScale;
-#pragma unroll
-        for (int pc = 0; pc < PIECES; ++pc) {
-          pf[pc][kb * 2 + (e >> 3)][e & 7] = (T)rest;
-          if (pc + 1 < PIECES) rest -= to_f32<T>(pf[pc][kb * 2 + (e >> 3)][e & 7]);
-        }
+      for (int e = 0; e < 32; ++e) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[e >> 4][e & 15], c, -m_use));
+        sum[e & 3] += x;
+        pf[0][e >> 3][e & 7] = (T)x;
       }
+      l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    } else {
+      float pr[32];
 #pragma unroll
-    for (int w = 16; w >= 1; w >>= 1)
+      for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-      for (int e = 0; e < w; ++e) pr[e] += pr[e + w];
-    l_run += pr[0];
-    if constexpr (decltype(careful)::value) {
-      // values that are not finite: out of the products, then per feature the visible keys with +inf or
-      // NaN, and those with -inf or NaN, are counted by products of ones, and the sum takes an infinity of
-      // that sign (both make a NaN; a visible key of probability 0 counts for both: 0 * inf)
-      auto keys = [&](uint32_t bits, int s) {
-        u16x8 x;
+        for (int e = 0; e < 16; ++e) {
+          pr[kb * 16 + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[kb][e], c, -m_use));
+          float rest = pr[kb * 16 + e] * kPieceScale;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = (bits >> (8 * s + j)) & 1 ? Bits16<T>::kOne : 0;
-        return __builtin_bit_cast(frag, x);
-      };
-#pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt) {
-        __builtin_amdgcn_sched_barrier(0);
-        f32x16 count[2] = {};
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          u16x8 x = __builtin_bit_cast(u16x8, read_tr_frag<frag>(sb + s * 16 * L::KROW + v_raddr[dt],
-                                                                 sb + (s * 16 + 8) * L::KROW + v_raddr[dt]));
-          u16x8 one[2], any;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const uint16_t mag = x[j] & 0x7fff;
-            any[j] = mag >= Bits16<T>::kInf ? Bits16<T>::kOne : 0;
-            one[0][j] = mag > Bits16<T>::kInf || x[j] >> 15 == 0 ? any[j] : 0;
-            one[1][j] = mag > Bits16<T>::kInf || x[j] >> 15 == 1 ? any[j] : 0;
-            if (mag >= Bits16<T>::kInf) x[j] = 0;
-          }
-#pragma unroll
-          for (int pc = 0; pc < PIECES; ++pc) oacc[dt] = Mfma<T>::run(__builtin_bit_cast(frag, x), pf[pc][s], oacc[dt]);
-#pragma unroll
-          for (int sign = 0; sign < 2; ++sign) {
-            count[sign] = Mfma<T>::run(__builtin_bit_cast(frag, one[sign]), keys(seen, s), count[sign]);
-            count[sign] = Mfma<T>::run(__builtin_bit_cast(frag, any), keys(none, s), count[sign]);
+          for (int pc = 0; pc < PIECES; ++pc) {
+            pf[pc][kb * 2 + (e >> 3)][e & 7] = (T)rest;
+            if (pc + 1 < PIECES) rest -= to_f32<T>(pf[pc][kb * 2 + (e >> 3)][e & 7]);
           }
         }
 #pragma unroll
-        for (int sign = 0; sign < 2; ++sign)
+      for (int w = 16; w >= 1; w >>= 1)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            uint32_t add = count[sign][e] > 0.f ? (sign ? 0xff800000u : 0x7f800000u) : 0x80000000u;
-            asm volatile("" : "+v"(add));  // the file is compiled as if no NaN occurred
-            oacc[dt][e] += __uint_as_float(add);
-          }
-      }
-      return;
+        for (int e = 0; e < w; ++e) pr[e] += pr[e + w];
+      l_run += pr[0];
     }
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt) {
@@ -536,104 +520,201 @@ __global__ __launch_bounds__(NTHREADS, 2) void paged_chunk_kernel(const ChunkPar
 #pragma unroll
         for (int pc = 0; pc < PIECES; ++pc) oacc[dt] = Mfma<T>::run(vf[s], pf[pc][s], oacc[dt]);
     }
-    __builtin_amdgcn_sched_group_barrier(0x100, 8, 1);
+    if constexpr (!lean(D, PIECES)) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 8, 1);
 #pragma unroll
-    for (int j = 0; j < D / 32 - 1; ++j) {
+      for (int j = 0; j < D / 32 - 1; ++j) {
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        __builtin_amdgcn_sched_group_barrier(0x008, PIECES, 1);
-        __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+        for (int s = 0; s < 4; ++s) {
+          __builtin_amdgcn_sched_group_barrier(0x008, PIECES, 1);
+          __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+        }
       }
+      __builtin_amdgcn_sched_group_barrier(0x008, 4 * PIECES, 1);
     }
-    __builtin_amdgcn_sched_group_barrier(0x008, 4 * PIECES, 1);
   };
 
-  // ---- the stream over this run's tiles
-  auto stream = [&](auto careful) {
-    for (int base = t_first; base < t_last; base += POS ? LIST_CAP : t_last - t_first) {
-      int nt = t_last - base;
+  // ---- the second time over the tiles.  Values that are not finite are taken out of this wave's rows of a
+  // tile as they land, and the tile is marked ...
+  auto clean_share = [&](int stage, int i) {
+    char* v = smem + stage * L::STAGE_BYTES + L::K_BYTES + wave_kv + lane * 16;
+    bool found = false;
+#pragma unroll
+    for (int l = 0; l < L::KV_LOADS; ++l) {
+      u16x8 x = *(const u16x8*)(v + l * 1024);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const bool odd = (x[j] & 0x7fff) >= Bits16<T>::kInf;
+        found = found || odd;
+        x[j] = odd ? 0 : x[j];
+      }
+      *(u16x8*)(v + l * 1024) = x;
+    }
+    if (__ballot(found) != 0 && lane == 0) atomicOr(&marks[i >> 5], 1u << (i & 31));
+    wait_lgkmcnt0();  // before the barrier that hands the tile to the other waves
+  };
+  // ... and a marked tile, V as it is, counts per feature the visible keys with +inf or NaN, then those with
+  // -inf or NaN, by products with ones; the sum takes an infinity of that sign (both make a NaN; a
+  // visible key of probability 0 counts for both: 0 * inf).
+  auto mark = [&](int stage, int slot0, int mode) {
+    const char* sb = smem + stage * L::STAGE_BYTES;
+    f32x16 sacc[2];
+    scores(stage, slot0, mode, sacc);
+    uint32_t seen = 0, none = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const float x = sacc[i >> 4][i & 15];
+      const bool vis = __float_as_uint(x) != 0xff800000u;
+      seen |= (vis ? 1u : 0u) << i;
+      none |= (vis && __builtin_amdgcn_exp2f(__builtin_fmaf(x, c, -m_use)) == 0.f ? 1u : 0u) << i;
+    }
+    auto keys = [&](uint32_t bits, int s) {
+      u16x8 x;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = (bits >> (8 * s + j)) & 1 ? Bits16<T>::kOne : 0;
+      return __builtin_bit_cast(frag, x);
+    };
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int sign = 0; sign < 2; ++sign) {
+        __builtin_amdgcn_sched_barrier(0);
+        f32x16 count = {};
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const u16x8 x = __builtin_bit_cast(u16x8, read_tr_frag<frag>(sb + s * 16 * L::KROW + v_raddr[dt],
+                                                                       sb + (s * 16 + 8) * L::KROW + v_raddr[dt]));
+          u16x8 one, any;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const uint16_t mag = x[j] & 0x7fff;
+            any[j] = mag >= Bits16<T>::kInf ? Bits16<T>::kOne : 0;
+            one[j] = mag > Bits16<T>::kInf || (x[j] >> 15) == sign ? any[j] : 0;
+          }
+          count = Mfma<T>::run(__builtin_bit_cast(frag, one), keys(seen, s), count);
+          count = Mfma<T>::run(__builtin_bit_cast(frag, any), keys(none, s), count);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          uint32_t add = count[e] > 0.f ? (sign ? 0xff800000u : 0x7f800000u) : 0x80000000u;
+          asm volatile("" : "+v"(add));  // the file is compiled as if no NaN occurred
+          oacc[dt][e] += __uint_as_float(add);
+        }
+      }
+  };
+
+  // ---- the passes over this run's tiles: the pages' indices (and the list of the tiles needed), then the
+  // stream
+  auto stream = [&](bool careful) {
+    for (int base = t_first; base < t_last; base += PASS) {
+      const int span = min(PASS, t_last - base);
+      int nt = span;
+      pg0 = page_of(base * BN);
+      const int npg = page_of(min((base + span) * BN, n) - 1) - pg0 + 1;
+      bool lost = false;
+      for (int i = tid; i < npg; i += NTHREADS) {
+        const int64_t id = p.tables[b * p.ts_b + (int64_t)(pg0 + i) * p.ts_w];
+        const bool ok = (uint64_t)id < (uint64_t)p.P;
+        ids[i] = ok ? (int)id : -1;
+        lost = lost || !ok;
+      }
+      if (careful && tid < PASS / 32) marks[tid] = 0;
       if constexpr (POS) {
         const TileInfo* tinfo = c_.tiles + (int64_t)b * c_.ntiles;
-        const int span = min(LIST_CAP, nt);
-        nt = 0;
-        for (int r0 = 0; r0 < span; r0 += NTHREADS) {
-          const int t = base + r0 + tid;
-          bool need = false;
-          int modes = 0;
-          if (r0 + tid < span) {
-            const TileInfo ti = tinfo[t];
-            need = ti.n_valid > 0 && !(p.causal && max_wg < ti.min_valid);
+        bool need = false;
+        int modes = 0;
+        if (tid < span) {
+          const TileInfo ti = tinfo[base + tid];
+          need = ti.n_valid > 0 && !(p.causal && max_wg < ti.min_valid);
 #pragma unroll
-            for (int w = 0; w < NWAVES; ++w) {
-              int m;
-              if (!red_act[w] || ti.n_valid == 0 || (p.causal && red_max[w] < ti.min_valid)) m = 0;
-              else if (ti.n_valid == BN && (!p.causal || ti.max_valid <= red_min[w])) m = 1;
-              else m = 2;
-              modes |= m << (2 * w);
-            }
+          for (int w = 0; w < NWAVES; ++w) {
+            int m;
+            if (!red_act[w] || ti.n_valid == 0 || (p.causal && red_max[w] < ti.min_valid)) m = 0;
+            else if (ti.n_valid == BN && (!p.causal || ti.max_valid <= red_min[w])) m = 1;
+            else m = ti.pad[0] ? 3 : 2;
+            modes |= m << (2 * w);
           }
-          const uint64_t bal = __ballot(need);
-          if (lane == 0) wave_cnt[wave] = __builtin_popcountll(bal);
-          __syncthreads();
-          int off = nt;
-          for (int w = 0; w < wave; ++w) off += wave_cnt[w];
-          int tot = nt;
-          for (int w = 0; w < NWAVES; ++w) tot += wave_cnt[w];
-          if (need)
-            tile_list[off + __builtin_amdgcn_mbcnt_hi((uint32_t)(bal >> 32),
-                                                      __builtin_amdgcn_mbcnt_lo((uint32_t)bal, 0))] = make_int2(t, modes);
-          __syncthreads();
-          nt = tot;
         }
-        nt = uniform(nt);
-        if (nt == 0) continue;
+        const uint64_t bal = __ballot(need);
+        if (lane == 0) wave_cnt[wave] = __builtin_popcountll(bal);
+        __syncthreads();
+        int off = 0;
+        for (int w = 0; w < wave; ++w) off += wave_cnt[w];
+        nt = 0;
+        for (int w = 0; w < NWAVES; ++w) nt += wave_cnt[w];
+        if (need)
+          tile_list[off + __builtin_amdgcn_mbcnt_hi((uint32_t)(bal >> 32),
+                                                    __builtin_amdgcn_mbcnt_lo((uint32_t)bal, 0))] =
+              make_int2(base + tid, modes);
+        nt = scalar(nt);
+      } else if (__ballot(lost) != 0 && lane == 0) {
+        flags[0] = 1;
       }
-      auto tile_of = [&](int i) -> int {
-        if constexpr (POS) return uniform(tile_list[i].x);
-        else return base + i;
+      __syncthreads();
+      const bool bad = !POS && scalar(flags[0]) != 0;
+      auto tile_of = [&](int i) -> int { return POS ? scalar(tile_list[i].x) : base + i; };
+      auto mode_of = [&](int tile, int e) -> int {
+        int m;
+        if constexpr (POS) m = scalar((e >> (2 * wave)) & 3);
+        else m = tile * BN >= lim_max ? 0 : bad ? 3 : (tile + 1) * BN <= lim_min ? 1 : 2;
+        return m;
       };
-      const int bad = uniform(flags[0]);
       int issued = 0;
-      for (; issued < nt && issued < NSTAGE - 1; ++issued) load_tile(tile_of(issued), id_of(tile_of(issued)), issued);
-      // the tile to load next, and its page, are known a step ahead of its load
-      int t_load = issued < nt ? tile_of(issued) : base;
-      int64_t id_load = id_of(t_load);
-      int e_cur = 0;
-      if constexpr (POS) e_cur = tile_list[0].y;
+      for (; issued < nt && issued < NSTAGE - 1; ++issued)
+        load_tile(tile_of(issued), scalar(id_of(tile_of(issued))), issued);
+      // what the next step needs is read from LDS right after a barrier and used behind that step's work:
+      // the tile to load next and its page, the next tile's mode
+      int t_load = base, id_load = -1;
+      if (issued < nt) t_load = tile_of(issued), id_load = scalar(id_of(t_load));
+      int t_cur = base, e_cur = 0;
+      if constexpr (POS)
+        if (nt > 0) t_cur = tile_of(0), e_cur = tile_list[0].y;
       for (int i = 0; i < nt; ++i) {
-        wait_tiles_ahead<L::LPT>(issued - i - 1);
+        if (POS && wave == 0) wait_tiles_ahead<L::LPT + 1>(issued - i - 1);
+        else wait_tiles_ahead<L::LPT>(issued - i - 1);
+        if (careful) clean_share((int)((unsigned)i % NSTAGE), i);
         barrier_no_fence();  // tile i landed for every wave; the stage of tile i-1 is free
         if (issued < nt) {
           load_tile(t_load, id_load, (int)((unsigned)issued % NSTAGE));
           ++issued;
         }
-        int tile, mode;
-        int2 e_nxt = make_int2(0, 0), l_nxt = make_int2(0, 0);
+        int2 e_nxt = make_int2(t_cur + 1, 0);
+        int l_nxt = t_load, id_nxt = 0;
         if constexpr (POS) {
-          tile = uniform(tile_list[i].x);
-          mode = uniform((e_cur >> (2 * wave)) & 3);
           e_nxt = tile_list[i + 1 < nt ? i + 1 : i];
-          l_nxt = tile_list[issued < nt ? issued : 0];
+          l_nxt = tile_list[issued < nt ? issued : 0].x;
+          id_nxt = id_of(scalar(l_nxt));
         } else {
-          tile = base + i;
-          mode = tile * BN >= lim_max ? 0 : (tile + 1) * BN <= lim_min ? 1 : 2;
-          if (issued < nt) t_load = base + issued, id_load = id_of(t_load);
+          l_nxt = issued < nt ? base + issued : t_load;
+          id_nxt = id_of(l_nxt);
         }
-        if (bad && mode != 0) mode = 3;
-        if (mode != 0) compute((int)((unsigned)i % NSTAGE), tile * BN, mode, careful);
-        if constexpr (POS) {
-          e_cur = e_nxt.y;
-          if (issued < nt) t_load = uniform(l_nxt.x), id_load = id_of(t_load);
-        }
+        const int mode = mode_of(t_cur, e_cur);
+        if (mode != 0) compute((int)((unsigned)i % NSTAGE), t_cur * BN, mode);
+        t_cur = scalar(e_nxt.x);
+        e_cur = e_nxt.y;
+        t_load = scalar(l_nxt);
+        id_load = scalar(id_nxt);
       }
-      __syncthreads();  // the next pass rewrites the list and the stages
+      __syncthreads();  // the next pass rewrites the lists and the stages
+      if (!careful) continue;
+      for (int i = 0; i < nt; ++i) {
+        if (!((scalar(marks[i >> 5]) >> (i & 31)) & 1)) continue;
+        const int tile = tile_of(i);
+        load_tile(tile, scalar(id_of(tile)), 0);
+        wait_vmcnt<0>();
+        __syncthreads();
+        const int mode = mode_of(tile, POS ? tile_list[i].y : 0);
+        if (mode != 0) mark(0, tile * BN, mode);
+        __syncthreads();
+      }
     }
   };
 
-  __syncthreads();  // flags[0]
   clear();
-  stream(std::false_type());
-  {
+  bool careful = false;
+  while (true) {
+    stream(careful);
+    if (careful) break;
     uint32_t worst = 0;
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt)
@@ -641,10 +722,9 @@ __global__ __launch_bounds__(NTHREADS, 2) void paged_chunk_kernel(const ChunkPar
       for (int e = 0; e < 16; ++e) worst = max(worst, __float_as_uint(oacc[dt][e]) & 0x7fffffffu);
     if (__ballot(sees && worst >= 0x7f800000u) != 0 && lane == 0) flags[1] = 1;
     __syncthreads();
-    if (flags[1] != 0) {
-      clear();
-      stream(std::true_type());
-    }
+    if (flags[1] == 0) break;
+    careful = true;
+    clear();
   }
 
   // ---- epilogue.  A row's sum is 0 exactly where it saw no key (a NaN is kept).
@@ -702,7 +782,7 @@ size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
 struct ChunkPlan {
   int hp, splits;
-  size_t tiles, part_out, part_lse;  // bytes: summaries, one split's partial result
+  size_t tiles, pos32, part_out, part_lse;  // bytes: summaries, positions, one split's partial result
 };
 
 ChunkPlan plan_chunk(int64_t B, int64_t Sq, int64_t Hq, int group, int64_t D, int64_t slots, bool pos) {
@@ -710,6 +790,7 @@ ChunkPlan plan_chunk(int64_t B, int64_t Sq, int64_t Hq, int group, int64_t D, in
   r.hp = prefill_heads_per_wg(Sq, group);
   r.splits = prefill_key_splits(B, Sq, Hq, slots, r.hp);
   r.tiles = pos ? align256((size_t)B * ((slots + BN - 1) / BN) * sizeof(TileInfo)) : 0;
+  r.pos32 = pos ? align256((size_t)B * ((slots + BN - 1) / BN) * BN * sizeof(int32_t)) : 0;
   r.part_out = align256((size_t)B * Sq * Hq * D * sizeof(float));
   r.part_lse = align256((size_t)B * Sq * Hq * sizeof(float));
   return r;
@@ -719,7 +800,7 @@ ChunkPlan plan_chunk(int64_t B, int64_t Sq, int64_t Hq, int group, int64_t D, in
 
 size_t paged_chunk_workspace_bytes(int64_t B, int64_t Sq, int64_t Hq, int group, int64_t D, int64_t slots, bool pos) {
   const ChunkPlan r = plan_chunk(B, Sq, Hq, group, D, slots, pos);
-  return r.tiles + (r.splits > 1 ? r.splits * (r.part_out + r.part_lse) : 0);
+  return r.tiles + r.pos32 + (r.splits > 1 ? r.splits * (r.part_out + r.part_lse) : 0);
 }
 
 bool paged_chunk_supported(const PagedParams& p, const HeadMap& map) {
@@ -744,11 +825,12 @@ int launch_paged_chunk(const PagedParams& params, const HeadMap& map, void* ws, 
   char* at = (char*)ws;
   if (o.pos) {
     c.tiles = (const TileInfo*)at;
+    c.pos32 = (const int32_t*)(at + r.tiles);
     c.ntiles = (int32_t)((slots + BN - 1) / BN);
-    hipLaunchKernelGGL(paged_tile_info_kernel, dim3((unsigned)c.ntiles, (unsigned)o.B), dim3(64), 0, st, o, c.ntiles,
-                       (TileInfo*)at);
+    hipLaunchKernelGGL(paged_tile_info_kernel, dim3((unsigned)std::min((c.ntiles + 3) / 4, 64), (unsigned)o.B),
+                       dim3(256), 0, st, o, c.ntiles, (TileInfo*)at, (int32_t*)(at + r.tiles));
     CEA_CHECK_LAUNCH("paged_tile_info");
-    at += r.tiles;
+    at += r.tiles + r.pos32;
   }
   // query heads that an XCD takes together: whole KV heads, as many as 5 MB of keys and values hold (by
   // the table's width: the lengths are on the device), in sets of even size
