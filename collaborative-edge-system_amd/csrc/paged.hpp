@@ -61,6 +61,15 @@ bool paged_chunk_supported(const PagedParams& p, const HeadMap& map);
 size_t paged_chunk_workspace_bytes(int64_t B, int64_t Sq, int64_t Hq, int group, int64_t D, int64_t slots, bool pos);
 int launch_paged_chunk(const PagedParams& p, const HeadMap& map, void* ws, hipStream_t s);
 
+// f32, head size 64 or 128.  Scratch: the partial results of key splits.
+bool paged_f32_supported(const PagedParams& p, const HeadMap& map);
+size_t paged_f32_workspace_bytes(int64_t B, int64_t Sq, int64_t Hq, int group, int64_t D, int64_t slots);
+int launch_paged_f32(const PagedParams& p, const HeadMap& map, void* ws, hipStream_t s);
+
+// Merges the f32 partial results of `splits` key splits (the first at part.out / part.lse) into p's.
+int merge_paged_splits(const PagedParams& p, const PagedParams& part, int splits, int64_t split_out,
+                       int64_t split_lse, hipStream_t s);
+
 int launch_paged_generic(const PagedParams& p, const HeadMap& map, hipStream_t s);
 
 // Appends, one row of k and v per token and head; null tensors are left out.

@@ -64,6 +64,25 @@ bool paged_tiles_supported(const PagedParams& p) {
   return p.pos == nullptr || p.ps_s == 1;
 }
 
+int merge_paged_splits(const PagedParams& o, const PagedParams& part, int splits, int64_t split_out,
+                       int64_t split_lse, hipStream_t st) {
+  MergeParams m;
+  memset(&m, 0, sizeof(m));
+  m.n = splits;
+  m.B = o.B, m.Sq = o.Sq, m.H = o.Hq, m.D = o.D;
+  m.dtype = CEA_F32, m.out_dtype = o.out_dtype;
+  for (int i = 0; i < splits; ++i) {
+    m.outs[i] = (const float*)part.out + i * split_out;
+    m.lses[i] = (const float*)part.lse + i * split_lse;
+    m.os[i][0] = part.os_b, m.os[i][1] = part.os_s, m.os[i][2] = part.os_h;
+    m.ls[i][0] = part.ls_b, m.ls[i][1] = part.ls_h, m.ls[i][2] = part.ls_s;
+  }
+  m.out = o.out, m.lse = o.lse;
+  m.dos[0] = o.os_b, m.dos[1] = o.os_s, m.dos[2] = o.os_h;
+  m.dls[0] = o.ls_b, m.dls[1] = o.ls_h, m.dls[2] = o.ls_s;
+  return launch_merge(m, st);
+}
+
 }  // namespace cea
 
 using namespace cea;
@@ -117,13 +136,14 @@ int cea_paged_kv_append(const cea_tensor* k, const cea_tensor* v, const cea_tens
 
 size_t cea_paged_attention_workspace_bytes(int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int64_t D,
                                            int64_t W, int64_t page, int32_t in_dtype) {
-  if (!(in_dtype == CEA_BF16 || in_dtype == CEA_F16) || !(D == 64 || D == 128)) return 0;
+  if (!(in_dtype == CEA_BF16 || in_dtype == CEA_F16 || in_dtype == CEA_F32) || !(D == 64 || D == 128)) return 0;
   if (B <= 0 || Sq <= 0 || Hq <= 0 || Hkv <= 0 || W <= 0 || page <= 0 || page % 16) return 0;
   // (an explicit map takes the place of an even grouping, or there is none: room for either)
   const int64_t slots = W * page;
   size_t most = 0;
   for (const int group : {0, Hq % Hkv == 0 ? (int)(Hq / Hkv) : 0})
-    most = std::max({most, paged_token_workspace_bytes(B, Sq, Hq, Hkv, group, D, slots),
+    if (in_dtype == CEA_F32) most = std::max(most, paged_f32_workspace_bytes(B, Sq, Hq, group, D, slots));
+    else most = std::max({most, paged_token_workspace_bytes(B, Sq, Hq, Hkv, group, D, slots),
                      paged_chunk_workspace_bytes(B, Sq, Hq, group, D, slots, true)});
   return most;
 }
@@ -202,6 +222,12 @@ int cea_paged_attention(const cea_tensor* q, const cea_tensor* k_pages, const ce
                   "%s: workspace of %zu bytes needed, %zu given", what, need, workspace_bytes);
       return token ? launch_paged_token(p, map, workspace, st) : launch_paged_chunk(p, map, workspace, st);
     }
+  }
+  if (paged_f32_supported(p, map)) {
+    const size_t need = paged_f32_workspace_bytes(B, Sq, Hq, map.group, D, W * page);
+    CEA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), CEA_ENOSPACE,
+                "%s: workspace of %zu bytes needed, %zu given", what, need, workspace_bytes);
+    return launch_paged_f32(p, map, workspace, st);
   }
   return launch_paged_generic(p, map, st);
 }

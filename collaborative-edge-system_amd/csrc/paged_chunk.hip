@@ -858,21 +858,7 @@ int launch_paged_chunk(const PagedParams& params, const HeadMap& map, void* ws, 
   else
     rc = o.D == 128 ? launch_td<f16, 128>(c, f32, st) : launch_td<f16, 64>(c, f32, st);
   if (rc || r.splits == 1) return rc;
-  MergeParams m;
-  memset(&m, 0, sizeof(m));
-  m.n = r.splits;
-  m.B = o.B, m.Sq = o.Sq, m.H = o.Hq, m.D = o.D;
-  m.dtype = CEA_F32, m.out_dtype = o.out_dtype;
-  for (int i = 0; i < r.splits; ++i) {
-    m.outs[i] = (const float*)c.p.out + i * c.split_out;
-    m.lses[i] = (const float*)c.p.lse + i * c.split_lse;
-    m.os[i][0] = c.p.os_b, m.os[i][1] = c.p.os_s, m.os[i][2] = c.p.os_h;
-    m.ls[i][0] = c.p.ls_b, m.ls[i][1] = c.p.ls_h, m.ls[i][2] = c.p.ls_s;
-  }
-  m.out = o.out, m.lse = o.lse;
-  m.dos[0] = o.os_b, m.dos[1] = o.os_s, m.dos[2] = o.os_h;
-  m.dls[0] = o.ls_b, m.dls[1] = o.ls_h, m.dls[2] = o.ls_s;
-  return launch_merge(m, st);
+  return merge_paged_splits(o, c.p, r.splits, c.split_out, c.split_lse, st);
 }
 
 }  // namespace cea
