@@ -17,8 +17,9 @@
 //     a prefix of the row and every mask is one 32-bit comparison with the query row's limit; with
 //     them a launch before this one summarises the tiles and writes the positions in 32 bits,
 //     and the workgroup lists the tiles it needs;
-//   * lengths are known on the device alone: a launch with few query blocks is cut into key splits by
-//     the table's width, and each split takes an equal run of the tiles that the row really has;
+//   * lengths are known on the device alone: a launch with few query blocks has room for up to 16 key
+//     splits by the table's width, and the device gives every row as many as its tiles are worth, each
+//     an equal run of them; a second launch joins the rows that were cut;
 //   * hidden keys may hold anything.  Their scores are masked; a value that is not finite shows up as
 //     a result that is not, and the workgroup then goes over its tiles once more: such values are taken
 //     out of the tiles as they land, and the tiles that had some are visited again to add, per row and
@@ -77,8 +78,10 @@ struct ChunkParams {
   const int32_t* pos32;      // does not fit 31 bits), and [B, ntiles * 64] positions, kHidden32 where no key
   int32_t ntiles;
   int32_t hp;                // query heads of a workgroup: 1, 2, 4, 8
-  int32_t splits;            // key splits
-  int64_t split_out, split_lse;  // elements between the splits' partial results
+  int32_t splits;            // rows may be cut into key splits: at most so many splits in all (0: no)
+  int32_t kv_units;          // units of query heads that share keys: KV heads (or all heads)
+  float* part;               // partial results of the splits: [splits, Sq, Hq, D] and [splits, Hq, Sq]
+  float* part_lse;
   int32_t order_units, order_per_kv;  // workgroup columns that an XCD works through together
   int32_t page16;
   uint32_t magic;            // ceil(2^32 / page16), for page16 > 1
@@ -157,6 +160,54 @@ template <int LPT> __device__ __forceinline__ void wait_tiles_ahead(int ahead) {
   else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
+// Key splits: row b's tiles are cut into as many equal runs as they are worth where the tiles of all rows
+// make about two workgroups per compute unit (at least 4 tiles each: a split costs its start and its
+// part of the join), whatever the rows' lengths.  The splits of all rows are one line.
+constexpr int kSplitWgs = 512, kSplitTiles = 4;
+struct Split {
+  int b, split, first, count;  // a row, one of its splits, the place of its first one, how many it has
+};
+
+__device__ __forceinline__ int scan64(int v) {  // inclusive prefix sum over the lanes
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int x = __shfl_up(v, off, 64);
+    if (lane >= off) v += x;
+  }
+  return v;
+}
+
+// The split at place `at` (count 0 past the line's end), or with at < 0 row `b`'s.  per_row: workgroups of a
+// row's split.
+__device__ __forceinline__ Split find_split(const ChunkParams& c, int per_row, int at, int b) {
+  const PagedParams& p = c.p;
+  const int lane = threadIdx.x & 63;
+  auto tiles_of = [&](int row) { return row < p.B ? ((int)paged_slots(p, row) + BN - 1) / BN : 0; };
+  const int mine = tiles_of(lane);  // of the first 64 rows
+  int total = wave_sum_i32(mine);
+  for (int b0 = 64; b0 < p.B; b0 += 64) total += wave_sum_i32(tiles_of(b0 + lane));
+  const int per = (int)max(((int64_t)total * per_row + kSplitWgs - 1) / kSplitWgs, (int64_t)kSplitTiles);
+  Split r = {0, 0, 0, 0};
+  int before = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    const int tiles = b0 == 0 ? mine : tiles_of(b0 + lane);
+    const int n = b0 + lane < p.B ? max(1, min((tiles + per - 1) / per, kMaxKeySplits)) : 0;
+    const int sums = scan64(n);
+    const uint64_t found = at >= 0 ? __ballot(before + sums > at) : (b - b0 < 64 ? 1ull << (b - b0) : 0ull);
+    if (found != 0) {
+      const int l = (int)__builtin_ctzll(found);
+      r.b = b0 + l;
+      r.count = __builtin_amdgcn_readlane(n, l);
+      r.first = before + __builtin_amdgcn_readlane(sums, l) - r.count;
+      r.split = at - r.first;
+      break;
+    }
+    before += __builtin_amdgcn_readlane(sums, 63);
+  }
+  return r;
+}
+
 // Summaries and 32-bit positions of a row's tiles, a wave per tile; the row's length, not the table's
 // width, decides how many there are.
 __global__ __launch_bounds__(256) void paged_tile_info_kernel(const PagedParams p, int ntiles, TileInfo* out,
@@ -216,16 +267,18 @@ __global__ __launch_bounds__(NTHREADS, lean(D, PIECES) ? 4 : 2) void paged_chunk
   const int rows_pb = BM >> hp_log2;
   const int nqb = (p.Sq + rows_pb - 1) >> (__builtin_ctz(BM) - hp_log2);
   const int ngroups = p.Hq >> hp_log2, units = ngroups * p.B, total = nqb * units;
-  const int nsplit = c_.splits, all = total * nsplit;
-  int blk = blockIdx.x, split = 0, qb, b, hg;
-  if (nsplit > 1) {
-    if ((all & 7) == 0) blk = (blk & 7) * (all >> 3) + (blk >> 3);
-    split = blk / total;
-    blk -= split * total;
-    const int bh = blk / nqb;
-    qb = nqb - 1 - (blk - bh * nqb);
-    b = bh / ngroups;
-    hg = bh - b * ngroups;
+  int blk = blockIdx.x, split = 0, nsplit = 1, place = 0, qb, b, hg;
+  if (c_.splits > 0) {
+    // (split, KV head) in turn over the XCDs, the workgroups that share its keys together
+    const int per_kv = ngroups / c_.kv_units, shared = per_kv * nqb;
+    const int i = blk >> 3, set = i / shared, in = i - set * shared;
+    const int u = uniform(set * 8 + (blk & 7));
+    place = u / c_.kv_units;
+    const Split x = find_split(c_, nqb * ngroups, place, 0);
+    if (x.count == 0) return;
+    b = x.b, split = x.split, nsplit = x.count;
+    qb = nqb - 1 - in / per_kv;
+    hg = (u - place * c_.kv_units) * per_kv + in % per_kv;
   } else {
     int unit;
     if (nqb == 1) {
@@ -734,11 +787,14 @@ __global__ __launch_bounds__(NTHREADS, lean(D, PIECES) ? 4 : 2) void paged_chunk
   asm volatile("" : "+v"(l_bits));  // (compared as a float, a NaN might be taken for 0 in this file)
   const bool empty = !sees || (l_bits << 1) == 0;
   const float inv = empty ? 0.f : 1.f / (l_tot * kPieceScale);
-  if (p.lse && g == 0) {
-    float* lp = (float*)p.lse + split * c_.split_lse + b * p.ls_b + h * p.ls_h + (int64_t)row * p.ls_s;
+  if ((p.lse || nsplit > 1) && g == 0) {
+    float* lp = nsplit > 1 ? c_.part_lse + ((int64_t)place * p.Hq + h) * p.Sq + row
+                           : (float*)p.lse + b * p.ls_b + h * p.ls_h + (int64_t)row * p.ls_s;
     *lp = empty ? -__builtin_inff() : (m_run * fabsf(scale) + logf(l_tot)) - kExpShift * 0.69314718055994531f;
   }
-  const int64_t orow = split * c_.split_out + b * p.os_b + (int64_t)row * p.os_s + h * p.os_h;
+  const int64_t orow = nsplit > 1 ? (((int64_t)place * p.Sq + row) * p.Hq + h) * D
+                                  : b * p.os_b + (int64_t)row * p.os_s + h * p.os_h;
+  float* fout = nsplit > 1 ? c_.part : p.out_dtype == CEA_F32 ? (float*)p.out : nullptr;
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
@@ -747,8 +803,8 @@ __global__ __launch_bounds__(NTHREADS, lean(D, PIECES) ? 4 : 2) void paged_chunk
 #pragma unroll
       for (int j = 0; j < 4; ++j) x[j] = empty ? 0.f : oacc[dt][i4 * 4 + j] * inv;
       const int64_t at = orow + dt * 32 + i4 * 8 + g * 4;
-      if (p.out_dtype == CEA_F32) {
-        *(float4*)((float*)p.out + at) = make_float4(x[0], x[1], x[2], x[3]);
+      if (fout) {
+        *(float4*)(fout + at) = make_float4(x[0], x[1], x[2], x[3]);
       } else {
         const T v4[4] = {(T)x[0], (T)x[1], (T)x[2], (T)x[3]};
         uint2 raw;
@@ -758,17 +814,77 @@ __global__ __launch_bounds__(NTHREADS, lean(D, PIECES) ? 4 : 2) void paged_chunk
     }
 }
 
+// Joins a row's key splits by their log-sum-exp, four features a thread; every read is under way before
+// the first weight is known.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void paged_chunk_join_kernel(const ChunkParams c, int per_row) {
+  const PagedParams& p = c.p;
+  const int b = blockIdx.y;
+  const Split cut = find_split(c, per_row, -1, b);
+  const int n = uniform(cut.count);
+  if (n == 1) return;  // written by its workgroups
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (int64_t)p.Sq * p.Hq * (D / 4)) return;
+  const int f = (int)(i % (D / 4)) * 4;
+  const int h = (int)(i / (D / 4) % p.Hq), s = (int)(i / ((int64_t)(D / 4) * p.Hq));
+  const int64_t o_split = (int64_t)p.Sq * p.Hq * D, l_split = (int64_t)p.Hq * p.Sq;
+  const float* o = c.part + cut.first * o_split + ((int64_t)s * p.Hq + h) * D + f;
+  const float* l = c.part_lse + cut.first * l_split + (int64_t)h * p.Sq + s;
+  float4 x[kMaxKeySplits];
+  float lse[kMaxKeySplits], m = -__builtin_inff();
+#pragma unroll
+  for (int k = 0; k < kMaxKeySplits; ++k)
+    if (k < n) lse[k] = l[k * l_split], x[k] = *(const float4*)(o + k * o_split);
+#pragma unroll
+  for (int k = 0; k < kMaxKeySplits; ++k)
+    if (k < n) m = fmaxf(m, lse[k]);
+  const float shift = m == -__builtin_inff() ? 0.f : m;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < kMaxKeySplits; ++k)
+    if (k < n) {
+      const float w = expf(lse[k] - shift);  // 0 for a split that the row sees nothing of, whose output is 0
+      sum += w;
+      acc.x += x[k].x * w, acc.y += x[k].y * w, acc.z += x[k].z * w, acc.w += x[k].w * w;
+    }
+  uint32_t bits = __float_as_uint(sum);
+  asm volatile("" : "+v"(bits));  // (the file is compiled as if no NaN occurred)
+  const bool empty = bits == 0;
+  const float inv = empty ? 0.f : 1.f / sum;
+  const float r[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+  const int64_t at = b * p.os_b + s * p.os_s + h * p.os_h + f;
+  if (p.out_dtype == CEA_F32) {
+    *(float4*)((float*)p.out + at) = make_float4(r[0], r[1], r[2], r[3]);
+  } else {
+    const T v4[4] = {(T)r[0], (T)r[1], (T)r[2], (T)r[3]};
+    uint2 raw;
+    __builtin_memcpy(&raw, v4, 8);
+    *(uint2*)((T*)p.out + at) = raw;
+  }
+  if (p.lse && f == 0)
+    ((float*)p.lse)[b * p.ls_b + h * p.ls_h + s * p.ls_s] = empty ? -__builtin_inff() : shift + logf(sum);
+}
+
 template <typename T, int D, bool POS, int PIECES>
 int launch_form(const ChunkParams& c, hipStream_t st) {
   const PagedParams& p = c.p;
   const int nqb = (p.Sq + BM / c.hp - 1) / (BM / c.hp);
-  const int64_t total = (int64_t)nqb * (p.Hq / c.hp) * p.B * c.splits;
+  const int64_t per_row = (int64_t)nqb * (p.Hq / c.hp);
+  int64_t total = per_row * p.B;
+  if (c.splits > 0) total = ((int64_t)c.splits * c.kv_units + 7) / 8 * 8 * (per_row / c.kv_units);
   constexpr int lds = Layout<D, POS>::LDS_BYTES;
   const hipError_t e = reserve_lds<paged_chunk_kernel<T, D, POS, PIECES>>(lds);
   CEA_REQUIRE(e == hipSuccess, CEA_ELAUNCH, "paged_attention: cannot reserve %d bytes of LDS: %s", lds,
               hipGetErrorString(e));
   hipLaunchKernelGGL((paged_chunk_kernel<T, D, POS, PIECES>), dim3((unsigned)total), dim3(NTHREADS), lds, st, c);
   CEA_CHECK_LAUNCH("paged_chunk");
+  if (c.splits > 0) {
+    const int64_t vectors = (int64_t)p.Sq * p.Hq * (D / 4);
+    hipLaunchKernelGGL((paged_chunk_join_kernel<T, D>), dim3((unsigned)((vectors + 255) / 256), (unsigned)p.B), dim3(256),
+                       0, st, c, (int)per_row);
+    CEA_CHECK_LAUNCH("paged_chunk_join");
+  }
   return CEA_OK;
 }
 
@@ -782,17 +898,22 @@ size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
 struct ChunkPlan {
   int hp, splits;
-  size_t tiles, pos32, part_out, part_lse;  // bytes: summaries, positions, one split's partial result
+  size_t tiles, pos32, part_out, part_lse;  // bytes: summaries, positions, the splits' partial results
 };
 
 ChunkPlan plan_chunk(int64_t B, int64_t Sq, int64_t Hq, int group, int64_t D, int64_t slots, bool pos) {
   ChunkPlan r;
   r.hp = prefill_heads_per_wg(Sq, group);
-  r.splits = prefill_key_splits(B, Sq, Hq, slots, r.hp);
+  // Below a workgroup per compute unit the rows may be cut; their splits are at most the workgroups that the
+  // tiles are dealt to, over those of a row's split, and one a row more for what does not divide.
+  const int64_t per_row = (Sq + BM / r.hp - 1) / (BM / r.hp) * (Hq / r.hp), tiles = (slots + BN - 1) / BN;
+  r.splits = 0;
+  if (per_row * B < 256 && tiles >= 2 * kSplitTiles)
+    r.splits = (int)std::min<int64_t>(B * kMaxKeySplits, kSplitWgs / per_row + 1 + B);
   r.tiles = pos ? align256((size_t)B * ((slots + BN - 1) / BN) * sizeof(TileInfo)) : 0;
   r.pos32 = pos ? align256((size_t)B * ((slots + BN - 1) / BN) * BN * sizeof(int32_t)) : 0;
-  r.part_out = align256((size_t)B * Sq * Hq * D * sizeof(float));
-  r.part_lse = align256((size_t)B * Sq * Hq * sizeof(float));
+  r.part_out = align256((size_t)r.splits * Sq * Hq * D * sizeof(float));
+  r.part_lse = align256((size_t)r.splits * Sq * Hq * sizeof(float));
   return r;
 }
 
@@ -800,7 +921,7 @@ ChunkPlan plan_chunk(int64_t B, int64_t Sq, int64_t Hq, int group, int64_t D, in
 
 size_t paged_chunk_workspace_bytes(int64_t B, int64_t Sq, int64_t Hq, int group, int64_t D, int64_t slots, bool pos) {
   const ChunkPlan r = plan_chunk(B, Sq, Hq, group, D, slots, pos);
-  return r.tiles + r.pos32 + (r.splits > 1 ? r.splits * (r.part_out + r.part_lse) : 0);
+  return r.tiles + r.pos32 + r.part_out + r.part_lse;
 }
 
 bool paged_chunk_supported(const PagedParams& p, const HeadMap& map) {
@@ -843,22 +964,11 @@ int launch_paged_chunk(const PagedParams& params, const HeadMap& map, void* ws, 
   c.order_units = (int)((heads + sets - 1) / sets * per_kv);
   if (o.B == 1 && heads == 1) c.order_units = 1;
 
-  if (r.splits > 1) {  // partial results (f32), merged below
-    c.p.out = at;
-    c.p.out_dtype = CEA_F32;
-    c.p.os_h = o.D, c.p.os_s = (int64_t)o.Hq * o.D, c.p.os_b = c.p.os_s * o.Sq;
-    c.p.lse = at + r.splits * r.part_out;
-    c.p.ls_s = 1, c.p.ls_h = o.Sq, c.p.ls_b = (int64_t)o.Hq * o.Sq;
-    c.split_out = (int64_t)(r.part_out / sizeof(float)), c.split_lse = (int64_t)(r.part_lse / sizeof(float));
-  }
+  c.kv_units = map.group > 0 ? o.Hkv : o.Hq;
+  c.part = (float*)at, c.part_lse = (float*)(at + r.part_out);
   const bool f32 = o.out_dtype == CEA_F32;
-  int rc;
-  if (o.in_dtype == CEA_BF16)
-    rc = o.D == 128 ? launch_td<bf16, 128>(c, f32, st) : launch_td<bf16, 64>(c, f32, st);
-  else
-    rc = o.D == 128 ? launch_td<f16, 128>(c, f32, st) : launch_td<f16, 64>(c, f32, st);
-  if (rc || r.splits == 1) return rc;
-  return merge_paged_splits(o, c.p, r.splits, c.split_out, c.split_lse, st);
+  if (o.in_dtype == CEA_BF16) return o.D == 128 ? launch_td<bf16, 128>(c, f32, st) : launch_td<bf16, 64>(c, f32, st);
+  return o.D == 128 ? launch_td<f16, 128>(c, f32, st) : launch_td<f16, 64>(c, f32, st);
 }
 
 }  // namespace cea
