@@ -210,9 +210,13 @@ int cea_paged_attention(const cea_tensor* q, const cea_tensor* k_pages, const ce
   if (page == 0 || p.P == 0) p.W = 0, p.page = 1;  // no slots: every row is empty
   hipStream_t st = (hipStream_t)stream;
   if (paged_tiles_supported(p)) {
-    // the token form while one unit holds a KV head's queries, so its keys are read once; and for single
-    // tokens of larger groups
-    const bool few = Sq == 1 || map.group <= 0 || Sq * map.group <= 16;
+    // The token form while one unit holds a KV head's queries, so its keys are read once, and for single
+    // tokens of larger groups; two units where a key is small or a unit one workgroup (us, token / chunk
+    // form, 32 query rows of a KV head: 4 rows of up to 500 keys, D = 64, 8.5 / 13.9; 16 of up to 2500, D = 64,
+    // 27.8 / 30.5; 24 and 32 query rows at D = 128: 8 rows of up to 4096 keys 49.9 / 42.0, 32 of up to 2500
+    // 118 / 72).
+    const int64_t rows = Sq * map.group;
+    const bool few = Sq == 1 || map.group <= 0 || rows <= 16 || (rows <= 32 && (D == 64 || W * page <= 1024));
     const bool token = few && paged_token_supported(p, map);
     if (token || paged_chunk_supported(p, map)) {
       const int64_t slots = W * page;

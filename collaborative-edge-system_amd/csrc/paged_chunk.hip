@@ -142,6 +142,8 @@ __device__ __forceinline__ int wave_max_i32(int v) {
   for (int off = 32; off >= 1; off >>= 1) v = max(v, __shfl_xor(v, off, 64));
   return v;
 }
+typedef const int64_t __attribute__((address_space(4))) * scalar_i64;  // read through the scalar cache
+
 // A wave-uniform value in scalar registers, whatever the compiler makes of where it came from.
 template <typename X> __device__ __forceinline__ X scalar(X v) {
   if constexpr (sizeof(X) == 4) {
@@ -161,9 +163,11 @@ template <int LPT> __device__ __forceinline__ void wait_tiles_ahead(int ahead) {
 }
 
 // Key splits: row b's tiles are cut into as many equal runs as they are worth where the tiles of all rows
-// make about two workgroups per compute unit (at least 4 tiles each: a split costs its start and its
-// part of the join), whatever the rows' lengths.  The splits of all rows are one line.
-constexpr int kSplitWgs = 512, kSplitTiles = 4;
+// make 384 workgroups (at least 4 tiles each: a split costs its start and its part of the join),
+// whatever the rows' lengths.  The splits of all rows are one line.  (us, 256 / 384 / 512 workgroups: four
+// chunks of 300 over 700 to 4001 keys, 32/4 heads of 64, 65.9 / 63.7 / 70.3; 6 tokens of 8 rows of 100 to 4096,
+// 32/8 heads of 128, 43.4 / 41.0 / 39.9; 128 tokens over 32768 96.1 / 94.7 / 96.5)
+constexpr int kSplitWgs = 384, kSplitTiles = 4;
 struct Split {
   int b, split, first, count;  // a row, one of its splits, the place of its first one, how many it has
 };
@@ -240,23 +244,26 @@ __global__ __launch_bounds__(256) void paged_tile_info_kernel(const PagedParams 
   }
 }
 
+template <bool POS> struct Shared {
+  int64_t red_max[NWAVES], red_min[NWAVES];  // what the waves' rows see
+  int red_act[NWAVES], wave_cnt[NWAVES];
+  int lost[NWAVES];                          // a page of the pass that is not there, by finder
+  int odd_result;                            // a result that is not finite
+  uint32_t marks[PASS / 32];                 // tiles that hold a value that is not finite
+  int32_t ids[PASS * BN / 16];               // page indices of the pass, -1 where none
+  int2 tile_list[POS ? PASS : 1];            // (tile, 2-bit mode of every wave)
+};
+
 // PIECES: 16-bit numbers whose sum enters the value product for a probability: one for 16-bit results
 // (p rounded once, half a step of the type, as the result's own rounding is), three of bf16 or two of f16
 // for f32 results (p to 2^-23 and better).
-constexpr bool lean(int D, int pieces) { return false; }
-template <typename T, int D, bool POS, int PIECES>
-__global__ __launch_bounds__(NTHREADS, lean(D, PIECES) ? 4 : 2) void paged_chunk_kernel(const ChunkParams c_) {
+// AGAIN: over the tiles a second time, after values that are not finite.  Returns whether that is needed
+// (nothing has been written then).
+template <typename T, int D, bool POS, int PIECES, bool AGAIN>
+__device__ __forceinline__ bool chunk_body(const ChunkParams& c_, char* smem, Shared<POS>& sh) {
   typedef Layout<D, POS> L;
   typedef typename Mfma<T>::frag frag;
   const PagedParams& p = c_.p;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ int2 tile_list[POS ? PASS : 1];      // (tile, 2-bit mode of every wave)
-  __shared__ int32_t ids[PASS * BN / 16];         // page indices of the pass, -1 where none
-  __shared__ uint32_t marks[PASS / 32];           // tiles that hold a value that is not finite
-  __shared__ int64_t red_max[NWAVES], red_min[NWAVES];
-  __shared__ int red_act[NWAVES], wave_cnt[NWAVES];
-  __shared__ int flags[2];  // some page of the run is not there; some result is not finite
-
   const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63;
   const int r = lane & 31, g = lane >> 5;
 
@@ -275,7 +282,7 @@ __global__ __launch_bounds__(NTHREADS, lean(D, PIECES) ? 4 : 2) void paged_chunk
     const int u = uniform(set * 8 + (blk & 7));
     place = u / c_.kv_units;
     const Split x = find_split(c_, nqb * ngroups, place, 0);
-    if (x.count == 0) return;
+    if (x.count == 0) return false;
     b = x.b, split = x.split, nsplit = x.count;
     qb = nqb - 1 - in / per_kv;
     hg = (u - place * c_.kv_units) * per_kv + in % per_kv;
@@ -315,10 +322,54 @@ __global__ __launch_bounds__(NTHREADS, lean(D, PIECES) ? 4 : 2) void paged_chunk
   const int kvh = p.group > 0 ? hg * hp / p.group : c_.kv[hg * hp];
   const int row = qb * rows_pb + (wave & ((1 << waves_log2) - 1)) * 32 + r;
   const bool row_ok = row < p.Sq;
+  // ---- everything that the start reads is under way before any of it is used: positions and queries, the
+  // row's length through the scalar cache, then the first pass's page indices, which the length alone decides
   const int64_t qpos = row_ok ? p.q_pos[b * p.qps_b + (int64_t)row * p.qps_s] : -1;
-  const int n = scalar(uniform((int)paged_slots(p, b)));
+  uint4 qraw[D / 16];
+  {
+    const T* qrow = (const T*)p.q + b * p.qs_b + (int64_t)row * p.qs_s + h * p.qs_h;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      qraw[ks] = make_uint4(0, 0, 0, 0);
+      if (row_ok) qraw[ks] = *(const uint4*)(qrow + ks * 16 + g * 8);
+    }
+  }
+  const int64_t len = ((scalar_i64)(uintptr_t)p.lengths)[b * p.ns_b];
+  const int n = scalar((int)max((int64_t)0, min(len, (int64_t)p.W * p.page)));
   const int page16 = scalar(c_.page16);
   const uint32_t magic = scalar(c_.magic);
+  auto page_of = [&](int slot) -> int {
+    const uint32_t u = (uint32_t)slot >> 4;
+    return (int)(page16 == 1 ? u : __umulhi(u, magic));
+  };
+  // this split's run of the row's tiles (what its queries cannot see is left out below)
+  const int row_tiles = (n + BN - 1) / BN;
+  const int per_split = nsplit > 1 ? (row_tiles + nsplit - 1) / nsplit : row_tiles;
+  const int t_first = scalar(min(row_tiles, split * per_split));
+  int t_last = scalar(min(row_tiles, t_first + per_split));
+
+  // the page indices and summaries of a pass, from memory to registers and from there to LDS
+  constexpr int kIdsPer = PASS * BN / 16 / NTHREADS;
+  struct PassRegs {
+    int64_t id[kIdsPer];
+    TileInfo ti;
+  };
+  int pg0 = 0;  // page of the pass's first slot
+  auto fetch_pass = [&](int base, int last, PassRegs& x) {
+    const int span = min(PASS, last - base);
+    pg0 = page_of(base * BN);
+    const int npg = span > 0 ? page_of(min((base + span) * BN, n) - 1) - pg0 + 1 : 0;
+    const int64_t* tab = p.tables + b * p.ts_b + pg0 * p.ts_w;
+#pragma unroll
+    for (int i = 0; i < kIdsPer; ++i) {
+      x.id[i] = 0;
+      if (i * NTHREADS + tid < npg) x.id[i] = tab[(int64_t)(i * NTHREADS + tid) * p.ts_w];
+    }
+    if constexpr (POS)
+      if (tid < span) x.ti = c_.tiles[(int64_t)b * c_.ntiles + base + tid];
+  };
+  PassRegs regs;
+  if constexpr (!POS) fetch_pass(t_first, t_last, regs);
 
   // ---- what the rows see: slots [0, lim) of this lane's row by their number (POS: positions to qpos)
   const bool sees = row_ok && (!p.causal || qpos >= 0);
@@ -327,48 +378,17 @@ __global__ __launch_bounds__(NTHREADS, lean(D, PIECES) ? 4 : 2) void paged_chunk
   if constexpr (POS) {
     const int64_t mn = wave_min_i64(sees ? qpos : INT64_MAX), mx = wave_max_i64(sees ? qpos : INT64_MIN);
     const bool act = __ballot(sees) != 0;
-    if (lane == 0) red_max[wave] = mx, red_min[wave] = mn, red_act[wave] = act ? 1 : 0;
+    if (lane == 0) sh.red_max[wave] = mx, sh.red_min[wave] = mn, sh.red_act[wave] = act ? 1 : 0;
   } else {
     lim_min = uniform(wave_min_i32(lim > 0 ? lim : INT32_MAX));
     lim_max = uniform(wave_max_i32(lim));
-    if (lane == 0) red_max[wave] = lim_max;
+    if (lane == 0) sh.red_max[wave] = lim_max;
   }
-  if (tid < 2) flags[tid] = 0;
-  __syncthreads();
-  int64_t max_wg = red_max[0];
-#pragma unroll
-  for (int w = 1; w < NWAVES; ++w) max_wg = max(max_wg, red_max[w]);
-  bool any_wg = !POS;
-  if constexpr (POS)
-#pragma unroll
-    for (int w = 0; w < NWAVES; ++w) any_wg = any_wg || red_act[w] != 0;
+  if (tid == 0) sh.odd_result = 0;
 
-  // ---- this split's run of tiles
-  const int seen_tiles = uniform(!any_wg ? 0 : ((POS ? n : (int)max_wg) + BN - 1) / BN);
-  const int per_split = (seen_tiles + nsplit - 1) / nsplit;
-  const int t_first = scalar(min(seen_tiles, split * per_split));
-  const int t_last = scalar(min(seen_tiles, t_first + per_split));
-
-  auto page_of = [&](int slot) -> int {
-    const uint32_t u = (uint32_t)slot >> 4;
-    return (int)(page16 == 1 ? u : __umulhi(u, magic));
-  };
   const float scale = (float)p.scale;
   const float c = fabsf(scale) * 1.4426950408889634f;
   const float grow_thr = kRescaleLog2 / c;
-  const uint32_t qflip = scale < 0.f ? 0x80008000u : 0u;
-  frag qf[D / 16];
-  {
-    const T* qrow = (const T*)p.q + b * p.qs_b + (int64_t)row * p.qs_s + h * p.qs_h;
-#pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) {
-      uint4 raw = make_uint4(0, 0, 0, 0);
-      if (sees) raw = *(const uint4*)(qrow + ks * 16 + g * 8);
-      raw.x ^= qflip; raw.y ^= qflip; raw.z ^= qflip; raw.w ^= qflip;
-      __builtin_memcpy(&qf[ks], &raw, 16);
-    }
-  }
-
   const uint32_t krow = scalar((uint32_t)(p.ks_s * 2)), vrow = scalar((uint32_t)(p.vs_s * 2));
   uint32_t k_voff[L::KV_LOADS], v_voff[L::KV_LOADS];
 #pragma unroll
@@ -379,15 +399,13 @@ __global__ __launch_bounds__(NTHREADS, lean(D, PIECES) ? 4 : 2) void paged_chunk
     const int lgv = (((pg >> 2) ^ v_swz<D>(key)) << 2) | (pg & 3);
     v_voff[i] = local * vrow + (lgv << 4);
   }
-  uint32_t k_raddr[D / 16], v_raddr[D / 32];
-#pragma unroll
-  for (int ks = 0; ks < D / 16; ++ks) k_raddr[ks] = r * L::KROW + (((2 * ks + g) ^ k_swz<D>(r)) << 4);
+  // fragment reads: the swizzles are exclusive ors of bits that the features' offsets have to themselves
+  const uint32_t k_read0 = r * L::KROW + ((g ^ k_swz<D>(r)) << 4);
+  uint32_t v_read0;
   {
     const int src = lane & 15, grp = lane >> 4;
     const int vr = g * 4 + (src >> 2);
-#pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
-      v_raddr[dt] = L::K_BYTES + vr * L::KROW + ((dt ^ v_swz<D>(vr)) << 6) + (16 * (grp & 1) + 4 * (src & 3)) * 2;
+    v_read0 = L::K_BYTES + vr * L::KROW + (v_swz<D>(vr) << 6) + (16 * (grp & 1) + 4 * (src & 3)) * 2;
   }
   const uint32_t smem_lds = lds_addr(smem);
   const uint32_t wave_kv = wave * (L::KV_LOADS * 1024);
@@ -396,9 +414,8 @@ __global__ __launch_bounds__(NTHREADS, lean(D, PIECES) ? 4 : 2) void paged_chunk
   const int64_t ks_p = scalar(p.ks_p * 2), vs_p = scalar(p.vs_p * 2);
   const int32_t* pos32 = POS ? scalar(c_.pos32 + (int64_t)b * c_.ntiles * BN) : nullptr;
 
-  int pg0 = 0;  // page of the pass's first slot
   // the page index of this wave's rows of a tile (behind the row's end: the last one's)
-  auto id_of = [&](int tile) -> int { return ids[page_of(min(tile * BN + wave * WROWS, n - 1)) - pg0]; };
+  auto id_of = [&](int tile) -> int { return sh.ids[page_of(min(tile * BN + wave * WROWS, n - 1)) - pg0]; };
   auto load_tile = [&](int tile, int id, int stage) {
     const int slot = tile * BN + wave * WROWS;
     const int rows = min(n - slot, WROWS);  // rows behind the row's end, and of no page, read 0
@@ -425,17 +442,9 @@ __global__ __launch_bounds__(NTHREADS, lean(D, PIECES) ? 4 : 2) void paged_chunk
   constexpr bool kF16 = std::is_same<T, f16>::value;
   constexpr float kExpShift = kF16 && PIECES == 1 ? 7.f : 0.f;
   constexpr float kPieceScale = kF16 && PIECES > 1 ? 128.f : 1.f;
+  frag qf[D / 16];
   f32x16 oacc[D / 32];
-  float m_run, m_use, l_run;
-  auto clear = [&]() {
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) oacc[i][e] = 0.f;
-    m_run = -__builtin_inff();
-    m_use = -kExpShift;
-    l_run = 0.f;
-  };
+  float m_run = -__builtin_inff(), m_use = -kExpShift, l_run = 0.f;
 
   // The scores of a tile.  mode: 1 every key visible to every row of the wave that sees anything, 2 masked,
   // 3 masked and looked up: a page of the pass that is not there, or (POS) a position beyond 31 bits.
@@ -446,21 +455,20 @@ __global__ __launch_bounds__(NTHREADS, lean(D, PIECES) ? 4 : 2) void paged_chunk
     for (int kb = 0; kb < 2; ++kb) {
       frag kf[D / 16];
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) kf[ks] = *(const frag*)(sb + kb * 32 * L::KROW + k_raddr[ks]);
+      for (int ks = 0; ks < D / 16; ++ks) kf[ks] = *(const frag*)(sb + kb * 32 * L::KROW + (k_read0 ^ (ks << 5)));
       f32x16 acc = {};
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) acc = Mfma<T>::run(kf[ks], qf[ks], acc);
       sacc[kb] = acc;
     }
-    if constexpr (!lean(D, PIECES)) {
-      __builtin_amdgcn_sched_group_barrier(0x100, D / 16, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, D / 16, 0);
 #pragma unroll
-      for (int j = 0; j < D / 16; ++j) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      }
-      __builtin_amdgcn_sched_group_barrier(0x008, D / 16, 0);
+    for (int j = 0; j < D / 16; ++j) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }
+    __builtin_amdgcn_sched_group_barrier(0x008, D / 16, 0);
+    
     if (mode == 1) return;
     if (mode == 2) {
       if constexpr (POS) {
@@ -491,7 +499,7 @@ __global__ __launch_bounds__(NTHREADS, lean(D, PIECES) ? 4 : 2) void paged_chunk
       const int slot = slot0 + (x >> 4) * 32 + ((x >> 2) & 3) * 8 + g * 4 + (x & 3);
       bool vis = slot < lim;
       if (vis) {
-        const int pg = page_of(slot), id = ids[pg - pg0];
+        const int pg = page_of(slot), id = sh.ids[pg - pg0];
         vis = id >= 0;
         if (POS && vis) {
           const int64_t pos = p.pos[(int64_t)id * p.ps_p + slot - pg * (page16 * 16)];
@@ -533,58 +541,45 @@ __global__ __launch_bounds__(NTHREADS, lean(D, PIECES) ? 4 : 2) void paged_chunk
         for (int e = 0; e < 16; ++e) oacc[dt][e] *= alpha;
     }
     frag pf[PIECES][4];
-    if constexpr (lean(D, PIECES)) {
-      float sum[4] = {};
+    float pr[32];
 #pragma unroll
-      for (int e = 0; e < 32; ++e) {
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[e >> 4][e & 15], c, -m_use));
-        sum[e & 3] += x;
-        pf[0][e >> 3][e & 7] = (T)x;
-      }
-      l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    } else {
-      float pr[32];
+    for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
+      for (int e = 0; e < 16; ++e) {
+        pr[kb * 16 + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[kb][e], c, -m_use));
+        float rest = pr[kb * 16 + e] * kPieceScale;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          pr[kb * 16 + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[kb][e], c, -m_use));
-          float rest = pr[kb * 16 + e] * kPieceScale;
-#pragma unroll
-          for (int pc = 0; pc < PIECES; ++pc) {
-            pf[pc][kb * 2 + (e >> 3)][e & 7] = (T)rest;
-            if (pc + 1 < PIECES) rest -= to_f32<T>(pf[pc][kb * 2 + (e >> 3)][e & 7]);
-          }
+        for (int pc = 0; pc < PIECES; ++pc) {
+          pf[pc][kb * 2 + (e >> 3)][e & 7] = (T)rest;
+          if (pc + 1 < PIECES) rest -= to_f32<T>(pf[pc][kb * 2 + (e >> 3)][e & 7]);
         }
+      }
 #pragma unroll
-      for (int w = 16; w >= 1; w >>= 1)
+    for (int w = 16; w >= 1; w >>= 1)
 #pragma unroll
-        for (int e = 0; e < w; ++e) pr[e] += pr[e + w];
-      l_run += pr[0];
-    }
+      for (int e = 0; e < w; ++e) pr[e] += pr[e + w];
+    l_run += pr[0];
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt) {
       frag vf[4];
 #pragma unroll
       for (int s = 0; s < 4; ++s)
-        vf[s] = read_tr_frag<frag>(sb + s * 16 * L::KROW + v_raddr[dt], sb + (s * 16 + 8) * L::KROW + v_raddr[dt]);
+        vf[s] = read_tr_frag<frag>(sb + s * 16 * L::KROW + (v_read0 ^ (dt << 6)), sb + (s * 16 + 8) * L::KROW + (v_read0 ^ (dt << 6)));
 #pragma unroll
       for (int s = 0; s < 4; ++s)
 #pragma unroll
         for (int pc = 0; pc < PIECES; ++pc) oacc[dt] = Mfma<T>::run(vf[s], pf[pc][s], oacc[dt]);
     }
-    if constexpr (!lean(D, PIECES)) {
-      __builtin_amdgcn_sched_group_barrier(0x100, 8, 1);
+    __builtin_amdgcn_sched_group_barrier(0x100, 8, 1);
 #pragma unroll
-      for (int j = 0; j < D / 32 - 1; ++j) {
+    for (int j = 0; j < D / 32 - 1; ++j) {
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          __builtin_amdgcn_sched_group_barrier(0x008, PIECES, 1);
-          __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
-        }
+      for (int s = 0; s < 4; ++s) {
+        __builtin_amdgcn_sched_group_barrier(0x008, PIECES, 1);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
       }
-      __builtin_amdgcn_sched_group_barrier(0x008, 4 * PIECES, 1);
     }
+    __builtin_amdgcn_sched_group_barrier(0x008, 4 * PIECES, 1);
   };
 
   // ---- the second time over the tiles.  Values that are not finite are taken out of this wave's rows of a
@@ -603,7 +598,7 @@ __global__ __launch_bounds__(NTHREADS, lean(D, PIECES) ? 4 : 2) void paged_chunk
       }
       *(u16x8*)(v + l * 1024) = x;
     }
-    if (__ballot(found) != 0 && lane == 0) atomicOr(&marks[i >> 5], 1u << (i & 31));
+    if (__ballot(found) != 0 && lane == 0) atomicOr(&sh.marks[i >> 5], 1u << (i & 31));
     wait_lgkmcnt0();  // before the barrier that hands the tile to the other waves
   };
   // ... and a marked tile, V as it is, counts per feature the visible keys with +inf or NaN, then those with
@@ -635,8 +630,8 @@ __global__ __launch_bounds__(NTHREADS, lean(D, PIECES) ? 4 : 2) void paged_chunk
         f32x16 count = {};
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-          const u16x8 x = __builtin_bit_cast(u16x8, read_tr_frag<frag>(sb + s * 16 * L::KROW + v_raddr[dt],
-                                                                       sb + (s * 16 + 8) * L::KROW + v_raddr[dt]));
+          const u16x8 x = __builtin_bit_cast(u16x8, read_tr_frag<frag>(sb + s * 16 * L::KROW + (v_read0 ^ (dt << 6)),
+                                                                       sb + (s * 16 + 8) * L::KROW + (v_read0 ^ (dt << 6))));
           u16x8 one, any;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
@@ -658,54 +653,71 @@ __global__ __launch_bounds__(NTHREADS, lean(D, PIECES) ? 4 : 2) void paged_chunk
 
   // ---- the passes over this run's tiles: the pages' indices (and the list of the tiles needed), then the
   // stream
-  auto stream = [&](bool careful) {
+  int64_t max_wg = 0;
+  bool any_wg = !POS;
+  auto stream = [&]() {
     for (int base = t_first; base < t_last; base += PASS) {
+      if (POS || base != t_first) fetch_pass(base, t_last, regs);
       const int span = min(PASS, t_last - base);
       int nt = span;
-      pg0 = page_of(base * BN);
-      const int npg = page_of(min((base + span) * BN, n) - 1) - pg0 + 1;
       bool lost = false;
-      for (int i = tid; i < npg; i += NTHREADS) {
-        const int64_t id = p.tables[b * p.ts_b + (int64_t)(pg0 + i) * p.ts_w];
-        const bool ok = (uint64_t)id < (uint64_t)p.P;
-        ids[i] = ok ? (int)id : -1;
+#pragma unroll
+      for (int i = 0; i < kIdsPer; ++i) {
+        const bool ok = (uint64_t)regs.id[i] < (uint64_t)p.P;
+        sh.ids[i * NTHREADS + tid] = ok ? (int)regs.id[i] : -1;
         lost = lost || !ok;
       }
-      if (careful && tid < PASS / 32) marks[tid] = 0;
+      const bool lost_w = __ballot(lost) != 0;
+      if (lane == 0) sh.lost[wave] = lost_w ? 1 : 0;
+      if (AGAIN && tid < PASS / 32) sh.marks[tid] = 0;
+      __syncthreads();
+      if (base == t_first) {
+        max_wg = sh.red_max[0];
+#pragma unroll
+        for (int w = 1; w < NWAVES; ++w) max_wg = max(max_wg, sh.red_max[w]);
+        if constexpr (POS)
+#pragma unroll
+          for (int w = 0; w < NWAVES; ++w) any_wg = any_wg || sh.red_act[w] != 0;
+        if (!any_wg) t_last = t_first;
+        if (!POS) t_last = scalar(min(t_last, ((int)max_wg + BN - 1) / BN));
+        if (t_first >= t_last) break;
+        nt = min(nt, t_last - base);
+      }
       if constexpr (POS) {
-        const TileInfo* tinfo = c_.tiles + (int64_t)b * c_.ntiles;
         bool need = false;
         int modes = 0;
         if (tid < span) {
-          const TileInfo ti = tinfo[base + tid];
+          const TileInfo ti = regs.ti;
           need = ti.n_valid > 0 && !(p.causal && max_wg < ti.min_valid);
 #pragma unroll
           for (int w = 0; w < NWAVES; ++w) {
             int m;
-            if (!red_act[w] || ti.n_valid == 0 || (p.causal && red_max[w] < ti.min_valid)) m = 0;
-            else if (ti.n_valid == BN && (!p.causal || ti.max_valid <= red_min[w])) m = 1;
+            if (!sh.red_act[w] || ti.n_valid == 0 || (p.causal && sh.red_max[w] < ti.min_valid)) m = 0;
+            else if (ti.n_valid == BN && (!p.causal || ti.max_valid <= sh.red_min[w])) m = 1;
             else m = ti.pad[0] ? 3 : 2;
             modes |= m << (2 * w);
           }
         }
         const uint64_t bal = __ballot(need);
-        if (lane == 0) wave_cnt[wave] = __builtin_popcountll(bal);
+        if (lane == 0) sh.wave_cnt[wave] = __builtin_popcountll(bal);
         __syncthreads();
         int off = 0;
-        for (int w = 0; w < wave; ++w) off += wave_cnt[w];
+        for (int w = 0; w < wave; ++w) off += sh.wave_cnt[w];
         nt = 0;
-        for (int w = 0; w < NWAVES; ++w) nt += wave_cnt[w];
+        for (int w = 0; w < NWAVES; ++w) nt += sh.wave_cnt[w];
         if (need)
-          tile_list[off + __builtin_amdgcn_mbcnt_hi((uint32_t)(bal >> 32),
-                                                    __builtin_amdgcn_mbcnt_lo((uint32_t)bal, 0))] =
+          sh.tile_list[off + __builtin_amdgcn_mbcnt_hi((uint32_t)(bal >> 32),
+                                                       __builtin_amdgcn_mbcnt_lo((uint32_t)bal, 0))] =
               make_int2(base + tid, modes);
         nt = scalar(nt);
-      } else if (__ballot(lost) != 0 && lane == 0) {
-        flags[0] = 1;
+        __syncthreads();
       }
-      __syncthreads();
-      const bool bad = !POS && scalar(flags[0]) != 0;
-      auto tile_of = [&](int i) -> int { return POS ? scalar(tile_list[i].x) : base + i; };
+      int lost_any = 0;
+      if constexpr (!POS)
+#pragma unroll
+        for (int w = 0; w < NWAVES; ++w) lost_any |= sh.lost[w];
+      const bool bad = !POS && scalar(lost_any) != 0;
+      auto tile_of = [&](int i) -> int { return POS ? scalar(sh.tile_list[i].x) : base + i; };
       auto mode_of = [&](int tile, int e) -> int {
         int m;
         if constexpr (POS) m = scalar((e >> (2 * wave)) & 3);
@@ -721,11 +733,11 @@ __global__ __launch_bounds__(NTHREADS, lean(D, PIECES) ? 4 : 2) void paged_chunk
       if (issued < nt) t_load = tile_of(issued), id_load = scalar(id_of(t_load));
       int t_cur = base, e_cur = 0;
       if constexpr (POS)
-        if (nt > 0) t_cur = tile_of(0), e_cur = tile_list[0].y;
+        if (nt > 0) t_cur = tile_of(0), e_cur = sh.tile_list[0].y;
       for (int i = 0; i < nt; ++i) {
         if (POS && wave == 0) wait_tiles_ahead<L::LPT + 1>(issued - i - 1);
         else wait_tiles_ahead<L::LPT>(issued - i - 1);
-        if (careful) clean_share((int)((unsigned)i % NSTAGE), i);
+        if constexpr (AGAIN) clean_share((int)((unsigned)i % NSTAGE), i);
         barrier_no_fence();  // tile i landed for every wave; the stage of tile i-1 is free
         if (issued < nt) {
           load_tile(t_load, id_load, (int)((unsigned)issued % NSTAGE));
@@ -734,8 +746,8 @@ __global__ __launch_bounds__(NTHREADS, lean(D, PIECES) ? 4 : 2) void paged_chunk
         int2 e_nxt = make_int2(t_cur + 1, 0);
         int l_nxt = t_load, id_nxt = 0;
         if constexpr (POS) {
-          e_nxt = tile_list[i + 1 < nt ? i + 1 : i];
-          l_nxt = tile_list[issued < nt ? issued : 0].x;
+          e_nxt = sh.tile_list[i + 1 < nt ? i + 1 : i];
+          l_nxt = sh.tile_list[issued < nt ? issued : 0].x;
           id_nxt = id_of(scalar(l_nxt));
         } else {
           l_nxt = issued < nt ? base + issued : t_load;
@@ -749,39 +761,45 @@ __global__ __launch_bounds__(NTHREADS, lean(D, PIECES) ? 4 : 2) void paged_chunk
         id_load = scalar(id_nxt);
       }
       __syncthreads();  // the next pass rewrites the lists and the stages
-      if (!careful) continue;
+      if constexpr (!AGAIN) continue;
       for (int i = 0; i < nt; ++i) {
-        if (!((scalar(marks[i >> 5]) >> (i & 31)) & 1)) continue;
+        if (!((scalar(sh.marks[i >> 5]) >> (i & 31)) & 1)) continue;
         const int tile = tile_of(i);
         load_tile(tile, scalar(id_of(tile)), 0);
         wait_vmcnt<0>();
         __syncthreads();
-        const int mode = mode_of(tile, POS ? tile_list[i].y : 0);
+        const int mode = mode_of(tile, POS ? sh.tile_list[i].y : 0);
         if (mode != 0) mark(0, tile * BN, mode);
         __syncthreads();
       }
     }
   };
 
-  clear();
-  bool careful = false;
-  while (true) {
-    stream(careful);
-    if (careful) break;
+  if (scale < 0.f) {  // the sign goes into the queries
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks)
+      qraw[ks].x ^= 0x80008000u, qraw[ks].y ^= 0x80008000u, qraw[ks].z ^= 0x80008000u, qraw[ks].w ^= 0x80008000u;
+  }
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks) __builtin_memcpy(&qf[ks], &qraw[ks], 16);
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) oacc[i][e] = 0.f;
+  stream();
+  if constexpr (!AGAIN) {
     uint32_t worst = 0;
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
       for (int e = 0; e < 16; ++e) worst = max(worst, __float_as_uint(oacc[dt][e]) & 0x7fffffffu);
-    if (__ballot(sees && worst >= 0x7f800000u) != 0 && lane == 0) flags[1] = 1;
+    if (__ballot(sees && worst >= 0x7f800000u) != 0 && lane == 0) sh.odd_result = 1;
     __syncthreads();
-    if (flags[1] == 0) break;
-    careful = true;
-    clear();
+    if (sh.odd_result != 0) return true;
   }
 
   // ---- epilogue.  A row's sum is 0 exactly where it saw no key (a NaN is kept).
-  if (!row_ok) return;
+  if (!row_ok) return false;
   const float l_tot = sum_halves(l_run);
   uint32_t l_bits = __float_as_uint(l_tot);
   asm volatile("" : "+v"(l_bits));  // (compared as a float, a NaN might be taken for 0 in this file)
@@ -812,7 +830,25 @@ __global__ __launch_bounds__(NTHREADS, lean(D, PIECES) ? 4 : 2) void paged_chunk
         *(uint2*)((T*)p.out + at) = raw;
       }
     }
+  return false;
 }
+
+// The second time over the tiles is a function of its own, so its registers are not those of the first.
+typedef const void __attribute__((address_space(4))) * kernel_args_ptr;
+typedef __attribute__((address_space(3))) char* lds_ptr;
+template <typename T, int D, bool POS, int PIECES>
+__device__ __noinline__ void chunk_again(kernel_args_ptr args, lds_ptr smem, lds_ptr sh) {
+  chunk_body<T, D, POS, PIECES, true>(*(const ChunkParams*)args, (char*)smem, *(Shared<POS>*)(char*)sh);
+}
+
+template <typename T, int D, bool POS, int PIECES>
+__global__ __launch_bounds__(NTHREADS, 2) void paged_chunk_kernel(const ChunkParams c_) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ Shared<POS> sh;
+  if (chunk_body<T, D, POS, PIECES, false>(c_, smem, sh))
+    chunk_again<T, D, POS, PIECES>((kernel_args_ptr)__builtin_amdgcn_kernarg_segment_ptr(), (lds_ptr)smem, (lds_ptr)(char*)&sh);
+}
+
 
 // Joins a row's key splits by their log-sum-exp, four features a thread; every read is under way before
 // the first weight is known.
