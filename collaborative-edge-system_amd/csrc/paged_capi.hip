@@ -3,8 +3,8 @@
 #include <string.h>
 
 #include <algorithm>
+#include <memory>
 #include <new>
-#include <unordered_set>
 
 #include "paged.hpp"
 
@@ -253,23 +253,18 @@ int cea_copy_pages(int32_t n, const cea_tensor* pools, const int64_t* src, const
                   "%s: pages overlap", what);
   }
   const int64_t P = pools[0].size[1];
-  try {
-    std::unordered_set<int64_t> written;
-    written.reserve((size_t)moves);
-    for (int64_t i = 0; i < moves; ++i) {
-      CEA_REQUIRE(src[i] >= 0 && src[i] < P && dst[i] >= 0 && dst[i] < P, CEA_EINVAL,
-                  "%s: move %lld (%lld to %lld) leaves the %lld pages", what, (long long)i,
-                  (long long)src[i], (long long)dst[i], (long long)P);
-      CEA_REQUIRE(written.insert(dst[i]).second, CEA_EINVAL, "%s: page %lld is written twice", what,
-                  (long long)dst[i]);
-    }
-    for (int64_t i = 0; i < moves; ++i)
-      CEA_REQUIRE(!written.count(src[i]), CEA_EINVAL, "%s: page %lld is both read and written", what,
-                  (long long)src[i]);
-  } catch (const std::bad_alloc&) {
-    set_error("%s: out of host memory", what);
-    return CEA_ELAUNCH;
+  for (int64_t i = 0; i < moves; ++i)
+    CEA_REQUIRE(src[i] >= 0 && src[i] < P && dst[i] >= 0 && dst[i] < P, CEA_EINVAL,
+                "%s: move %lld (%lld to %lld) leaves the %lld pages", what, (long long)i, (long long)src[i],
+                (long long)dst[i], (long long)P);
+  std::unique_ptr<bool[]> written(new (std::nothrow) bool[(size_t)std::max<int64_t>(P, 1)]());
+  CEA_REQUIRE(written != nullptr, CEA_ELAUNCH, "%s: out of host memory", what);
+  for (int64_t i = 0; i < moves; ++i) {
+    CEA_REQUIRE(!written[dst[i]], CEA_EINVAL, "%s: page %lld is written twice", what, (long long)dst[i]);
+    written[dst[i]] = true;
   }
+  for (int64_t i = 0; i < moves; ++i)
+    CEA_REQUIRE(!written[src[i]], CEA_EINVAL, "%s: page %lld is both read and written", what, (long long)src[i]);
   if (moves == 0) return CEA_OK;
   return launch_copy_pages(n, pools, src, dst, moves, (hipStream_t)stream);
 }
