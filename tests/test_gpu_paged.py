@@ -193,6 +193,29 @@ def test_hidden_keys_hold_anything(cea, dev, bad, n, D):
         P.check(c, ref, torch.where(hit, ref.out.to(out.dtype), out), got[1] if with_lse else None)
 
 
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("n,D", [(1, 64), (3, 128), (20, 64), (20, 128)])
+def test_hidden_keys_of_long_rows_hold_anything(cea, dev, bad, n, D):
+    """The same where a row is cut into parts and splits: only the parts that hold such a value differ."""
+    c = P.make(B=2, n=n, Hq=4, Hkv=1, D=D, page=64, lengths=(5003, 1100), explicit=True, stale=bad, seed=22)
+    for b, js in ((0, (7, 2500, 5001)), (1, (64,))):
+        for j in js:
+            p, i = int(c.tables[b, j // 64]), j % 64
+            c.pos_pages[p, i] = -1
+            c.k_pages[p, :, i], c.v_pages[p, :, i] = bad, bad
+    _check(cea, dev, c)
+    c = P.make(B=2, n=n, Hq=4, Hkv=1, D=D, page=64, lengths=(5003, 1100), stale=bad, seed=23)
+    p, i = int(c.tables[0, 5002 // 64]), 5002 % 64  # the last token, which only the last query sees
+    ref = P.reference(c)
+    c.v_pages[p, 0, i, 9] = bad
+    out, lse = P.call(cea, P.to(c, dev), True)
+    out = out.cpu()
+    hit = torch.zeros_like(out, dtype=torch.bool)
+    hit[0, n - 1, :, 9] = True
+    assert bool((out[hit].isnan() if math.isnan(bad) else out[hit] == bad).all())
+    P.check(c, ref, torch.where(hit, ref.out.float(), out), lse, pieces_left=2.0 ** -23)
+
+
 def test_values_of_probability_zero(cea, dev):
     """A visible key whose probability underflows to 0 still meets its infinite value: 0 * inf."""
     for n in (1, 40):
@@ -290,6 +313,64 @@ def test_a_row_of_a_wide_table(cea, dev):
 def test_many_rows(cea, dev):
     c = P.make(B=150, n=1, Hq=4, Hkv=2, D=64, page=16, lengths=[(7 * b) % 90 for b in range(150)], seed=15)
     _check(cea, dev, c)
+
+
+@pytest.mark.parametrize("explicit", [False, True])
+@pytest.mark.parametrize("Hq,Hkv,D,page", [(4, 1, 64, 16), (2, 2, 128, 48)])
+def test_long_rows(cea, dev, explicit, Hq, Hkv, D, page):
+    """Tens of thousands of keys: a unit cut into hundreds of parts, a chunk in several passes."""
+    for n in (1, 3, 35):
+        _check(cea, dev, P.make(B=1, n=n, Hq=Hq, Hkv=Hkv, D=D, page=page, lengths=(41003,), explicit=explicit, seed=n))
+
+
+def test_long_rows_f32(cea, dev):
+    for n in (1, 20):
+        for explicit in (False, True):
+            _check(cea, dev, P.make(B=2, n=n, Hq=4, Hkv=2, D=64, page=16, lengths=(9001, 300), dtype=F32,
+                                    explicit=explicit, seed=n))
+
+
+@pytest.mark.parametrize("n", [1, 2, 20])
+@pytest.mark.parametrize("explicit", [False, True])
+def test_more_rows_than_lanes(cea, dev, n, explicit):
+    """More than 64 rows, of lengths from none to long, behind a wide table: runs over many rows, rows cut
+    between workgroups and rows that are not."""
+    lengths = [0 if b % 7 == 3 else n + (37 * b) % 61 + (1500 if b % 50 == 9 else 0) for b in range(135)]
+    _check(cea, dev, P.make(B=135, n=n, Hq=4, Hkv=2, D=64, page=16, lengths=lengths, width=130, explicit=explicit,
+                            seed=18))
+
+
+@pytest.mark.parametrize("n", [1, 3, 40])
+def test_positions_beyond_31_bits(cea, dev, n):
+    """Positions of any size, on both sides of 2^31 and far above, in one row and one tile."""
+    c = P.make(B=2, n=n, Hq=4, Hkv=2, D=64, page=16, lengths=(n + 300, n + 40), explicit=True, seed=19)
+    base = 2 ** 31 - 200
+    c.pos_pages = torch.where(c.pos_pages >= 0, c.pos_pages + base, c.pos_pages)
+    c.q_pos += base
+    for b in range(2):
+        for j in (5, 60, 61):
+            p, i = int(c.tables[b, j // 16 if j < int(c.lengths[b]) else 0]), j % 16
+            c.pos_pages[p, i] = 2 ** 31 - 1 if j == 5 else 2 ** 62 + j
+    c.q_pos[0, -1] = 2 ** 62 + 60
+    _check(cea, dev, c)
+    c.causal = False
+    _check(cea, dev, c)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("n", [1, 60])
+def test_large_scores(cea, dev, dtype, n):
+    """Scores of hundreds: one key takes nearly everything, and the running maximum moves often."""
+    _check(cea, dev, P.make(B=2, n=n, Hq=4, Hkv=2, D=64, page=16, lengths=(n + 400, n + 30), dtype=dtype,
+                            q_scale=30.0, seed=20))
+
+
+def test_same_page_in_two_rows(cea, dev):
+    """Rows that share a prefix name the same pages."""
+    for n in (1, 50):
+        c = P.make(B=3, n=n, Hq=4, Hkv=2, D=64, page=16, lengths=(n + 200, n + 180, n + 64), seed=21)
+        c.tables[1, :4], c.tables[2, :4] = c.tables[0, :4], c.tables[0, :4]
+        _check(cea, dev, c)
 
 
 def test_merges_with_another_share(cea, dev):
@@ -506,12 +587,13 @@ def test_another_stream_than_the_default(cea, dev):
             assert torch.equal(o, outs[0])
 
 
-@pytest.mark.parametrize("n", [1, 4, 40])
-def test_captured_calls_follow_their_tensors(cea, dev, n):
+@pytest.mark.parametrize("n,W,explicit", [(1, 40, False), (4, 40, True), (1, 140, False), (3, 140, True), (40, 140, False),
+                                         (40, 140, True)])
+def test_captured_calls_follow_their_tensors(cea, dev, n, W, explicit):
     """An append and an attention in one graph, replayed as the row grows: every replay equals the
     eager calls on the same contents, bit for bit; two graphs replayed in turn do not disturb each
     other."""
-    H, D, page, W = 2, 64, 16, 40
+    H, D, page = 2, 64, 16
     pages = 3 * W
     g = torch.Generator().manual_seed(n)
     kp = torch.randn(pages, H, page, D, generator=g).to(BF16).to(dev)
@@ -523,12 +605,13 @@ def test_captured_calls_follow_their_tensors(cea, dev, n):
     after = torch.zeros(3, dtype=torch.int64, device=dev)
     q_pos = torch.zeros(3, n, dtype=torch.int64, device=dev)
     steps = torch.arange(n, device=dev)
+    pp = torch.arange(page, device=dev).expand(pages, page).contiguous() if explicit else None
 
     def step():
         after.copy_(lengths + n)
         q_pos.copy_(lengths.view(3, 1) + steps)
-        cea.paged_kv_append(kp, vp, tables, lengths, k, v)
-        return cea.paged_attention(q, kp, vp, tables, after, q_pos)
+        cea.paged_kv_append(kp, vp, tables, lengths, k, v, pos_pages=pp, pos=q_pos if explicit else None)
+        return cea.paged_attention(q, kp, vp, tables, after, q_pos, pos_pages=pp)
 
     side = torch.cuda.Stream()
     with torch.cuda.stream(side):
