@@ -373,7 +373,7 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, char* smem, Sh
 
   // ---- what the rows see: slots [0, lim) of this lane's row by their number (POS: positions to qpos)
   const bool sees = row_ok && (!p.causal || qpos >= 0);
-  const int lim = !sees ? 0 : p.causal && !POS ? (int)min(qpos + 1, (int64_t)n) : n;
+  const int lim = !sees ? 0 : p.causal && !POS && qpos < n ? (int)qpos + 1 : n;
   int lim_min = 0, lim_max = 0;  // of the wave's rows that see anything
   if constexpr (POS) {
     const int64_t mn = wave_min_i64(sees ? qpos : INT64_MAX), mx = wave_max_i64(sees ? qpos : INT64_MIN);
@@ -468,7 +468,7 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, char* smem, Sh
       __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }
     __builtin_amdgcn_sched_group_barrier(0x008, D / 16, 0);
-    
+
     if (mode == 1) return;
     if (mode == 2) {
       if constexpr (POS) {
@@ -965,7 +965,10 @@ bool paged_chunk_supported(const PagedParams& p, const HeadMap& map) {
   for (int64_t s : {p.os_b, p.os_s, p.os_h})
     if (s % 4) return false;
   if ((uintptr_t)p.out % 16 || (p.pos && (uintptr_t)p.pos % 8)) return false;
-  return p.B < 65536 && (int64_t)p.B * p.Hq * ((p.Sq + 31) / 32) * kMaxKeySplits < ((int64_t)1 << 31);
+  // (all rows' tiles, and all workgroups, are counted in 32 bits)
+  const int64_t tiles = ((int64_t)p.W * p.page + BN - 1) / BN;
+  return p.B < 65536 && p.B * tiles < ((int64_t)1 << 31) &&
+         (int64_t)p.B * p.Hq * ((p.Sq + 31) / 32) * kMaxKeySplits < ((int64_t)1 << 31);
 }
 
 int launch_paged_chunk(const PagedParams& params, const HeadMap& map, void* ws, hipStream_t st) {

@@ -105,7 +105,7 @@ __global__ __launch_bounds__(NW * 64) void paged_f32_kernel(const F32Params t) {
   const int n = uniform((int)paged_slots(p, b));
   // this lane's row sees slots [0, lim) (POS: of those, the positions up to qpos)
   const bool sees = row_ok && (!p.causal || qpos >= 0);
-  const int lim = !sees ? 0 : p.causal && !POS ? (int)min(qpos + 1, (int64_t)n) : n;
+  const int lim = !sees ? 0 : p.causal && !POS && qpos < n ? (int)qpos + 1 : n;
   int lim_max = lim;
 #pragma unroll
   for (int off = 8; off >= 1; off >>= 1) lim_max = max(lim_max, __shfl_xor(lim_max, off, 64));

@@ -296,7 +296,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void paged_token_kernel(c
     int lim = n, lim_all = n, lim_any = n;
     if (POS && p.causal && __ballot(row_real && qpos >= 0) == 0) lim_any = 0;
     if (!POS && p.causal) {
-      lim = (int)max((int64_t)0, min(qpos + 1, (int64_t)n));
+      lim = qpos >= n ? n : (int)max((int64_t)0, qpos + 1);
       lim_all = row_real ? lim : n;
       lim_any = row_real ? lim : 0;
       if (p.Sq > 1) {

@@ -262,8 +262,11 @@ class PagedKVCache:
             cache.append(layer, step, k, v, cos=cos, sin=sin)
             out = cache.attention(layer, step, q, q_pos)
 
-    A step made before :meth:`free`, :meth:`truncate` or :meth:`compact` is refused after it: its
-    pages may be another's.  Everything runs on the current stream.
+    A step made before :meth:`fork`, :meth:`free`, :meth:`truncate` or :meth:`compact` is refused
+    after it: its pages may be another's (a fork shares tokens, so they are written before it).
+    Everything runs on the current stream.  A captured graph holds appends and attention; ``extend``
+    and ``compact`` come between its replays, and are refused in a capture, which would not run them.
+    One thread at a time calls a cache.
     """
 
     def __init__(self, layers: int, pages: int, page: int, heads: int, head_dim: int, *,
@@ -292,7 +295,9 @@ class PagedKVCache:
     def fork(self, seq: int) -> int:
         """A new sequence that shares the tokens of ``seq``; the page that both would write next is
         copied when one of them is extended."""
-        return self.book.fork(seq)
+        child = self.book.fork(seq)
+        self._epoch += 1
+        return child
 
     def free(self, seq: int) -> None:
         """Ends a sequence and gives its pages back."""
@@ -313,8 +318,13 @@ class PagedKVCache:
             pools.append(self.pos_pages.unsqueeze(0))
         copy_pages(pools, src, dst, dim=1)
 
+    def _outside_capture(self, what: str) -> None:
+        if self.kv.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"{what} belongs before a graph's replay, not into its capture")
+
     def compact(self) -> int:
         """Moves the held pages to the lowest indices; returns how many moved."""
+        self._outside_capture("compact")
         moves = self.book.compact()
         self._copy(moves)
         self._epoch += 1
@@ -325,6 +335,7 @@ class PagedKVCache:
         """Room for ``counts[i]`` new tokens of ``seqs[i]`` (0: the sequence is only read) and the
         step's tensors.  With ``into`` a step of the same number of rows is filled in place, its
         width allowing, for a captured graph that reads it."""
+        self._outside_capture("extend")
         seqs = list(seqs)
         counts = [int(counts)] * len(seqs) if isinstance(counts, int) else [int(n) for n in counts]
         if into is not None:
@@ -353,7 +364,7 @@ class PagedKVCache:
 
     def _check(self, step: PagedStep) -> None:
         if step.epoch != self._epoch:
-            raise RuntimeError("the step is older than the last free, truncate or compact")
+            raise RuntimeError("the step is older than the last fork, free, truncate or compact")
 
     def append(self, layer: int, step: PagedStep, k: torch.Tensor, v: torch.Tensor, *,
                cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,

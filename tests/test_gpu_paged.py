@@ -357,6 +357,18 @@ def test_positions_beyond_31_bits(cea, dev, n):
     _check(cea, dev, c)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32, F64])
+@pytest.mark.parametrize("explicit", [False, True])
+@pytest.mark.parametrize("n", [1, 3, 40])
+def test_the_largest_query_position(cea, dev, dtype, explicit, n):
+    """A query at the largest 64-bit position sees every key under the causal rule."""
+    c = P.make(B=2, n=n, Hq=4, Hkv=2, D=64, page=16, lengths=(n + 300, n + 5), dtype=dtype, explicit=explicit, seed=24)
+    c.q_pos[0, 0] = c.q_pos[1, -1] = torch.iinfo(torch.int64).max
+    if explicit:
+        c.pos_pages[int(c.tables[0, 3]), 5] = torch.iinfo(torch.int64).max
+    _check(cea, dev, c)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("n", [1, 60])
 def test_large_scores(cea, dev, dtype, n):
@@ -635,6 +647,29 @@ def test_captured_calls_follow_their_tensors(cea, dev, n, W, explicit):
         assert torch.equal(out, want) and torch.equal(kp, kept)
         lengths += n
         torch.randn(1 << 16, device=dev).sum().item()
+
+
+def test_pages_are_not_handed_out_in_a_capture(cea, dev):
+    cache = cea.PagedKVCache(1, 6, 16, 2, 64, device=dev)
+    a = cache.new()
+    step = cache.extend([a], 5)
+    q = torch.randn(1, 1, 2, 64, device=dev, dtype=BF16)
+    pos = torch.tensor([[4]], device=dev)
+    kv = torch.randn(1, 5, 2, 64, device=dev, dtype=BF16)
+    cache.append(0, step, kv, kv)
+    want = cache.attention(0, step, q, pos)
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=stream):
+        with pytest.raises(RuntimeError, match="capture"):
+            cache.extend([a], 1)
+        with pytest.raises(RuntimeError, match="capture"):
+            cache.compact()
+        out = cache.attention(0, step, q, pos)
+    assert cache.length(a) == 5 and cache.free_pages == 5
+    for _ in range(3):
+        graph.replay()
+        assert torch.equal(out, want)
 
 
 @pytest.mark.parametrize("positions", [False, True])

@@ -233,3 +233,16 @@ def test_a_step_is_refused_after_its_pages_may_have_changed_hands(cea):
     with pytest.raises(ValueError, match="rows"):
         cache.extend([], [], into=again)
     assert cache.length(b) == 22
+
+
+def test_a_step_is_refused_after_a_fork(cea):
+    """Its tokens may not be written yet, and a page that the child copies would lack them."""
+    cache = cea.PagedKVCache(1, 4, 16, 2, 64, device="cpu")
+    a = cache.new()
+    step = cache.extend([a], 5)
+    child = cache.fork(a)
+    k = torch.zeros(1, 5, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="older"):
+        cache.append(0, step, k, k)
+    assert cache.length(child) == 5
+    cache._check(cache.extend([child], 0))
