@@ -211,12 +211,12 @@ int cea_paged_attention(const cea_tensor* q, const cea_tensor* k_pages, const ce
   hipStream_t st = (hipStream_t)stream;
   if (paged_tiles_supported(p)) {
     // The token form while one unit holds a KV head's queries, so its keys are read once, and for single
-    // tokens of larger groups; two units where a key is small or a unit one workgroup (us, token / chunk
-    // form, 32 query rows of a KV head: 4 rows of up to 500 keys, D = 64, 8.5 / 13.9; 16 of up to 2500, D = 64,
-    // 27.8 / 30.5; 24 and 32 query rows at D = 128: 8 rows of up to 4096 keys 49.9 / 42.0, 32 of up to 2500
-    // 118 / 72).
+    // tokens of larger groups; two units where all is one launch of small tiles (us, token / chunk form: 32
+    // query rows of a KV head, 4 rows of up to 900 keys, D = 64, 12.6 / 15.7, D = 128, 18.5 / 17.5; 16 rows of up
+    // to 2500, D = 64, 28.2 / 23.7; 16 query rows, 32 rows of up to 8000, D = 128, 154 / 170, 8 of up to 4096
+    // 31.7 / 26.3, 16 of up to 2500, D = 64, 21.0 / 22.1).
     const int64_t rows = Sq * map.group;
-    const bool few = Sq == 1 || map.group <= 0 || rows <= 16 || (rows <= 32 && (D == 64 || W * page <= 1024));
+    const bool few = Sq == 1 || map.group <= 0 || rows <= 16 || (rows <= 32 && D == 64 && W * page <= 1024);
     const bool token = few && paged_token_supported(p, map);
     if (token || paged_chunk_supported(p, map)) {
       const int64_t slots = W * page;

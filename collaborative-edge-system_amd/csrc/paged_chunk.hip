@@ -3,20 +3,28 @@
 //
 //   out = sum_j p_j v_j / sum_j p_j,  p_j = exp(s_j - m),  s_j = scale * q.k_j,  lse = m + log sum_j p_j
 //
-// Bound by the matrix cores and the LDS reads that feed them.  The tile body is the prefill kernel's: a workgroup
-// of 8 waves holds 256 query rows of one query head (or, for short chunks, of 2, 4 or 8 heads of one KV
-// head), a wave 32 of them; S^T = K.Q^T per 64-key tile with v_mfma_f32_32x32x16 (a lane holds one
-// row's scores, so its statistics are scalars), O^T += V^T.P^T from the score registers, V
-// transposed on its way out of LDS; K and V go global -> LDS directly through a ring of 4 tiles, 3 in
-// flight; exp2 domain, the reference maximum moved only when a row's grows by 2^8.  What the pages
-// change:
-//   * a wave loads 8 rows of a tile, and pages are multiples of 16 slots, so they lie in one page:
-//     its address stays scalar; the page indices of 512 tiles at a time wait in LDS (read through the
+// The tile body is the prefill kernel's: a wave holds 32 query rows of one query head; S^T = K.Q^T per
+// 64-key tile with v_mfma_f32_32x32x16 (a lane holds one row's scores, so its statistics are scalars),
+// O^T += V^T.P^T from the score registers, V transposed on its way out of LDS; K and V go global -> LDS
+// directly; exp2 domain, the reference maximum moved only when a row's grows by 2^8.  A workgroup is 4
+// waves, 128 rows of one query head (or, for short chunks, of 2 or 4 heads of one KV head), with two
+// tiles in LDS, the next one loading: two workgroups fit a compute unit at D = 128, three at D =
+// 64, and while one waits at its barrier or for its products another has its softmax to do.  (8 waves, 4
+// tiles, one workgroup a compute unit: chunks of 500 tokens over 4000 to 9000 keys, 32/8 heads of 128, 248 us
+// against 232; four chunks of 300 over 700 to 4001, 32/4 heads of 64, 63.3 against 51.2; two prompts of
+// 2000, 32/4 heads of 64, 58.4 against 53.3, of 128 85.9 and 85.9; 12 tokens of 4 rows of up to 10000 49
+// against 31; 128 tokens over 32768 keys 90.4 against 93.4, whose keys cross the L2 twice as often.)
+// Bound by the matrix cores (40 % busy over two prompts of 2000), the LDS reads that feed them and the
+// softmax's vector instructions, each near half of the time.  What the pages change:
+//   * a wave loads 16 rows of a tile, and pages are multiples of 16 slots, so they lie in one page:
+//     its address stays scalar; the page indices of 256 tiles at a time wait in LDS (read through the
 //     scalar cache, each delayed the next tile's first product);
 //   * without positions in the pool slot j is position j, so the tiles that a workgroup visits are
 //     a prefix of the row and every mask is one 32-bit comparison with the query row's limit; with
-//     them a launch before this one summarises the tiles and writes the positions in 32 bits,
-//     and the workgroup lists the tiles it needs;
+//     them a launch before this one summarises the tiles, writes the positions in 32 bits and
+//     what a score starts with, 0 or -inf where no key is, and the workgroup lists the tiles it needs; the
+//     products add to that start, so empty slots cost no comparisons (82 us to 61 with the smaller
+//     workgroups, four chunks of 300 over 700 to 4001 slots with 2 % of them empty);
 //   * lengths are known on the device alone: a launch with few query blocks has room for up to 16 key
 //     splits by the table's width, and the device gives every row as many as its tiles are worth, each
 //     an equal run of them; a second launch joins the rows that were cut;
@@ -62,22 +70,23 @@ template <typename T> struct Bits16;
 template <> struct Bits16<bf16> { static constexpr uint16_t kInf = 0x7f80, kOne = 0x3f80; };
 template <> struct Bits16<f16> { static constexpr uint16_t kInf = 0x7c00, kOne = 0x3c00; };
 
-constexpr int NWAVES = 8;
+constexpr int NWAVES = 4;
 constexpr int NTHREADS = NWAVES * 64;
 constexpr int BM = NWAVES * 32;       // query rows per workgroup
 constexpr int BN = kTileKeys;         // keys per tile
 constexpr int WROWS = BN / NWAVES;    // rows of a tile that a wave loads
-constexpr int NSTAGE = 4;             // LDS ring depth
-constexpr int PASS = 512;             // tiles of a pass: their page indices (and list) are in LDS
+constexpr int PASS = 256;             // tiles of a pass: their page indices (and list) are in LDS
+static_assert(PASS <= NTHREADS, "a thread looks at one tile of a pass");
 constexpr int32_t kHidden32 = INT32_MAX;  // no key; visible positions end below it
 constexpr float kRescaleLog2 = 8.0f;
 
 struct ChunkParams {
   PagedParams p;
   const TileInfo* tiles;     // with positions in the pool: [B, ntiles] summaries (pad[0]: some position
-  const int32_t* pos32;      // does not fit 31 bits), and [B, ntiles * 64] positions, kHidden32 where no key
+  const int32_t* pos32;      // does not fit 31 bits), and [B, ntiles, 2, 64]: positions, kHidden32 where no
+                             // key, and what a score starts with: 0, or -inf where no key
   int32_t ntiles;
-  int32_t hp;                // query heads of a workgroup: 1, 2, 4, 8
+  int32_t hp;                // query heads of a workgroup: 1, 2, 4
   int32_t splits;            // rows may be cut into key splits: at most so many splits in all (0: no)
   int32_t kv_units;          // units of query heads that share keys: KV heads (or all heads)
   float* part;               // partial results of the splits: [splits, Sq, Hq, D] and [splits, Hq, Sq]
@@ -93,12 +102,11 @@ template <int D, bool POS> struct Layout {
   static constexpr int NCG = D / 8;
   static constexpr int K_BYTES = BN * KROW;
   static constexpr int V_BYTES = BN * KROW;
-  static constexpr int STAGE_BYTES = K_BYTES + V_BYTES + (POS ? BN * 4 : 0);
-  static constexpr int LDS_BYTES = NSTAGE * STAGE_BYTES;
+  static constexpr int STAGE_BYTES = K_BYTES + V_BYTES + (POS ? BN * 8 : 0);
+  static constexpr int LDS_BYTES = 2 * STAGE_BYTES;
   static constexpr int KV_LOADS = K_BYTES / (NTHREADS * 16);
   static constexpr int ROWS_PER_LOAD = 1024 / KROW;
-  static constexpr int LPT = 2 * KV_LOADS;  // loads of one wave per tile (wave 0: and the positions)
-  static_assert(KV_LOADS * ROWS_PER_LOAD == WROWS, "a wave loads 8 rows");
+  static_assert(KV_LOADS * ROWS_PER_LOAD == WROWS && WROWS == 16, "a wave loads 16 rows, which lie in one page");
 };
 
 template <int D> __device__ __forceinline__ int k_swz(int key) {
@@ -155,19 +163,13 @@ template <typename X> __device__ __forceinline__ X scalar(X v) {
     return (X)(((uint64_t)hi << 32) | lo);
   }
 }
-template <int LPT> __device__ __forceinline__ void wait_tiles_ahead(int ahead) {
-  static_assert(NSTAGE == 4, "wait ladder written for 2 tiles ahead at most");
-  if (ahead >= 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LPT) : "memory");
-  else if (ahead == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LPT) : "memory");
-  else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-}
 
 // Key splits: row b's tiles are cut into as many equal runs as they are worth where the tiles of all rows
-// make 384 workgroups (at least 4 tiles each: a split costs its start and its part of the join),
-// whatever the rows' lengths.  The splits of all rows are one line.  (us, 256 / 384 / 512 workgroups: four
-// chunks of 300 over 700 to 4001 keys, 32/4 heads of 64, 65.9 / 63.7 / 70.3; 6 tokens of 8 rows of 100 to 4096,
-// 32/8 heads of 128, 43.4 / 41.0 / 39.9; 128 tokens over 32768 96.1 / 94.7 / 96.5)
-constexpr int kSplitWgs = 384, kSplitTiles = 4;
+// make 512 workgroups (at least 4 tiles each: a split costs its start and its part of the join),
+// whatever the rows' lengths.  The splits of all rows are one line.  (us, 384 / 512 / 640 / 768 workgroups:
+// four chunks of 300 over 700 to 4001 keys, 32/4 heads of 64, 54.6 / 52.4 / 56.7 / 56.2; 6 tokens of 8 rows of 100
+// to 4096, 32/8 heads of 128, - / 25.4 / - / 33.8; 128 tokens over 32768 - / 93.5 / - / 94.7)
+constexpr int kSplitWgs = 512, kSplitTiles = 4;
 struct Split {
   int b, split, first, count;  // a row, one of its splits, the place of its first one, how many it has
 };
@@ -231,7 +233,8 @@ __global__ __launch_bounds__(256) void paged_tile_info_kernel(const PagedParams 
     const int64_t mx = wave_max_i64(valid ? pos : INT64_MIN);
     const uint64_t some = __ballot(valid), far = __ballot(wide);
     const int64_t at = (int64_t)b * ntiles + t;
-    pos32[at * BN + lane] = valid && !wide ? (int32_t)pos : kHidden32;
+    pos32[at * (2 * BN) + lane] = valid && !wide ? (int32_t)pos : kHidden32;
+    pos32[at * (2 * BN) + BN + lane] = valid ? 0 : (int32_t)0xff800000u;
     if (lane == 0) {
       TileInfo ti;
       ti.min_valid = mn;
@@ -412,7 +415,7 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, char* smem, Sh
   const char* kh = scalar((const char*)((const T*)p.k + (int64_t)kvh * p.ks_h));
   const char* vh = scalar((const char*)((const T*)p.v + (int64_t)kvh * p.vs_h));
   const int64_t ks_p = scalar(p.ks_p * 2), vs_p = scalar(p.vs_p * 2);
-  const int32_t* pos32 = POS ? scalar(c_.pos32 + (int64_t)b * c_.ntiles * BN) : nullptr;
+  const int32_t* pos32 = POS ? scalar(c_.pos32 + (int64_t)b * c_.ntiles * (2 * BN)) : nullptr;
 
   // the page index of this wave's rows of a tile (behind the row's end: the last one's)
   auto id_of = [&](int tile) -> int { return sh.ids[page_of(min(tile * BN + wave * WROWS, n - 1)) - pg0]; };
@@ -431,8 +434,8 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, char* smem, Sh
     for (int i = 0; i < L::KV_LOADS; ++i) buffer_load_lds16_m0(vrs, st + L::K_BYTES + wave_kv + i * 1024, v_voff[i]);
     if constexpr (POS) {
       if (wave == 0) {
-        const i32x4 prs = make_rsrc(pos32 + (int64_t)tile * BN, BN * 4);
-        if (lane < BN / 4) buffer_load_lds16_m0(prs, st + L::K_BYTES + L::V_BYTES, lane * 16);
+        const i32x4 prs = make_rsrc(pos32 + (int64_t)tile * (2 * BN), BN * 8);
+        if (lane < BN / 2) buffer_load_lds16_m0(prs, st + L::K_BYTES + L::V_BYTES, lane * 16);
       }
     }
   };
@@ -447,7 +450,9 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, char* smem, Sh
   float m_run = -__builtin_inff(), m_use = -kExpShift, l_run = 0.f;
 
   // The scores of a tile.  mode: 1 every key visible to every row of the wave that sees anything, 2 masked,
-  // 3 masked and looked up: a page of the pass that is not there, or (POS) a position beyond 31 bits.
+  // 3 masked and looked up: a page of the pass that is not there, or (POS) a position beyond 31 bits.  (POS: in
+  // mode 1 slots may be empty.  Their scores are -inf plus a product, which is -inf unless the slot holds a value
+  // that is not finite; those show up in the results, and the second time over the tiles masks them.)
   const int qlim32 = !sees ? -1 : p.causal ? (int)min(qpos, (int64_t)kHidden32 - 1) : kHidden32 - 1;
   auto scores = [&](int stage, int slot0, int mode, f32x16 (&sacc)[2]) {
     const char* sb = smem + stage * L::STAGE_BYTES;
@@ -457,6 +462,14 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, char* smem, Sh
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) kf[ks] = *(const frag*)(sb + kb * 32 * L::KROW + (k_read0 ^ (ks << 5)));
       f32x16 acc = {};
+      if constexpr (POS) {  // 0, or -inf where no key
+        const char* start = sb + L::K_BYTES + L::V_BYTES + BN * 4 + (kb * 32 + g * 4) * 4;
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4) {
+          const float4 x = *(const float4*)(start + i4 * 32);
+          acc[i4 * 4 + 0] = x.x, acc[i4 * 4 + 1] = x.y, acc[i4 * 4 + 2] = x.z, acc[i4 * 4 + 3] = x.w;
+        }
+      }
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) acc = Mfma<T>::run(kf[ks], qf[ks], acc);
       sacc[kb] = acc;
@@ -693,7 +706,7 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, char* smem, Sh
           for (int w = 0; w < NWAVES; ++w) {
             int m;
             if (!sh.red_act[w] || ti.n_valid == 0 || (p.causal && sh.red_max[w] < ti.min_valid)) m = 0;
-            else if (ti.n_valid == BN && (!p.causal || ti.max_valid <= sh.red_min[w])) m = 1;
+            else if (!AGAIN && (!p.causal || ti.max_valid <= sh.red_min[w])) m = 1;
             else m = ti.pad[0] ? 3 : 2;
             modes |= m << (2 * w);
           }
@@ -725,8 +738,7 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, char* smem, Sh
         return m;
       };
       int issued = 0;
-      for (; issued < nt && issued < NSTAGE - 1; ++issued)
-        load_tile(tile_of(issued), scalar(id_of(tile_of(issued))), issued);
+      if (nt > 0) load_tile(tile_of(0), scalar(id_of(tile_of(0))), 0), issued = 1;
       // what the next step needs is read from LDS right after a barrier and used behind that step's work:
       // the tile to load next and its page, the next tile's mode
       int t_load = base, id_load = -1;
@@ -735,12 +747,11 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, char* smem, Sh
       if constexpr (POS)
         if (nt > 0) t_cur = tile_of(0), e_cur = sh.tile_list[0].y;
       for (int i = 0; i < nt; ++i) {
-        if (POS && wave == 0) wait_tiles_ahead<L::LPT + 1>(issued - i - 1);
-        else wait_tiles_ahead<L::LPT>(issued - i - 1);
-        if constexpr (AGAIN) clean_share((int)((unsigned)i % NSTAGE), i);
+        wait_vmcnt<0>();
+        if constexpr (AGAIN) clean_share(i & 1, i);
         barrier_no_fence();  // tile i landed for every wave; the stage of tile i-1 is free
         if (issued < nt) {
-          load_tile(t_load, id_load, (int)((unsigned)issued % NSTAGE));
+          load_tile(t_load, id_load, issued & 1);
           ++issued;
         }
         int2 e_nxt = make_int2(t_cur + 1, 0);
@@ -754,7 +765,7 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, char* smem, Sh
           id_nxt = id_of(l_nxt);
         }
         const int mode = mode_of(t_cur, e_cur);
-        if (mode != 0) compute((int)((unsigned)i % NSTAGE), t_cur * BN, mode);
+        if (mode != 0) compute(i & 1, t_cur * BN, mode);
         t_cur = scalar(e_nxt.x);
         e_cur = e_nxt.y;
         t_load = scalar(l_nxt);
@@ -842,7 +853,7 @@ __device__ __noinline__ void chunk_again(kernel_args_ptr args, lds_ptr smem, lds
 }
 
 template <typename T, int D, bool POS, int PIECES>
-__global__ __launch_bounds__(NTHREADS, 2) void paged_chunk_kernel(const ChunkParams c_) {
+__global__ __launch_bounds__(NTHREADS, D == 64 && PIECES == 1 ? 3 : 2) void paged_chunk_kernel(const ChunkParams c_) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ Shared<POS> sh;
   if (chunk_body<T, D, POS, PIECES, false>(c_, smem, sh))
@@ -932,6 +943,15 @@ template <typename T, int D> int launch_td(const ChunkParams& c, bool f32, hipSt
 
 size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
+// Query heads of a workgroup: the fewest padded query rows per head, the smallest number on ties.
+int heads_per_wg(int64_t Sq, int64_t group) {
+  auto padding = [&](int hp) { return (Sq + BM / hp - 1) / (BM / hp) * (BM / hp) - Sq; };
+  int best = 1;
+  for (int hp = 2; hp <= NWAVES && group > 0 && group % hp == 0; hp *= 2)
+    if (padding(hp) < padding(best)) best = hp;
+  return best;
+}
+
 struct ChunkPlan {
   int hp, splits;
   size_t tiles, pos32, part_out, part_lse;  // bytes: summaries, positions, the splits' partial results
@@ -939,15 +959,15 @@ struct ChunkPlan {
 
 ChunkPlan plan_chunk(int64_t B, int64_t Sq, int64_t Hq, int group, int64_t D, int64_t slots, bool pos) {
   ChunkPlan r;
-  r.hp = prefill_heads_per_wg(Sq, group);
-  // Below a workgroup per compute unit the rows may be cut; their splits are at most the workgroups that the
+  r.hp = heads_per_wg(Sq, group);
+  // Below two workgroups per compute unit the rows may be cut; their splits are at most the workgroups that the
   // tiles are dealt to, over those of a row's split, and one a row more for what does not divide.
   const int64_t per_row = (Sq + BM / r.hp - 1) / (BM / r.hp) * (Hq / r.hp), tiles = (slots + BN - 1) / BN;
   r.splits = 0;
-  if (per_row * B < 256 && tiles >= 2 * kSplitTiles)
+  if (per_row * B < kSplitWgs && tiles >= 2 * kSplitTiles)
     r.splits = (int)std::min<int64_t>(B * kMaxKeySplits, kSplitWgs / per_row + 1 + B);
   r.tiles = pos ? align256((size_t)B * ((slots + BN - 1) / BN) * sizeof(TileInfo)) : 0;
-  r.pos32 = pos ? align256((size_t)B * ((slots + BN - 1) / BN) * BN * sizeof(int32_t)) : 0;
+  r.pos32 = pos ? align256((size_t)B * ((slots + BN - 1) / BN) * 2 * BN * sizeof(int32_t)) : 0;
   r.part_out = align256((size_t)r.splits * Sq * Hq * D * sizeof(float));
   r.part_lse = align256((size_t)r.splits * Sq * Hq * sizeof(float));
   return r;
