@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import math
+import random
 
 import pytest
 import torch
@@ -752,3 +753,28 @@ def test_a_life_of_the_cache(cea, dev, positions):
     moved = cache.compact()
     assert moved > 0 and cache.free_pages == 64 - len({p for s in (a, d, e) for p in cache.book.table(s)})
     step([a, d, e], [1, 30, 2])
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_random_calls(cea, dev, seed):
+    """Types, heads, page sizes, lengths, masks, layouts and bad pages drawn together."""
+    rng = random.Random(1000 + seed)
+    dtype = rng.choice([BF16, BF16, F16, F16, F32, F64])
+    D = rng.choice([64, 64, 128, 128, 40])
+    page = rng.choice([16, 32, 48, 64, 128, 20])
+    Hkv, g = rng.choice([1, 2, 3]), rng.choice([1, 2, 3, 4, 8])
+    Hq = Hkv * g
+    n = rng.choice([1, 1, 2, 3, 5, 9, 17, 33, 65, 130, 200])
+    B = rng.choice([1, 2, 3, 5])
+    while B > 1 and B * n * Hq > 1600:
+        B -= 1
+    lengths = [rng.choice([0, n, n + rng.randint(0, 70), n + rng.randint(0, 700), rng.randint(0, 1500)]) for _ in range(B)]
+    kv_map = [rng.randrange(Hkv) for _ in range(Hq)] if rng.random() < 0.2 else None
+    c = P.make(B=B, n=n, Hq=Hq, Hkv=Hkv, D=D, page=page, lengths=lengths, dtype=dtype, explicit=rng.random() < 0.5,
+               causal=rng.random() < 0.8, scale=rng.choice([None, None, 0.5, -0.2]), kv_map=kv_map, seed=seed,
+               layout=rng.choice(["hnd", "nhd"]), stale=rng.choice([None, math.nan, math.inf]),
+               width=max([-(-x // page) for x in lengths] + [1]) + rng.choice([0, 0, 1, 30]),
+               pad_rows=[(rng.randrange(B), rng.randrange(n)) for _ in range(rng.choice([0, 0, 2]))])
+    if rng.random() < 0.3:
+        c.tables[rng.randrange(B), rng.randrange(c.W)] = rng.choice([-1, c.P, 2 ** 40])
+    _check(cea, dev, c)
