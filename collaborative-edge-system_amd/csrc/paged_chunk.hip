@@ -749,6 +749,7 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, char* smem, Sh
       for (int i = 0; i < nt; ++i) {
         wait_vmcnt<0>();
         if constexpr (AGAIN) clean_share(i & 1, i);
+        wait_lgkmcnt0();     // tile i-1 is in registers, wherever the compiler puts the products
         barrier_no_fence();  // tile i landed for every wave; the stage of tile i-1 is free
         if (issued < nt) {
           load_tile(t_load, id_load, issued & 1);
