@@ -247,7 +247,7 @@ class PagedStep:
         self.buffer = torch.empty(rows * (width + 3), dtype=torch.int64, device=device)
         self.tables = self.buffer[3 * rows:].view(rows, width)
         self.offsets, self.counts, self.lengths = self.buffer[:3 * rows].view(3, rows)
-        self.epoch = -1
+        self.cache, self.epoch = None, -1
 
 
 class PagedKVCache:
@@ -359,10 +359,12 @@ class PagedKVCache:
             host += t + [-1] * (width - len(t))
         staged = torch.tensor(host, dtype=torch.int64, pin_memory=self.kv.is_cuda)
         step.buffer.copy_(staged, non_blocking=True)
-        step.epoch = self._epoch
+        step.cache, step.epoch = self, self._epoch
         return step
 
     def _check(self, step: PagedStep) -> None:
+        if step.cache is not self:
+            raise RuntimeError("the step is not this cache's")
         if step.epoch != self._epoch:
             raise RuntimeError("the step is older than the last fork, free, truncate or compact")
 

@@ -246,3 +246,17 @@ def test_a_step_is_refused_after_a_fork(cea):
         cache.append(0, step, k, k)
     assert cache.length(child) == 5
     cache._check(cache.extend([child], 0))
+
+
+def test_a_step_of_another_cache_is_refused(cea):
+    one, two = (cea.PagedKVCache(1, 4, 16, 2, 64, device="cpu") for _ in range(2))
+    a, b = one.new(), two.new()
+    step, other = one.extend([a], 5), two.extend([b], 3)
+    q = torch.zeros(1, 1, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="this cache"):
+        two.attention(0, step, q, torch.zeros(1, 1, dtype=torch.int64))
+    two.extend([b], 1, into=step)  # filled anew, it is the other one's
+    two._check(step)
+    two._check(other)
+    with pytest.raises(RuntimeError, match="this cache"):
+        one._check(step)
