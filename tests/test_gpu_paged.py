@@ -650,6 +650,31 @@ def test_captured_calls_follow_their_tensors(cea, dev, n, W, explicit):
         torch.randn(1 << 16, device=dev).sum().item()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("n", [1, 40])
+def test_two_graphs_replayed_at_once(cea, dev, dtype, n):
+    """Calls that cut their rows, captured twice and replayed on two streams together, share no scratch."""
+    cases = [P.to(P.make(B=2, n=n, Hq=4, Hkv=1, D=64, page=16, lengths=(2500, 1800), dtype=dtype, seed=25 + i), dev)
+             for i in range(2)]
+    want = [P.call(cea, c, True) for c in cases]
+    torch.cuda.synchronize()
+    streams, graphs, got = [torch.cuda.Stream() for _ in cases], [], []
+    for c, s in zip(cases, streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            outs = [P.call(cea, c, True) for _ in range(8)]
+        graphs.append(g)
+        got.append(outs)
+    for _ in range(4):
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for outs, ref in zip(got, want):
+            for o in outs:
+                assert torch.equal(o[0], ref[0]) and torch.equal(o[1], ref[1])
+
+
 def test_pages_are_not_handed_out_in_a_capture(cea, dev):
     cache = cea.PagedKVCache(1, 6, 16, 2, 64, device=dev)
     a = cache.new()
