@@ -251,7 +251,7 @@ template <bool POS> struct Shared {
   int64_t red_max[NWAVES], red_min[NWAVES];  // what the waves' rows see
   int red_act[NWAVES], wave_cnt[NWAVES];
   int lost[NWAVES];                          // a page of the pass that is not there, by finder
-  int odd_result;                            // a result that is not finite
+  int odd_result;                            // a result that is not finite; the first pass's alone
   uint32_t marks[PASS / 32];                 // tiles that hold a value that is not finite
   int32_t ids[PASS * BN / 16];               // page indices of the pass, -1 where none
   int2 tile_list[POS ? PASS : 1];            // (tile, 2-bit mode of every wave)
@@ -387,7 +387,10 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, char* smem, Sh
     lim_max = uniform(wave_max_i32(lim));
     if (lane == 0) sh.red_max[wave] = lim_max;
   }
-  if (tid == 0) sh.odd_result = 0;
+  // (the first time alone: a wave that is late to read what the first pass found shares this word with waves
+  // that are in the second already, and no barrier lies between)
+  if constexpr (!AGAIN)
+    if (tid == 0) sh.odd_result = 0;
 
   const float scale = (float)p.scale;
   const float c = fabsf(scale) * 1.4426950408889634f;

@@ -232,6 +232,37 @@ def test_values_of_probability_zero(cea, dev):
         assert bool(torch.isfinite(out[:, :, 1]).all())
 
 
+@pytest.mark.parametrize("D,explicit", [(64, False), (64, True), (128, True)])
+def test_every_workgroup_looks_at_its_tiles_again(cea, dev, D, explicit):
+    """Hidden values that are not finite under every query block of many equal rows: each goes over its
+    tiles twice, and every time every row is the same and right."""
+    n, copies = 130, 48
+    c = P.make(B=2, n=n, Hq=4, Hkv=2, D=D, page=16, lengths=(n + 150, n + 33), explicit=explicit, seed=26)
+    ref = P.reference(c)
+    for b in range(2):  # a slot that nobody sees, or (by its number) the last query alone
+        j = 20 if explicit else int(c.lengths[b]) - 1
+        p, i = int(c.tables[b, j // 16]), j % 16
+        if explicit:
+            c.pos_pages[p, i] = -1
+        c.v_pages[p, :, i] = math.nan
+    if explicit:
+        ref = P.reference(c)
+    d = P.to(c, dev)
+    for name in ("q", "tables", "lengths", "q_pos"):
+        t = getattr(d, name)
+        setattr(d, name, t.repeat(copies, *[1] * (t.dim() - 1)))
+    first = None
+    for _ in range(20):
+        out = P.call(cea, d).view(copies, 2, n, 4, D)
+        first = out[0].clone() if first is None else first
+        assert torch.equal(out.nan_to_num(7.0), first.nan_to_num(7.0).expand_as(out))
+    got = first.cpu()
+    if not explicit:
+        assert bool(got[:, n - 1].isnan().all())
+        got[:, n - 1] = ref.out[:, n - 1].to(got.dtype)
+    P.check(c, ref, got)
+
+
 @pytest.mark.parametrize("n", [1, 30])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_not_a_number_in_a_visible_place(cea, dev, n, dtype):

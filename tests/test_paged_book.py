@@ -3,11 +3,15 @@ compacted, and the argument checks of its entry points (no kernel runs here)."""
 
 import ctypes
 import random
+import re
+from pathlib import Path
 
 import pytest
 import torch
 
 from test_abi import _t
+
+REPO = Path(__file__).resolve().parents[1]
 
 
 def contents_model(book, store, moves):
@@ -260,3 +264,15 @@ def test_a_step_of_another_cache_is_refused(cea):
     two._check(other)
     with pytest.raises(RuntimeError, match="this cache"):
         one._check(step)
+
+
+def test_the_second_pass_does_not_touch_the_flag_of_the_first():
+    """The chunk kernel's waves read `odd_result` behind the first pass's last barrier and go into the
+    second pass without another one, so a store there would race with a late reader."""
+    text = (REPO / "collaborative-edge-system_amd" / "csrc" / "paged_chunk.hip").read_text()
+    body = text[text.index("chunk_body(const ChunkParams"):text.index("chunk_again(kernel_args_ptr")]
+    stores = [m.start() for m in re.finditer(r"odd_result\s*=[^=]", body)]
+    assert len(stores) == 2
+    for at in stores:  # the innermost `if constexpr` above each: only where this is not the second pass
+        guards = re.findall(r"if constexpr \(([^\n]*)\)", body[:at])
+        assert guards[-1].startswith("!AGAIN"), body[at - 200:at + 40]
