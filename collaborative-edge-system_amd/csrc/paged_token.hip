@@ -537,6 +537,8 @@ __global__ __launch_bounds__(256) void paged_token_join_kernel(const TokenParams
     }
     const float shift = m_new == -__builtin_inff() ? 0.f : m_new;
     const float a = m == -__builtin_inff() ? 1.f : expf(m - shift);
+    // (parts that saw a key: one whose weight underflows to 0 still counts, as its infinities make a NaN there)
+    const uint64_t saw = __ballot(pl != 0.f);
     const float wt = pl == 0.f ? 0.f : pm == -__builtin_inff() ? 1.f : expf(pm - shift);
     float sum = pl * wt;
 #pragma unroll
@@ -550,7 +552,7 @@ __global__ __launch_bounds__(256) void paged_token_join_kernel(const TokenParams
       const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wt), wave + 4 * k));
 #pragma unroll
       for (int i = 0; i < FPL; ++i)
-        if (w != 0.f) o[i] = __builtin_fmaf(x[k][i], w, o[i]);
+        if ((saw >> (wave + 4 * k)) & 1) o[i] = __builtin_fmaf(x[k][i], w, o[i]);
     }
   }
 #pragma unroll

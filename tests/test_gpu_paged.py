@@ -263,6 +263,39 @@ def test_every_workgroup_looks_at_its_tiles_again(cea, dev, D, explicit):
     P.check(c, ref, got)
 
 
+def _zero_probability_case(n, length, dtype, explicit, top, bad):
+    """One key of slot `top` takes every query's whole sum (scores of 6400 against a few), so slot 3, which
+    every query sees as well, has probability 0 in any precision; its value is `bad` in KV head 0's feature 7."""
+    c = P.make(B=1, n=n, Hq=4, Hkv=2, D=64, page=16, lengths=(length,), dtype=dtype, explicit=explicit, seed=27)
+    c.q[:] = 4.0
+    for j in (3, top):
+        p, i = int(c.tables[0, j // 16]), j % 16
+        c.k_pages[p, :, i] = 200.0 if j == top else 0.0
+        if explicit:
+            c.pos_pages[p, i] = 2 * j
+    ref = P.reference(c)
+    c.v_pages[int(c.tables[0, 0]), 0, 3, 7] = bad
+    hit = torch.zeros(1, n, 4, 64, dtype=torch.bool)
+    hit[:, :, :2, 7] = True  # 0 * inf and 0 * NaN
+    return c, ref, hit
+
+
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("explicit", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32, F64])
+@pytest.mark.parametrize("n,length", [(1, 70), (1, 1500), (1, 9000), (4, 2100), (40, 90), (40, 1900)])
+def test_a_visible_value_of_probability_zero_is_still_met(cea, dev, n, length, dtype, explicit, bad):
+    """0 * inf is NaN wherever rows are cut: the key that takes the sum lies in the first tile, or far behind."""
+    for top in (0, length - n - 1):
+        c, ref, hit = _zero_probability_case(n, length, dtype, explicit, top, bad)
+        d = P.to(c, dev)
+        for with_lse in (False, True):
+            got = P.call(cea, d, with_lse)
+            out = (got[0] if with_lse else got).cpu()
+            assert bool(out[hit].isnan().all()), (top, with_lse)
+            P.check(c, ref, torch.where(hit, ref.out.to(out.dtype), out), got[1] if with_lse else None)
+
+
 @pytest.mark.parametrize("n", [1, 30])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_not_a_number_in_a_visible_place(cea, dev, n, dtype):
