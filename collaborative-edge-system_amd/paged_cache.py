@@ -219,6 +219,18 @@ class PageBook:
                 table.append(self._take())
         return copies
 
+    def _retract(self, seqs: Sequence[int], lengths: Sequence[int],
+                 copies: List[Tuple[int, int]]) -> None:
+        """Takes the last :meth:`extend` back, given the lengths before it and what it returned."""
+        came_from = {b: a for a, b in copies}
+        for seq, length in zip(seqs, lengths):
+            self.truncate(seq, length)
+            table = self._tables[seq]
+            if table and table[-1] in came_from:
+                own, table[-1] = table[-1], came_from[table[-1]]
+                self._holders[table[-1]] += 1
+                self._give_back(own)
+
     def _take(self) -> int:
         page = heapq.heappop(self._free)
         self._holders[page] = 1
@@ -227,16 +239,22 @@ class PageBook:
     def compact(self) -> List[Tuple[int, int]]:
         """Renames the held pages to the lowest indices; returns the page copies ``(from, to)`` that
         have to be done before the tables are used."""
+        moves = self._moves()
+        self._rename(moves)
+        return moves
+
+    def _moves(self) -> List[Tuple[int, int]]:
         held = [p for p in range(self.pages) if self._holders[p]]
         holes = [p for p in range(len(held)) if not self._holders[p]]
-        moves = [(p, holes.pop(0)) for p in reversed(held) if p >= len(held)]
+        return list(zip((p for p in reversed(held) if p >= len(held)), holes))
+
+    def _rename(self, moves: List[Tuple[int, int]]) -> None:
         to = dict(moves)
         for table in self._tables.values():
             table[:] = [to.get(p, p) for p in table]
         for a, b in moves:
             self._holders[b], self._holders[a] = self._holders[a], 0
-        self._free = list(range(len(held), self.pages))
-        return moves
+        self._free = [p for p in range(self.pages) if not self._holders[p]]
 
 
 class PagedStep:
@@ -325,8 +343,9 @@ class PagedKVCache:
     def compact(self) -> int:
         """Moves the held pages to the lowest indices; returns how many moved."""
         self._outside_capture("compact")
-        moves = self.book.compact()
-        self._copy(moves)
+        moves = self.book._moves()
+        self._copy(moves)  # (into free pages: a copy that fails changes no table)
+        self.book._rename(moves)
         self._epoch += 1
         return len(moves)
 
@@ -334,7 +353,7 @@ class PagedKVCache:
                into: Optional[PagedStep] = None) -> PagedStep:
         """Room for ``counts[i]`` new tokens of ``seqs[i]`` (0: the sequence is only read) and the
         step's tensors.  With ``into`` a step of the same number of rows is filled in place, its
-        width allowing, for a captured graph that reads it."""
+        width allowing, for a captured graph that reads it.  A call that fails adds no tokens."""
         self._outside_capture("extend")
         seqs = list(seqs)
         counts = [int(counts)] * len(seqs) if isinstance(counts, int) else [int(n) for n in counts]
@@ -348,17 +367,22 @@ class PagedKVCache:
                 if widest > into.tables.shape[1]:
                     raise ValueError(f"the step is {into.tables.shape[1]} pages wide, {widest} needed")
         offsets = [self.length(s) for s in seqs]
-        self._copy(self.book.extend(seqs, counts))
-        tables = [self.book.table(s) for s in seqs]
-        step = into
-        if step is None:
-            step = PagedStep(len(seqs), max(map(len, tables), default=0), self.kv.device)
-        width = step.tables.shape[1]
-        host = offsets + counts + [self.length(s) for s in seqs]
-        for t in tables:
-            host += t + [-1] * (width - len(t))
-        staged = torch.tensor(host, dtype=torch.int64, pin_memory=self.kv.is_cuda)
-        step.buffer.copy_(staged, non_blocking=True)
+        copies = self.book.extend(seqs, counts)
+        try:
+            self._copy(copies)
+            tables = [self.book.table(s) for s in seqs]
+            step = into
+            if step is None:
+                step = PagedStep(len(seqs), max(map(len, tables), default=0), self.kv.device)
+            width = step.tables.shape[1]
+            host = offsets + counts + [self.length(s) for s in seqs]
+            for t in tables:
+                host += t + [-1] * (width - len(t))
+            staged = torch.tensor(host, dtype=torch.int64, pin_memory=self.kv.is_cuda)
+            step.buffer.copy_(staged, non_blocking=True)
+        except BaseException:  # (no memory for the step, a copy refused: without a step nothing is added)
+            self.book._retract(seqs, offsets, copies)
+            raise
         step.cache, step.epoch = self, self._epoch
         return step
 

@@ -2,6 +2,7 @@
 compacted, and the argument checks of its entry points (no kernel runs here)."""
 
 import ctypes
+import importlib
 import random
 import re
 from pathlib import Path
@@ -138,6 +139,66 @@ def test_extend_argument_errors(cea):
             book.extend(seqs, counts)
     with pytest.raises(ValueError):
         cea.PageBook(0, 4)
+
+
+def _state(book):
+    return ({s: (book.length(s), book.table(s)) for s in book.sequences()}, list(book._holders), sorted(book._free))
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_an_extension_taken_back_leaves_the_book_as_it_was(cea, seed):
+    rng = random.Random(50 + seed)
+    book = cea.PageBook(60, 4)
+    seqs = [book.new() for _ in range(4)]
+    for _ in range(200):
+        if len(seqs) < 9 and rng.random() < 0.4:
+            seqs.append(book.fork(rng.choice(seqs)))
+        for s in seqs:
+            if book.length(s) > 24:
+                book.truncate(s, rng.randint(0, 11))
+        some = rng.sample(seqs, rng.randint(1, len(seqs)))
+        counts, before = [rng.randint(0, 6) for _ in some], _state(book)
+        lengths = [book.length(s) for s in some]
+        try:
+            copies = book.extend(some, counts)
+        except RuntimeError:
+            continue
+        after = _state(book)
+        book._retract(some, lengths, copies)
+        assert _state(book) == before
+        assert book.extend(some, counts) == copies and _state(book) == after
+
+
+def test_a_cache_call_that_fails_changes_nothing(cea, monkeypatch):
+    """A page copy that is refused (host pools), and no memory for a step: the tokens are not counted,
+    their pages are free, and earlier steps still hold."""
+    cache = cea.PagedKVCache(1, 8, 4, 2, 64, device="cpu")
+    a, b = cache.new(), cache.new()
+    step = cache.extend([b, a], [4, 6])
+    cache.free(b)
+    c = cache.fork(a)
+    step = cache.extend([a, c], 0)
+    before = _state(cache.book)
+    with pytest.raises(RuntimeError):
+        cache.extend([a], 1)  # its own page 2 has to be copied first
+    assert _state(cache.book) == before
+    with pytest.raises(RuntimeError):
+        cache.compact()
+    assert _state(cache.book) == before
+    cache._check(step)
+    cache.free(c)
+    step, before = cache.extend([a], 0), _state(cache.book)
+
+    def no_memory(*args):
+        raise MemoryError
+
+    monkeypatch.setattr(importlib.import_module(cea.__name__ + ".paged_cache"), "PagedStep", no_memory)
+    with pytest.raises(MemoryError):
+        cache.extend([a], 9)
+    assert _state(cache.book) == before
+    cache._check(step)
+    cache.extend([a], 1, into=step)
+    assert step.lengths.tolist() == [7] and cache.length(a) == 7
 
 
 def _refs(*ts):
