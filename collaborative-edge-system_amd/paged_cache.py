@@ -266,6 +266,7 @@ class PagedStep:
         self.tables = self.buffer[3 * rows:].view(rows, width)
         self.offsets, self.counts, self.lengths = self.buffer[:3 * rows].view(3, rows)
         self.cache, self.epoch = None, -1
+        self.most = 0  # new tokens of a row at most
 
 
 class PagedKVCache:
@@ -353,7 +354,8 @@ class PagedKVCache:
                into: Optional[PagedStep] = None) -> PagedStep:
         """Room for ``counts[i]`` new tokens of ``seqs[i]`` (0: the sequence is only read) and the
         step's tensors.  With ``into`` a step of the same number of rows is filled in place, its
-        width allowing, for a captured graph that reads it.  A call that fails adds no tokens."""
+        width allowing, for a captured graph that reads it (its appends write as many tokens a row as
+        they were captured with, so ``counts`` stays within those).  A call that fails adds no tokens."""
         self._outside_capture("extend")
         seqs = list(seqs)
         counts = [int(counts)] * len(seqs) if isinstance(counts, int) else [int(n) for n in counts]
@@ -383,7 +385,7 @@ class PagedKVCache:
         except BaseException:  # (no memory for the step, a copy refused: without a step nothing is added)
             self.book._retract(seqs, offsets, copies)
             raise
-        step.cache, step.epoch = self, self._epoch
+        step.cache, step.epoch, step.most = self, self._epoch, max(counts, default=0)
         return step
 
     def _check(self, step: PagedStep) -> None:
@@ -395,8 +397,11 @@ class PagedKVCache:
     def append(self, layer: int, step: PagedStep, k: torch.Tensor, v: torch.Tensor, *,
                cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,
                pos: Optional[torch.Tensor] = None) -> None:
-        """Writes a layer's new keys and values (:func:`paged_kv_append`)."""
+        """Writes a layer's new keys and values (:func:`paged_kv_append`); rows with fewer new tokens
+        than ``k`` and ``v`` hold are padded."""
         self._check(step)
+        if k.dim() == 4 and k.shape[1] < step.most:
+            raise ValueError(f"the step adds up to {step.most} tokens to a row, k holds {k.shape[1]}")
         k_pages, v_pages = self.pages(layer)
         paged_kv_append(k_pages, v_pages, step.tables, step.offsets, k, v, cos=cos, sin=sin,
                         counts=step.counts, pos_pages=self.pos_pages, pos=pos)

@@ -337,3 +337,16 @@ def test_the_second_pass_does_not_touch_the_flag_of_the_first():
     for at in stores:  # the innermost `if constexpr` above each: only where this is not the second pass
         guards = re.findall(r"if constexpr \(([^\n]*)\)", body[:at])
         assert guards[-1].startswith("!AGAIN"), body[at - 200:at + 40]
+
+
+def test_an_append_of_fewer_tokens_than_the_step_counts_is_refused(cea):
+    """The others would be counted and read, and never written."""
+    cache = cea.PagedKVCache(1, 4, 16, 2, 64, device="cpu")
+    a, b = cache.new(), cache.new()
+    step = cache.extend([a, b], [2, 5])
+    k = torch.zeros(2, 4, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="up to 5 tokens"):
+        cache.append(0, step, k, k)
+    cache.extend([a, b], [4, 0], into=step)
+    with pytest.raises(RuntimeError):  # as many as k holds: on to the operator, which wants the GPU
+        cache.append(0, step, k, k)
