@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import heapq
 import math
+import operator
 from typing import Dict, List, Optional, Sequence, Tuple, Union
 
 import torch
@@ -97,6 +98,15 @@ def paged_attention_with_lse(q: torch.Tensor, k_pages: torch.Tensor, v_pages: to
     return out, lse
 
 
+def _page_list(pages: Union[torch.Tensor, Sequence[int]]) -> torch.Tensor:
+    if isinstance(pages, torch.Tensor):
+        return pages
+    try:
+        return torch.tensor([operator.index(p) for p in pages], dtype=torch.int64)
+    except TypeError:
+        raise ValueError("page indices must be whole numbers") from None
+
+
 def copy_pages(pools: Union[torch.Tensor, Sequence[torch.Tensor]],
                src: Union[torch.Tensor, Sequence[int]], dst: Union[torch.Tensor, Sequence[int]], *,
                dim: int = 0) -> None:
@@ -106,12 +116,11 @@ def copy_pages(pools: Union[torch.Tensor, Sequence[torch.Tensor]],
     contiguous, and what precedes it (layers, keys and values) holds more pools of the same pages.
     ``src`` and ``dst`` are host lists (the pages are handed out on the host): they go with the
     launch, without a transfer, and a captured call copies the same pages on every replay.
-    ``ValueError`` if a page is written twice, or both read and written, or does not exist.
+    ``ValueError`` if a page is written twice, or both read and written, or does not exist, and for
+    indices that are not whole numbers.
     """
     pools = [pools] if isinstance(pools, torch.Tensor) else list(pools)
-    src = src if isinstance(src, torch.Tensor) else torch.tensor(list(src), dtype=torch.int64)
-    dst = dst if isinstance(dst, torch.Tensor) else torch.tensor(list(dst), dtype=torch.int64)
-    nat.ops().copy_pages(pools, int(dim), src, dst)
+    nat.ops().copy_pages(pools, int(dim), _page_list(src), _page_list(dst))
 
 
 class PageBook:
@@ -192,6 +201,7 @@ class PageBook:
         has too few free pages."""
         if len(seqs) != len(counts) or len(set(seqs)) != len(seqs):
             raise ValueError("need distinct sequences with a count each")
+        counts = [operator.index(n) for n in counts]
         if any(n < 0 for n in counts):
             raise ValueError("counts must not be negative")
         need, left = 0, {}
@@ -358,7 +368,7 @@ class PagedKVCache:
         they were captured with, so ``counts`` stays within those).  A call that fails adds no tokens."""
         self._outside_capture("extend")
         seqs = list(seqs)
-        counts = [int(counts)] * len(seqs) if isinstance(counts, int) else [int(n) for n in counts]
+        counts = [int(counts)] * len(seqs) if isinstance(counts, int) else [operator.index(n) for n in counts]
         if into is not None:
             if into.tables.shape[0] != len(seqs):
                 raise ValueError(f"the step has {into.tables.shape[0]} rows, not {len(seqs)}")

@@ -350,3 +350,19 @@ def test_an_append_of_fewer_tokens_than_the_step_counts_is_refused(cea):
     cache.extend([a, b], [4, 0], into=step)
     with pytest.raises(RuntimeError):  # as many as k holds: on to the operator, which wants the GPU
         cache.append(0, step, k, k)
+
+
+def test_parts_of_pages_and_tokens_are_refused(cea):
+    """Not cut to the next whole number."""
+    pool = torch.zeros(4, 2, 16, 64)
+    for src, dst in (([0.7], [1]), ([0], [1.0]), ([0], ["1"])):
+        with pytest.raises(ValueError, match="whole"):
+            cea.copy_pages(pool, src, dst)
+    cache = cea.PagedKVCache(1, 4, 16, 2, 64, device="cpu")
+    a = cache.new()
+    for give in (lambda: cache.extend([a], [1.5]), lambda: cache.book.extend([a], [1.5])):
+        with pytest.raises(TypeError):
+            give()
+        assert cache.length(a) == 0
+    cache.extend([a], torch.tensor([3]))
+    assert cache.length(a) == 3
