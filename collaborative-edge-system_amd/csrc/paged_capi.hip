@@ -42,6 +42,17 @@ int check_pos_pages(const cea_tensor* pp, const cea_tensor* kp, const char* what
   return CEA_OK;
 }
 
+// The pages [N, P] of a pool [N, P, E] are apart: along the dimension of the smaller stride by a page at
+// least, along the other one by all that this one spans.  Views of a tensor that holds each element once are.
+bool pages_apart(const cea_tensor& t) {
+  if (t.size[0] == 0 || t.size[1] == 0) return true;
+  int near = t.stride[0] <= t.stride[1] ? 0 : 1;
+  if (t.size[near] == 1) near = 1 - near;  // (the stride of a single one says nothing)
+  const int far = 1 - near;
+  const int64_t span = t.size[near] > 1 ? t.stride[near] * (t.size[near] - 1) + t.size[2] : t.size[2];
+  return (t.size[near] <= 1 || t.stride[near] >= t.size[2]) && (t.size[far] <= 1 || t.stride[far] >= span);
+}
+
 }  // namespace
 
 bool paged_tiles_supported(const PagedParams& p) {
@@ -248,9 +259,7 @@ int cea_copy_pages(int32_t n, const cea_tensor* pools, const int64_t* src, const
     if ((rc = check_tensor(&pools[i], "pool", 3, -1, true))) return rc;
     CEA_REQUIRE(pools[i].size[1] == pools[0].size[1], CEA_EINVAL,
                 "%s: the pools differ in their number of pages", what);
-    for (int j = 0; j < 2; ++j)
-      CEA_REQUIRE(pools[i].size[j] <= 1 || pools[i].stride[j] >= pools[i].size[2], CEA_EINVAL,
-                  "%s: pages overlap", what);
+    CEA_REQUIRE(pages_apart(pools[i]), CEA_EINVAL, "%s: pages overlap", what);
   }
   const int64_t P = pools[0].size[1];
   for (int64_t i = 0; i < moves; ++i)

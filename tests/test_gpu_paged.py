@@ -629,6 +629,17 @@ def test_copy_many_pages_through_several_pools(cea, dev):
         assert torch.equal(t, w)
 
 
+def test_copy_pages_of_a_pool_with_pages_first(cea, dev):
+    """[P, layers, 2, page, D], handed over as a view with the pages behind the layers."""
+    pool = torch.randint(-99, 99, (7, 3, 2, 16, 8), device=dev).to(BF16)
+    want = pool.clone()
+    want[torch.tensor([4, 1], device=dev)] = pool[torch.tensor([0, 3], device=dev)]
+    cea.copy_pages(pool.permute(1, 2, 0, 3, 4), [0, 3], [4, 1], dim=2)
+    assert torch.equal(pool, want)
+    with pytest.raises(ValueError, match="overlap"):
+        cea.copy_pages(pool.view(-1).as_strided((2, 6, 32), (32, 32, 1)), [0], [1], dim=1)
+
+
 def test_copy_pages_refusals(cea, dev):
     pool = torch.zeros(2, 6, 4, 8, device=dev)
     for src, dst in (([0], [6]), ([0, 1], [2, 2]), ([0, 1], [1, 2]), ([0], [1, 2])):

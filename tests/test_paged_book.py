@@ -366,3 +366,22 @@ def test_parts_of_pages_and_tokens_are_refused(cea):
         assert cache.length(a) == 0
     cache.extend([a], torch.tensor([3]))
     assert cache.length(a) == 3
+
+
+def test_pools_whose_pages_overlap_are_refused(cea):
+    """By their two strides together; the ways in which views of one tensor lie apart are not."""
+    nat = cea._native
+    lib = nat.load_library()
+    one, other = (ctypes.c_int64 * 1)(0), (ctypes.c_int64 * 1)(1)
+
+    def copy(size, stride):
+        t = _t((*size, 32), 1)
+        t.stride[0], t.stride[1], t.stride[2] = *stride, 1
+        return lib.cea_copy_pages(1, (nat.CeaTensor * 1)(t), one, other, 1, None)
+
+    for size, stride in (((2, 6), (32, 32)), ((2, 6), (160, 32)), ((3, 6), (32, 64)), ((2, 6), (0, 32)),
+                         ((2, 6), (192, 16)), ((2, 6), (192, -32)), ((1, 6), (5, 31)), ((2, 6), (16, 400))):
+        assert copy(size, stride) == nat.EINVAL and "overlap" in nat.last_error(), (size, stride)
+    if not torch.cuda.is_available():  # (these go on to the launch, which fails here, before it reads anything)
+        for size, stride in (((2, 6), (192, 32)), ((2, 6), (32, 64)), ((1, 6), (0, 32)), ((3, 6), (40, 120))):
+            assert copy(size, stride) != nat.EINVAL, (size, stride)
