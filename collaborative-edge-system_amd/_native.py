@@ -134,6 +134,11 @@ _SIGNATURES = {
         ctypes.c_size_t,
         [ctypes.c_int64] * 7 + [ctypes.c_int32],
     ),
+    "cea_paged_attention_workspace": (
+        ctypes.c_int,
+        [_P] * 7 + [ctypes.c_int32, ctypes.c_double, ctypes.POINTER(ctypes.c_int32), ctypes.c_int32,
+                    _P, _P, ctypes.POINTER(ctypes.c_size_t)],
+    ),
     "cea_paged_attention": (
         ctypes.c_int,
         [_P] * 7 + [ctypes.c_int32, ctypes.c_double, ctypes.POINTER(ctypes.c_int32), ctypes.c_int32,

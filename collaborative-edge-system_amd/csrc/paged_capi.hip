@@ -42,6 +42,99 @@ int check_pos_pages(const cea_tensor* pp, const cea_tensor* kp, const char* what
   return CEA_OK;
 }
 
+// An attention call: its parameters, the kernel that it takes and the scratch of that kernel.
+enum class Form { none, token, chunk, f32, generic };
+struct Attention {
+  PagedParams p;
+  HeadMap map;
+  Form form;
+  size_t bytes;
+};
+
+int prepare_attention(Attention& c, const cea_tensor* q, const cea_tensor* k_pages, const cea_tensor* v_pages,
+                      const cea_tensor* pos_pages, const cea_tensor* tables, const cea_tensor* lengths,
+                      const cea_tensor* q_pos, int32_t causal, double scale, const int32_t* kv_map,
+                      int32_t kv_map_len, const cea_tensor* out, const cea_tensor* lse) {
+  memset(&c, 0, sizeof(c));
+  const char* what = "paged_attention";
+  int rc;
+  if ((rc = check_tensor(q, "q", 4, -1, true))) return rc;
+  const int dt = q->dtype;
+  CEA_REQUIRE(dt != CEA_I64, CEA_EUNSUPPORTED, "%s: unsupported dtype int64", what);
+  const int64_t B = q->size[0], Sq = q->size[1], Hq = q->size[2], D = q->size[3];
+  CEA_REQUIRE(D >= 1, CEA_EINVAL, "%s: empty head dimension", what);
+  CEA_REQUIRE(k_pages != nullptr, CEA_EINVAL, "k_pages: missing tensor");
+  const int64_t Hkv = k_pages->ndim == 4 ? k_pages->size[1] : 0;
+  if ((rc = check_pages(k_pages, v_pages, dt, Hkv, D, what))) return rc;
+  if ((rc = check_rows(tables, lengths, "lengths", B, what))) return rc;
+  if (pos_pages && (rc = check_pos_pages(pos_pages, k_pages, what))) return rc;
+  if ((rc = check_tensor(q_pos, "q_pos", 2, CEA_I64, false))) return rc;
+  CEA_REQUIRE(q_pos->size[0] == B && q_pos->size[1] == Sq, CEA_EINVAL, "%s: q_pos must be [B, Sq]",
+              what);
+  const int acc = dt == CEA_F64 ? CEA_F64 : CEA_F32;
+  if ((rc = check_tensor(out, "out", 4, -1, true))) return rc;
+  CEA_REQUIRE(out->size[0] == B && out->size[1] == Sq && out->size[2] == Hq && out->size[3] == D,
+              CEA_EINVAL, "%s: out must be [B, Sq, Hq, D]", what);
+  CEA_REQUIRE(out->dtype == acc || out->dtype == dt, CEA_EINVAL, "%s: out must be %s or %s", what,
+              dtype_name(acc), dtype_name(dt));
+  if (lse) {
+    if ((rc = check_tensor(lse, "lse", 3, acc, false))) return rc;
+    CEA_REQUIRE(lse->size[0] == B && lse->size[1] == Hq && lse->size[2] == Sq, CEA_EINVAL,
+                "%s: lse must be [B, Hq, Sq]", what);
+  }
+  if ((rc = make_head_map(&c.map, Hq, Hkv, kv_map, kv_map_len))) return rc;
+  const int64_t page = k_pages->size[2], W = tables->size[1];
+  CEA_REQUIRE(W == 0 || page < ((int64_t)1 << 40) / W, CEA_EUNSUPPORTED, "%s: tables too wide", what);
+
+  PagedParams& p = c.p;
+  p.q = q->data, p.k = k_pages->data, p.v = v_pages->data;
+  p.q_pos = (const int64_t*)q_pos->data;
+  p.pos = pos_pages ? (const int64_t*)pos_pages->data : nullptr;
+  p.tables = (const int64_t*)tables->data, p.lengths = (const int64_t*)lengths->data;
+  p.out = out->data, p.lse = lse ? lse->data : nullptr;
+  p.P = k_pages->size[0];
+  p.B = (int)B, p.Sq = (int)Sq, p.Hq = (int)Hq, p.Hkv = (int)Hkv, p.D = (int)D;
+  p.W = (int)W, p.page = (int)page;
+  p.qs_b = q->stride[0], p.qs_s = q->stride[1], p.qs_h = q->stride[2];
+  p.ks_p = k_pages->stride[0], p.ks_h = k_pages->stride[1], p.ks_s = k_pages->stride[2];
+  p.vs_p = v_pages->stride[0], p.vs_h = v_pages->stride[1], p.vs_s = v_pages->stride[2];
+  if (pos_pages) p.ps_p = pos_pages->stride[0], p.ps_s = pos_pages->stride[1];
+  p.ts_b = tables->stride[0], p.ts_w = tables->stride[1], p.ns_b = lengths->stride[0];
+  p.qps_b = q_pos->stride[0], p.qps_s = q_pos->stride[1];
+  p.os_b = out->stride[0], p.os_s = out->stride[1], p.os_h = out->stride[2];
+  if (lse) p.ls_b = lse->stride[0], p.ls_h = lse->stride[1], p.ls_s = lse->stride[2];
+  p.scale = scale;
+  p.causal = causal ? 1 : 0;
+  p.in_dtype = dt, p.out_dtype = out->dtype;
+  p.group = c.map.group;
+  if (B == 0 || Sq == 0 || Hq == 0) return CEA_OK;
+  if (page == 0 || p.P == 0) p.W = 0, p.page = 1;  // no slots: every row is empty
+  const int group = c.map.group;
+  const int64_t slots = (int64_t)p.W * p.page;
+  if (paged_tiles_supported(p)) {
+    // The token form while one unit holds a KV head's queries, so its keys are read once, and for single
+    // tokens of larger groups; two units where all is one launch of small tiles (us, token / chunk form: 32
+    // query rows of a KV head, 4 rows of up to 900 keys, D = 64, 12.6 / 15.7, D = 128, 18.5 / 17.5; 16 rows of up
+    // to 2500, D = 64, 28.2 / 23.7; 16 query rows, 32 rows of up to 8000, D = 128, 154 / 170, 8 of up to 4096
+    // 31.7 / 26.3, 16 of up to 2500, D = 64, 21.0 / 22.1).
+    const int64_t rows = Sq * group;
+    const bool few = Sq == 1 || group <= 0 || rows <= 16 || (rows <= 32 && D == 64 && slots <= 1024);
+    if (few && paged_token_supported(p, c.map)) {
+      c.form = Form::token;
+      c.bytes = paged_token_workspace_bytes(B, Sq, Hq, Hkv, group, D, slots);
+    } else if (paged_chunk_supported(p, c.map)) {
+      c.form = Form::chunk;
+      c.bytes = paged_chunk_workspace_bytes(B, Sq, Hq, group, D, slots, p.pos != nullptr);
+    }
+  }
+  if (c.form == Form::none && paged_f32_supported(p, c.map)) {
+    c.form = Form::f32;
+    c.bytes = paged_f32_workspace_bytes(B, Sq, Hq, group, D, slots);
+  }
+  if (c.form == Form::none) c.form = Form::generic;
+  return CEA_OK;
+}
+
 // The pages [N, P] of a pool [N, P, E] are apart: along the dimension of the smaller stride by a page at
 // least, along the other one by all that this one spans.  Views of a tensor that holds each element once are.
 bool pages_apart(const cea_tensor& t) {
@@ -159,92 +252,39 @@ size_t cea_paged_attention_workspace_bytes(int64_t B, int64_t Sq, int64_t Hq, in
   return most;
 }
 
+int cea_paged_attention_workspace(const cea_tensor* q, const cea_tensor* k_pages, const cea_tensor* v_pages,
+                                  const cea_tensor* pos_pages, const cea_tensor* tables,
+                                  const cea_tensor* lengths, const cea_tensor* q_pos, int32_t causal,
+                                  double scale, const int32_t* kv_map, int32_t kv_map_len,
+                                  const cea_tensor* out, const cea_tensor* lse, size_t* bytes) {
+  CEA_REQUIRE(bytes != nullptr, CEA_EINVAL, "paged_attention: missing arguments");
+  Attention c;
+  const int rc = prepare_attention(c, q, k_pages, v_pages, pos_pages, tables, lengths, q_pos, causal, scale, kv_map,
+                                   kv_map_len, out, lse);
+  *bytes = rc ? 0 : c.bytes;
+  return rc;
+}
+
 int cea_paged_attention(const cea_tensor* q, const cea_tensor* k_pages, const cea_tensor* v_pages,
                         const cea_tensor* pos_pages, const cea_tensor* tables,
                         const cea_tensor* lengths, const cea_tensor* q_pos, int32_t causal,
                         double scale, const int32_t* kv_map, int32_t kv_map_len, cea_tensor* out,
                         cea_tensor* lse, void* workspace, size_t workspace_bytes, void* stream) {
-  const char* what = "paged_attention";
-  int rc;
-  if ((rc = check_tensor(q, "q", 4, -1, true))) return rc;
-  const int dt = q->dtype;
-  CEA_REQUIRE(dt != CEA_I64, CEA_EUNSUPPORTED, "%s: unsupported dtype int64", what);
-  const int64_t B = q->size[0], Sq = q->size[1], Hq = q->size[2], D = q->size[3];
-  CEA_REQUIRE(D >= 1, CEA_EINVAL, "%s: empty head dimension", what);
-  CEA_REQUIRE(k_pages != nullptr, CEA_EINVAL, "k_pages: missing tensor");
-  const int64_t Hkv = k_pages->ndim == 4 ? k_pages->size[1] : 0;
-  if ((rc = check_pages(k_pages, v_pages, dt, Hkv, D, what))) return rc;
-  if ((rc = check_rows(tables, lengths, "lengths", B, what))) return rc;
-  if (pos_pages && (rc = check_pos_pages(pos_pages, k_pages, what))) return rc;
-  if ((rc = check_tensor(q_pos, "q_pos", 2, CEA_I64, false))) return rc;
-  CEA_REQUIRE(q_pos->size[0] == B && q_pos->size[1] == Sq, CEA_EINVAL, "%s: q_pos must be [B, Sq]",
-              what);
-  const int acc = dt == CEA_F64 ? CEA_F64 : CEA_F32;
-  if ((rc = check_tensor(out, "out", 4, -1, true))) return rc;
-  CEA_REQUIRE(out->size[0] == B && out->size[1] == Sq && out->size[2] == Hq && out->size[3] == D,
-              CEA_EINVAL, "%s: out must be [B, Sq, Hq, D]", what);
-  CEA_REQUIRE(out->dtype == acc || out->dtype == dt, CEA_EINVAL, "%s: out must be %s or %s", what,
-              dtype_name(acc), dtype_name(dt));
-  if (lse) {
-    if ((rc = check_tensor(lse, "lse", 3, acc, false))) return rc;
-    CEA_REQUIRE(lse->size[0] == B && lse->size[1] == Hq && lse->size[2] == Sq, CEA_EINVAL,
-                "%s: lse must be [B, Hq, Sq]", what);
-  }
-  HeadMap map;
-  if ((rc = make_head_map(&map, Hq, Hkv, kv_map, kv_map_len))) return rc;
-  const int64_t page = k_pages->size[2], W = tables->size[1];
-  CEA_REQUIRE(W == 0 || page < ((int64_t)1 << 40) / W, CEA_EUNSUPPORTED, "%s: tables too wide", what);
-
-  PagedParams p;
-  memset(&p, 0, sizeof(p));
-  p.q = q->data, p.k = k_pages->data, p.v = v_pages->data;
-  p.q_pos = (const int64_t*)q_pos->data;
-  p.pos = pos_pages ? (const int64_t*)pos_pages->data : nullptr;
-  p.tables = (const int64_t*)tables->data, p.lengths = (const int64_t*)lengths->data;
-  p.out = out->data, p.lse = lse ? lse->data : nullptr;
-  p.P = k_pages->size[0];
-  p.B = (int)B, p.Sq = (int)Sq, p.Hq = (int)Hq, p.Hkv = (int)Hkv, p.D = (int)D;
-  p.W = (int)W, p.page = (int)page;
-  p.qs_b = q->stride[0], p.qs_s = q->stride[1], p.qs_h = q->stride[2];
-  p.ks_p = k_pages->stride[0], p.ks_h = k_pages->stride[1], p.ks_s = k_pages->stride[2];
-  p.vs_p = v_pages->stride[0], p.vs_h = v_pages->stride[1], p.vs_s = v_pages->stride[2];
-  if (pos_pages) p.ps_p = pos_pages->stride[0], p.ps_s = pos_pages->stride[1];
-  p.ts_b = tables->stride[0], p.ts_w = tables->stride[1], p.ns_b = lengths->stride[0];
-  p.qps_b = q_pos->stride[0], p.qps_s = q_pos->stride[1];
-  p.os_b = out->stride[0], p.os_s = out->stride[1], p.os_h = out->stride[2];
-  if (lse) p.ls_b = lse->stride[0], p.ls_h = lse->stride[1], p.ls_s = lse->stride[2];
-  p.scale = scale;
-  p.causal = causal ? 1 : 0;
-  p.in_dtype = dt, p.out_dtype = out->dtype;
-  p.group = map.group;
-  if (B == 0 || Sq == 0 || Hq == 0) return CEA_OK;
-  if (page == 0 || p.P == 0) p.W = 0, p.page = 1;  // no slots: every row is empty
+  Attention c;
+  const int rc = prepare_attention(c, q, k_pages, v_pages, pos_pages, tables, lengths, q_pos, causal, scale, kv_map,
+                                   kv_map_len, out, lse);
+  if (rc) return rc;
+  CEA_REQUIRE(c.bytes == 0 || (workspace && workspace_bytes >= c.bytes), CEA_ENOSPACE,
+              "paged_attention: workspace of %zu bytes needed, %zu given", c.bytes, workspace_bytes);
   hipStream_t st = (hipStream_t)stream;
-  if (paged_tiles_supported(p)) {
-    // The token form while one unit holds a KV head's queries, so its keys are read once, and for single
-    // tokens of larger groups; two units where all is one launch of small tiles (us, token / chunk form: 32
-    // query rows of a KV head, 4 rows of up to 900 keys, D = 64, 12.6 / 15.7, D = 128, 18.5 / 17.5; 16 rows of up
-    // to 2500, D = 64, 28.2 / 23.7; 16 query rows, 32 rows of up to 8000, D = 128, 154 / 170, 8 of up to 4096
-    // 31.7 / 26.3, 16 of up to 2500, D = 64, 21.0 / 22.1).
-    const int64_t rows = Sq * map.group;
-    const bool few = Sq == 1 || map.group <= 0 || rows <= 16 || (rows <= 32 && D == 64 && W * page <= 1024);
-    const bool token = few && paged_token_supported(p, map);
-    if (token || paged_chunk_supported(p, map)) {
-      const int64_t slots = W * page;
-      const size_t need = token ? paged_token_workspace_bytes(B, Sq, Hq, Hkv, map.group, D, slots)
-                                : paged_chunk_workspace_bytes(B, Sq, Hq, map.group, D, slots, p.pos != nullptr);
-      CEA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), CEA_ENOSPACE,
-                  "%s: workspace of %zu bytes needed, %zu given", what, need, workspace_bytes);
-      return token ? launch_paged_token(p, map, workspace, st) : launch_paged_chunk(p, map, workspace, st);
-    }
+  switch (c.form) {
+    case Form::none: return CEA_OK;  // no query rows
+    case Form::token: return launch_paged_token(c.p, c.map, workspace, st);
+    case Form::chunk: return launch_paged_chunk(c.p, c.map, workspace, st);
+    case Form::f32: return launch_paged_f32(c.p, c.map, workspace, st);
+    case Form::generic: break;
   }
-  if (paged_f32_supported(p, map)) {
-    const size_t need = paged_f32_workspace_bytes(B, Sq, Hq, map.group, D, W * page);
-    CEA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), CEA_ENOSPACE,
-                "%s: workspace of %zu bytes needed, %zu given", what, need, workspace_bytes);
-    return launch_paged_f32(p, map, workspace, st);
-  }
-  return launch_paged_generic(p, map, st);
+  return launch_paged_generic(c.p, c.map, st);
 }
 
 int cea_copy_pages(int32_t n, const cea_tensor* pools, const int64_t* src, const int64_t* dst,

@@ -586,16 +586,19 @@ std::vector<Tensor> paged_attention(const Tensor& q_in, const Tensor& k_pages, c
   Tensor out = at::empty({B, Sq, Hq, D}, o_opts);
   Tensor lse = with_lse ? at::empty({B, Hq, Sq}, o_opts.dtype(acc)) : Tensor();
   const std::vector<int32_t> m = map_of(kv_map);
-  const size_t bytes = cea_paged_attention_workspace_bytes(B, Sq, Hq, k_pages.size(1), D, tables.size(1),
-                                                           k_pages.size(2), code_of(q.scalar_type()));
-  const Scratch ws = bytes ? workspace(bytes) : Scratch();
   cea_tensor a[6] = {arg(q), arg(k_pages), arg(v_pages), arg(tables), arg(lengths), arg(qp)};
   cea_tensor pa, o = arg(out), l;
   if (pp.defined()) pa = arg(pp);
   if (with_lse) l = arg(lse);
-  check_rc(cea_paged_attention(&a[0], &a[1], &a[2], pp.defined() ? &pa : nullptr, &a[3], &a[4], &a[5],
-                               causal ? 1 : 0, scale, m.empty() ? nullptr : m.data(), (int32_t)m.size(), &o,
-                               with_lse ? &l : nullptr, ws.data(), ws.size, stream_of(dev)),
+  const cea_tensor* pos = pp.defined() ? &pa : nullptr;
+  const int32_t* map = m.empty() ? nullptr : m.data();
+  size_t bytes = 0;
+  check_rc(cea_paged_attention_workspace(&a[0], &a[1], &a[2], pos, &a[3], &a[4], &a[5], causal ? 1 : 0, scale, map,
+                                         (int32_t)m.size(), &o, with_lse ? &l : nullptr, &bytes),
+           "paged_attention");
+  const Scratch ws = bytes ? workspace(bytes) : Scratch();
+  check_rc(cea_paged_attention(&a[0], &a[1], &a[2], pos, &a[3], &a[4], &a[5], causal ? 1 : 0, scale, map,
+                               (int32_t)m.size(), &o, with_lse ? &l : nullptr, ws.data(), ws.size, stream_of(dev)),
            "paged_attention");
   if (with_lse) return {out, lse};
   return {out};

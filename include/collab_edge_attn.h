@@ -396,11 +396,18 @@ int cea_paged_kv_append(const cea_tensor* k, const cea_tensor* v, const cea_tens
  * The paged form of attention / attention_with_lse (collab_infer/parallel/attention.py:201-239,
  * 270-301) over a LayerKVCache view.
  *   out [B,Sq,Hq,D] in q's dtype or the accumulation dtype; lse [B,Hq,Sq] in the latter, or NULL.
- *   workspace: device memory of cea_paged_attention_workspace_bytes() bytes (16-byte aligned,
- *   contents need no initialisation), not shared with a call that may run at the same time.
+ *   workspace: device memory (16-byte aligned, contents need no initialisation), not shared with a call
+ *   that may run at the same time, of what cea_paged_attention_workspace() gives for the same arguments
+ *   (no data is read), or of cea_paged_attention_workspace_bytes() bytes: enough for any layout and head
+ *   map of these sizes, with positions in the pool, which take 8.5 bytes per slot of the tables.
  */
 size_t cea_paged_attention_workspace_bytes(int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int64_t D,
                                            int64_t W, int64_t page, int32_t in_dtype);
+int cea_paged_attention_workspace(const cea_tensor* q, const cea_tensor* k_pages, const cea_tensor* v_pages,
+                                  const cea_tensor* pos_pages, const cea_tensor* tables,
+                                  const cea_tensor* lengths, const cea_tensor* q_pos, int32_t causal,
+                                  double scale, const int32_t* kv_map, int32_t kv_map_len,
+                                  const cea_tensor* out, const cea_tensor* lse, size_t* bytes);
 int cea_paged_attention(const cea_tensor* q, const cea_tensor* k_pages, const cea_tensor* v_pages,
                         const cea_tensor* pos_pages, const cea_tensor* tables,
                         const cea_tensor* lengths, const cea_tensor* q_pos, int32_t causal,

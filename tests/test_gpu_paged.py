@@ -471,6 +471,21 @@ def test_merges_with_another_share(cea, dev):
     P.check(c, ref, out, lse, pieces_left=2.0 ** -22)
 
 
+@pytest.mark.parametrize("n", [1, 30])
+def test_wide_tables_without_positions_take_no_scratch_for_them(cea, dev, n):
+    """64 rows of tables of 131072 slots (71 MB of positions and summaries, if there were any)."""
+    c = P.make(B=64, n=n, Hq=4, Hkv=1, D=64, page=64, lengths=[n + 3 * b for b in range(64)], width=2048, seed=28)
+    d = P.to(c, dev)
+    P.call(cea, d)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = P.call(cea, d)
+    parts = 64 * 16 * n * 4 * 65 * 4 if n > 1 else 512 * 2 * 4 * 66 * 4  # of all key splits, or of all runs
+    assert torch.cuda.max_memory_allocated() - before <= out.numel() * 2 + parts + (1 << 20)
+    P.check(c, P.reference(c), out)
+
+
 # ---------------------------------------------------------------------------------------
 # append
 # ---------------------------------------------------------------------------------------

@@ -385,3 +385,51 @@ def test_pools_whose_pages_overlap_are_refused(cea):
     if not torch.cuda.is_available():  # (these go on to the launch, which fails here, before it reads anything)
         for size, stride in (((2, 6), (192, 32)), ((2, 6), (32, 64)), ((1, 6), (0, 32)), ((3, 6), (40, 120))):
             assert copy(size, stride) != nat.EINVAL, (size, stride)
+
+
+def test_scratch_is_that_of_the_kernel_that_runs(cea):
+    """What a call asks for: the bound for any layout of its sizes covers it; single tokens need their parts
+    alone and chunks without positions no summaries, however wide the tables are."""
+    nat = cea._native
+    lib = nat.load_library()
+    bf16, i64, f32 = 1, 4, 0
+
+    def needed(B, n, Hq, Hkv, D, W, page, dt=bf16, pos=False, kv_map=None, out=None, page_pad=0):
+        P = 8
+        q, kp, vp = (_t(x, dt) for x in ((B, n, Hq, D), (P, Hkv, page, D), (P, Hkv, page, D)))
+        if page_pad:  # (rows off the 16-byte grid: the generic kernel)
+            kp.stride[2] += page_pad
+        tab, ln, qp, o = _t((B, W), i64), _t((B,), i64), _t((B, n), i64), _t((B, n, Hq, D), dt if out is None else out)
+        pp = _t((P, page), i64) if pos else None
+        m = None if kv_map is None else (ctypes.c_int32 * Hq)(*kv_map)
+        got = ctypes.c_size_t(7)
+        rc = lib.cea_paged_attention_workspace(*_refs(q, kp, vp, pp, tab, ln, qp), 1, 0.125, m, Hq if m else 0,
+                                               *_refs(o, None), ctypes.byref(got))
+        assert rc == 0, nat.last_error()
+        most = lib.cea_paged_attention_workspace_bytes(B, n, Hq, Hkv, D, W, page, dt)
+        assert got.value <= most
+        if got.value:  # the call itself wants as much
+            assert lib.cea_paged_attention(*_refs(q, kp, vp, pp, tab, ln, qp), 1, 0.125, m, Hq if m else 0,
+                                           *_refs(o, None), 1 << 20, got.value - 1, None) == nat.ENOSPACE
+            assert f"{got.value} bytes" in nat.last_error()
+        return got.value
+
+    # 512 workgroups x 2 parts of 4 rows of 130 numbers
+    assert needed(32, 1, 32, 8, 128, 2048, 64) == 512 * 2 * 4 * 130 * 4 == needed(32, 1, 32, 8, 128, 2048, 64, pos=True)
+    assert needed(32, 1, 32, 8, 128, 16, 64) == 0  # short tables: one launch
+    wide = needed(1, 500, 32, 8, 128, 20000, 64)
+    assert needed(1, 500, 32, 8, 128, 40000, 64) == wide > 0
+    assert needed(1, 500, 32, 8, 128, 20000, 64, pos=True) - wide == 20000 * (512 + 32)
+    assert needed(1, 1, 8, 8, 80, 20000, 64) == 0 == needed(1, 1, 8, 8, 64, 2000, 64, page_pad=1)
+    assert needed(1, 20, 8, 8, 64, 2000, 64, dt=f32) > 0
+    rng = random.Random(3)
+    for _ in range(300):
+        Hkv, D, page = rng.choice([1, 2, 8]), rng.choice([64, 128]), rng.choice([16, 64, 128])
+        Hq = Hkv * rng.choice([1, 3, 4, 16])
+        kv_map = [rng.randrange(Hkv) for _ in range(Hq)] if rng.random() < 0.3 else None
+        needed(rng.choice([1, 3, 70]), rng.choice([1, 2, 9, 40, 700]), Hq, Hkv, D, rng.choice([1, 20, 3000]), page,
+               dt=rng.choice([bf16, f32]), pos=rng.random() < 0.5, kv_map=kv_map, out=rng.choice([None, f32]))
+    got = ctypes.c_size_t(7)
+    bad = _t((2, 3, 8, 64), bf16)
+    assert lib.cea_paged_attention_workspace(*_refs(bad, bad, None, None, None, None, None), 1, 1.0, None, 0, None, None,
+                                             ctypes.byref(got)) == nat.EINVAL and got.value == 0
