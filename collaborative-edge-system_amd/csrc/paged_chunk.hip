@@ -452,6 +452,26 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, char* smem, Sh
   f32x16 oacc[D / 32];
   float m_run = -__builtin_inff(), m_use = -kExpShift, l_run = 0.f;
 
+  // Which of this lane's keys its row does not see, bit by bit, looked up one by one (rare: the pool's positions
+  // are read in place, which waits for every load).
+  auto hidden = [&](int slot0) -> uint32_t {
+    uint32_t hide = 0;
+#pragma unroll 1
+    for (int x = 0; x < 32; ++x) {
+      const int slot = slot0 + (x >> 4) * 32 + ((x >> 2) & 3) * 8 + g * 4 + (x & 3);
+      bool vis = slot < lim;
+      if (vis) {
+        const int pg = page_of(slot), id = sh.ids[pg - pg0];
+        vis = id >= 0;
+        if (POS && vis) {
+          const int64_t pos = p.pos[(int64_t)id * p.ps_p + slot - pg * (page16 * 16)];
+          vis = pos >= 0 && (!p.causal || pos <= qpos);
+        }
+      }
+      hide |= (vis ? 0u : 1u) << x;
+    }
+    return hide;
+  };
   // The scores of a tile.  mode: 1 every key visible to every row of the wave that sees anything, 2 masked,
   // 3 masked and looked up: a page of the pass that is not there, or (POS) a position beyond 31 bits.  (POS: in
   // mode 1 slots may be empty.  Their scores are -inf plus a product, which is -inf unless the slot holds a value
@@ -509,21 +529,7 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, char* smem, Sh
       }
       return;
     }
-    uint32_t hide = 0;
-#pragma unroll 1
-    for (int x = 0; x < 32; ++x) {  // (rare: the pool's positions are read in place, which waits for every load)
-      const int slot = slot0 + (x >> 4) * 32 + ((x >> 2) & 3) * 8 + g * 4 + (x & 3);
-      bool vis = slot < lim;
-      if (vis) {
-        const int pg = page_of(slot), id = sh.ids[pg - pg0];
-        vis = id >= 0;
-        if (POS && vis) {
-          const int64_t pos = p.pos[(int64_t)id * p.ps_p + slot - pg * (page16 * 16)];
-          vis = pos >= 0 && (!p.causal || pos <= qpos);
-        }
-      }
-      hide |= (vis ? 0u : 1u) << x;
-    }
+    const uint32_t hide = hidden(slot0);
 #pragma unroll
     for (int i = 0; i < 32; ++i)
       if ((hide >> i) & 1u) sacc[i >> 4][i & 15] = -__builtin_inff();
@@ -620,18 +626,19 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, char* smem, Sh
   // ... and a marked tile, V as it is, counts per feature the visible keys with +inf or NaN, then those with
   // -inf or NaN, by products with ones; the sum takes an infinity of that sign (both make a NaN; a
   // visible key of probability 0 counts for both: 0 * inf).
-  auto mark = [&](int stage, int slot0, int mode) {
+  auto mark = [&](int stage, int slot0) {
     const char* sb = smem + stage * L::STAGE_BYTES;
     f32x16 sacc[2];
-    scores(stage, slot0, mode, sacc);
-    uint32_t seen = 0, none = 0;
+    scores(stage, slot0, 1, sacc);
+    // (a key's score does not say whether it is visible: -inf is a score as well)
+    const uint32_t seen = ~hidden(slot0);
+    uint32_t none = 0;
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
       const float x = sacc[i >> 4][i & 15];
-      const bool vis = __float_as_uint(x) != 0xff800000u;
-      seen |= (vis ? 1u : 0u) << i;
-      none |= (vis && __builtin_amdgcn_exp2f(__builtin_fmaf(x, c, -m_use)) == 0.f ? 1u : 0u) << i;
+      none |= (__builtin_amdgcn_exp2f(__builtin_fmaf(x, c, -m_use)) == 0.f ? 1u : 0u) << i;
     }
+    none &= seen;
     auto keys = [&](uint32_t bits, int s) {
       u16x8 x;
 #pragma unroll
@@ -784,7 +791,7 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, char* smem, Sh
         wait_vmcnt<0>();
         __syncthreads();
         const int mode = mode_of(tile, POS ? sh.tile_list[i].y : 0);
-        if (mode != 0) mark(0, tile * BN, mode);
+        if (mode != 0) mark(0, tile * BN);
         __syncthreads();
       }
     }

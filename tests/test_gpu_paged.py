@@ -296,6 +296,29 @@ def test_a_visible_value_of_probability_zero_is_still_met(cea, dev, n, length, d
             P.check(c, ref, torch.where(hit, ref.out.to(out.dtype), out), got[1] if with_lse else None)
 
 
+@pytest.mark.parametrize("explicit", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32, F64])
+@pytest.mark.parametrize("n,length", [(1, 70), (1, 1500), (40, 90), (40, 1900)])
+def test_a_visible_score_of_minus_infinity(cea, dev, n, length, dtype, explicit):
+    """Its probability is 0 as any other's that underflows, and the key is visible all the same: an infinite
+    value there makes a NaN, a finite one nothing."""
+    c = P.make(B=1, n=n, Hq=4, Hkv=2, D=64, page=16, lengths=(length,), dtype=dtype, explicit=explicit, seed=29)
+    c.q = c.q.abs() + 1  # of one sign: a feature of -inf makes a score of -inf
+    page = int(c.tables[0, 0])
+    c.k_pages[page, :, 3] = -200.0
+    if explicit:
+        c.pos_pages[page, 3] = 0
+    ref = P.reference(c)
+    c.k_pages[page, :, 3, 11] = -math.inf
+    P.check(c, ref, P.call(cea, P.to(c, dev)))
+    c.v_pages[page, 0, 3, 7] = math.inf
+    hit = torch.zeros(1, n, 4, 64, dtype=torch.bool)
+    hit[:, :, :2, 7] = True
+    out = P.call(cea, P.to(c, dev)).cpu()
+    assert bool(out[hit].isnan().all())
+    P.check(c, ref, torch.where(hit, ref.out.to(out.dtype), out))
+
+
 @pytest.mark.parametrize("n", [1, 30])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_not_a_number_in_a_visible_place(cea, dev, n, dtype):
