@@ -113,10 +113,11 @@ int prepare_attention(Attention& c, const cea_tensor* q, const cea_tensor* k_pag
   const int64_t slots = (int64_t)p.W * p.page;
   if (paged_tiles_supported(p)) {
     // The token form while one unit holds a KV head's queries, so its keys are read once, and for single
-    // tokens of larger groups; two units where all is one launch of small tiles (us, token / chunk form: 32
-    // query rows of a KV head, 4 rows of up to 900 keys, D = 64, 12.6 / 15.7, D = 128, 18.5 / 17.5; 16 rows of up
-    // to 2500, D = 64, 28.2 / 23.7; 16 query rows, 32 rows of up to 8000, D = 128, 154 / 170, 8 of up to 4096
-    // 31.7 / 26.3, 16 of up to 2500, D = 64, 21.0 / 22.1).
+    // tokens of larger groups; two units where all is one launch of small tiles.  us, token / chunk form: 16 query
+    // rows of a KV head, D = 64, 16 rows of up to 2500 keys 21.5 / 23.0; 14, 2 rows of up to 8000 15.4 / 18.3; 16,
+    // D = 128, 32 rows of up to 8000 157 / 170, but 8 of 100 to 4096 32.1 / 26.4, which the rule does not tell
+    // apart; 32 query rows, 4 rows of up to 900, D = 64, 13.1 / 14.9, D = 128, 18.5 / 17.5; 28, 4 of up to 500,
+    // D = 64, 11.2 / 14.5; 32, 16 of up to 2500, D = 64, 28.2 / 23.7.
     const int64_t rows = Sq * group;
     const bool few = Sq == 1 || group <= 0 || rows <= 16 || (rows <= 32 && D == 64 && slots <= 1024);
     if (few && paged_token_supported(p, c.map)) {

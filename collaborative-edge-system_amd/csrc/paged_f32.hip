@@ -14,7 +14,7 @@
 //   * 8 waves take every 8th tile each and are joined in LDS; long tables with few query rows are cut
 //     into up to 16 key splits by the table's width (each takes an equal run of the row's own tiles),
 //     merged by the list merge.
-//   * Bound by latency: a prompt of 512 keys is 4 tiles a wave, 13.9 us for 8 heads of 64.
+//   * Bound by latency: a prompt of 512 keys is 4 tiles a wave, 14.2 us for 8 heads of 64.
 //   * A value that is not finite and hidden from some query would reach it as 0 * inf.  The results show
 //     that (they are not finite either), and the workgroup then goes over its tiles again and sums products
 //     one by one, over each query's visible keys.

@@ -1,7 +1,7 @@
 // Writing a paged KV cache: the append of new tokens with the rotary of K fused in, and copies of
 // whole pages through any number of pools.  Both are HBM-bound: every row is read and written once.
-// Measured: 2 x 4096 tokens of 8 heads of 128 (71 MB, which the Infinity Cache holds) 11.6 us, 6.1 TB/s; 32 single
-// tokens 8.8 us a call and 3.7 of it on the GPU; 300 pages of 128 KB through 16 pools (1.26 GB) 252 us, 5.0 TB/s,
+// Measured: 2 x 4096 tokens of 8 heads of 128 (71 MB, which the Infinity Cache holds) 11.7 us, 6.1 TB/s; 32 single
+// tokens 8.6 us a call and 3.5 of it on the GPU; 300 pages of 128 KB through 16 pools (1.26 GB) 254 us, 5.0 TB/s,
 // a large copy's rate; 16 pages through 44 pools 8.1 us a call and 3.7 on the GPU.
 #include <algorithm>
 

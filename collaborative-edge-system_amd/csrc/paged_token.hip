@@ -20,9 +20,9 @@
 //     unnormalised (o, m, l) go to the workspace, and a second launch joins the parts of the
 //     units that were cut.  Short tables (kTokenWhole) take one workgroup of 4 to 16 waves per
 //     unit and one launch.
-//   * Measured: 32 rows of 1024 to 32768 keys, 32/8 heads of 128, bf16: 355 us for 2.2 GB, 6.2 TB/s (reads
-//     reach 6.3 here, a copy 4.9); 8 rows of 100 to 4096 keys in f16 22.6 us, 18 of them the stream and 4
-//     the join; one row of 777 keys, 32/4 heads of 64, 10.9 us, a chain of dependent trips to memory (length,
+//   * Measured: 32 rows of 1024 to 32768 keys, 32/8 heads of 128, bf16: 358 us for 2.2 GB, 6.2 TB/s (reads
+//     reach 6.3 here, a copy 4.9), 364 with f32 results; 8 rows of 100 to 4096 keys in f16 22.6 us, 18 of them
+//     the stream and 4.5 the join; one row of 777 keys, 32/4 heads of 64, 10.7 us, a chain of dependent trips to memory (length,
 //     page index, keys) and 4 tiles a wave.
 //   * Hidden keys are masked in the scores, and tiles behind the last visible slot are not read.  A
 //     value that is not finite would meet the zero probabilities of hidden keys and the zero or
@@ -626,9 +626,11 @@ int unit_heads(int64_t Sq, int64_t Hq, int64_t Hkv, int group) {
   return 0;
 }
 
-// Slots of a table up to which a unit is one workgroup's: the second launch costs the host 3 us, and the
-// GPU as much as the split saves (us, whole / split: 4 units of 777 keys, D = 64, 9.8 / 9.7; 4 of 1500
-// 14.1 / 9.9; D = 128: 8 of 777 12.6 / 10.8, 64 of up to 1000 16.4 / 14.8, 320 24.5 / 33.1).
+// Slots of a table up to which a unit is one workgroup's.  The second launch of a split costs the host 3 us,
+// and more on the GPU than it saves from a few hundred units on; a captured call of few units at D = 128 would
+// gain by it.  us, whole / split, in a stream of calls (in a graph): 4 units of 300 keys, D = 64, 11.7 / 14.9 (6.9 /
+// 9.7), 4 of 777 11.7 / 14.8 (9.8 / 9.9), 4 of 1500 - (14.1 / 9.9), 256 of up to 1000 13.7 / 26.4; D = 128: 8 of 777
+// 13.1 / 15.0 (12.4 / 10.8), 64 of up to 1000 16.7 / 15.8 (16.3 / 14.9), 320 24.5 / 32.9, 512 of up to 700 26.1 / 42.2.
 constexpr int64_t kTokenWhole = 1024;
 
 TokenPlan plan_token(int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int group, int64_t slots) {

@@ -81,6 +81,11 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     :func:`~.attention.attention`.  Queries with position -1 are padding under the causal rule; rows
     without a visible key are 0.  The new tokens are appended first, and ``lengths`` counts them.
     What hidden slots hold does not reach a result, infinities and NaN included.
+
+    Probabilities keep f32's bits for single and few tokens (up to 16 query rows of a KV head); those of
+    bf16 and f16 chunks on the matrix cores are rounded to the type once before they weigh the values, so
+    a row's result may differ by such a rounding with the number of tokens in the call.
+    :func:`paged_attention_with_lse` keeps them in every form.
     """
     return _attend(q, k_pages, v_pages, tables, lengths, q_pos, pos_pages, causal, scale, kv_map,
                    False)[0]
