@@ -57,6 +57,11 @@ from .paged_cache import (  # noqa: F401
     paged_attention,
     paged_attention_with_lse,
     paged_kv_append,
+    paged_kv_keep,
+    paged_kv_read,
+    paged_tree_attention,
+    paged_tree_attention_with_lse,
+    tree_masks,
 )
 from .partition import HeadShard, SequenceLayout, partition_heads, split_sizes  # noqa: F401
 from .projection import FusedColumnParallelLinear, fused_linear, linear, linear_gated  # noqa: F401

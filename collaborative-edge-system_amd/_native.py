@@ -36,6 +36,8 @@ DTYPE_CODES = {
     torch.float16: 2,
     torch.float64: 3,
     torch.int64: 4,
+    torch.float8_e4m3fn: 5,
+    torch.uint8: 6,
 }
 
 OK, EINVAL, EUNSUPPORTED, ELAUNCH, ENOSPACE = 0, -1, -2, -3, -4
@@ -144,6 +146,30 @@ _SIGNATURES = {
         [_P] * 7 + [ctypes.c_int32, ctypes.c_double, ctypes.POINTER(ctypes.c_int32), ctypes.c_int32,
                     _P, _P, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
     ),
+    "cea_paged_kv_append8": (ctypes.c_int, [_P] * 13 + [ctypes.c_void_p]),
+    "cea_paged_attention8_workspace": (
+        ctypes.c_int,
+        [_P] * 9 + [ctypes.c_int32, ctypes.c_double, ctypes.POINTER(ctypes.c_int32), ctypes.c_int32,
+                    _P, _P, ctypes.POINTER(ctypes.c_size_t)],
+    ),
+    "cea_paged_attention8": (
+        ctypes.c_int,
+        [_P] * 9 + [ctypes.c_int32, ctypes.c_double, ctypes.POINTER(ctypes.c_int32), ctypes.c_int32,
+                    _P, _P, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
+    ),
+    "cea_paged_kv_read": (ctypes.c_int, [_P] * 9 + [ctypes.c_void_p]),
+    "cea_paged_tree_attention_workspace": (
+        ctypes.c_int,
+        [_P] * 9 + [ctypes.c_double, ctypes.POINTER(ctypes.c_int32), ctypes.c_int32, _P, _P,
+                    ctypes.POINTER(ctypes.c_size_t)],
+    ),
+    "cea_paged_tree_attention": (
+        ctypes.c_int,
+        [_P] * 9 + [ctypes.c_double, ctypes.POINTER(ctypes.c_int32), ctypes.c_int32, _P, _P,
+                    ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
+    ),
+    "cea_tree_masks": (ctypes.c_int, [_P] * 4 + [ctypes.c_void_p]),
+    "cea_paged_kv_keep": (ctypes.c_int, [_P, _P, ctypes.c_int32, _P, _P, _P, _P, ctypes.c_void_p]),
     "cea_copy_pages": (
         ctypes.c_int,
         [ctypes.c_int32, _P, ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int64),

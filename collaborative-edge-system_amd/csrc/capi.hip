@@ -30,6 +30,8 @@ int check_tensor(const cea_tensor* t, const char* name, int ndim, int dtype, boo
               dtype_name(dtype), dtype_name(t->dtype));
   CEA_REQUIRE(dtype_size(t->dtype) != 0, CEA_EINVAL, "%s: unknown dtype code %d", name,
               t->dtype);
+  CEA_REQUIRE(dtype != kAnyType || dtype_size(t->dtype) > 1, CEA_EUNSUPPORTED, "%s: unsupported dtype %s", name,
+              dtype_name(t->dtype));
   int64_t numel = 1;
   for (int i = 0; i < ndim; ++i) {
     CEA_REQUIRE(t->size[i] >= 0, CEA_EINVAL, "%s: negative size", name);

@@ -76,6 +76,8 @@ inline size_t dtype_size(int32_t dt) {
     case CEA_F16: return 2;
     case CEA_F64: return 8;
     case CEA_I64: return 8;
+    case CEA_F8: return 1;
+    case CEA_U8: return 1;
     default: return 0;
   }
 }
@@ -87,12 +89,16 @@ inline const char* dtype_name(int32_t dt) {
     case CEA_F16: return "float16";
     case CEA_F64: return "float64";
     case CEA_I64: return "int64";
+    case CEA_F8: return "float8_e4m3fn";
+    case CEA_U8: return "uint8";
     default: return "unknown";
   }
 }
 
-// Checks rank, dtype and (optionally) a unit innermost stride.  Returns 0 or an error code.
-int check_tensor(const cea_tensor* t, const char* name, int ndim, int dtype_or_minus1,
+// Checks rank, dtype (kAnyType: any but those of 8 bits) and (optionally) a unit innermost stride.  Returns 0 or
+// an error code.
+constexpr int kAnyType = -1, kAnyBytes = -2;
+int check_tensor(const cea_tensor* t, const char* name, int ndim, int dtype,
                  bool inner_contiguous);
 
 // ---------------------------------------------------------------------------------------

@@ -42,6 +42,36 @@ int check_pos_pages(const cea_tensor* pp, const cea_tensor* kp, const char* what
   return CEA_OK;
 }
 
+// The scales of 8-bit pages (whose type is checked), both of them.
+int check_scales(const cea_tensor* ks, const cea_tensor* vs, const cea_tensor* kp, const char* what) {
+  int rc;
+  if ((rc = check_tensor(ks, "k_scales", 3, CEA_U8, false))) return rc;
+  if ((rc = check_tensor(vs, "v_scales", 3, CEA_U8, false))) return rc;
+  for (const cea_tensor* t : {ks, vs})
+    for (int i = 0; i < 3; ++i)
+      CEA_REQUIRE(t->size[i] == kp->size[i], CEA_EINVAL, "%s: k_scales and v_scales must be [P, H, page]", what);
+  return CEA_OK;
+}
+
+int check_counts(const cea_tensor* counts, int64_t B, const char* what) {
+  int rc;
+  if ((rc = check_tensor(counts, "counts", 1, CEA_I64, false))) return rc;
+  CEA_REQUIRE(counts->size[0] == B, CEA_EINVAL, "%s: counts must be [B]", what);
+  return CEA_OK;
+}
+
+// What an attention call is given: scales for 8-bit pages, q_pos (and pos_pages) for a sequence, counts and
+// masks for a tree.
+struct AttentionArgs {
+  const char* what;
+  const cea_tensor *q, *k_pages, *v_pages, *k_scales, *v_scales, *pos_pages, *tables, *lengths, *q_pos, *counts, *masks;
+  int32_t causal;
+  double scale;
+  const int32_t* kv_map;
+  int32_t kv_map_len;
+  const cea_tensor *out, *lse;
+};
+
 // An attention call: its parameters, the kernel that it takes and the scratch of that kernel.
 enum class Form { none, token, chunk, f32, generic };
 struct Attention {
@@ -51,26 +81,39 @@ struct Attention {
   size_t bytes;
 };
 
-int prepare_attention(Attention& c, const cea_tensor* q, const cea_tensor* k_pages, const cea_tensor* v_pages,
-                      const cea_tensor* pos_pages, const cea_tensor* tables, const cea_tensor* lengths,
-                      const cea_tensor* q_pos, int32_t causal, double scale, const int32_t* kv_map,
-                      int32_t kv_map_len, const cea_tensor* out, const cea_tensor* lse) {
+int prepare_attention(Attention& c, const AttentionArgs& a) {
   memset(&c, 0, sizeof(c));
-  const char* what = "paged_attention";
+  const char* what = a.what;
+  const cea_tensor *q = a.q, *k_pages = a.k_pages, *v_pages = a.v_pages, *pos_pages = a.pos_pages;
+  const cea_tensor *tables = a.tables, *lengths = a.lengths, *q_pos = a.q_pos, *out = a.out, *lse = a.lse;
   int rc;
-  if ((rc = check_tensor(q, "q", 4, -1, true))) return rc;
+  if ((rc = check_tensor(q, "q", 4, kAnyType, true))) return rc;
   const int dt = q->dtype;
   CEA_REQUIRE(dt != CEA_I64, CEA_EUNSUPPORTED, "%s: unsupported dtype int64", what);
   const int64_t B = q->size[0], Sq = q->size[1], Hq = q->size[2], D = q->size[3];
   CEA_REQUIRE(D >= 1, CEA_EINVAL, "%s: empty head dimension", what);
   CEA_REQUIRE(k_pages != nullptr, CEA_EINVAL, "k_pages: missing tensor");
   const int64_t Hkv = k_pages->ndim == 4 ? k_pages->size[1] : 0;
-  if ((rc = check_pages(k_pages, v_pages, dt, Hkv, D, what))) return rc;
+  const bool bytes8 = a.k_scales != nullptr || a.v_scales != nullptr;
+  if ((rc = check_pages(k_pages, v_pages, bytes8 ? CEA_F8 : dt, Hkv, D, what))) return rc;
+  if (bytes8) {
+    CEA_REQUIRE(dt != CEA_F64, CEA_EUNSUPPORTED, "%s: 8-bit pages take bf16, f16 or f32 queries", what);
+    if ((rc = check_scales(a.k_scales, a.v_scales, k_pages, what))) return rc;
+  }
   if ((rc = check_rows(tables, lengths, "lengths", B, what))) return rc;
   if (pos_pages && (rc = check_pos_pages(pos_pages, k_pages, what))) return rc;
-  if ((rc = check_tensor(q_pos, "q_pos", 2, CEA_I64, false))) return rc;
-  CEA_REQUIRE(q_pos->size[0] == B && q_pos->size[1] == Sq, CEA_EINVAL, "%s: q_pos must be [B, Sq]",
-              what);
+  if (a.masks) {
+    if ((rc = check_counts(a.counts, B, what))) return rc;
+    if ((rc = check_tensor(a.masks, "masks", 3, CEA_I64, false))) return rc;
+    CEA_REQUIRE(a.masks->size[0] == B && a.masks->size[1] == Sq && a.masks->size[2] == (Sq + 63) / 64, CEA_EINVAL,
+                "%s: masks must be [B, T, ceil(T / 64)]", what);
+    CEA_REQUIRE(Sq <= CEA_MAX_TREE, CEA_EUNSUPPORTED, "%s: trees of up to %d nodes, got %lld", what, CEA_MAX_TREE,
+                (long long)Sq);
+  } else {
+    if ((rc = check_tensor(q_pos, "q_pos", 2, CEA_I64, false))) return rc;
+    CEA_REQUIRE(q_pos->size[0] == B && q_pos->size[1] == Sq, CEA_EINVAL, "%s: q_pos must be [B, Sq]",
+                what);
+  }
   const int acc = dt == CEA_F64 ? CEA_F64 : CEA_F32;
   if ((rc = check_tensor(out, "out", 4, -1, true))) return rc;
   CEA_REQUIRE(out->size[0] == B && out->size[1] == Sq && out->size[2] == Hq && out->size[3] == D,
@@ -82,13 +125,13 @@ int prepare_attention(Attention& c, const cea_tensor* q, const cea_tensor* k_pag
     CEA_REQUIRE(lse->size[0] == B && lse->size[1] == Hq && lse->size[2] == Sq, CEA_EINVAL,
                 "%s: lse must be [B, Hq, Sq]", what);
   }
-  if ((rc = make_head_map(&c.map, Hq, Hkv, kv_map, kv_map_len))) return rc;
+  if ((rc = make_head_map(&c.map, Hq, Hkv, a.kv_map, a.kv_map_len))) return rc;
   const int64_t page = k_pages->size[2], W = tables->size[1];
   CEA_REQUIRE(W == 0 || page < ((int64_t)1 << 40) / W, CEA_EUNSUPPORTED, "%s: tables too wide", what);
 
   PagedParams& p = c.p;
   p.q = q->data, p.k = k_pages->data, p.v = v_pages->data;
-  p.q_pos = (const int64_t*)q_pos->data;
+  p.q_pos = a.masks ? nullptr : (const int64_t*)q_pos->data;
   p.pos = pos_pages ? (const int64_t*)pos_pages->data : nullptr;
   p.tables = (const int64_t*)tables->data, p.lengths = (const int64_t*)lengths->data;
   p.out = out->data, p.lse = lse ? lse->data : nullptr;
@@ -100,12 +143,23 @@ int prepare_attention(Attention& c, const cea_tensor* q, const cea_tensor* k_pag
   p.vs_p = v_pages->stride[0], p.vs_h = v_pages->stride[1], p.vs_s = v_pages->stride[2];
   if (pos_pages) p.ps_p = pos_pages->stride[0], p.ps_s = pos_pages->stride[1];
   p.ts_b = tables->stride[0], p.ts_w = tables->stride[1], p.ns_b = lengths->stride[0];
-  p.qps_b = q_pos->stride[0], p.qps_s = q_pos->stride[1];
+  if (a.masks) {
+    p.masks = (const int64_t*)a.masks->data, p.counts = (const int64_t*)a.counts->data;
+    p.ms_b = a.masks->stride[0], p.ms_s = a.masks->stride[1], p.ms_w = a.masks->stride[2];
+    p.cs_b = a.counts->stride[0];
+  } else {
+    p.qps_b = q_pos->stride[0], p.qps_s = q_pos->stride[1];
+  }
+  if (bytes8) {
+    p.k_scales = (const uint8_t*)a.k_scales->data, p.v_scales = (const uint8_t*)a.v_scales->data;
+    p.kss_p = a.k_scales->stride[0], p.kss_h = a.k_scales->stride[1], p.kss_s = a.k_scales->stride[2];
+    p.vss_p = a.v_scales->stride[0], p.vss_h = a.v_scales->stride[1], p.vss_s = a.v_scales->stride[2];
+  }
   p.os_b = out->stride[0], p.os_s = out->stride[1], p.os_h = out->stride[2];
   if (lse) p.ls_b = lse->stride[0], p.ls_h = lse->stride[1], p.ls_s = lse->stride[2];
-  p.scale = scale;
-  p.causal = causal ? 1 : 0;
-  p.in_dtype = dt, p.out_dtype = out->dtype;
+  p.scale = a.scale;
+  p.causal = a.causal ? 1 : 0;
+  p.in_dtype = dt, p.kv_dtype = bytes8 ? CEA_F8 : dt, p.out_dtype = out->dtype;
   p.group = c.map.group;
   if (B == 0 || Sq == 0 || Hq == 0) return CEA_OK;
   if (page == 0 || p.P == 0) p.W = 0, p.page = 1;  // no slots: every row is empty
@@ -150,6 +204,7 @@ bool pages_apart(const cea_tensor& t) {
 }  // namespace
 
 bool paged_tiles_supported(const PagedParams& p) {
+  if (p.kv_dtype == CEA_F8 || p.masks) return false;
   if (!(p.in_dtype == CEA_BF16 || p.in_dtype == CEA_F16) || !(p.D == 64 || p.D == 128)) return false;
   if (p.page % 16 != 0 || p.W == 0) return false;
   // slots and places in 32 bits, and page numbers by multiplication (u / m = u * ceil(2^32 / m) >> 32
@@ -188,32 +243,52 @@ int merge_paged_splits(const PagedParams& o, const PagedParams& part, int splits
   return launch_merge(m, st);
 }
 
-}  // namespace cea
+namespace {
 
-using namespace cea;
+int attention_workspace(const AttentionArgs& a, size_t* bytes) {
+  CEA_REQUIRE(bytes != nullptr, CEA_EINVAL, "%s: missing arguments", a.what);
+  Attention c;
+  const int rc = prepare_attention(c, a);
+  *bytes = rc ? 0 : c.bytes;
+  return rc;
+}
 
-extern "C" {
+int run_attention(const AttentionArgs& a, void* workspace, size_t workspace_bytes, void* stream) {
+  Attention c;
+  const int rc = prepare_attention(c, a);
+  if (rc) return rc;
+  CEA_REQUIRE(c.bytes == 0 || (workspace && workspace_bytes >= c.bytes), CEA_ENOSPACE,
+              "%s: workspace of %zu bytes needed, %zu given", a.what, c.bytes, workspace_bytes);
+  hipStream_t st = (hipStream_t)stream;
+  switch (c.form) {
+    case Form::none: return CEA_OK;  // no query rows
+    case Form::token: return launch_paged_token(c.p, c.map, workspace, st);
+    case Form::chunk: return launch_paged_chunk(c.p, c.map, workspace, st);
+    case Form::f32: return launch_paged_f32(c.p, c.map, workspace, st);
+    case Form::generic: break;
+  }
+  return launch_paged_generic(c.p, c.map, st);
+}
 
-int cea_paged_kv_append(const cea_tensor* k, const cea_tensor* v, const cea_tensor* pos,
-                        const cea_tensor* cos, const cea_tensor* sin, const cea_tensor* tables,
-                        const cea_tensor* offsets, const cea_tensor* counts, cea_tensor* k_pages,
-                        cea_tensor* v_pages, cea_tensor* pos_pages, void* stream) {
-  const char* what = "paged_kv_append";
+// An append into pages of the rows' type (no scales), or of 8 bits.
+int append(const char* what, const cea_tensor* k, const cea_tensor* v, const cea_tensor* pos, const cea_tensor* cos,
+           const cea_tensor* sin, const cea_tensor* tables, const cea_tensor* offsets, const cea_tensor* counts,
+           cea_tensor* k_pages, cea_tensor* v_pages, bool bytes8, cea_tensor* k_scales, cea_tensor* v_scales,
+           cea_tensor* pos_pages, void* stream) {
   int rc;
-  if ((rc = check_tensor(k, "k", 4, -1, true))) return rc;
+  if ((rc = check_tensor(k, "k", 4, kAnyType, true))) return rc;
   const int dt = k->dtype;
   CEA_REQUIRE(dt != CEA_I64, CEA_EUNSUPPORTED, "%s: unsupported dtype int64", what);
+  CEA_REQUIRE(!bytes8 || dt != CEA_F64, CEA_EUNSUPPORTED, "%s: 8-bit pages take bf16, f16 or f32 rows", what);
   if ((rc = check_tensor(v, "v", 4, dt, true))) return rc;
   const int64_t B = k->size[0], n = k->size[1], H = k->size[2], D = k->size[3];
   for (int i = 0; i < 4; ++i)
     CEA_REQUIRE(v->size[i] == k->size[i], CEA_EINVAL, "%s: v must match k [B,n,H,D]", what);
   CEA_REQUIRE(D % 2 == 0, CEA_EINVAL, "%s: head size must be even", what);
-  if ((rc = check_pages(k_pages, v_pages, dt, H, D, what))) return rc;
+  if ((rc = check_pages(k_pages, v_pages, bytes8 ? CEA_F8 : dt, H, D, what))) return rc;
+  if (bytes8 && (rc = check_scales(k_scales, v_scales, k_pages, what))) return rc;
   if ((rc = check_rows(tables, offsets, "offsets", B, what))) return rc;
-  if (counts) {
-    if ((rc = check_tensor(counts, "counts", 1, CEA_I64, false))) return rc;
-    CEA_REQUIRE(counts->size[0] == B, CEA_EINVAL, "%s: counts must be [B]", what);
-  }
+  if (counts && (rc = check_counts(counts, B, what))) return rc;
   CEA_REQUIRE((pos == nullptr) == (pos_pages == nullptr), CEA_EINVAL,
               "%s: give both positions and pos_pages or neither", what);
   if (pos) {
@@ -235,8 +310,36 @@ int cea_paged_kv_append(const cea_tensor* k, const cea_tensor* v, const cea_tens
     if (c.size[0] == 1) c.stride[0] = 0;  // broadcast over the batch
     if (sn.size[0] == 1) sn.stride[0] = 0;
   }
+  if (bytes8)
+    return launch_paged_append8(k, v, pos, cos ? &c : nullptr, cos ? &sn : nullptr, tables, offsets, counts, k_pages,
+                                v_pages, k_scales, v_scales, pos_pages, (hipStream_t)stream);
   return launch_paged_append(k, v, pos, cos ? &c : nullptr, cos ? &sn : nullptr, tables, offsets,
                              counts, k_pages, v_pages, pos_pages, (hipStream_t)stream);
+}
+
+}  // namespace
+
+}  // namespace cea
+
+using namespace cea;
+
+extern "C" {
+
+int cea_paged_kv_append(const cea_tensor* k, const cea_tensor* v, const cea_tensor* pos,
+                        const cea_tensor* cos, const cea_tensor* sin, const cea_tensor* tables,
+                        const cea_tensor* offsets, const cea_tensor* counts, cea_tensor* k_pages,
+                        cea_tensor* v_pages, cea_tensor* pos_pages, void* stream) {
+  return append("paged_kv_append", k, v, pos, cos, sin, tables, offsets, counts, k_pages, v_pages, false, nullptr,
+                nullptr, pos_pages, stream);
+}
+
+int cea_paged_kv_append8(const cea_tensor* k, const cea_tensor* v, const cea_tensor* pos,
+                         const cea_tensor* cos, const cea_tensor* sin, const cea_tensor* tables,
+                         const cea_tensor* offsets, const cea_tensor* counts, cea_tensor* k_pages,
+                         cea_tensor* v_pages, cea_tensor* k_scales, cea_tensor* v_scales,
+                         cea_tensor* pos_pages, void* stream) {
+  return append("paged_kv_append", k, v, pos, cos, sin, tables, offsets, counts, k_pages, v_pages, true, k_scales,
+                v_scales, pos_pages, stream);
 }
 
 size_t cea_paged_attention_workspace_bytes(int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int64_t D,
@@ -258,12 +361,8 @@ int cea_paged_attention_workspace(const cea_tensor* q, const cea_tensor* k_pages
                                   const cea_tensor* lengths, const cea_tensor* q_pos, int32_t causal,
                                   double scale, const int32_t* kv_map, int32_t kv_map_len,
                                   const cea_tensor* out, const cea_tensor* lse, size_t* bytes) {
-  CEA_REQUIRE(bytes != nullptr, CEA_EINVAL, "paged_attention: missing arguments");
-  Attention c;
-  const int rc = prepare_attention(c, q, k_pages, v_pages, pos_pages, tables, lengths, q_pos, causal, scale, kv_map,
-                                   kv_map_len, out, lse);
-  *bytes = rc ? 0 : c.bytes;
-  return rc;
+  return attention_workspace({"paged_attention", q, k_pages, v_pages, nullptr, nullptr, pos_pages, tables, lengths,
+                              q_pos, nullptr, nullptr, causal, scale, kv_map, kv_map_len, out, lse}, bytes);
 }
 
 int cea_paged_attention(const cea_tensor* q, const cea_tensor* k_pages, const cea_tensor* v_pages,
@@ -271,21 +370,110 @@ int cea_paged_attention(const cea_tensor* q, const cea_tensor* k_pages, const ce
                         const cea_tensor* lengths, const cea_tensor* q_pos, int32_t causal,
                         double scale, const int32_t* kv_map, int32_t kv_map_len, cea_tensor* out,
                         cea_tensor* lse, void* workspace, size_t workspace_bytes, void* stream) {
-  Attention c;
-  const int rc = prepare_attention(c, q, k_pages, v_pages, pos_pages, tables, lengths, q_pos, causal, scale, kv_map,
-                                   kv_map_len, out, lse);
-  if (rc) return rc;
-  CEA_REQUIRE(c.bytes == 0 || (workspace && workspace_bytes >= c.bytes), CEA_ENOSPACE,
-              "paged_attention: workspace of %zu bytes needed, %zu given", c.bytes, workspace_bytes);
-  hipStream_t st = (hipStream_t)stream;
-  switch (c.form) {
-    case Form::none: return CEA_OK;  // no query rows
-    case Form::token: return launch_paged_token(c.p, c.map, workspace, st);
-    case Form::chunk: return launch_paged_chunk(c.p, c.map, workspace, st);
-    case Form::f32: return launch_paged_f32(c.p, c.map, workspace, st);
-    case Form::generic: break;
+  return run_attention({"paged_attention", q, k_pages, v_pages, nullptr, nullptr, pos_pages, tables, lengths, q_pos,
+                        nullptr, nullptr, causal, scale, kv_map, kv_map_len, out, lse},
+                       workspace, workspace_bytes, stream);
+}
+
+int cea_paged_attention8_workspace(const cea_tensor* q, const cea_tensor* k_pages, const cea_tensor* v_pages,
+                                   const cea_tensor* k_scales, const cea_tensor* v_scales,
+                                   const cea_tensor* pos_pages, const cea_tensor* tables,
+                                   const cea_tensor* lengths, const cea_tensor* q_pos, int32_t causal,
+                                   double scale, const int32_t* kv_map, int32_t kv_map_len,
+                                   const cea_tensor* out, const cea_tensor* lse, size_t* bytes) {
+  CEA_REQUIRE(k_scales && v_scales, CEA_EINVAL, "paged_attention: missing scales");
+  return attention_workspace({"paged_attention", q, k_pages, v_pages, k_scales, v_scales, pos_pages, tables, lengths,
+                              q_pos, nullptr, nullptr, causal, scale, kv_map, kv_map_len, out, lse}, bytes);
+}
+
+int cea_paged_attention8(const cea_tensor* q, const cea_tensor* k_pages, const cea_tensor* v_pages,
+                         const cea_tensor* k_scales, const cea_tensor* v_scales,
+                         const cea_tensor* pos_pages, const cea_tensor* tables,
+                         const cea_tensor* lengths, const cea_tensor* q_pos, int32_t causal,
+                         double scale, const int32_t* kv_map, int32_t kv_map_len, cea_tensor* out,
+                         cea_tensor* lse, void* workspace, size_t workspace_bytes, void* stream) {
+  CEA_REQUIRE(k_scales && v_scales, CEA_EINVAL, "paged_attention: missing scales");
+  return run_attention({"paged_attention", q, k_pages, v_pages, k_scales, v_scales, pos_pages, tables, lengths, q_pos,
+                        nullptr, nullptr, causal, scale, kv_map, kv_map_len, out, lse},
+                       workspace, workspace_bytes, stream);
+}
+
+int cea_paged_tree_attention_workspace(const cea_tensor* q, const cea_tensor* k_pages, const cea_tensor* v_pages,
+                                       const cea_tensor* k_scales, const cea_tensor* v_scales,
+                                       const cea_tensor* tables, const cea_tensor* lengths,
+                                       const cea_tensor* counts, const cea_tensor* masks, double scale,
+                                       const int32_t* kv_map, int32_t kv_map_len, const cea_tensor* out,
+                                       const cea_tensor* lse, size_t* bytes) {
+  CEA_REQUIRE(masks && counts, CEA_EINVAL, "paged_tree_attention: missing masks or counts");
+  return attention_workspace({"paged_tree_attention", q, k_pages, v_pages, k_scales, v_scales, nullptr, tables, lengths,
+                              nullptr, counts, masks, 1, scale, kv_map, kv_map_len, out, lse}, bytes);
+}
+
+int cea_paged_tree_attention(const cea_tensor* q, const cea_tensor* k_pages, const cea_tensor* v_pages,
+                             const cea_tensor* k_scales, const cea_tensor* v_scales, const cea_tensor* tables,
+                             const cea_tensor* lengths, const cea_tensor* counts, const cea_tensor* masks,
+                             double scale, const int32_t* kv_map, int32_t kv_map_len, cea_tensor* out,
+                             cea_tensor* lse, void* workspace, size_t workspace_bytes, void* stream) {
+  CEA_REQUIRE(masks && counts, CEA_EINVAL, "paged_tree_attention: missing masks or counts");
+  return run_attention({"paged_tree_attention", q, k_pages, v_pages, k_scales, v_scales, nullptr, tables, lengths,
+                        nullptr, counts, masks, 1, scale, kv_map, kv_map_len, out, lse},
+                       workspace, workspace_bytes, stream);
+}
+
+int cea_paged_kv_read(const cea_tensor* k_pages, const cea_tensor* v_pages, const cea_tensor* k_scales,
+                      const cea_tensor* v_scales, const cea_tensor* tables, const cea_tensor* offsets,
+                      const cea_tensor* counts, cea_tensor* k, cea_tensor* v, void* stream) {
+  const char* what = "paged_kv_read";
+  int rc;
+  if ((rc = check_tensor(k, "k", 4, kAnyType, true))) return rc;
+  CEA_REQUIRE(k->dtype != CEA_I64, CEA_EUNSUPPORTED, "%s: unsupported dtype int64", what);
+  if ((rc = check_tensor(v, "v", 4, k->dtype, true))) return rc;
+  for (int i = 0; i < 4; ++i)
+    CEA_REQUIRE(v->size[i] == k->size[i], CEA_EINVAL, "%s: v must match k [B,n,H,D]", what);
+  const bool bytes8 = k_scales != nullptr || v_scales != nullptr;
+  CEA_REQUIRE(!bytes8 || k->dtype != CEA_F64, CEA_EUNSUPPORTED, "%s: 8-bit pages are read as bf16, f16 or f32", what);
+  if ((rc = check_pages(k_pages, v_pages, bytes8 ? CEA_F8 : k->dtype, k->size[2], k->size[3], what))) return rc;
+  if (bytes8 && (rc = check_scales(k_scales, v_scales, k_pages, what))) return rc;
+  if ((rc = check_rows(tables, offsets, "offsets", k->size[0], what))) return rc;
+  if (counts && (rc = check_counts(counts, k->size[0], what))) return rc;
+  return launch_paged_read(k_pages, v_pages, k_scales, v_scales, tables, offsets, counts, k, v, (hipStream_t)stream);
+}
+
+int cea_tree_masks(const cea_tensor* parents, const cea_tensor* counts, cea_tensor* masks, cea_tensor* depths,
+                   void* stream) {
+  const char* what = "tree_masks";
+  int rc;
+  if ((rc = check_tensor(parents, "parents", 2, CEA_I64, false))) return rc;
+  const int64_t B = parents->size[0], T = parents->size[1];
+  if (counts && (rc = check_counts(counts, B, what))) return rc;
+  if ((rc = check_tensor(masks, "masks", 3, CEA_I64, false))) return rc;
+  if ((rc = check_tensor(depths, "depths", 2, CEA_I64, false))) return rc;
+  CEA_REQUIRE(masks->size[0] == B && masks->size[1] == T && masks->size[2] == (T + 63) / 64, CEA_EINVAL,
+              "%s: masks must be [B, T, ceil(T / 64)]", what);
+  CEA_REQUIRE(depths->size[0] == B && depths->size[1] == T, CEA_EINVAL, "%s: depths must be [B, T]", what);
+  CEA_REQUIRE(T <= CEA_MAX_TREE, CEA_EUNSUPPORTED, "%s: trees of up to %d nodes, got %lld", what, CEA_MAX_TREE,
+              (long long)T);
+  return launch_tree_masks(parents, counts, masks, depths, (hipStream_t)stream);
+}
+
+int cea_paged_kv_keep(cea_tensor* kv, cea_tensor* scales, int32_t page, const cea_tensor* tables,
+                      const cea_tensor* offsets, const cea_tensor* counts, const cea_tensor* path, void* stream) {
+  const char* what = "paged_kv_keep";
+  int rc;
+  if ((rc = check_tensor(kv, "kv", 4, kAnyBytes, true))) return rc;
+  CEA_REQUIRE(page >= 0 && (page == 0 ? kv->size[3] == 0 : kv->size[3] % page == 0), CEA_EINVAL,
+              "%s: kv must be [N, P, H, page * D]", what);
+  CEA_REQUIRE((scales != nullptr) == (kv->dtype == CEA_F8), CEA_EINVAL, "%s: scales go with 8-bit pages", what);
+  if (scales) {
+    if ((rc = check_tensor(scales, "scales", 4, CEA_U8, false))) return rc;
+    CEA_REQUIRE(scales->size[0] == kv->size[0] && scales->size[1] == kv->size[1] && scales->size[2] == kv->size[2] &&
+                    scales->size[3] == page,
+                CEA_EINVAL, "%s: scales must be [N, P, H, page]", what);
   }
-  return launch_paged_generic(c.p, c.map, st);
+  if ((rc = check_tensor(path, "path", 2, CEA_I64, false))) return rc;
+  if ((rc = check_rows(tables, offsets, "offsets", path->size[0], what))) return rc;
+  if (counts && (rc = check_counts(counts, path->size[0], what))) return rc;
+  return launch_paged_keep(kv, scales, page, tables, offsets, counts, path, (hipStream_t)stream);
 }
 
 int cea_copy_pages(int32_t n, const cea_tensor* pools, const int64_t* src, const int64_t* dst,
@@ -297,7 +485,7 @@ int cea_copy_pages(int32_t n, const cea_tensor* pools, const int64_t* src, const
   CEA_REQUIRE(pools != nullptr && moves >= 0 && (moves == 0 || (src && dst)), CEA_EINVAL,
               "%s: missing arguments", what);
   for (int i = 0; i < n; ++i) {
-    if ((rc = check_tensor(&pools[i], "pool", 3, -1, true))) return rc;
+    if ((rc = check_tensor(&pools[i], "pool", 3, kAnyBytes, true))) return rc;
     CEA_REQUIRE(pools[i].size[1] == pools[0].size[1], CEA_EINVAL,
                 "%s: the pools differ in their number of pages", what);
     CEA_REQUIRE(pages_apart(pools[i]), CEA_EINVAL, "%s: pages overlap", what);

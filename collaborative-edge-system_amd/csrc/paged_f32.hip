@@ -315,7 +315,7 @@ size_t paged_f32_workspace_bytes(int64_t B, int64_t Sq, int64_t Hq, int group, i
 }
 
 bool paged_f32_supported(const PagedParams& p, const HeadMap& map) {
-  if (p.in_dtype != CEA_F32 || !(p.D == 64 || p.D == 128) || p.page % KT != 0 || p.W == 0) return false;
+  if (p.kv_dtype != CEA_F32 || p.masks || !(p.D == 64 || p.D == 128) || p.page % KT != 0 || p.W == 0) return false;
   if (map.group <= 0 && (p.Hq > kPagedMapHeads || p.Hkv > 256)) return false;
   if (!std::isfinite(p.scale)) return false;
   // (32-bit slots; u / m = u * ceil(2^32 / m) >> 32 while u * m < 2^32)

@@ -194,7 +194,8 @@ int copy_moves(const CopyPool* pools, int npools, int64_t chunks, int vec, const
     const dim3 grid((unsigned)(p.moves * chunks));
     if (vec == 16) hipLaunchKernelGGL((copy_pages_kernel<u32x4, NP, NM>), grid, dim3(256), 0, st, p);
     else if (vec == 4) hipLaunchKernelGGL((copy_pages_kernel<uint32_t, NP, NM>), grid, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((copy_pages_kernel<uint16_t, NP, NM>), grid, dim3(256), 0, st, p);
+    else if (vec == 2) hipLaunchKernelGGL((copy_pages_kernel<uint16_t, NP, NM>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((copy_pages_kernel<uint8_t, NP, NM>), grid, dim3(256), 0, st, p);
     CEA_CHECK_LAUNCH("copy_pages");
   }
   return CEA_OK;
@@ -245,7 +246,7 @@ int launch_copy_pages(int n, const cea_tensor* pools, const int64_t* src, const 
                       int64_t m, hipStream_t st) {
   CopyPool pool[CEA_MAX_PARTS] = {};
   int npools = 0;
-  bool v16 = true, v4 = true;
+  bool v16 = true, v4 = true, v2 = true;
   int64_t chunks = 0;
   for (int i = 0; i < n; ++i) {
     const cea_tensor& t = pools[i];
@@ -263,11 +264,11 @@ int launch_copy_pages(int n, const cea_tensor* pools, const int64_t* src, const 
                 "copy_pages: pages too large");
     c.chunks = (int32_t)per_page;
     const int64_t a = (int64_t)(uintptr_t)c.base | (c.n > 1 ? c.stride_n : 0) | c.stride_p | c.bytes;
-    v16 = v16 && a % 16 == 0, v4 = v4 && a % 4 == 0;
+    v16 = v16 && a % 16 == 0, v4 = v4 && a % 4 == 0, v2 = v2 && a % 2 == 0;
     ++npools;
   }
   if (npools == 0) return CEA_OK;
-  const int vec = v16 ? 16 : v4 ? 4 : 2;
+  const int vec = v16 ? 16 : v4 ? 4 : v2 ? 2 : 1;
   if (npools == 1 && m <= kFewMoves) return copy_moves<1, kFewMoves>(pool, npools, chunks, vec, src, dst, m, st);
   return copy_moves<CEA_MAX_PARTS, kMoves>(pool, npools, chunks, vec, src, dst, m, st);
 }

@@ -35,9 +35,14 @@ int32_t code_of(c10::ScalarType t) {
   }
 }
 
-cea_tensor arg(const Tensor& t) {
+// The same with the types of 8-bit pages, which the paged cache's operators alone take.
+int32_t page_code_of(c10::ScalarType t) {
+  return t == at::kFloat8_e4m3fn ? CEA_F8 : t == at::kByte ? CEA_U8 : code_of(t);
+}
+
+cea_tensor arg(const Tensor& t, bool pages = false) {
   cea_tensor a;
-  const int32_t code = code_of(t.scalar_type());
+  const int32_t code = pages ? page_code_of(t.scalar_type()) : code_of(t.scalar_type());
   TORCH_CHECK_NOT_IMPLEMENTED(code >= 0, "dtype ", t.scalar_type(), " is not supported by the kernels");
   TORCH_CHECK_VALUE(t.dim() <= CEA_MAX_DIMS, "at most ", CEA_MAX_DIMS, " dimensions supported, got ",
                     t.dim());
@@ -543,72 +548,220 @@ void check_pools(const Tensor& k_pages, const Tensor& v_pages) {
   TORCH_CHECK_VALUE(k_pages.dim() == 4 && v_pages.dim() == 4, "k_pages and v_pages must be [P, H, page, D]");
 }
 
+// Pages of 8 bits come with both scales, others with neither.
+bool bytes8(const Tensor& k_pages, const Tensor& v_pages, const Tensor& ks, const Tensor& vs) {
+  const bool f8 = k_pages.scalar_type() == at::kFloat8_e4m3fn;
+  TORCH_CHECK_VALUE(f8 == (v_pages.scalar_type() == at::kFloat8_e4m3fn), "k_pages and v_pages must share one dtype");
+  TORCH_CHECK_VALUE(ks.defined() == f8 && vs.defined() == f8,
+                    "k_scales and v_scales go with float8_e4m3fn pages, both of them");
+  return f8;
+}
+
+// Arguments of a C call: a tensor that is not given is a null pointer.
+template <size_t N> struct Args {
+  cea_tensor a[N];
+  cea_tensor* p[N];
+  explicit Args(const Tensor* const (&t)[N]) {
+    for (size_t i = 0; i < N; ++i) {
+      p[i] = nullptr;
+      if (t[i]->defined()) a[i] = arg(*t[i], true), p[i] = &a[i];
+    }
+  }
+  cea_tensor* operator[](size_t i) const { return p[i]; }
+};
+
 void paged_kv_append(Tensor k_pages, Tensor v_pages, const c10::optional<Tensor>& pos_pages_in,
                      const Tensor& tables_in, const Tensor& offsets_in, const c10::optional<Tensor>& counts_in,
                      const Tensor& k_in, const Tensor& v_in, const c10::optional<Tensor>& pos_in,
-                     const c10::optional<Tensor>& cos_in, const c10::optional<Tensor>& sin_in) {
+                     const c10::optional<Tensor>& cos_in, const c10::optional<Tensor>& sin_in,
+                     const c10::optional<Tensor>& k_scales_in, const c10::optional<Tensor>& v_scales_in) {
   const Tensor pp = given(pos_pages_in), counts0 = given(counts_in), pos0 = given(pos_in);
-  const Tensor cos0 = given(cos_in), sin0 = given(sin_in);
-  const at::Device dev = device_of({&k_pages, &v_pages, &pp, &tables_in, &offsets_in, &counts0, &k_in, &v_in,
+  const Tensor cos0 = given(cos_in), sin0 = given(sin_in), ks = given(k_scales_in), vs = given(v_scales_in);
+  const at::Device dev = device_of({&k_pages, &v_pages, &ks, &vs, &pp, &tables_in, &offsets_in, &counts0, &k_in, &v_in,
                                     &pos0, &cos0, &sin0});
   check_pools(k_pages, v_pages);
+  const bool f8 = bytes8(k_pages, v_pages, ks, vs);
   TORCH_CHECK_VALUE(cos0.defined() == sin0.defined(), "give both rotary tables or neither");
   c10::DeviceGuard guard(dev);
   const Tensor k = inner(k_in), v = inner(v_in), tables = as_i64(tables_in), offsets = as_i64(offsets_in);
   const Tensor counts = counts0.defined() ? as_i64(counts0) : counts0, pos = pos0.defined() ? as_i64(pos0) : pos0;
   const Tensor cos = cos0.defined() ? inner(cos0.to(k.scalar_type())) : cos0;
   const Tensor sin = sin0.defined() ? inner(sin0.to(k.scalar_type())) : sin0;
-  cea_tensor a[11];
-  const Tensor* t[11] = {&k, &v, &pos, &cos, &sin, &tables, &offsets, &counts, &k_pages, &v_pages, &pp};
-  cea_tensor* p[11];
-  for (int i = 0; i < 11; ++i) {
-    p[i] = nullptr;
-    if (t[i]->defined()) a[i] = arg(*t[i]), p[i] = &a[i];
-  }
-  check_rc(cea_paged_kv_append(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], p[8], p[9], p[10], stream_of(dev)),
+  const Args<13> p({&k, &v, &pos, &cos, &sin, &tables, &offsets, &counts, &k_pages, &v_pages, &ks, &vs, &pp});
+  check_rc(f8 ? cea_paged_kv_append8(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], p[8], p[9], p[10], p[11], p[12],
+                                     stream_of(dev))
+              : cea_paged_kv_append(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], p[8], p[9], p[12], stream_of(dev)),
            "paged_kv_append");
+}
+
+std::vector<Tensor> paged_kv_read(const Tensor& k_pages, const Tensor& v_pages, const c10::optional<Tensor>& k_scales_in,
+                                  const c10::optional<Tensor>& v_scales_in, const Tensor& tables_in,
+                                  const Tensor& offsets_in, const c10::optional<Tensor>& counts_in, int64_t n,
+                                  at::ScalarType dtype) {
+  const Tensor ks = given(k_scales_in), vs = given(v_scales_in), counts0 = given(counts_in);
+  const at::Device dev = device_of({&k_pages, &v_pages, &ks, &vs, &tables_in, &offsets_in, &counts0});
+  check_pools(k_pages, v_pages);
+  const bool f8 = bytes8(k_pages, v_pages, ks, vs);
+  TORCH_CHECK_VALUE(n >= 0, "n must not be negative");
+  TORCH_CHECK_VALUE(tables_in.dim() == 2, "tables must be [B, W]");
+  TORCH_CHECK_VALUE(f8 || dtype == k_pages.scalar_type(), "pages of ", k_pages.scalar_type(),
+                    " are read in their own dtype");
+  c10::DeviceGuard guard(dev);
+  const Tensor tables = as_i64(tables_in), offsets = as_i64(offsets_in);
+  const Tensor counts = counts0.defined() ? as_i64(counts0) : counts0;
+  const auto opts = at::TensorOptions().device(dev).dtype(dtype);
+  Tensor k = at::empty({tables.size(0), n, k_pages.size(1), k_pages.size(3)}, opts), v = at::empty_like(k);
+  const Args<9> p({&k_pages, &v_pages, &ks, &vs, &tables, &offsets, &counts, &k, &v});
+  check_rc(cea_paged_kv_read(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], p[8], stream_of(dev)), "paged_kv_read");
+  return {k, v};
+}
+
+// Outputs of an attention call, and the call with the scratch it asks for.
+template <typename Sizes, typename Call>
+std::vector<Tensor> attend(const Tensor& q, bool with_lse, const at::Device& dev, const char* what, Sizes sizes,
+                           Call call) {
+  const at::ScalarType acc = acc_of(q.scalar_type());
+  const auto o_opts = at::TensorOptions().device(dev).dtype(with_lse ? acc : q.scalar_type());
+  Tensor out = at::empty(q.sizes(), o_opts);
+  Tensor lse = with_lse ? at::empty({q.size(0), q.size(2), q.size(1)}, o_opts.dtype(acc)) : Tensor();
+  cea_tensor o = arg(out), l;
+  if (with_lse) l = arg(lse);
+  cea_tensor* lp = with_lse ? &l : nullptr;
+  size_t bytes = 0;
+  check_rc(sizes(&o, lp, &bytes), what);
+  const Scratch ws = bytes ? workspace(bytes) : Scratch();
+  check_rc(call(&o, lp, ws.data(), ws.size), what);
+  if (with_lse) return {out, lse};
+  return {out};
 }
 
 std::vector<Tensor> paged_attention(const Tensor& q_in, const Tensor& k_pages, const Tensor& v_pages,
                                     const c10::optional<Tensor>& pos_pages_in, const Tensor& tables_in,
                                     const Tensor& lengths_in, const Tensor& q_pos_in, bool causal, double scale,
-                                    c10::optional<at::IntArrayRef> kv_map, bool with_lse) {
-  const Tensor pp = given(pos_pages_in);
-  const at::Device dev = device_of({&q_in, &k_pages, &v_pages, &pp, &tables_in, &lengths_in, &q_pos_in});
+                                    c10::optional<at::IntArrayRef> kv_map, bool with_lse,
+                                    const c10::optional<Tensor>& k_scales_in,
+                                    const c10::optional<Tensor>& v_scales_in) {
+  const Tensor pp = given(pos_pages_in), ks = given(k_scales_in), vs = given(v_scales_in);
+  const at::Device dev = device_of({&q_in, &k_pages, &v_pages, &ks, &vs, &pp, &tables_in, &lengths_in, &q_pos_in});
   check_pools(k_pages, v_pages);
+  const bool f8 = bytes8(k_pages, v_pages, ks, vs);
   TORCH_CHECK_VALUE(q_in.dim() == 4, "q must be [B, S, H, D]");
   TORCH_CHECK_VALUE(tables_in.dim() == 2, "tables must be [B, W]");
   c10::DeviceGuard guard(dev);
   const Tensor q = inner(q_in), tables = as_i64(tables_in), lengths = as_i64(lengths_in), qp = as_i64(q_pos_in);
-  const int64_t B = q.size(0), Sq = q.size(1), Hq = q.size(2), D = q.size(3);
-  const at::ScalarType acc = acc_of(q.scalar_type());
-  const auto o_opts = at::TensorOptions().device(dev).dtype(with_lse ? acc : q.scalar_type());
-  Tensor out = at::empty({B, Sq, Hq, D}, o_opts);
-  Tensor lse = with_lse ? at::empty({B, Hq, Sq}, o_opts.dtype(acc)) : Tensor();
   const std::vector<int32_t> m = map_of(kv_map);
-  cea_tensor a[6] = {arg(q), arg(k_pages), arg(v_pages), arg(tables), arg(lengths), arg(qp)};
-  cea_tensor pa, o = arg(out), l;
-  if (pp.defined()) pa = arg(pp);
-  if (with_lse) l = arg(lse);
-  const cea_tensor* pos = pp.defined() ? &pa : nullptr;
   const int32_t* map = m.empty() ? nullptr : m.data();
-  size_t bytes = 0;
-  check_rc(cea_paged_attention_workspace(&a[0], &a[1], &a[2], pos, &a[3], &a[4], &a[5], causal ? 1 : 0, scale, map,
-                                         (int32_t)m.size(), &o, with_lse ? &l : nullptr, &bytes),
-           "paged_attention");
-  const Scratch ws = bytes ? workspace(bytes) : Scratch();
-  check_rc(cea_paged_attention(&a[0], &a[1], &a[2], pos, &a[3], &a[4], &a[5], causal ? 1 : 0, scale, map,
-                               (int32_t)m.size(), &o, with_lse ? &l : nullptr, ws.data(), ws.size, stream_of(dev)),
-           "paged_attention");
-  if (with_lse) return {out, lse};
-  return {out};
+  const int32_t len = (int32_t)m.size(), c = causal ? 1 : 0;
+  const Args<9> p({&q, &k_pages, &v_pages, &pp, &tables, &lengths, &qp, &ks, &vs});
+  return attend(
+      q, with_lse, dev, "paged_attention",
+      [&](cea_tensor* o, cea_tensor* l, size_t* bytes) {
+        return f8 ? cea_paged_attention8_workspace(p[0], p[1], p[2], p[7], p[8], p[3], p[4], p[5], p[6], c, scale, map,
+                                                   len, o, l, bytes)
+                  : cea_paged_attention_workspace(p[0], p[1], p[2], p[3], p[4], p[5], p[6], c, scale, map, len, o, l,
+                                                  bytes);
+      },
+      [&](cea_tensor* o, cea_tensor* l, void* ws, size_t size) {
+        return f8 ? cea_paged_attention8(p[0], p[1], p[2], p[7], p[8], p[3], p[4], p[5], p[6], c, scale, map, len, o, l,
+                                         ws, size, stream_of(dev))
+                  : cea_paged_attention(p[0], p[1], p[2], p[3], p[4], p[5], p[6], c, scale, map, len, o, l, ws, size,
+                                        stream_of(dev));
+      });
+}
+
+std::vector<Tensor> paged_tree_attention(const Tensor& q_in, const Tensor& k_pages, const Tensor& v_pages,
+                                         const c10::optional<Tensor>& k_scales_in,
+                                         const c10::optional<Tensor>& v_scales_in, const Tensor& tables_in,
+                                         const Tensor& lengths_in, const Tensor& counts_in, const Tensor& masks_in,
+                                         double scale, c10::optional<at::IntArrayRef> kv_map, bool with_lse) {
+  const Tensor ks = given(k_scales_in), vs = given(v_scales_in);
+  const at::Device dev =
+      device_of({&q_in, &k_pages, &v_pages, &ks, &vs, &tables_in, &lengths_in, &counts_in, &masks_in});
+  check_pools(k_pages, v_pages);
+  bytes8(k_pages, v_pages, ks, vs);
+  TORCH_CHECK_VALUE(q_in.dim() == 4, "q must be [B, T, H, D]");
+  TORCH_CHECK_VALUE(masks_in.scalar_type() == at::kLong, "masks must be int64 words");
+  c10::DeviceGuard guard(dev);
+  const Tensor q = inner(q_in), tables = as_i64(tables_in), lengths = as_i64(lengths_in), counts = as_i64(counts_in);
+  const std::vector<int32_t> m = map_of(kv_map);
+  const int32_t* map = m.empty() ? nullptr : m.data();
+  const int32_t len = (int32_t)m.size();
+  const Args<9> p({&q, &k_pages, &v_pages, &ks, &vs, &tables, &lengths, &counts, &masks_in});
+  return attend(
+      q, with_lse, dev, "paged_tree_attention",
+      [&](cea_tensor* o, cea_tensor* l, size_t* bytes) {
+        return cea_paged_tree_attention_workspace(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], p[8], scale, map, len,
+                                                  o, l, bytes);
+      },
+      [&](cea_tensor* o, cea_tensor* l, void* ws, size_t size) {
+        return cea_paged_tree_attention(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], p[8], scale, map, len, o, l, ws,
+                                        size, stream_of(dev));
+      });
+}
+
+std::vector<Tensor> tree_masks(const Tensor& parents_in, const c10::optional<Tensor>& counts_in) {
+  const Tensor counts0 = given(counts_in);
+  const at::Device dev = device_of({&parents_in, &counts0});
+  TORCH_CHECK_VALUE(parents_in.dim() == 2, "parents must be [B, T]");
+  c10::DeviceGuard guard(dev);
+  const Tensor parents = as_i64(parents_in), counts = counts0.defined() ? as_i64(counts0) : counts0;
+  const int64_t B = parents.size(0), T = parents.size(1);
+  const auto opts = at::TensorOptions().device(dev).dtype(at::kLong);
+  Tensor masks = at::empty({B, T, (T + 63) / 64}, opts), depths = at::empty({B, T}, opts);
+  const Args<4> p({&parents, &counts, &masks, &depths});
+  check_rc(cea_tree_masks(p[0], p[1], p[2], p[3], stream_of(dev)), "tree_masks");
+  return {masks, depths};
+}
+
+// The pools of all layers as [N, P, H, page * D] (scales: [N, P, H, page]): the dimensions before the pages
+// have to collapse into one.
+cea_tensor pools_arg(const Tensor& t, int64_t rest, const char* what) {
+  cea_tensor a;
+  a.dtype = page_code_of(t.scalar_type());
+  TORCH_CHECK_NOT_IMPLEMENTED(a.dtype >= 0, "dtype ", t.scalar_type(), " is not supported by the kernels");
+  const int64_t lead = t.dim() - rest;
+  int64_t n = 1, stride = 0;
+  for (int64_t i = lead - 1; i >= 0; --i) {
+    if (t.size(i) == 1) continue;
+    TORCH_CHECK_VALUE(n == 1 || t.stride(i) == stride * n || t.numel() == 0,
+                      "paged_kv_keep: the dimensions of ", what, " before the pages must collapse");
+    if (n == 1) stride = t.stride(i);
+    n *= t.size(i);
+  }
+  a.data = t.numel() > 0 ? t.data_ptr() : nullptr;
+  a.ndim = 4;
+  a.size[0] = n, a.stride[0] = stride;
+  for (int i = 0; i < 3; ++i) a.size[1 + i] = t.size(lead + i), a.stride[1 + i] = t.stride(lead + i);
+  return a;
+}
+
+void paged_kv_keep(Tensor kv, const c10::optional<Tensor>& scales_in, const Tensor& tables_in, const Tensor& offsets_in,
+                   const c10::optional<Tensor>& counts_in, const Tensor& path_in) {
+  const Tensor scales = given(scales_in), counts0 = given(counts_in);
+  const at::Device dev = device_of({&kv, &scales, &tables_in, &offsets_in, &counts0, &path_in});
+  TORCH_CHECK_VALUE(kv.dim() >= 4, "kv must be [..., P, H, page, D]");
+  TORCH_CHECK_VALUE(!scales.defined() || scales.dim() == kv.dim() - 1, "scales must be [..., P, H, page]");
+  TORCH_CHECK_VALUE(scales.defined() == (kv.scalar_type() == at::kFloat8_e4m3fn),
+                    "scales go with float8_e4m3fn pages");
+  const int64_t page = kv.size(-2), D = kv.size(-1);
+  TORCH_CHECK_VALUE(kv.numel() == 0 || ((D == 1 || kv.stride(-1) == 1) && (page == 1 || kv.stride(-2) == D)),
+                    "paged_kv_keep: a head's slots of a page must be contiguous");
+  c10::DeviceGuard guard(dev);
+  const Tensor tables = as_i64(tables_in), offsets = as_i64(offsets_in), path = as_i64(path_in);
+  const Tensor counts = counts0.defined() ? as_i64(counts0) : counts0;
+  cea_tensor a = pools_arg(kv, 4, "kv"), sc;
+  a.size[3] = page * D, a.stride[3] = 1;
+  if (scales.defined()) sc = pools_arg(scales, 3, "scales");
+  const Args<4> p({&tables, &offsets, &counts, &path});
+  check_rc(cea_paged_kv_keep(&a, scales.defined() ? &sc : nullptr, (int32_t)page, p[0], p[1], p[2], p[3], stream_of(dev)),
+           "paged_kv_keep");
 }
 
 // A pool tensor with its page dimension `dim` as [N, P, E]: the dimensions before it have to
 // collapse into one, those after it to be contiguous (they are copied as bytes).
 cea_tensor pool_arg(const Tensor& t, int64_t dim) {
   cea_tensor a;
-  a.dtype = code_of(t.scalar_type());
+  a.dtype = page_code_of(t.scalar_type());
   TORCH_CHECK_NOT_IMPLEMENTED(a.dtype >= 0, "dtype ", t.scalar_type(), " is not supported by the kernels");
   TORCH_CHECK_VALUE(dim >= 0 && dim < t.dim(), "copy_pages: a pool of ", t.dim(), " dimensions has no dimension ",
                     dim);
@@ -680,9 +833,19 @@ TORCH_LIBRARY(collab_edge, m) {
   m.def("kv_append(Tensor(a!) cache_k, Tensor(b!) cache_v, Tensor(c!) cache_pos, int offset, Tensor k, "
         "Tensor v, Tensor pos, Tensor? cos, Tensor? sin) -> ()");
   m.def("paged_kv_append(Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor(c!)? pos_pages, Tensor tables, "
-        "Tensor offsets, Tensor? counts, Tensor k, Tensor v, Tensor? pos, Tensor? cos, Tensor? sin) -> ()");
+        "Tensor offsets, Tensor? counts, Tensor k, Tensor v, Tensor? pos, Tensor? cos, Tensor? sin, "
+        "Tensor(d!)? k_scales=None, Tensor(e!)? v_scales=None) -> ()");
+  m.def("paged_kv_read(Tensor k_pages, Tensor v_pages, Tensor? k_scales, Tensor? v_scales, Tensor tables, "
+        "Tensor offsets, Tensor? counts, int n, ScalarType dtype) -> Tensor[]");
   m.def("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor? pos_pages, Tensor tables, "
-        "Tensor lengths, Tensor q_pos, bool causal, float scale, int[]? kv_map, bool with_lse) -> Tensor[]");
+        "Tensor lengths, Tensor q_pos, bool causal, float scale, int[]? kv_map, bool with_lse, "
+        "Tensor? k_scales=None, Tensor? v_scales=None) -> Tensor[]");
+  m.def("paged_tree_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor? k_scales, Tensor? v_scales, "
+        "Tensor tables, Tensor lengths, Tensor counts, Tensor masks, float scale, int[]? kv_map, bool with_lse) "
+        "-> Tensor[]");
+  m.def("tree_masks(Tensor parents, Tensor? counts) -> Tensor[]");
+  m.def("paged_kv_keep(Tensor(a!) kv, Tensor(b!)? scales, Tensor tables, Tensor offsets, Tensor? counts, Tensor path) "
+        "-> ()");
   m.def("copy_pages(Tensor(a!)[] pools, int dim, Tensor src, Tensor dst) -> ()");
 }
 
@@ -707,6 +870,10 @@ TORCH_LIBRARY_IMPL(collab_edge, CompositeExplicitAutograd, m) {
   m.impl("linear_gated", linear_gated);
   m.impl("kv_append", kv_append);
   m.impl("paged_kv_append", paged_kv_append);
+  m.impl("paged_kv_read", paged_kv_read);
   m.impl("paged_attention", paged_attention);
+  m.impl("paged_tree_attention", paged_tree_attention);
+  m.impl("tree_masks", tree_masks);
+  m.impl("paged_kv_keep", paged_kv_keep);
   m.impl("copy_pages", copy_pages);
 }

@@ -9,10 +9,20 @@ of row ``b`` is place ``j % page`` of page ``tables[b, j // page]``.  The operat
 * :func:`paged_attention` / :func:`paged_attention_with_lse` - attention over a row's slots, one new
   token or a chunk of them, by the masking rule and with the ``(out, lse)`` convention of
   :mod:`.attention`,
+* :func:`paged_tree_attention` / :func:`paged_tree_attention_with_lse` - the same for a tree of drafted
+  tokens in the row's last slots (:func:`tree_masks` from the nodes' parents),
+* :func:`paged_kv_keep` - the accepted nodes' rows moved into line, in all layers' pools,
+* :func:`paged_kv_read` - a row's slots as contiguous keys and values,
 * :func:`copy_pages` - copies of whole pages through all layers' pools,
 
 read tables and lengths on the device, so nothing waits for the host and a captured graph follows
 what its tensors hold.  A page index outside the pool is a page that holds nothing.
+
+Pages of ``torch.float8_e4m3fn`` take half the memory, and half the reads of a decode step.  With them go
+``k_scales`` / ``v_scales`` ``[P, H, page]`` (uint8): the numbers ``q`` of a slot and head stand for
+``q * 2^(s - 127)``, ``s`` its scale byte.  The append chooses it per row: ``s - 127`` is the smallest
+whole number ``e >= -117`` with ``max |x| <= 448 * 2^e``.  Values keep 4 significant bits (half a step is
+``2^-4`` of a value); infinities and NaN become NaN.
 
 :class:`PageBook` keeps which sequence holds which pages (sharing, copy on write, compaction) on the
 host, and :class:`PagedKVCache` is the pools of a model's layers with their book.
@@ -36,7 +46,9 @@ def paged_kv_append(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.
                     cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,
                     counts: Optional[torch.Tensor] = None,
                     pos_pages: Optional[torch.Tensor] = None,
-                    pos: Optional[torch.Tensor] = None) -> None:
+                    pos: Optional[torch.Tensor] = None,
+                    k_scales: Optional[torch.Tensor] = None,
+                    v_scales: Optional[torch.Tensor] = None) -> None:
     """Writes ``k`` (rotated with ``cos``/``sin`` ``[B, n, D]`` when given) and ``v`` ``[B, n, H, D]``
     into row ``b``'s slots ``offsets[b] .. offsets[b] + counts[b] - 1``, in place.
 
@@ -45,34 +57,54 @@ def paged_kv_append(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.
     is that of :func:`~.layers.apply_rotary`, rounded once at its end (``apply_rotary`` rounds its
     products too).  A slot is written by one token: pages that rows share are full ones, or copied
     before (:func:`copy_pages`).  Tokens of slots that a row has no page for are dropped.
+
+    Into 8-bit pages (with both scales) go rows of bf16, f16 or f32; keys are rotated in f32 and rounded to
+    e4m3 alone.
     """
     if (cos is None) != (sin is None):
         raise ValueError("give both rotary tables or neither")
     if (pos is None) != (pos_pages is None):
         raise ValueError("give both pos and pos_pages or neither")
-    if v.dtype != k.dtype or k_pages.dtype != k.dtype or v_pages.dtype != k.dtype:
-        raise ValueError("k, v and the pages must share one dtype")
+    if v.dtype != k.dtype:
+        raise ValueError("k and v must share one dtype")
+    _check_pages(k.dtype, k_pages, v_pages, k_scales, v_scales, "k, v")
     nat.ops().paged_kv_append(k_pages, v_pages, pos_pages, tables, offsets, counts, k, v, pos, cos,
-                              sin)
+                              sin, k_scales, v_scales)
 
 
-def _attend(q, k_pages, v_pages, tables, lengths, q_pos, pos_pages, causal, scale, kv_map, with_lse):
+def _check_pages(dtype, k_pages, v_pages, k_scales, v_scales, what):
+    if k_scales is None and v_scales is None:
+        if k_pages.dtype != dtype or v_pages.dtype != dtype:
+            raise ValueError(f"{what}, k_pages and v_pages must share a dtype, got {dtype}, "
+                             f"{k_pages.dtype}, {v_pages.dtype} (8-bit pages need their scales)")
+    elif k_scales is None or v_scales is None:
+        raise ValueError("give both scales or neither")
+    elif k_pages.dtype != torch.float8_e4m3fn or v_pages.dtype != torch.float8_e4m3fn:
+        raise ValueError(f"scales go with float8_e4m3fn pages, got {k_pages.dtype}, {v_pages.dtype}")
+
+
+def _check_attention(q, k_pages, v_pages, k_scales, v_scales, scale, kv_map):
     if q.dim() != 4 or k_pages.dim() != 4:
         raise ValueError("q must be [B, S, H, D] and k_pages [P, H, page, D]")
-    if k_pages.dtype != q.dtype or v_pages.dtype != q.dtype:
-        raise ValueError(f"q, k_pages and v_pages must share a dtype, got {q.dtype}, "
-                         f"{k_pages.dtype}, {v_pages.dtype}")
+    _check_pages(q.dtype, k_pages, v_pages, k_scales, v_scales, "q")
     mapping = _kv_map_list(kv_map)
     _check_heads(q.shape[2], k_pages.shape[1], mapping)
-    scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale)
+    return 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale), mapping
+
+
+def _attend(q, k_pages, v_pages, tables, lengths, q_pos, pos_pages, causal, scale, kv_map, with_lse,
+            k_scales, v_scales):
+    scale, mapping = _check_attention(q, k_pages, v_pages, k_scales, v_scales, scale, kv_map)
     return nat.ops().paged_attention(q, k_pages, v_pages, pos_pages, tables, lengths, q_pos,
-                                     bool(causal), scale, mapping, with_lse)
+                                     bool(causal), scale, mapping, with_lse, k_scales, v_scales)
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                     tables: torch.Tensor, lengths: torch.Tensor, q_pos: torch.Tensor, *,
                     pos_pages: Optional[torch.Tensor] = None, causal: bool = True,
-                    scale: Optional[float] = None, kv_map: KVMap = None) -> torch.Tensor:
+                    scale: Optional[float] = None, kv_map: KVMap = None,
+                    k_scales: Optional[torch.Tensor] = None,
+                    v_scales: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of ``q`` ``[B, S, H, D]`` over slots ``0 .. lengths[b]-1`` of each row's pages;
     returns ``[B, S, H, D]`` in ``q.dtype``.
 
@@ -86,21 +118,114 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     bf16 and f16 chunks on the matrix cores are rounded to the type once before they weigh the values, so
     a row's result may differ by such a rounding with the number of tokens in the call.
     :func:`paged_attention_with_lse` keeps them in every form.
+
+    8-bit pages (with both scales) are attended as the values that they stand for, by queries of bf16, f16
+    or f32; f16 ones meet values that f16 holds (f16 rows leave no others in the pages).
     """
     return _attend(q, k_pages, v_pages, tables, lengths, q_pos, pos_pages, causal, scale, kv_map,
-                   False)[0]
+                   False, k_scales, v_scales)[0]
 
 
 def paged_attention_with_lse(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                              tables: torch.Tensor, lengths: torch.Tensor, q_pos: torch.Tensor, *,
                              pos_pages: Optional[torch.Tensor] = None, causal: bool = True,
-                             scale: Optional[float] = None, kv_map: KVMap = None
-                             ) -> Tuple[torch.Tensor, torch.Tensor]:
+                             scale: Optional[float] = None, kv_map: KVMap = None,
+                             k_scales: Optional[torch.Tensor] = None,
+                             v_scales: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """:func:`paged_attention` returning ``(out, lse)`` in accumulation precision, for the exact
     merges of partial results (:func:`~.attention.merge_attention`); empty rows give ``(0, -inf)``."""
     out, lse = _attend(q, k_pages, v_pages, tables, lengths, q_pos, pos_pages, causal, scale, kv_map,
-                       True)
+                       True, k_scales, v_scales)
     return out, lse
+
+
+def tree_masks(parents: torch.Tensor, counts: Optional[torch.Tensor] = None
+               ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``(masks, depths)`` of trees of up to 512 drafted tokens, on the device.
+
+    ``parents`` ``[B, T]`` names each node's parent, an earlier node; anything else (-1) makes a node
+    follow the sequence itself.  ``masks`` ``[B, T, ceil(T / 64)]`` (int64) has bit ``j % 64`` of word ``j //
+    64`` set in node ``i``'s row where ``j`` is ``i`` or one of its ancestors; ``depths`` ``[B, T]`` counts a
+    node's ancestors, so its position is that of the first new slot plus its depth.  Nodes from
+    ``counts[b]`` on have no bits and depth 0.
+    """
+    masks, depths = nat.ops().tree_masks(parents, counts)
+    return masks, depths
+
+
+def _tree(q, k_pages, v_pages, tables, lengths, counts, masks, scale, kv_map, with_lse, k_scales, v_scales):
+    scale, mapping = _check_attention(q, k_pages, v_pages, k_scales, v_scales, scale, kv_map)
+    if masks.dim() == 3 and masks.shape[0] == 1 and q.shape[0] != 1:
+        masks = masks.expand(q.shape[0], -1, -1)
+    return nat.ops().paged_tree_attention(q, k_pages, v_pages, k_scales, v_scales, tables, lengths, counts,
+                                          masks, scale, mapping, with_lse)
+
+
+def paged_tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                         tables: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor,
+                         masks: torch.Tensor, *, scale: Optional[float] = None, kv_map: KVMap = None,
+                         k_scales: Optional[torch.Tensor] = None,
+                         v_scales: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of ``q`` ``[B, T, H, D]``, the nodes of a tree of drafted tokens in the last ``counts[b]``
+    of each row's ``lengths[b]`` slots; returns ``[B, T, H, D]`` in ``q.dtype``.
+
+    Node ``i`` is in slot ``lengths[b] - counts[b] + i``, appended like any token.  It sees every slot
+    before the tree, and the slots of the nodes ``j`` whose bit is set in ``masks`` ``[B, T, ceil(T / 64)]``
+    (int64, bit ``j % 64`` of word ``j // 64``; a first dimension of 1 is every row's): those of
+    :func:`tree_masks`, or any other.  Nodes from ``counts[b]`` on are padding, and 0, as is a node that
+    sees nothing.  ``T`` is up to 512.  Precision, 8-bit pages and what hidden slots may hold are
+    :func:`paged_attention`'s.
+    """
+    return _tree(q, k_pages, v_pages, tables, lengths, counts, masks, scale, kv_map, False, k_scales,
+                 v_scales)[0]
+
+
+def paged_tree_attention_with_lse(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                                  tables: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor,
+                                  masks: torch.Tensor, *, scale: Optional[float] = None,
+                                  kv_map: KVMap = None, k_scales: Optional[torch.Tensor] = None,
+                                  v_scales: Optional[torch.Tensor] = None
+                                  ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """:func:`paged_tree_attention` returning ``(out, lse)`` in accumulation precision (for a rank that
+    holds the tree and a share of the sequence; the other ranks' shares by :func:`paged_attention_with_lse`)."""
+    out, lse = _tree(q, k_pages, v_pages, tables, lengths, counts, masks, scale, kv_map, True, k_scales,
+                     v_scales)
+    return out, lse
+
+
+def paged_kv_keep(kv: torch.Tensor, tables: torch.Tensor, offsets: torch.Tensor, path: torch.Tensor, *,
+                  counts: Optional[torch.Tensor] = None, scales: Optional[torch.Tensor] = None) -> None:
+    """Moves the accepted nodes of a tree into line, in place: slot ``offsets[b] + i`` of row ``b`` takes
+    what slot ``offsets[b] + path[b, i]`` held, in every pool of ``kv`` ``[..., P, H, page, D]`` (all
+    layers' keys and values; what precedes the pages collapses into one dimension) and of ``scales`` ``[...,
+    P, H, page]``, which 8-bit pages have.
+
+    ``path`` ``[B, n]`` names the accepted nodes in order, on the device, padded with -1.  A node is never
+    before its place in line, so entries below their index move nothing, nor do those from ``counts[b]`` on,
+    the row's nodes, where ``counts`` ``[B]`` is given.
+    """
+    nat.ops().paged_kv_keep(kv, scales, tables, offsets, counts, path)
+
+
+def paged_kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor,
+                  offsets: torch.Tensor, n: int, *, counts: Optional[torch.Tensor] = None,
+                  dtype: Optional[torch.dtype] = None, k_scales: Optional[torch.Tensor] = None,
+                  v_scales: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``(k, v)`` ``[B, n, H, D]``: what row ``b``'s slots ``offsets[b] .. offsets[b] + counts[b] - 1`` hold
+    (``n`` of them without ``counts``, and at most), and 0 from there on and where a row has no page.
+
+    8-bit pages are read as ``dtype``: bf16 (the default), f16 or f32, which hold their values as they are (but
+    for magnitudes outside f16's normal numbers, which are rounded); others as their own.
+    """
+    if dtype is None:
+        dtype = torch.bfloat16 if k_pages.dtype == torch.float8_e4m3fn else k_pages.dtype
+    if k_scales is None and v_scales is None:
+        _check_pages(dtype, k_pages, v_pages, None, None, "dtype")
+    else:
+        _check_pages(None, k_pages, v_pages, k_scales, v_scales, "dtype")
+    k, v = nat.ops().paged_kv_read(k_pages, v_pages, k_scales, v_scales, tables, offsets, counts,
+                                   operator.index(n), dtype)
+    return k, v
 
 
 def _page_list(pages: Union[torch.Tensor, Sequence[int]]) -> torch.Tensor:
@@ -282,6 +407,9 @@ class PagedStep:
         self.offsets, self.counts, self.lengths = self.buffer[:3 * rows].view(3, rows)
         self.cache, self.epoch = None, -1
         self.most = 0  # new tokens of a row at most
+        self.seqs: List[int] = []  # the rows' sequences, and their lengths before the step and with it
+        self.starts: List[int] = []
+        self.ends: List[int] = []
 
 
 class PagedKVCache:
@@ -296,6 +424,17 @@ class PagedKVCache:
             cache.append(layer, step, k, v, cos=cos, sin=sin)
             out = cache.attention(layer, step, q, q_pos)
 
+    With a tree of drafted tokens in each row::
+
+        step = cache.extend(seqs, nodes)
+        masks, depths = tree_masks(parents)
+        for layer in range(layers):                    # tables of position offset + depth
+            cache.append(layer, step, k, v, cos=cos, sin=sin)
+            out = cache.tree_attention(layer, step, q, masks)
+        cache.keep(step, path, kept)                   # the accepted nodes, the others are dropped
+
+    With ``dtype=torch.float8_e4m3fn`` keys and values are held in 8 bits, with their scale bytes.
+
     A step made before :meth:`fork`, :meth:`free`, :meth:`truncate` or :meth:`compact` is refused
     after it: its pages may be another's (a fork shares tokens, so they are written before it).
     Everything runs on the current stream.  A captured graph holds appends and attention; ``extend``
@@ -307,6 +446,8 @@ class PagedKVCache:
                  dtype: torch.dtype = torch.bfloat16, device="cuda", positions: bool = False) -> None:
         self.book = PageBook(pages, page)
         self.kv = torch.empty(layers, 2, pages, heads, page, head_dim, dtype=dtype, device=device)
+        self.scales = (torch.empty(layers, 2, pages, heads, page, dtype=torch.uint8, device=device)
+                       if dtype == torch.float8_e4m3fn else None)
         self.pos_pages = (torch.full((pages, page), -1, dtype=torch.int64, device=device)
                           if positions else None)
         self._epoch = 0
@@ -314,6 +455,12 @@ class PagedKVCache:
     def pages(self, layer: int) -> Tuple[torch.Tensor, torch.Tensor]:
         """``(k_pages, v_pages)`` of a layer."""
         return self.kv[layer, 0], self.kv[layer, 1]
+
+    def _scales(self, layer: int) -> Dict[str, torch.Tensor]:
+        """The arguments that 8-bit pages add to a call."""
+        if self.scales is None:
+            return {}
+        return {"k_scales": self.scales[layer, 0], "v_scales": self.scales[layer, 1]}
 
     @property
     def free_pages(self) -> int:
@@ -348,6 +495,8 @@ class PagedKVCache:
             return
         src, dst = zip(*moves)
         pools = [self.kv.flatten(0, 1)]
+        if self.scales is not None:
+            pools.append(self.scales.flatten(0, 1))
         if self.pos_pages is not None:
             pools.append(self.pos_pages.unsqueeze(0))
         copy_pages(pools, src, dst, dim=1)
@@ -401,6 +550,7 @@ class PagedKVCache:
             self.book._retract(seqs, offsets, copies)
             raise
         step.cache, step.epoch, step.most = self, self._epoch, max(counts, default=0)
+        step.seqs, step.starts, step.ends = seqs, offsets, host[2 * len(seqs):3 * len(seqs)]
         return step
 
     def _check(self, step: PagedStep) -> None:
@@ -419,7 +569,7 @@ class PagedKVCache:
             raise ValueError(f"the step adds up to {step.most} tokens to a row, k holds {k.shape[1]}")
         k_pages, v_pages = self.pages(layer)
         paged_kv_append(k_pages, v_pages, step.tables, step.offsets, k, v, cos=cos, sin=sin,
-                        counts=step.counts, pos_pages=self.pos_pages, pos=pos)
+                        counts=step.counts, pos_pages=self.pos_pages, pos=pos, **self._scales(layer))
 
     def attention(self, layer: int, step: PagedStep, q: torch.Tensor, q_pos: torch.Tensor, *,
                   causal: bool = True, scale: Optional[float] = None, kv_map: KVMap = None
@@ -427,7 +577,8 @@ class PagedKVCache:
         """A layer's attention over the step's sequences (:func:`paged_attention`)."""
         self._check(step)
         return paged_attention(q, *self.pages(layer), step.tables, step.lengths, q_pos,
-                               pos_pages=self.pos_pages, causal=causal, scale=scale, kv_map=kv_map)
+                               pos_pages=self.pos_pages, causal=causal, scale=scale, kv_map=kv_map,
+                               **self._scales(layer))
 
     def attention_with_lse(self, layer: int, step: PagedStep, q: torch.Tensor, q_pos: torch.Tensor,
                            *, causal: bool = True, scale: Optional[float] = None,
@@ -436,7 +587,49 @@ class PagedKVCache:
         self._check(step)
         return paged_attention_with_lse(q, *self.pages(layer), step.tables, step.lengths, q_pos,
                                         pos_pages=self.pos_pages, causal=causal, scale=scale,
-                                        kv_map=kv_map)
+                                        kv_map=kv_map, **self._scales(layer))
+
+    def tree_attention(self, layer: int, step: PagedStep, q: torch.Tensor, masks: torch.Tensor, *,
+                       scale: Optional[float] = None, kv_map: KVMap = None) -> torch.Tensor:
+        """A layer's attention of the step's new tokens as trees (:func:`paged_tree_attention`)."""
+        self._check_tree(step)
+        if q.dim() == 4 and q.shape[1] < step.most:
+            raise ValueError(f"the step adds up to {step.most} tokens to a row, q holds {q.shape[1]}")
+        return paged_tree_attention(q, *self.pages(layer), step.tables, step.lengths, step.counts, masks,
+                                    scale=scale, kv_map=kv_map, **self._scales(layer))
+
+    def _check_tree(self, step: PagedStep) -> None:
+        self._check(step)
+        if self.pos_pages is not None:
+            raise NotImplementedError("trees take a cache without positions of its own")
+
+    def keep(self, step: PagedStep, path: torch.Tensor, kept: Sequence[int]) -> None:
+        """Keeps the accepted nodes of the step's trees as the sequences' next tokens and drops the others:
+        row ``b`` keeps ``kept[b]`` nodes, the first of ``path[b]`` ``[B, n]`` (indices in order, on the
+        device).  ``kept`` is on the host, as the lengths are; the step is used up."""
+        self._check_tree(step)
+        self._outside_capture("keep")
+        kept = [operator.index(n) for n in kept]
+        if path.dim() != 2 or path.shape[0] != len(step.seqs) or len(kept) != len(step.seqs):
+            raise ValueError(f"path must be [{len(step.seqs)}, n], with a count each")
+        for seq, start, end, n in zip(step.seqs, step.starts, step.ends, kept):
+            if self.length(seq) != end:
+                raise RuntimeError(f"sequence {seq} was extended after the step")
+            if not 0 <= n <= min(end - start, path.shape[1]):
+                raise ValueError(f"sequence {seq} cannot keep {n} of {end - start} nodes, "
+                                 f"{path.shape[1]} in the path")
+        paged_kv_keep(self.kv, step.tables, step.offsets, path, counts=step.counts, scales=self.scales)
+        for seq, start, n in zip(step.seqs, step.starts, kept):
+            self.book.truncate(seq, start + n)
+        self._epoch += 1
+
+    def read(self, layer: int, step: PagedStep, n: int, *, dtype: Optional[torch.dtype] = None
+             ) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The first ``n`` slots of the step's sequences in a layer as ``(k, v)`` ``[B, n, H, D]``, 0 behind
+        a sequence's end (:func:`paged_kv_read`)."""
+        self._check(step)
+        return paged_kv_read(*self.pages(layer), step.tables, torch.zeros_like(step.lengths), n,
+                             counts=step.lengths, dtype=dtype, **self._scales(layer))
 
 
 __all__ = [
@@ -447,4 +640,9 @@ __all__ = [
     "paged_attention",
     "paged_attention_with_lse",
     "paged_kv_append",
+    "paged_kv_keep",
+    "paged_kv_read",
+    "paged_tree_attention",
+    "paged_tree_attention_with_lse",
+    "tree_masks",
 ]

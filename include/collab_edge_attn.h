@@ -32,6 +32,8 @@ extern "C" {
 #define CEA_F16 2
 #define CEA_F64 3
 #define CEA_I64 4
+#define CEA_F8 5   /* e4m3 with NaN and without infinities (torch.float8_e4m3fn): 8-bit pages */
+#define CEA_U8 6   /* the scale bytes of 8-bit pages                                         */
 
 /* status codes */
 #define CEA_OK 0
@@ -44,6 +46,8 @@ extern "C" {
 #define CEA_MAX_PARTS 16      /* maximum number of partial results one merge call combines   */
 #define CEA_MAX_MAPPED_HEADS 512 /* maximum query heads when an explicit kv_map is given     */
 
+#define CEA_MAX_TREE 512      /* maximum nodes of a row's tree of drafted tokens               */
+
 #define CEA_NOALLOC_SCRATCH_BYTES (32 << 20) /* per-GPU scratch of cea_attention_with_lse_noalloc */
 
 /* gated activations of cea_gated_mul: the reference's _ACTIVATIONS table (llama.py:44-49) */
@@ -54,7 +58,7 @@ extern "C" {
 
 typedef struct cea_tensor {
   void* data;                    /* device pointer to element [0, ..., 0]       */
-  int32_t dtype;                 /* CEA_F32 / CEA_BF16 / CEA_F16 / CEA_F64 / CEA_I64 */
+  int32_t dtype;                 /* one of the element types above             */
   int32_t ndim;                  /* number of used entries of size / stride    */
   int64_t size[CEA_MAX_DIMS];
   int64_t stride[CEA_MAX_DIMS];  /* in elements                                 */
@@ -413,6 +417,87 @@ int cea_paged_attention(const cea_tensor* q, const cea_tensor* k_pages, const ce
                         const cea_tensor* lengths, const cea_tensor* q_pos, int32_t causal,
                         double scale, const int32_t* kv_map, int32_t kv_map_len, cea_tensor* out,
                         cea_tensor* lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Pages of 8 bits.  k_pages, v_pages [P,H,page,D] are CEA_F8 and k_scales, v_scales [P,H,page] CEA_U8 (any
+ * strides): the numbers q of a slot and head stand for q * 2^(s - 127), s their scale byte.  D even.
+ *
+ * cea_paged_kv_append8 is cea_paged_kv_append into such pages, for bf16, f16 and f32 rows: K rotated in f32
+ * (products and sum rounded once each), then every row by its largest finite magnitude m,
+ *   e = the smallest whole number >= -117 with m <= 448 * 2^e,  s = e + 127,  q = x * 2^-e rounded to nearest
+ * (ties to even).  The rounding to 4 significant bits is all that is lost: within half a step, 2^-4 of a value
+ * (2^-10 * 2^e for those below 2^-6 * 2^e).  Values that are not finite become NaN; finite ones beyond the row's
+ * type count as its largest, and a row whose q would read back beyond the type is cut at q = 240.
+ *
+ * cea_paged_attention8 is cea_paged_attention over such pages, q bf16, f16 or f32.  f16 queries meet values
+ * that f16 holds: pages that f16 rows were appended to have no others.
+ */
+int cea_paged_kv_append8(const cea_tensor* k, const cea_tensor* v, const cea_tensor* pos,
+                         const cea_tensor* cos, const cea_tensor* sin, const cea_tensor* tables,
+                         const cea_tensor* offsets, const cea_tensor* counts, cea_tensor* k_pages,
+                         cea_tensor* v_pages, cea_tensor* k_scales, cea_tensor* v_scales,
+                         cea_tensor* pos_pages, void* stream);
+int cea_paged_attention8_workspace(const cea_tensor* q, const cea_tensor* k_pages, const cea_tensor* v_pages,
+                                   const cea_tensor* k_scales, const cea_tensor* v_scales,
+                                   const cea_tensor* pos_pages, const cea_tensor* tables,
+                                   const cea_tensor* lengths, const cea_tensor* q_pos, int32_t causal,
+                                   double scale, const int32_t* kv_map, int32_t kv_map_len,
+                                   const cea_tensor* out, const cea_tensor* lse, size_t* bytes);
+int cea_paged_attention8(const cea_tensor* q, const cea_tensor* k_pages, const cea_tensor* v_pages,
+                         const cea_tensor* k_scales, const cea_tensor* v_scales,
+                         const cea_tensor* pos_pages, const cea_tensor* tables,
+                         const cea_tensor* lengths, const cea_tensor* q_pos, int32_t causal,
+                         double scale, const int32_t* kv_map, int32_t kv_map_len, cea_tensor* out,
+                         cea_tensor* lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Reads slots offsets[b] .. offsets[b] + counts[b] - 1 (n of them with counts NULL, and at most) of every row
+ * into k, v [B,n,H,D]; slots that a row has no page for, and places from counts[b] on, are 0.  From 8-bit pages
+ * (with their scales) into bf16, f16 or f32, rounded once (f16 alone has values to round: those below its normal
+ * numbers or beyond its largest); from other pages (scales NULL) into their own type.
+ */
+int cea_paged_kv_read(const cea_tensor* k_pages, const cea_tensor* v_pages, const cea_tensor* k_scales,
+                      const cea_tensor* v_scales, const cea_tensor* tables, const cea_tensor* offsets,
+                      const cea_tensor* counts, cea_tensor* k, cea_tensor* v, void* stream);
+
+/*
+ * Drafted tokens as a tree.  q [B,T,Hq,D] are the nodes in the last counts[b] slots of each row, node i in slot
+ * lengths[b] - counts[b] + i; node i sees every slot before them, and the slot of node j where bit j % 64 of
+ * masks[b, i, j / 64] is set, masks int64 [B,T,ceil(T/64)] (any strides, any bits: those of its ancestors and
+ * itself make a tree).  Nodes from counts[b] on are padding: their results are those of a row without keys.
+ * Pages of any type, 8 bits with their scales (else NULL); T up to CEA_MAX_TREE; out, lse and the workspace as
+ * cea_paged_attention's.
+ */
+int cea_paged_tree_attention_workspace(const cea_tensor* q, const cea_tensor* k_pages, const cea_tensor* v_pages,
+                                       const cea_tensor* k_scales, const cea_tensor* v_scales,
+                                       const cea_tensor* tables, const cea_tensor* lengths,
+                                       const cea_tensor* counts, const cea_tensor* masks, double scale,
+                                       const int32_t* kv_map, int32_t kv_map_len, const cea_tensor* out,
+                                       const cea_tensor* lse, size_t* bytes);
+int cea_paged_tree_attention(const cea_tensor* q, const cea_tensor* k_pages, const cea_tensor* v_pages,
+                             const cea_tensor* k_scales, const cea_tensor* v_scales, const cea_tensor* tables,
+                             const cea_tensor* lengths, const cea_tensor* counts, const cea_tensor* masks,
+                             double scale, const int32_t* kv_map, int32_t kv_map_len, cea_tensor* out,
+                             cea_tensor* lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * masks[b, i]: the bits of node i and of its ancestors; depths[b, i]: how many ancestors it has (so a node's
+ * position is that of the first free slot plus its depth).  parents [B,T] int64, T up to CEA_MAX_TREE: the index
+ * of an earlier node, and anything else for a node that follows the sequence itself.  Nodes from counts[b] on
+ * (counts NULL: none) have no bits and depth 0.  masks [B,T,ceil(T/64)], depths [B,T] int64.
+ */
+int cea_tree_masks(const cea_tensor* parents, const cea_tensor* counts, cea_tensor* masks,
+                   cea_tensor* depths, void* stream);
+
+/*
+ * Keeps the accepted nodes of a tree whose first node is in slot offsets[b]: slot offsets[b] + i takes what slot
+ * offsets[b] + path[b, i] held before the call, in all N pools of kv [N,P,H,page*D] (the layers' keys and values;
+ * any type, `page` slots of D contiguous elements) and, for 8-bit pages, scales [N,P,H,page] (else NULL).  path
+ * [B,n] int64 on the device; entries below i (-1: none) move nothing, and nodes in order need no others, nor do
+ * entries from counts[b] on (the row's nodes; NULL: any).
+ */
+int cea_paged_kv_keep(cea_tensor* kv, cea_tensor* scales, int32_t page, const cea_tensor* tables,
+                      const cea_tensor* offsets, const cea_tensor* counts, const cea_tensor* path, void* stream);
 
 /*
  * Copies page src[i] to page dst[i] (host arrays of `moves` indices) in every pool: n tensors
