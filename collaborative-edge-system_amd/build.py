@@ -52,7 +52,9 @@ FILE_FLAGS = {
     "attn_prefill.hip": ["-fno-honor-nans", "-Wno-inline-asm"],
     "attn_decode.hip": ["-fno-honor-nans", "-Wno-inline-asm"],
     "paged_chunk.hip": ["-fno-honor-nans", "-Wno-inline-asm"],
+    "paged_chunk8.hip": ["-fno-honor-nans", "-Wno-inline-asm"],
     "paged_token.hip": ["-Wno-inline-asm"],
+    "paged_token8.hip": ["-Wno-inline-asm"],
     # the layer ops round every product to the tensor dtype before the next add, as the
     # reference's separate tensor ops do: no multiply-add contraction (without this flag
     # x*cos + rot*sin in f16 becomes an f16 fma, and f32 products fuse into the sums)

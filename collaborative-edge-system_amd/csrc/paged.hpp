@@ -74,14 +74,17 @@ __device__ __forceinline__ uint64_t tree_word(const PagedParams& p, int b, int64
   return left >= 64 ? x : x & (((uint64_t)1 << left) - 1);
 }
 
-// Layouts that the matrix-core kernels read: 16-bit types, head size 64 or 128, pages of a multiple
-// of 16 slots, rows of 16-byte vectors, contiguous positions.
+// What decides whether a query sees a slot: its number, a position in the pool, or a tree's mask.
+enum Vis { kNumber = 0, kPosition = 1, kTree = 2 };
+
+// Layouts that the matrix-core kernels read: 16-bit queries, pages of their type or of 8 bits, head size 64 or
+// 128, pages of a multiple of 16 slots, rows of 16-byte vectors, contiguous positions and scales.
 bool paged_tiles_supported(const PagedParams& p);
 
 // A few new tokens per row (at most 16 query rows of a unit; an explicit head map within kPagedMapHeads).
 bool paged_token_supported(const PagedParams& p, const HeadMap& map);
 size_t paged_token_workspace_bytes(int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int group, int64_t D,
-                                   int64_t slots);
+                                   int64_t slots, bool f8);
 int launch_paged_token(const PagedParams& p, const HeadMap& map, void* ws, hipStream_t s);
 
 // Any number of new tokens per row.  Scratch: tile summaries with positions in the pool, and the partial

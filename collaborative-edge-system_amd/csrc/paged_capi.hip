@@ -176,7 +176,7 @@ int prepare_attention(Attention& c, const AttentionArgs& a) {
     const bool few = Sq == 1 || group <= 0 || rows <= 16 || (rows <= 32 && D == 64 && slots <= 1024);
     if (few && paged_token_supported(p, c.map)) {
       c.form = Form::token;
-      c.bytes = paged_token_workspace_bytes(B, Sq, Hq, Hkv, group, D, slots);
+      c.bytes = paged_token_workspace_bytes(B, Sq, Hq, Hkv, group, D, slots, bytes8);
     } else if (paged_chunk_supported(p, c.map)) {
       c.form = Form::chunk;
       c.bytes = paged_chunk_workspace_bytes(B, Sq, Hq, group, D, slots, p.pos != nullptr);
@@ -204,7 +204,6 @@ bool pages_apart(const cea_tensor& t) {
 }  // namespace
 
 bool paged_tiles_supported(const PagedParams& p) {
-  if (p.kv_dtype == CEA_F8 || p.masks) return false;
   if (!(p.in_dtype == CEA_BF16 || p.in_dtype == CEA_F16) || !(p.D == 64 || p.D == 128)) return false;
   if (p.page % 16 != 0 || p.W == 0) return false;
   // slots and places in 32 bits, and page numbers by multiplication (u / m = u * ceil(2^32 / m) >> 32
@@ -213,11 +212,19 @@ bool paged_tiles_supported(const PagedParams& p) {
   if (slots >= (int64_t)1 << 30 || slots / 16 * (p.page / 16) >= (int64_t)1 << 32) return false;
   // exponents take |scale| * log2(e) as a factor, which has to be a normal number
   if (!(fabs(p.scale) >= 1e-30 && fabs(p.scale) <= 1e30)) return false;
-  const int64_t s8[] = {p.qs_b, p.qs_s, p.qs_h, p.ks_p, p.ks_h, p.ks_s, p.vs_p, p.vs_h, p.vs_s};
-  for (int64_t s : s8)
+  for (int64_t s : {p.qs_b, p.qs_s, p.qs_h})
     if (s % 8) return false;
-  for (const void* d : {p.q, p.k, p.v})
+  const int64_t per16 = p.kv_dtype == CEA_F8 ? 16 : 8;
+  for (int64_t s : {p.ks_p, p.ks_h, p.ks_s, p.vs_p, p.vs_h, p.vs_s})
+    if (s % per16) return false;
+  for (const void* d : {p.q, p.k, p.v, (const void*)p.k_scales, (const void*)p.v_scales})
     if ((uintptr_t)d % 16) return false;
+  // (16 scale bytes at a time, one after the other)
+  if (p.kv_dtype == CEA_F8) {
+    for (int64_t s : {p.kss_p, p.kss_h, p.vss_p, p.vss_h})
+      if (s % 16) return false;
+    if (p.kss_s != 1 || p.vss_s != 1) return false;
+  }
   // a 64-row tile spans less than 2^31 bytes
   for (int64_t s : {p.ks_s, p.vs_s})
     if (s < p.D || s >= (int64_t)1 << 23) return false;
@@ -351,7 +358,7 @@ size_t cea_paged_attention_workspace_bytes(int64_t B, int64_t Sq, int64_t Hq, in
   size_t most = 0;
   for (const int group : {0, Hq % Hkv == 0 ? (int)(Hq / Hkv) : 0})
     if (in_dtype == CEA_F32) most = std::max(most, paged_f32_workspace_bytes(B, Sq, Hq, group, D, slots));
-    else most = std::max({most, paged_token_workspace_bytes(B, Sq, Hq, Hkv, group, D, slots),
+    else most = std::max({most, paged_token_workspace_bytes(B, Sq, Hq, Hkv, group, D, slots, false),
                      paged_chunk_workspace_bytes(B, Sq, Hq, group, D, slots, true)});
   return most;
 }

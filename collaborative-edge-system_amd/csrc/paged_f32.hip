@@ -15,6 +15,8 @@
 //     into up to 16 key splits by the table's width (each takes an equal run of the row's own tiles),
 //     merged by the list merge.
 //   * Bound by latency: a prompt of 512 keys is 4 tiles a wave, 14.2 us for 8 heads of 64.
+//   * A tree's nodes see the slots before it as any rows do; in the last tiles a row's bits of the mask are read where
+//     they are needed, a few words of L2.
 //   * A value that is not finite and hidden from some query would reach it as 0 * inf.  The results show
 //     that (they are not finite either), and the workgroup then goes over its tiles again and sums products
 //     one by one, over each query's visible keys.
@@ -79,8 +81,9 @@ __device__ __forceinline__ float xor_sum(float x) {
   return __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
 }
 
-template <int D, bool POS>
+template <int D, int VIS>
 __global__ __launch_bounds__(NW * 64) void paged_f32_kernel(const F32Params t) {
+  constexpr bool POS = VIS == kPosition, TREE = VIS == kTree;
   constexpr int NB = D / 16;    // output feature blocks, and consecutive features of a lane
   const PagedParams& p = t.p;
   extern __shared__ __attribute__((aligned(16))) float red_o[];  // [NW][QB][D + 4]
@@ -101,11 +104,14 @@ __global__ __launch_bounds__(NW * 64) void paged_f32_kernel(const F32Params t) {
   const int row = qb * QB + c16;
   const bool row_ok = row < p.Sq * t.G;
   const int s = row_ok ? row / t.G : 0, h = h0 + (row_ok ? row - s * t.G : 0);
-  const int64_t qpos = p.q_pos[b * p.qps_b + (int64_t)s * p.qps_s];
+  const int64_t qpos = TREE ? 0 : p.q_pos[b * p.qps_b + (int64_t)s * p.qps_s];
   const int n = uniform((int)paged_slots(p, b));
-  // this lane's row sees slots [0, lim) (POS: of those, the positions up to qpos)
-  const bool sees = row_ok && (!p.causal || qpos >= 0);
-  const int lim = !sees ? 0 : p.causal && !POS && qpos < n ? (int)qpos + 1 : n;
+  const TreeOf nodes = TREE ? tree_of(p, b) : TreeOf{0, 0};
+  const int base = (int)max(nodes.base, -((int64_t)1 << 30));
+  // this lane's row sees slots [0, lim) (POS: of those, the positions up to qpos; TREE: those before base, and
+  // its nodes)
+  const bool sees = row_ok && (TREE ? s < nodes.nodes : !p.causal || qpos >= 0);
+  const int lim = !sees ? 0 : !TREE && p.causal && !POS && qpos < n ? (int)qpos + 1 : n;
   int lim_max = lim;
 #pragma unroll
   for (int off = 8; off >= 1; off >>= 1) lim_max = max(lim_max, __shfl_xor(lim_max, off, 64));
@@ -168,6 +174,10 @@ __global__ __launch_bounds__(NW * 64) void paged_f32_kernel(const F32Params t) {
       for (int i = 0; i < 4; ++i) {
         // (a position of -1, of a hole or of no page, is past every limit)
         vis[i] = sees && tile * KT + 4 * i + g < lim && cur.pos[i] >= 0 && (!POS || !p.causal || cur.pos[i] <= qpos);
+        if constexpr (TREE) {
+          const int node = tile * KT + 4 * i + g - base;
+          if (vis[i] && node >= 0) vis[i] = node < p.Sq && ((tree_word(p, b, s, node >> 6) >> (node & 63)) & 1);
+        }
         any = any || vis[i];
       }
       if (__ballot(any) != 0) {
@@ -270,13 +280,13 @@ __global__ __launch_bounds__(NW * 64) void paged_f32_kernel(const F32Params t) {
   }
 }
 
-template <int D, bool POS> int launch_form(const F32Params& t, hipStream_t st) {
+template <int D, int VIS> int launch_form(const F32Params& t, hipStream_t st) {
   constexpr int lds = NW * QB * (D + 4) * (int)sizeof(float);
-  const hipError_t e = reserve_lds<paged_f32_kernel<D, POS>>(lds);
+  const hipError_t e = reserve_lds<paged_f32_kernel<D, VIS>>(lds);
   CEA_REQUIRE(e == hipSuccess, CEA_ELAUNCH, "paged_attention: cannot reserve %d bytes of LDS: %s", lds,
               hipGetErrorString(e));
   const int64_t grid = (int64_t)t.nqb * (t.p.Hq / t.G) * t.p.B * t.splits;
-  hipLaunchKernelGGL((paged_f32_kernel<D, POS>), dim3((unsigned)grid), dim3(NW * 64), lds, st, t);
+  hipLaunchKernelGGL((paged_f32_kernel<D, VIS>), dim3((unsigned)grid), dim3(NW * 64), lds, st, t);
   CEA_CHECK_LAUNCH("paged_f32");
   return CEA_OK;
 }
@@ -315,7 +325,7 @@ size_t paged_f32_workspace_bytes(int64_t B, int64_t Sq, int64_t Hq, int group, i
 }
 
 bool paged_f32_supported(const PagedParams& p, const HeadMap& map) {
-  if (p.kv_dtype != CEA_F32 || p.masks || !(p.D == 64 || p.D == 128) || p.page % KT != 0 || p.W == 0) return false;
+  if (p.kv_dtype != CEA_F32 || !(p.D == 64 || p.D == 128) || p.page % KT != 0 || p.W == 0) return false;
   if (map.group <= 0 && (p.Hq > kPagedMapHeads || p.Hkv > 256)) return false;
   if (!std::isfinite(p.scale)) return false;
   // (32-bit slots; u / m = u * ceil(2^32 / m) >> 32 while u * m < 2^32)
@@ -348,8 +358,10 @@ int launch_paged_f32(const PagedParams& o, const HeadMap& map, void* ws, hipStre
     t.split_out = (int64_t)(r.part_out / sizeof(float)), t.split_lse = (int64_t)(r.part_lse / sizeof(float));
   }
   int rc;
-  if (o.D == 64) rc = o.pos ? launch_form<64, true>(t, st) : launch_form<64, false>(t, st);
-  else rc = o.pos ? launch_form<128, true>(t, st) : launch_form<128, false>(t, st);
+  if (o.D == 64)
+    rc = o.masks ? launch_form<64, kTree>(t, st) : o.pos ? launch_form<64, kPosition>(t, st) : launch_form<64, kNumber>(t, st);
+  else
+    rc = o.masks ? launch_form<128, kTree>(t, st) : o.pos ? launch_form<128, kPosition>(t, st) : launch_form<128, kNumber>(t, st);
   if (rc || r.splits == 1) return rc;
   return merge_paged_splits(o, t.p, r.splits, t.split_out, t.split_lse, st);
 }

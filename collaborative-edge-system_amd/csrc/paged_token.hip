@@ -28,40 +28,12 @@
 //     value that is not finite would meet the zero probabilities of hidden keys and the zero or
 //     negative later pieces of visible ones: a tile that holds one (rare; a look of two instructions
 //     per register) sums its products one by one, over each row's visible keys only.
-#include <math.h>
-
-#include <algorithm>
-
-#include "cea_lds_dma.hpp"
-#include "cea_mfma16.hpp"
-#include "paged.hpp"
+#include "paged_token.hpp"
 
 namespace cea {
 namespace {
 
 constexpr int TK = 16;                // keys per tile
-constexpr int ROWS = 16;              // query rows of a unit at most
-constexpr float kRescaleLog2 = 8.0f;  // the reference maximum moves when a row's grows by 2^8
-
-typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-typedef const int64_t __attribute__((address_space(4))) * scalar_i64;  // read through the scalar cache
-
-struct TokenParams {
-  PagedParams p;
-  int32_t G, units;       // query heads of a unit, units of a row
-  int32_t page16;         // page / 16
-  uint32_t magic;         // ceil(2^32 / page16), for page16 > 1
-  int32_t wgs;            // workgroups at most
-  float* partial;         // 2 x wgs parts of [rows][D + 2]: o, m, l
-  uint8_t kv[kPagedMapHeads];  // explicit head map (p.group == 0)
-};
-
-// The kernel's arguments behind a pointer that the compiler knows nothing about.
-typedef const void __attribute__((address_space(4))) * kernel_args_ptr;
-__device__ __forceinline__ kernel_args_ptr opaque(kernel_args_ptr p) {
-  asm volatile("" : "+s"(p));
-  return p;
-}
 
 template <int D> struct TLayout {
   static constexpr int ROW = D * 2;
@@ -72,104 +44,9 @@ template <int D> struct TLayout {
   static constexpr int LOADS = TILE_BYTES / 1024;
 };
 
-__device__ __forceinline__ int scan64(int v) {  // inclusive prefix sum over the lanes
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int x = __shfl_up(v, off, 64);
-    if (lane >= off) v += x;
-  }
-  return v;
-}
-
-// Slots of row b, a row that the whole wave works on (a scalar read).
-__device__ __forceinline__ int slots_of(const PagedParams& p, int b) {
-  const int64_t n = ((scalar_i64)(uintptr_t)p.lengths)[b * p.ns_b], cap = (int64_t)p.W * p.page;
-  return (int)(n < 0 ? 0 : n < cap ? n : cap);
-}
-
-// Key blocks of row b, at least one (which writes the result of a row without keys).
-template <int BLK> __device__ __forceinline__ int blocks_of(const PagedParams& p, int b) {
-  const int n = (int)paged_slots(p, b);
-  return n > 0 ? (n + BLK - 1) / BLK : 1;
-}
-
-// The line of blocks: the rows one after the other, each `units` stretches of its blocks.  Every
-// workgroup measures it from the lengths for itself, one wave-wide scan per 64 rows.
-struct Line {
-  int total;  // blocks of the line
-  int sums;   // this lane's prefix sum over the first 64 rows' blocks
-};
-struct LineRow {
-  int b, first, blocks;  // a row, the place of its first block, the blocks of each stretch
-};
-
-template <int BLK> __device__ __forceinline__ int prefix64(const PagedParams& p, int b0) {
-  const int b = b0 + (threadIdx.x & 63);
-  return scan64(b < p.B ? blocks_of<BLK>(p, b) : 0);
-}
-
-template <int BLK> __device__ __forceinline__ Line line_of(const TokenParams& t) {
-  Line line;
-  line.sums = prefix64<BLK>(t.p, 0);
-  line.total = __builtin_amdgcn_readlane(line.sums, 63);
-  for (int b0 = 64; b0 < t.p.B; b0 += 64)
-    line.total += __builtin_amdgcn_readlane(prefix64<BLK>(t.p, b0), 63);
-  line.total *= t.units;
-  return line;
-}
-
-// The row that holds block `at` (0 <= at < total), or with at < 0 row `b`.
-template <int BLK>
-__device__ __forceinline__ LineRow row_of(const TokenParams& t, const Line& line, int at, int b) {
-  LineRow r = {0, 0, 1};
-  int before = 0;
-  for (int b0 = 0; b0 < t.p.B; b0 += 64) {
-    const int sums = b0 == 0 ? line.sums : prefix64<BLK>(t.p, b0);
-    const uint64_t found =
-        at >= 0 ? __ballot((before + sums) * t.units > at) : (b - b0 < 64 ? 1ull << (b - b0) : 0ull);
-    if (found != 0) {
-      const int l = (int)__builtin_ctzll(found);
-      const int begin = l > 0 ? __builtin_amdgcn_readlane(sums, l - 1) : 0;
-      r.b = b0 + l;
-      r.first = (before + begin) * t.units;
-      r.blocks = __builtin_amdgcn_readlane(sums, l) - begin;
-      break;
-    }
-    before += __builtin_amdgcn_readlane(sums, 63);
-  }
-  return r;
-}
-
-// The line cut into runs: the first `more` workgroups take `run + 1` blocks, the others `run`.
-struct Runs {
-  int run, more;
-  __device__ __forceinline__ int start(int wg) const { return wg * run + min(wg, more); }
-  __device__ __forceinline__ int wg_of(int at) const {  // the workgroup that takes block `at`
-    const int big = more * (run + 1);
-    return at < big ? at / (run + 1) : more + (at - big) / run;
-  }
-};
-__device__ __forceinline__ Runs runs_of(const TokenParams& t, int total) {
-  const int wgs = max(1, min(t.wgs, total));
-  Runs r;
-  r.run = total / wgs;
-  r.more = total - r.run * wgs;
-  return r;
-}
-
-template <typename O> __device__ __forceinline__ void write_out(const PagedParams& p, int b, int s, int h, int d,
-                                                                float x) {
-  ((O*)p.out)[b * p.os_b + s * p.os_s + h * p.os_h + d] = (O)x;
-}
-template <typename T> __device__ __forceinline__ void write_row(const PagedParams& p, int b, int s, int h, int d,
-                                                                float x) {
-  if (p.out_dtype == CEA_F32) write_out<float>(p, b, s, h, d, x);
-  else write_out<T>(p, b, s, h, d, x);
-}
-
-template <typename T, int D, bool POS, int NW, bool SPLIT, int PC>
+template <typename T, int D, int VIS, int NW, bool SPLIT, int PC>
 __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void paged_token_kernel(const TokenParams args) {
+  constexpr bool POS = VIS == kPosition, TREE = VIS == kTree;
   typedef TLayout<D> L;
   typedef typename Mfma16<T>::frag8 frag8;
   constexpr int BLK = NW * TK;
@@ -280,7 +157,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void paged_token_kernel(c
     if (s0 < end) load_tile(s0, id0, 0);
     if (s0 + BLK < end) load_tile(s0 + BLK, id1, 1);
 
-    const int64_t qpos = p.q_pos[b * p.qps_b + rs * p.qps_s];
+    const int64_t qpos = TREE ? 0 : p.q_pos[b * p.qps_b + rs * p.qps_s];
     // this lane's query fragments (B operand of S = K.Q^T), the sign of a negative scale folded in
     frag8 qf[D / 32];
     {
@@ -298,11 +175,15 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void paged_token_kernel(c
     // this lane's row sees slots [0, lim) by their number, all rows see [0, lim_all), none beyond
     // lim_any (with positions in the pool the slots say nothing but where the row ends)
     int lim = n, lim_all = n, lim_any = n;
+    TreeRow tree = {0, 0};
+    bool row_sees = true;
     if (POS && p.causal && __ballot(row_real && qpos >= 0) == 0) lim_any = 0;
-    if (!POS && p.causal) {
-      lim = qpos >= n ? n : (int)max((int64_t)0, qpos + 1);
+    if (TREE || (!POS && p.causal)) {
+      const Limits x = limits_of<TREE>(p, b, n, qpos, rs, tree);
+      lim = x.lim;
+      row_sees = x.any > 0;
       lim_all = row_real ? lim : n;
-      lim_any = row_real ? lim : 0;
+      lim_any = row_real ? x.any : 0;
       if (p.Sq > 1) {
 #pragma unroll
         for (int off = 8; off >= 1; off >>= 1) {
@@ -346,9 +227,16 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void paged_token_kernel(c
         whole = __ballot(row_real && vis != 15u) == 0;
       } else {
         whole = ok && s0 + TK <= lim_all;
+        if constexpr (TREE) {
+          if (ok && row_sees) vis = tree_window<4>(tree, s0 + grp * 4);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (ok && s0 + grp * 4 + i < lim) vis |= 1u << i;
+          for (int i = 0; i < 4; ++i)
+            if (s0 + grp * 4 + i >= n) vis &= ~(1u << i);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (ok && s0 + grp * 4 + i < lim) vis |= 1u << i;
+        }
       }
       if (!row_real) vis = 0;
       // a value that is not finite (products with zero or negative pieces would spoil it)
@@ -431,55 +319,8 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void paged_token_kernel(c
       buf ^= 1;
     }
 
-    // ---- join the waves.  A row's sum is 0 exactly where it saw no key (a NaN is kept).
-    const float l_row = sum_halves(sum_rows16(l_run));
-    if (grp == 0) red_ml[row][wave] = make_float2(m_run, l_row);
-    float* red_o = (float*)wb;  // this wave's own buffers, no longer read as tiles
-    if (row_real) {
-#pragma unroll
-      for (int dt = 0; dt < D / 16; ++dt) *(f32x4*)(red_o + row * D + dt * 16 + grp * 4) = o[dt];
-    }
-    __syncthreads();
-    const bool all = lo == 0 && hi == blocks;
-    float* part = t.partial + ((int64_t)blockIdx.x * 2 + (lo == 0 ? 1 : 0)) * nrows * (D + 2);
-    for (int i = tid; i < nrows * D; i += NW * 64) {
-      const int r = i / D, d = i % D;
-      float2 ml[NW];
-      float x[NW];
-#pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        ml[w] = red_ml[r][w];
-        x[w] = ((const float*)(dsmem + w * L::WAVE_BYTES))[i];
-      }
-      float M = -__builtin_inff();  // of the raw scores
-#pragma unroll
-      for (int w = 0; w < NW; ++w) M = fmaxf(M, ml[w].x);
-      const float shift = M == -__builtin_inff() ? 0.f : M;
-      float acc = 0.f, sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        // (a wave that saw nothing has zeros; one whose scores are all NaN keeps its NaN)
-        const float wt = ml[w].x == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f((ml[w].x - shift) * c);
-        acc = __builtin_fmaf(x[w], wt, acc);
-        sum = __builtin_fmaf(ml[w].y, wt, sum);
-      }
-      acc *= 1.f / kPScale;
-      M *= fabsf(scale);
-      if (!SPLIT || all) {
-        const int s = r / t.G, h = unit * t.G + r - s * t.G;
-        write_row<T>(p, b, s, h, d, sum == 0.f ? 0.f : acc / sum);
-        if (p.lse && d == 0)
-          ((float*)p.lse)[b * p.ls_b + h * p.ls_h + s * p.ls_s] =
-              sum == 0.f ? -__builtin_inff() : (M == -__builtin_inff() ? 0.f : M) + logf(sum);
-      } else {
-        // non-temporal: written back past the caches, they disturb the reads of other workgroups least
-        __builtin_nontemporal_store(acc, part + r * (D + 2) + d);
-        if (d == 0) {
-          __builtin_nontemporal_store(M, part + r * (D + 2) + D);
-          __builtin_nontemporal_store(sum, part + r * (D + 2) + D + 1);
-        }
-      }
-    }
+    finish_unit<T, D, NW, !SPLIT>(t, o, m_run, l_run, red_ml, dsmem, L::WAVE_BYTES, b, unit, lo == 0, hi == blocks,
+                                  1.f / kPScale);
     if constexpr (!SPLIT) return;
     left -= hi - lo;
     if (left == 0) return;
@@ -494,93 +335,19 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void paged_token_kernel(c
   }
 }
 
-// Joins the parts of the units that the runs cut, one workgroup per (row, token, query head): every
-// wave weighs 64 parts at a time, a part a lane, and sums every fourth part's features, whose reads
-// are under way by then (one trip to memory for the lengths and one for up to 64 parts).
-template <typename T, int D, int NW>
-__global__ __launch_bounds__(256) void paged_token_join_kernel(const TokenParams t) {
-  constexpr int FPL = D / 64;  // features per lane
-  constexpr int PER = 16;      // parts of a wave among 64
-  __shared__ float o_s[4][D];
-  const PagedParams& p = t.p;
-  const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63;
-  const int h = blockIdx.x % p.Hq, s = (blockIdx.x / p.Hq) % p.Sq, b = blockIdx.x / (p.Hq * p.Sq);
-  const Line line = line_of<NW * TK>(t);
-  const LineRow r = row_of<NW * TK>(t, line, -1, b);
-  const Runs runs = runs_of(t, line.total);
-  const int unit = h / t.G, start = r.first + unit * r.blocks;
-  const int w0 = runs.wg_of(start), n = runs.wg_of(start + r.blocks - 1) - w0 + 1;
-  if (n == 1) return;  // finished by its workgroup
-  const int nrows = p.Sq * t.G;
-  // the first part is its workgroup's last unit (slot 1), the others' their first (slot 0)
-  const int64_t stride = 2 * (int64_t)nrows * (D + 2);
-  const float* base = t.partial + w0 * stride + (int64_t)(s * t.G + h - unit * t.G) * (D + 2);
-  auto part = [&](int j) { return base + j * stride + (j == 0 ? stride / 2 : 0); };
-  float m = -__builtin_inff(), l = 0.f, o[FPL] = {};
-  for (int j0 = 0; j0 < n; j0 += 64) {
-    float x[PER][FPL];
-#pragma unroll
-    for (int k = 0; k < PER; ++k) {
-      const int j = j0 + wave + 4 * k;
-      const float* q = part(j < n ? j : 0) + lane * FPL;
-#pragma unroll
-      for (int i = 0; i < FPL; ++i) x[k][i] = q[i];
-    }
-    const float* q = part(j0 + lane < n ? j0 + lane : 0);
-    const float pm = j0 + lane < n ? q[D] : -__builtin_inff(), pl = j0 + lane < n ? q[D + 1] : 0.f;
-    float m_new = m;
-    {
-      float v = pm;
-#pragma unroll
-      for (int off = 1; off < 16; off <<= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
-      m_new = fmaxf(m, max_halves(max_rows16(v)));
-    }
-    const float shift = m_new == -__builtin_inff() ? 0.f : m_new;
-    const float a = m == -__builtin_inff() ? 1.f : expf(m - shift);
-    // (parts that saw a key: one whose weight underflows to 0 still counts, as its infinities make a NaN there)
-    const uint64_t saw = __ballot(pl != 0.f);
-    const float wt = pl == 0.f ? 0.f : pm == -__builtin_inff() ? 1.f : expf(pm - shift);
-    float sum = pl * wt;
-#pragma unroll
-    for (int off = 1; off < 16; off <<= 1) sum += __shfl_xor(sum, off, 64);
-    m = m_new;
-    l = l * a + sum_halves(sum_rows16(sum));
-#pragma unroll
-    for (int i = 0; i < FPL; ++i) o[i] *= a;
-#pragma unroll
-    for (int k = 0; k < PER; ++k) {
-      const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wt), wave + 4 * k));
-#pragma unroll
-      for (int i = 0; i < FPL; ++i)
-        if ((saw >> (wave + 4 * k)) & 1) o[i] = __builtin_fmaf(x[k][i], w, o[i]);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < FPL; ++i) o_s[wave][lane * FPL + i] = o[i];
-  __syncthreads();
-  if (tid >= D) return;
-  const float acc = (o_s[0][tid] + o_s[1][tid]) + (o_s[2][tid] + o_s[3][tid]);
-  write_row<T>(p, b, s, h, tid, l == 0.f ? 0.f : acc / l);
-  if (p.lse && tid == 0)
-    ((float*)p.lse)[b * p.ls_b + h * p.ls_h + s * p.ls_s] =
-        l == 0.f ? -__builtin_inff() : (m == -__builtin_inff() ? 0.f : m) + logf(l);
-}
-
-constexpr int NW_SPLIT = 4;  // waves of a workgroup that takes a run
-
-template <typename T, int D, bool POS, int PC, int NW>
+template <typename T, int D, int VIS, int PC, int NW>
 int launch_whole(const TokenParams& t, hipStream_t st) {
   constexpr int lds = NW * TLayout<D>::WAVE_BYTES;
-  const hipError_t e = reserve_lds<paged_token_kernel<T, D, POS, NW, false, PC>>(lds);
+  const hipError_t e = reserve_lds<paged_token_kernel<T, D, VIS, NW, false, PC>>(lds);
   CEA_REQUIRE(e == hipSuccess, CEA_ELAUNCH, "paged_attention: cannot reserve %d bytes of LDS: %s", lds,
               hipGetErrorString(e));
-  hipLaunchKernelGGL((paged_token_kernel<T, D, POS, NW, false, PC>), dim3((unsigned)(t.p.B * t.units)), dim3(NW * 64),
+  hipLaunchKernelGGL((paged_token_kernel<T, D, VIS, NW, false, PC>), dim3((unsigned)(t.p.B * t.units)), dim3(NW * 64),
                      lds, st, t);
   CEA_CHECK_LAUNCH("paged_token");
   return CEA_OK;
 }
 
-template <typename T, int D, bool POS, int PC>
+template <typename T, int D, int VIS, int PC>
 int launch_form(const TokenParams& t, bool whole, hipStream_t st) {
   typedef TLayout<D> L;
   if (whole) {
@@ -588,18 +355,18 @@ int launch_form(const TokenParams& t, bool whole, hipStream_t st) {
     // 64, 14.9 / 10.3 / 9.8; 256 units of up to 1000, D = 64, 18.6 / 13.9 / 13.6; D = 128: 64 units
     // of up to 1000 keys 21.4 / 16.4 / -, 320 26.3 / 24.5 / -, 512 of up to 700 26.6 / 28.1 / -)
     const int64_t pairs = (int64_t)t.p.B * t.units;
-    if (D == 64 && pairs <= 256) return launch_whole<T, D, POS, PC, D == 64 ? 16 : 8>(t, st);
-    if (pairs <= (D == 64 ? 512 : 384)) return launch_whole<T, D, POS, PC, 8>(t, st);
-    return launch_whole<T, D, POS, PC, 4>(t, st);
+    if (D == 64 && pairs <= 256) return launch_whole<T, D, VIS, PC, D == 64 ? 16 : 8>(t, st);
+    if (pairs <= (D == 64 ? 512 : 384)) return launch_whole<T, D, VIS, PC, 8>(t, st);
+    return launch_whole<T, D, VIS, PC, 4>(t, st);
   }
   constexpr int lds = NW_SPLIT * L::WAVE_BYTES;
-  const hipError_t e = reserve_lds<paged_token_kernel<T, D, POS, NW_SPLIT, true, PC>>(lds);
+  const hipError_t e = reserve_lds<paged_token_kernel<T, D, VIS, NW_SPLIT, true, PC>>(lds);
   CEA_REQUIRE(e == hipSuccess, CEA_ELAUNCH, "paged_attention: cannot reserve %d bytes of LDS: %s", lds,
               hipGetErrorString(e));
-  hipLaunchKernelGGL((paged_token_kernel<T, D, POS, NW_SPLIT, true, PC>), dim3((unsigned)t.wgs), dim3(NW_SPLIT * 64),
+  hipLaunchKernelGGL((paged_token_kernel<T, D, VIS, NW_SPLIT, true, PC>), dim3((unsigned)t.wgs), dim3(NW_SPLIT * 64),
                      lds, st, t);
   CEA_CHECK_LAUNCH("paged_token");
-  hipLaunchKernelGGL((paged_token_join_kernel<T, D, NW_SPLIT>), dim3((unsigned)(t.p.B * t.p.Sq * t.p.Hq)), dim3(256),
+  hipLaunchKernelGGL((paged_token_join_kernel<T, D, NW_SPLIT * TK>), dim3((unsigned)(t.p.B * t.p.Sq * t.p.Hq)), dim3(256),
                      0, st, t);
   CEA_CHECK_LAUNCH("paged_token_join");
   return CEA_OK;
@@ -608,15 +375,12 @@ int launch_form(const TokenParams& t, bool whole, hipStream_t st) {
 template <typename T, int D> int launch_td(const TokenParams& t, bool whole, hipStream_t st) {
   constexpr int kFull = std::is_same<T, bf16>::value ? 3 : 2;  // pieces that hold an f32 probability
   const bool f32 = t.p.out_dtype == CEA_F32;
+  if (t.p.masks)
+    return f32 ? launch_form<T, D, kTree, kFull>(t, whole, st) : launch_form<T, D, kTree, 2>(t, whole, st);
   if (t.p.pos)
-    return f32 ? launch_form<T, D, true, kFull>(t, whole, st) : launch_form<T, D, true, 2>(t, whole, st);
-  return f32 ? launch_form<T, D, false, kFull>(t, whole, st) : launch_form<T, D, false, 2>(t, whole, st);
+    return f32 ? launch_form<T, D, kPosition, kFull>(t, whole, st) : launch_form<T, D, kPosition, 2>(t, whole, st);
+  return f32 ? launch_form<T, D, kNumber, kFull>(t, whole, st) : launch_form<T, D, kNumber, 2>(t, whole, st);
 }
-
-struct TokenPlan {
-  int32_t G, units, wgs;
-  bool whole;
-};
 
 // Query heads of a unit: a KV head's whole group, or the largest part of it whose rows fit.
 int unit_heads(int64_t Sq, int64_t Hq, int64_t Hkv, int group) {
@@ -633,12 +397,12 @@ int unit_heads(int64_t Sq, int64_t Hq, int64_t Hkv, int group) {
 // 13.1 / 15.0 (12.4 / 10.8), 64 of up to 1000 16.7 / 15.8 (16.3 / 14.9), 320 24.5 / 32.9, 512 of up to 700 26.1 / 42.2.
 constexpr int64_t kTokenWhole = 1024;
 
-TokenPlan plan_token(int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int group, int64_t slots) {
+TokenPlan plan_token(int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int group, int64_t slots, bool f8) {
   TokenPlan r;
   r.G = unit_heads(Sq, Hq, Hkv, group);
   r.units = r.G > 0 ? (int32_t)(Hq / r.G) : 0;
   r.whole = slots <= kTokenWhole;
-  const int64_t blocks = std::max<int64_t>(1, (slots + NW_SPLIT * TK - 1) / (NW_SPLIT * TK));
+  const int64_t block = NW_SPLIT * (f8 ? TK8 : TK), blocks = std::max<int64_t>(1, (slots + block - 1) / block);
   const int cus = device_cus() > 0 ? device_cus() : 256;
   // two workgroups per compute unit, as many as are resident at D = 128 (us, 512 / 1024: 8 rows of
   // 100 to 4096 keys, 32/8 heads of 128, 22.7 / 27.7; one row of 30000 31.4 / 37.1; 32 rows of 1024 to
@@ -650,8 +414,8 @@ TokenPlan plan_token(int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int group, 
 }  // namespace
 
 size_t paged_token_workspace_bytes(int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int group, int64_t D,
-                                   int64_t slots) {
-  const TokenPlan r = plan_token(B, Sq, Hq, Hkv, group, slots);
+                                   int64_t slots, bool f8) {
+  const TokenPlan r = plan_token(B, Sq, Hq, Hkv, group, slots, f8);
   if (r.G == 0 || r.whole) return 0;
   return (size_t)r.wgs * 2 * Sq * r.G * (D + 2) * sizeof(float);
 }
@@ -666,7 +430,8 @@ bool paged_token_supported(const PagedParams& p, const HeadMap& map) {
 }
 
 int launch_paged_token(const PagedParams& p, const HeadMap& map, void* ws, hipStream_t st) {
-  const TokenPlan r = plan_token(p.B, p.Sq, p.Hq, p.Hkv, map.group, (int64_t)p.W * p.page);
+  const TokenPlan r = plan_token(p.B, p.Sq, p.Hq, p.Hkv, map.group, (int64_t)p.W * p.page,
+                                 p.kv_dtype == CEA_F8);
   TokenParams t;
   t.p = p;
   t.G = r.G, t.units = r.units, t.wgs = r.wgs;
@@ -674,6 +439,7 @@ int launch_paged_token(const PagedParams& p, const HeadMap& map, void* ws, hipSt
   t.magic = t.page16 > 1 ? (uint32_t)((((uint64_t)1 << 32) + t.page16 - 1) / t.page16) : 0;
   t.partial = (float*)ws;
   for (int h = 0; h < kPagedMapHeads; ++h) t.kv[h] = map.group <= 0 && h < p.Hq ? (uint8_t)map.kv[h] : 0;
+  if (p.kv_dtype == CEA_F8) return launch_paged_token8(t, r.whole, st);
   if (p.in_dtype == CEA_BF16)
     return p.D == 128 ? launch_td<bf16, 128>(t, r.whole, st) : launch_td<bf16, 64>(t, r.whole, st);
   return p.D == 128 ? launch_td<f16, 128>(t, r.whole, st) : launch_td<f16, 64>(t, r.whole, st);
