@@ -6,11 +6,13 @@
 // j, or what pos_pages holds there when that is given.  Nothing outside the pools is read or
 // written whatever the tables, lengths and offsets hold.
 //
-// Pages of 8 bits hold e4m3 numbers, and a scale byte s per slot and head: the values q * 2^(s - 127).
+// Pages of 8 bits hold e4m3 numbers, and a scale byte s (1 to 254) per slot and head: the values q * 2^(s - 127).
 //
 // Drafts: with masks the queries are the nodes of a tree in the row's last counts[b] slots.  Node i sees
 // every slot before them, and slot lengths[b] - counts[b] + j where bit j of masks[b, i] is set.
 #pragma once
+
+#include <type_traits>
 
 #include "cea_kernels.hpp"
 
@@ -73,6 +75,17 @@ __device__ __forceinline__ uint64_t tree_word(const PagedParams& p, int b, int64
   const uint64_t x = (uint64_t)p.masks[b * p.ms_b + i * p.ms_s + w * p.ms_w];
   return left >= 64 ? x : x & (((uint64_t)1 << left) - 1);
 }
+
+// Two e4m3 numbers, the low or the high half of x, times a power of two, as 16-bit numbers: exact in bf16, and in
+// f16 but for what is below its normal numbers (rounded) or beyond its largest (infinite).
+template <typename T, bool HIGH> __device__ __forceinline__ uint32_t widen2(uint32_t x, float scale) {
+  if constexpr (std::is_same<T, bf16>::value)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, scale, HIGH));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, scale, HIGH));
+}
+// A scale byte (1 to 254) as the power of two that it stands for.
+__device__ __forceinline__ float scale_value(uint32_t s) { return __uint_as_float(s << 23); }
 
 // What decides whether a query sees a slot: its number, a position in the pool, or a tree's mask.
 enum Vis { kNumber = 0, kPosition = 1, kTree = 2 };

@@ -131,14 +131,6 @@ template <int D, int VIS, bool F8> struct Layout {
   static constexpr int pos(int i) { return K_BYTES + V_BYTES + i * (F8 ? POS_BYTES : STAGE_BYTES); }
 };
 
-// Two e4m3 numbers (the low or the high half of x) times a power of two as 16-bit numbers, exactly.
-template <typename T, bool HIGH> __device__ __forceinline__ uint32_t widen2(uint32_t x, float scale) {
-  if constexpr (std::is_same<T, bf16>::value)
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, scale, HIGH));
-  else
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, scale, HIGH));
-}
-
 template <int D> __device__ __forceinline__ int k_swz(int key) {
   if constexpr (D / 8 >= 16) return key & 15;
   else return (key >> 1) & 7;
@@ -486,7 +478,7 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, char* smem, Sh
         const int local = i * L::ROWS_PER_LOAD + lane / L::SRC_NCG, key = wave * WROWS + local;
         const uint4 x = *(const uint4*)(raw + kv * L::RAW_TILE + i * 1024 + lane * 16);
         const uint32_t s = ok && local < rows ? *(const uint8_t*)(raw + 2 * L::RAW_TILE + kv * WROWS + local) : 127u;
-        const float scale8 = __uint_as_float(s << 23);
+        const float scale8 = scale_value(s);
         const uint4 lo = make_uint4(widen2<T, false>(x.x, scale8), widen2<T, true>(x.x, scale8),
                                     widen2<T, false>(x.y, scale8), widen2<T, true>(x.y, scale8));
         const uint4 hi = make_uint4(widen2<T, false>(x.z, scale8), widen2<T, true>(x.z, scale8),

@@ -94,10 +94,9 @@ template <typename T> struct TypeTop { static constexpr int kScale = 247; };  //
 template <> struct TypeTop<f16> { static constexpr int kScale = 135; };       // below 2^16
 
 // Magnitude bits, 0 of what is not finite.
-__device__ __forceinline__ uint32_t finite_bits(float x) {
-  const uint32_t u = __float_as_uint(x) & 0x7fffffffu;
-  return u < 0x7f800000u ? u : 0u;
-}
+constexpr uint32_t kInfBits = 0x7f800000u;
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t finite_bits(float x) { return magnitude(x) < kInfBits ? magnitude(x) : 0u; }
 // (the rotary of f16 rows may leave f16's range, f32's sums do not)
 template <typename T> __device__ __forceinline__ float within(float x) {
   if constexpr (std::is_same<T, f16>::value)
@@ -105,6 +104,7 @@ template <typename T> __device__ __forceinline__ float within(float x) {
   else
     return x;
 }
+// Four values as numbers of the scale s, whatever they are.
 template <typename T> __device__ __forceinline__ uint32_t quantise4(const float* x, int s) {
   float q[4];
 #pragma unroll
@@ -116,6 +116,62 @@ template <typename T> __device__ __forceinline__ uint32_t quantise4(const float*
   int w = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
   w = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w, true);
   return (uint32_t)w;
+}
+// Eight values of a row that is finite and below its type's top scale, which is nearly every row: two an
+// instruction, v_cvt_scalef32_pk_fp8, which divides by the scale as it rounds.
+typedef short i16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u32x2 quantise8(const float* x, float scale) {
+  u32x2 w;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    i16x2 y = {0, 0};
+    y = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(y, x[4 * i], x[4 * i + 1], scale, false);
+    y = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(y, x[4 * i + 2], x[4 * i + 3], scale, true);
+    w[i] = __builtin_bit_cast(uint32_t, y);
+  }
+  return w;
+}
+template <typename T> __device__ __forceinline__ u32x2 quantise8(const T (&x)[8], float scale) {
+  if constexpr (sizeof(T) == 4) {
+    return quantise8(&x[0], scale);
+  } else {
+    typedef T pair __attribute__((ext_vector_type(2)));
+    u32x2 w;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      i16x2 y = {0, 0};
+      const pair a = {x[4 * i], x[4 * i + 1]}, b = {x[4 * i + 2], x[4 * i + 3]};
+      if constexpr (std::is_same<T, bf16>::value) {
+        y = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(y, a, scale, false);
+        y = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(y, b, scale, true);
+      } else {
+        y = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(y, a, scale, false);
+        y = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(y, b, scale, true);
+      }
+      w[i] = __builtin_bit_cast(uint32_t, y);
+    }
+    return w;
+  }
+}
+// The largest magnitude of eight values as an f32's bits, infinities and NaN among them.  (16-bit types: two
+// an instruction, in their own bits, whose order is that of the magnitudes.)
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+template <typename T> __device__ __forceinline__ uint32_t top8(const T (&x)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, magnitude(x[e]));
+    return top;
+  } else {
+    u32x4 raw;
+    __builtin_memcpy(&raw, x, 16);
+    u16x2 top = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, (uint32_t)(raw[i] & 0x7fff7fffu)));
+    const uint16_t one = max(top[0], top[1]);
+    return magnitude(to_f32<T>(__builtin_bit_cast(T, one)));
+  }
 }
 
 struct Append8Params {
@@ -159,37 +215,65 @@ __global__ __launch_bounds__(256) void paged_append8_kernel(const Append8Params 
   }
   const int64_t count = p.rows.counts ? p.rows.counts[b * p.rows.ns_b] : p.n;
   const Place at = place_of(p.rows, b, slot_after(p.rows.offsets[b * p.rows.os_b], s));
-  float x[4][VEC];
-  uint32_t top[2] = {0, 0};
+  float k[2][VEC];  // the rotated key
 #pragma unroll
   for (int e = 0; e < VEC; ++e) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i][e] = to_f32<T>(raw[i][e]);
+    const float a = to_f32<T>(raw[0][e]), z = to_f32<T>(raw[1][e]);
+    k[0][e] = a, k[1][e] = z;
     if constexpr (ROT) {
       // out_i = x_i c_i - x_{i+h} s_i, out_{i+h} = x_{i+h} c_{i+h} + x_i s_{i+h}: products and sum rounded once each
-      const float a = x[0][e], z = x[1][e];
-      x[0][e] = within<T>(add_rn(mul_rn(a, to_f32<T>(c1[e])), -mul_rn(z, to_f32<T>(s1[e]))));
-      x[1][e] = within<T>(add_rn(mul_rn(z, to_f32<T>(c2[e])), mul_rn(a, to_f32<T>(s2[e]))));
+      k[0][e] = add_rn(mul_rn(a, to_f32<T>(c1[e])), -mul_rn(z, to_f32<T>(s1[e])));
+      k[1][e] = add_rn(mul_rn(z, to_f32<T>(c2[e])), mul_rn(a, to_f32<T>(s2[e])));
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) top[i >> 1] = max(top[i >> 1], finite_bits(x[i][e]));
   }
+  uint32_t top[2] = {ROT ? max(top8(k[0]), top8(k[1])) : max(top8(raw[0]), top8(raw[1])), max(top8(raw[2]), top8(raw[3]))};
   for (uint32_t off = 1; off < nch; off <<= 1)
 #pragma unroll
     for (int i = 0; i < 2; ++i) top[i] = max(top[i], (uint32_t)__shfl_xor((int)top[i], (int)off, 64));
+  constexpr uint32_t kPlain = std::is_same<T, f16>::value ? 0x477fe000u : kInfBits - 1;  // the type's largest
+  bool plain = true;
+  int sc[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    sc[i] = scale_of(top[i]);
+    plain = plain && top[i] <= kPlain && sc[i] != TypeTop<T>::kScale;
+  }
+  u32x2 w[4];
+  if (__ballot(!plain) == 0) {
+    const float f[2] = {scale_value(sc[0]), scale_value(sc[1])};
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      w[g] = ROT ? quantise8(&k[g][0], f[0]) : quantise8<T>(raw[g], f[0]);
+      w[2 + g] = quantise8<T>(raw[2 + g], f[1]);
+    }
+  } else {
+    float x[4][VEC];
+    top[0] = top[1] = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        x[i][e] = i < 2 ? within<T>(k[i & 1][e]) : to_f32<T>(raw[i][e]);
+        top[i >> 1] = max(top[i >> 1], finite_bits(x[i][e]));
+      }
+    for (uint32_t off = 1; off < nch; off <<= 1)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) top[i] = max(top[i], (uint32_t)__shfl_xor((int)top[i], (int)off, 64));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      sc[i >> 1] = scale_of(top[i >> 1]);
+      w[i] = u32x2{quantise4<T>(x[i], sc[i >> 1]), quantise4<T>(x[i] + 4, sc[i >> 1])};
+    }
+  }
   if (!live || s >= count || at.id < 0) return;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int sc = scale_of(top[i]);
     const Pool& pool = i == 0 ? p.kp : p.vp;
     const Pool& scales = i == 0 ? p.ks : p.vs;
     char* o = pool.base + at_of(pool, at, h) + j;
-#pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      const u32x2 w = {quantise4<T>(x[2 * i + g], sc), quantise4<T>(x[2 * i + g] + 4, sc)};
-      *(u32x2*)(o + g * half) = w;
-    }
-    if (j == 0) scales.base[at_of(scales, at, h)] = (char)sc;
+    *(u32x2*)o = w[2 * i];
+    *(u32x2*)(o + half) = w[2 * i + 1];
+    if (j == 0) scales.base[at_of(scales, at, h)] = (char)sc[i];
   }
   if (p.pp && h == 0 && j == 0)
     p.pp[at.id * p.pps_p + at.at * p.pps_s] = p.pos[b * p.ps_b + s * p.ps_s];
@@ -259,54 +343,85 @@ struct ReadParams {
   Pool pool[2], scales[2];
   char* out[2];
   int64_t os_b[2], os_s[2], os_h[2];
-  int32_t B, n, H, D, total;
+  int32_t B, n, H, D, items, turns;  // items: vectors of a token; turns: groups of slots of a row
 };
 
-// VEC e4m3 numbers and their row's scale as values of O.  bf16 holds q * 2^(s - 127) as it is; f16 rounds
-// what is below its normal numbers and overflows to infinity.
-template <typename O, int VEC> __device__ __forceinline__ void widen(const uint8_t (&q)[VEC], int s, O (&x)[VEC]) {
+// VEC elements of the pages as values of O, two of 8 bits an instruction.
+template <typename I, typename O, int VEC> __device__ __forceinline__ void convert(const I (&q)[VEC], int s, O (&x)[VEC]) {
+  if constexpr (!std::is_same<I, uint8_t>::value) {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) x[i] = (O)ldexpf(__builtin_amdgcn_cvt_f32_fp8(q[i], 0), s - kScaleBias);
-}
-
-// A thread owns VEC features of a slot and head, of the keys or of the values.
-template <typename I, typename O, int VEC>
-__global__ __launch_bounds__(256) void paged_read_kernel(const ReadParams p) {
-  const uint32_t nch = p.D / VEC;
-  const uint32_t t = blockIdx.x * 256 + threadIdx.x;
-  if (t >= (uint32_t)p.total) return;
-  uint32_t r = t / nch;
-  const uint32_t j = (t - r * nch) * VEC;
-  const uint32_t h = r % (uint32_t)p.H;
-  r /= (uint32_t)p.H;
-  const uint32_t b = r / (uint32_t)p.n, s = r - b * p.n;
-  const int kv = blockIdx.y;
-  const int64_t count = p.rows.counts ? p.rows.counts[b * p.rows.ns_b] : p.n;
-  const Place at = s < count ? place_of(p.rows, b, slot_after(p.rows.offsets[b * p.rows.os_b], s)) : Place{-1, 0};
-  O x[VEC] = {};
-  if (at.id >= 0) {
-    const I* from = (const I*)p.pool[kv].base + at_of(p.pool[kv], at, h) + j;
-    if constexpr (std::is_same<I, uint8_t>::value) {
-      uint8_t q[VEC];
-      if constexpr (VEC == 1) q[0] = *from;
-      else load_bytes<std::conditional_t<VEC % 16 == 0, u32x4, u32x2>>(from, q);
-      widen<O, VEC>(q, ((const uint8_t*)p.scales[kv].base)[at_of(p.scales[kv], at, h)], x);
-    } else if constexpr (VEC == 1) {
-      x[0] = *from;
-    } else {
-      load_bytes<u32x4>(from, x);
+    for (int i = 0; i < VEC; ++i) x[i] = q[i];
+  } else if constexpr (sizeof(O) == 4) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) x[i] = ldexpf(__builtin_amdgcn_cvt_f32_fp8(q[i], 0), s - kScaleBias);
+  } else if constexpr (VEC == 8) {
+    u32x2 raw;
+    __builtin_memcpy(&raw, q, 8);
+    const float f = scale_value(s);
+    const u32x4 y = {widen2<O, false>(raw[0], f), widen2<O, true>(raw[0], f), widen2<O, false>(raw[1], f),
+                     widen2<O, true>(raw[1], f)};
+    __builtin_memcpy(x, &y, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const uint16_t y = (uint16_t)widen2<O, false>(q[i], scale_value(s));
+      __builtin_memcpy(&x[i], &y, 2);
     }
   }
-  O* to = (O*)p.out[kv] + b * p.os_b[kv] + s * p.os_s[kv] + h * p.os_h[kv] + j;
-  if constexpr (VEC == 1) *to = x[0];
-  else store_bytes<u32x4>(to, x);
+}
+
+// A wave owns kReadSlots slots of a row and takes the tokens' vectors 64 at a time: where the slots are is known
+// once for all of them, and keys and values of all its slots are under way together.
+constexpr int kReadSlots = 4;
+template <typename I, typename O, int VEC>
+__global__ __launch_bounds__(256) void paged_read_kernel(const ReadParams p) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t group = blockIdx.x * 4 + uniform(threadIdx.x >> 6);
+  const uint32_t b = group / (uint32_t)p.turns;
+  if (b >= (uint32_t)p.B) return;
+  const int s0 = (int)(group - b * p.turns) * kReadSlots;
+  const int64_t count = p.rows.counts ? p.rows.counts[b * p.rows.ns_b] : p.n;
+  const int64_t first = p.rows.offsets[b * p.rows.os_b];
+  Place at[kReadSlots];
+#pragma unroll
+  for (int i = 0; i < kReadSlots; ++i)
+    at[i] = s0 + i < count && s0 + i < p.n ? place_of(p.rows, b, slot_after(first, s0 + i)) : Place{-1, 0};
+  const uint32_t nch = p.D / VEC;
+  for (int item = lane; item < p.items; item += 64) {
+    const uint32_t h = (uint32_t)item / nch, j = ((uint32_t)item - h * nch) * VEC;
+    I q[2][kReadSlots][VEC] = {};
+    int s[2][kReadSlots] = {};
+#pragma unroll
+    for (int i = 0; i < kReadSlots; ++i)
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv)
+        if (at[i].id >= 0) {
+          const I* from = (const I*)p.pool[kv].base + at_of(p.pool[kv], at[i], h) + j;
+          if constexpr (VEC == 1) q[kv][i][0] = *from;
+          else load_bytes<std::conditional_t<sizeof(I) * VEC == 16, u32x4, u32x2>>(from, q[kv][i]);
+          if constexpr (std::is_same<I, uint8_t>::value)
+            s[kv][i] = ((const uint8_t*)p.scales[kv].base)[at_of(p.scales[kv], at[i], h)];
+        }
+#pragma unroll
+    for (int i = 0; i < kReadSlots; ++i)
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv)
+        if (s0 + i < p.n) {
+          O x[VEC];
+          convert<I, O, VEC>(q[kv][i], s[kv][i], x);
+          O* to = (O*)p.out[kv] + b * p.os_b[kv] + (s0 + i) * p.os_s[kv] + h * p.os_h[kv] + j;
+          if constexpr (VEC == 1) *to = x[0];
+          else store_bytes<u32x4>(to, x);
+        }
+  }
 }
 
 template <typename I, typename O, int VEC> int read_typed(ReadParams& p, hipStream_t st) {
-  const int64_t total = (int64_t)p.B * p.n * p.H * (p.D / VEC);
-  CEA_REQUIRE(total <= INT32_MAX - 256, CEA_EUNSUPPORTED, "paged_kv_read: too many tokens for one call");
-  p.total = (int32_t)total;
-  hipLaunchKernelGGL((paged_read_kernel<I, O, VEC>), dim3((unsigned)((total + 255) / 256), 2), dim3(256), 0, st, p);
+  const int64_t items = (int64_t)p.H * (p.D / VEC), turns = ((int64_t)p.n + kReadSlots - 1) / kReadSlots;
+  CEA_REQUIRE(items <= INT32_MAX - 64 && turns * p.B <= INT32_MAX - 4, CEA_EUNSUPPORTED,
+              "paged_kv_read: too many tokens for one call");
+  p.items = (int32_t)items, p.turns = (int32_t)turns;
+  hipLaunchKernelGGL((paged_read_kernel<I, O, VEC>), dim3((unsigned)((turns * p.B + 3) / 4)), dim3(256), 0, st, p);
   CEA_CHECK_LAUNCH("paged_kv_read");
   return CEA_OK;
 }
@@ -321,59 +436,69 @@ struct KeepParams {
   char *kv, *scales;
   int64_t s_n, s_p, s_h, s_s;      // bytes
   int64_t ss_n, ss_p, ss_h, ss_s;  // bytes
-  int32_t B, H, n, nch, all;       // nch: vectors of a row; all: pools * B * H
+  int32_t H, n, nch, pairs;        // nch: vectors of a row; pairs: pools times heads
 };
 
-// Slot base + i takes what slot base + path[i] held.  A thread owns a vector of a row, or its scale, in all
-// the slots of one sequence, head and pool, so it alone reads and writes there: eight are read, then written.
-// Entries with path[i] < i move nothing, so a source is never a slot that an earlier turn has written.
+// Slot base + i takes what slot base + path[i] held.  A workgroup serves kKeepPairs (pool, head) pairs of one
+// row: a wave finds where up to 64 entries' slots are and lists those that move, then every wave takes four
+// pairs and moves their vectors, 64 (entry, vector) at a time, of all four at once.  Entries with path[i] <= i
+// move nothing, so a source lies behind every slot that an earlier step of the wave has written, and within a
+// step all loads come before the stores.
+constexpr int kKeepPairs = 16;
 template <typename V>
 __global__ __launch_bounds__(256) void paged_keep_kernel(const KeepParams p) {
-  constexpr int TURN = 8;
-  const int per = p.nch + (p.scales ? 1 : 0);
-  const uint32_t t = blockIdx.x * 256 + threadIdx.x;
-  uint32_t r = t / (uint32_t)per;
-  if (r >= (uint32_t)p.all) return;
-  const int c = (int)(t - r * per);
-  const int h = (int)(r % (uint32_t)p.H);
-  r /= (uint32_t)p.H;
-  const int n = (int)(r / (uint32_t)p.B), b = (int)(r - (uint32_t)n * p.B);
-  const int64_t base = p.rows.offsets[b * p.rows.os_b];
-  const int64_t nodes = p.rows.counts ? p.rows.counts[b * p.rows.ns_b] : INT64_MAX;
-  const bool scale = c == p.nch;
-  char* pool = scale ? p.scales + n * p.ss_n + h * p.ss_h : p.kv + n * p.s_n + h * p.s_h + (int64_t)c * sizeof(V);
-  const int64_t s_p = scale ? p.ss_p : p.s_p, s_s = scale ? p.ss_s : p.s_s;
-  for (int i0 = 0; i0 < p.n; i0 += TURN) {
-    V x[TURN] = {};
-    char* to[TURN];
+  constexpr int PER = kKeepPairs / 4;
+  __shared__ int64_t src[64], dst[64], src_s[64], dst_s[64];
+  __shared__ int moves;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), b = blockIdx.y;
+  char *pool[PER], *scales[PER];
 #pragma unroll
-    for (int k = 0; k < TURN; ++k) {
-      const int i = i0 + k;
-      to[k] = nullptr;
-      if (i >= p.n) continue;
-      const int64_t node = p.path[b * p.ps_b + i * p.ps_i];
-      if (node <= i || node >= nodes) continue;  // (node i is in its place)
-      const Place from = place_of(p.rows, b, slot_after(base, node)), at = place_of(p.rows, b, slot_after(base, i));
-      if (from.id < 0 || at.id < 0) continue;
-      to[k] = pool + at.id * s_p + at.at * s_s;
-      const char* src = pool + from.id * s_p + from.at * s_s;
-      if (scale) {
-        const uint8_t y = *(const uint8_t*)src;
-        __builtin_memcpy(&x[k], &y, 1);
-      } else {
-        x[k] = *(const V*)src;
+  for (int k = 0; k < PER; ++k) {
+    const int pair = blockIdx.x * kKeepPairs + wave * PER + k, at = min(pair, p.pairs - 1);
+    const int n = at / p.H, h = at - n * p.H;
+    pool[k] = pair < p.pairs ? p.kv + n * p.s_n + h * p.s_h : nullptr;
+    scales[k] = p.scales ? p.scales + n * p.ss_n + h * p.ss_h : nullptr;
+  }
+  for (int i0 = 0; i0 < p.n; i0 += 64) {
+    if (i0 > 0) __syncthreads();  // the last list is used up
+    if (wave == 0) {
+      const int i = i0 + lane;
+      const int64_t base = p.rows.offsets[b * p.rows.os_b];
+      const int64_t nodes = p.rows.counts ? p.rows.counts[b * p.rows.ns_b] : INT64_MAX;
+      const int64_t node = i < p.n ? p.path[b * p.ps_b + i * p.ps_i] : -1;
+      const bool moves_on = node > i && node < nodes;  // (node i is in its place)
+      const Place from = moves_on ? place_of(p.rows, b, slot_after(base, node)) : Place{-1, 0};
+      const Place to = moves_on ? place_of(p.rows, b, slot_after(base, i)) : Place{-1, 0};
+      const bool move = from.id >= 0 && to.id >= 0;
+      const uint64_t all = __ballot(move);
+      if (move) {
+        const int k = __builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0));
+        src[k] = from.id * p.s_p + from.at * p.s_s, dst[k] = to.id * p.s_p + to.at * p.s_s;
+        src_s[k] = from.id * p.ss_p + from.at * p.ss_s, dst_s[k] = to.id * p.ss_p + to.at * p.ss_s;
       }
+      if (lane == 0) moves = __builtin_popcountll(all);
     }
+    __syncthreads();
+    const int m = moves;
+    for (int x = lane; x < m * p.nch; x += 64) {
+      const int e = (uint32_t)x / (uint32_t)p.nch, c = x - e * p.nch;
+      const int64_t from = src[e] + (int64_t)c * sizeof(V), to = dst[e] + (int64_t)c * sizeof(V);
+      V v[PER] = {};
 #pragma unroll
-    for (int k = 0; k < TURN; ++k) {
-      if (to[k] == nullptr) continue;
-      if (scale) {
-        uint8_t y;
-        __builtin_memcpy(&y, &x[k], 1);
-        *(uint8_t*)to[k] = y;
-      } else {
-        *(V*)to[k] = x[k];
-      }
+      for (int k = 0; k < PER; ++k)
+        if (pool[k]) v[k] = *(const V*)(pool[k] + from);
+#pragma unroll
+      for (int k = 0; k < PER; ++k)
+        if (pool[k]) *(V*)(pool[k] + to) = v[k];
+    }
+    if (p.scales && lane < m) {
+      uint8_t v[PER] = {};
+#pragma unroll
+      for (int k = 0; k < PER; ++k)
+        if (pool[k]) v[k] = *(const uint8_t*)(scales[k] + src_s[lane]);
+#pragma unroll
+      for (int k = 0; k < PER; ++k)
+        if (pool[k]) *(uint8_t*)(scales[k] + dst_s[lane]) = v[k];
     }
   }
 }
@@ -388,51 +513,46 @@ struct MaskParams {
   int32_t T, words;
 };
 
-// Every node starts with its own bit and a link to its parent, and takes, round by round, the bits of the
-// node that it links to and that node's link: after k rounds it holds 2^k nodes of its line.  A workgroup
-// per row; the lines are in LDS, what a round reads and what it writes apart.
-__global__ __launch_bounds__(512) void tree_masks_kernel(const MaskParams p) {
-  extern __shared__ uint64_t bits[];  // [2][T * words], then int16 links [2][T]
-  const int b = blockIdx.x, T = p.T, words = p.words, n = T * words;
-  int16_t* link = (int16_t*)(bits + 2 * n);
+// A wave per row, 64 nodes at a time.  Within them every node starts with its own bit and a link to its parent, and
+// takes, round by round, the bits of the node that it links to and that node's link: after k rounds it holds 2^k
+// nodes of its line.  Parents come first, so the lowest bit is the line's first node here, and that one's
+// parent, in LDS with all its words by now, brings the rest.
+__global__ __launch_bounds__(64) void tree_masks_kernel(const MaskParams p) {
+  extern __shared__ uint64_t line[];  // [T][words - 1]: the lines of the nodes before, by their words before the last
+  __shared__ int16_t depth[CEA_MAX_TREE];
+  const int b = blockIdx.x, lane = threadIdx.x, T = p.T, words = p.words;
   int64_t count = p.counts ? p.counts[b * p.ns_b] : T;
   count = count < 0 ? 0 : count < T ? count : T;
-  for (int i = threadIdx.x; i < T; i += blockDim.x) {
-    const int64_t up = i < count ? p.parents[b * p.ps_b + i * p.ps_t] : -1;
-    link[i] = (int16_t)(up >= 0 && up < i ? up : -1);
-  }
-  for (int x = threadIdx.x; x < n; x += blockDim.x) {
-    const int i = x / words, w = x - i * words;
-    bits[x] = i < count && w == i >> 6 ? (uint64_t)1 << (i & 63) : 0;
-  }
-  int cur = 0;
-  for (int span = 1; span < T; span *= 2) {
-    __syncthreads();
-    bool more = false;
-    const uint64_t* from = bits + cur * n;
-    uint64_t* to = bits + (cur ^ 1) * n;
-    for (int x = threadIdx.x; x < n; x += blockDim.x) {
-      const int i = x / words, w = x - i * words, up = link[cur * T + i];
-      to[x] = from[x] | (up >= 0 ? from[up * words + w] : 0);
-      if (w == 0) {
-        const int16_t next = up >= 0 ? link[cur * T + up] : (int16_t)-1;
-        link[(cur ^ 1) * T + i] = next;
-        more = more || next >= 0;
-      }
+  for (int w = 0; w < words; ++w) {
+    const int i = w * 64 + lane;
+    const bool real = i < count;
+    int64_t up64 = real ? p.parents[b * p.ps_b + i * p.ps_t] : -1;
+    const int up = up64 >= 0 && up64 < i ? (int)up64 : -1;
+    uint64_t own = real ? (uint64_t)1 << lane : 0;
+    int link = up >= w * 64 ? up - w * 64 : -1;
+    while (__ballot(link >= 0) != 0) {
+      const int from = link >= 0 ? link : lane;
+      const uint32_t lo = __shfl((int)(uint32_t)own, from, 64), hi = __shfl((int)(uint32_t)(own >> 32), from, 64);
+      const int next = __shfl(link, from, 64);
+      own |= ((uint64_t)hi << 32) | lo;
+      link = link >= 0 ? next : -1;
     }
-    cur ^= 1;
-    if (__syncthreads_or(more) == 0) break;
-  }
-  __syncthreads();
-  const uint64_t* done = bits + cur * n;
-  for (int x = threadIdx.x; x < n; x += blockDim.x) {
-    const int i = x / words, w = x - i * words;
-    p.masks[b * p.ms_b + i * p.ms_t + w * p.ms_w] = (int64_t)done[x];
-  }
-  for (int i = threadIdx.x; i < T; i += blockDim.x) {
-    int line = 0;
-    for (int w = 0; w < words; ++w) line += __builtin_popcountll(done[i * words + w]);
-    p.depths[b * p.ds_b + i * p.ds_t] = line > 0 ? line - 1 : 0;
+    const int first = own != 0 ? (int)__builtin_ctzll(own) : lane;
+    const int before = __shfl(up, first, 64);  // the line's last node before these, or none
+    int d = __builtin_popcountll(own) - 1;
+    if (before >= 0 && real) d += depth[before] + 1;
+    if (i < T) {
+      int64_t* out = p.masks + b * p.ms_b + i * p.ms_t;
+      for (int k = 0; k < words; ++k) {
+        uint64_t x = k == w ? own : 0;
+        if (k < w && before >= 0 && real) x = line[before * (words - 1) + k];
+        out[k * p.ms_w] = (int64_t)x;
+        if (k < words - 1) line[i * (words - 1) + k] = x;
+      }
+      depth[i] = (int16_t)d;
+      p.depths[b * p.ds_b + i * p.ds_t] = real ? d : 0;
+    }
+    __syncthreads();  // (one wave: what it wrote is there)
   }
 }
 
@@ -524,14 +644,15 @@ int launch_paged_keep(cea_tensor* kv, cea_tensor* scales, int page, const cea_te
     p.scales = (char*)scales->data;
     p.ss_n = scales->stride[0], p.ss_p = scales->stride[1], p.ss_h = scales->stride[2], p.ss_s = scales->stride[3];
   }
-  p.B = (int)B, p.H = (int)H, p.n = (int)path->size[1];
+  p.H = (int)H, p.n = (int)path->size[1];
   const int64_t bits = (int64_t)(uintptr_t)p.kv | (N > 1 ? p.s_n : 0) | p.s_p | p.s_h | p.s_s;
   const int vec = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : bits % 2 == 0 ? 2 : 1;
   p.nch = (int)(p.s_s / vec);
-  const int64_t all = N * B * H, threads = all * (p.nch + (scales ? 1 : 0));
-  CEA_REQUIRE(threads <= INT32_MAX - 256, CEA_EUNSUPPORTED, "paged_kv_keep: too many rows for one call");
-  p.all = (int)all;
-  const dim3 grid((unsigned)((threads + 255) / 256));
+  // (a turn's 64 entries times their vectors are counted in 32 bits, rows by the grid's second dimension)
+  CEA_REQUIRE(N * H <= INT32_MAX - kKeepPairs && p.s_s / vec < ((int64_t)1 << 24) && B < 65536, CEA_EUNSUPPORTED,
+              "paged_kv_keep: too many rows for one call");
+  p.pairs = (int)(N * H);
+  const dim3 grid((unsigned)((p.pairs + kKeepPairs - 1) / kKeepPairs), (unsigned)B);
   switch (vec) {
     case 16: hipLaunchKernelGGL((paged_keep_kernel<u32x4>), grid, dim3(256), 0, st, p); break;
     case 4: hipLaunchKernelGGL((paged_keep_kernel<uint32_t>), grid, dim3(256), 0, st, p); break;
@@ -553,13 +674,9 @@ int launch_tree_masks(const cea_tensor* parents, const cea_tensor* counts, cea_t
   p.T = (int)parents->size[1], p.words = (int)masks->size[2];
   const int64_t B = parents->size[0];
   if (B == 0 || p.T == 0) return CEA_OK;
-  const int lds = 2 * p.T * p.words * 8 + 2 * p.T * 2;
-  constexpr int most = 2 * CEA_MAX_TREE * (CEA_MAX_TREE / 64) * 8 + 2 * CEA_MAX_TREE * 2;
-  const hipError_t e = reserve_lds<tree_masks_kernel>(most);
-  CEA_REQUIRE(e == hipSuccess, CEA_ELAUNCH, "tree_masks: cannot reserve %d bytes of LDS: %s", most,
-              hipGetErrorString(e));
-  const int threads = std::min(512, (p.T * p.words + 63) / 64 * 64);
-  hipLaunchKernelGGL(tree_masks_kernel, dim3((unsigned)B), dim3(threads), lds, st, p);
+  // (up to 28 KB: within what a launch has without asking)
+  const int lds = p.T * (p.words - 1) * 8;
+  hipLaunchKernelGGL(tree_masks_kernel, dim3((unsigned)B), dim3(64), lds, st, p);
   CEA_CHECK_LAUNCH("tree_masks");
   return CEA_OK;
 }

@@ -16,8 +16,6 @@
 //   * a number that is not finite can only be NaN.  In a tile that all rows see it makes the NaN that the
 //     definition makes.  In others (the last ones of a unit) what no row sees is taken as 0, and a NaN that some rows
 //     see sums its tile's products one by one.
-#include <type_traits>
-
 #include "paged_token.hpp"
 
 namespace cea {
@@ -49,13 +47,6 @@ template <int D> __device__ __forceinline__ int v8_swz(int key) {
   else return ((key >> 1) & 1) | (key >> 4) << 1;
 }
 
-// Two e4m3 numbers, the low or the high half of x, times a power of two: exact in either type.
-template <typename T, bool HIGH> __device__ __forceinline__ uint32_t widen2(uint32_t x, float scale) {
-  if constexpr (std::is_same<T, bf16>::value)
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, scale, HIGH));
-  else
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, scale, HIGH));
-}
 template <typename T> __device__ __forceinline__ typename Mfma16<T>::frag8 widen8(uint32_t a, uint32_t b, float scale) {
   const u32x4 x = {widen2<T, false>(a, scale), widen2<T, true>(a, scale), widen2<T, false>(b, scale),
                    widen2<T, true>(b, scale)};
@@ -264,7 +255,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void paged_token8_kernel(
       uint32_t vscale[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        kscale[h] = __uint_as_float((uint32_t)*(const uint8_t*)(tb + L::SCALES + 16 * h + row) << 23);
+        kscale[h] = scale_value(*(const uint8_t*)(tb + L::SCALES + 16 * h + row));
         vscale[h] = *(const uint32_t*)(tb + L::SCALES + TK8 + 16 * h + 4 * grp);
       }
       // which of this lane's keys (bits 0-3: 4 grp + i, bits 4-7: 16 + 4 grp + i) its row sees

@@ -20,7 +20,7 @@ what its tensors hold.  A page index outside the pool is a page that holds nothi
 
 Pages of ``torch.float8_e4m3fn`` take half the memory, and half the reads of a decode step.  With them go
 ``k_scales`` / ``v_scales`` ``[P, H, page]`` (uint8): the numbers ``q`` of a slot and head stand for
-``q * 2^(s - 127)``, ``s`` its scale byte.  The append chooses it per row: ``s - 127`` is the smallest
+``q * 2^(s - 127)``, ``s`` its scale byte, 1 to 254.  The append chooses it per row: ``s - 127`` is the smallest
 whole number ``e >= -117`` with ``max |x| <= 448 * 2^e``.  Values keep 4 significant bits (half a step is
 ``2^-4`` of a value); infinities and NaN become NaN.
 

@@ -420,7 +420,7 @@ int cea_paged_attention(const cea_tensor* q, const cea_tensor* k_pages, const ce
 
 /*
  * Pages of 8 bits.  k_pages, v_pages [P,H,page,D] are CEA_F8 and k_scales, v_scales [P,H,page] CEA_U8 (any
- * strides): the numbers q of a slot and head stand for q * 2^(s - 127), s their scale byte.  D even.
+ * strides): the numbers q of a slot and head stand for q * 2^(s - 127), s their scale byte, 1 to 254.  D even.
  *
  * cea_paged_kv_append8 is cea_paged_kv_append into such pages, for bf16, f16 and f32 rows: K rotated in f32
  * (products and sum rounded once each), then every row by its largest finite magnitude m,
