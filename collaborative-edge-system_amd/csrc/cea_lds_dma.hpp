@@ -48,6 +48,16 @@ __device__ __forceinline__ void buffer_load_lds16_m0(i32x4 rs, uint32_t lds, uin
                ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voffset), "s"(rs) : "memory", "m0");
 }
 
+__device__ __forceinline__ void buffer_load_lds16_nt_m0(i32x4 rs, uint32_t lds, uint32_t voffset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds"
+               ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voffset), "s"(rs) : "memory", "m0");
+}
+// 16 bytes of each lane's own address to LDS at lds + 16 * lane.
+__device__ __forceinline__ void global_load_lds16_m0(uint64_t address, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(address) : "memory", "m0");
+}
+
 // 16-byte load with a wave-uniform byte offset (soffset) added to the per-lane offset.
 __device__ __forceinline__ void buffer_load_lds16_m0_so(i32x4 rs, uint32_t lds, uint32_t voffset,
                                                         uint32_t soffset) {

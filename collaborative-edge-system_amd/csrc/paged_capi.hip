@@ -224,6 +224,8 @@ bool paged_tiles_supported(const PagedParams& p) {
     for (int64_t s : {p.kss_p, p.kss_h, p.vss_p, p.vss_h})
       if (s % 16) return false;
     if (p.kss_s != 1 || p.vss_s != 1) return false;
+    for (int64_t s : {p.ks_p, p.vs_p, p.kss_p, p.vss_p, p.ts_w})  // (in 32 bits)
+      if (s < 0 || s >= (int64_t)1 << 32) return false;
   }
   // a 64-row tile spans less than 2^31 bytes
   for (int64_t s : {p.ks_s, p.vs_s})

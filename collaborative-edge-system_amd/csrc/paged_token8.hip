@@ -5,8 +5,9 @@
 //   k_j = kq_j * 2^(ks_j - 127),  v_j = vq_j * 2^(vs_j - 127)
 //
 // Units, runs, joins and the softmax are the 16-bit form's (paged_token.hip).  What 8 bits change:
-//   * a wave's tile is 32 keys, as many bytes as 16 of the 16-bit form: two halves of 16 rows, each in one page
-//     with an address of its own, and their 64 scale bytes by one load of four lanes;
+//   * a wave's tile is 32 keys, as many bytes as 16 of the 16-bit form: two halves of 16 rows, in one page where
+//     pages are multiples of 32 slots, else each with an address of its own, and their 64 scale bytes by one load of
+//     four lanes;
 //   * S = K.Q^T with v_mfma_f32_16x16x32: a lane reads 16 numbers of a key (the queries' features are in the same
 //     order) and turns them into the queries' type with the key's scale, two an instruction, exactly;
 //   * O^T += V^T.P^T with v_mfma_f32_16x16x32_bf16: ds_read_b64_tr_b8 gives a lane 8 keys of one feature, which become
@@ -16,6 +17,8 @@
 //   * a number that is not finite can only be NaN.  In a tile that all rows see it makes the NaN that the
 //     definition makes.  In others (the last ones of a unit) what no row sees is taken as 0, and a NaN that some rows
 //     see sums its tile's products one by one.
+#include <type_traits>
+
 #include "paged_token.hpp"
 
 namespace cea {
@@ -53,10 +56,11 @@ template <typename T> __device__ __forceinline__ typename Mfma16<T>::frag8 widen
   return __builtin_bit_cast(typename Mfma16<T>::frag8, x);
 }
 
-// 16 bytes of each lane's own address into LDS at a base + 16 * lane.
-__device__ __forceinline__ void global_load_lds16(const void* p, const char* lds_base) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-               ::"s"(lds_addr(lds_base)), "v"(p) : "memory", "m0");
+// A wave-uniform value that stays in a scalar register (read again from the arguments, it would be waited for where
+// it is used, with every LDS read before it).
+template <typename X> __device__ __forceinline__ X in_sgpr(X v) {
+  asm volatile("" : "+s"(v));
+  return v;
 }
 
 template <typename T, int D, int VIS, int NW, bool SPLIT, int PC>
@@ -73,6 +77,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void paged_token8_kernel(
   const bool row_real = row < nrows;
   const int rs = row_real ? row / args.G : 0, rg = row_real ? row - rs * args.G : 0;
   char* wb = dsmem + wave * L::WAVE_BYTES;
+  const uint32_t wave_lds = lds_addr(dsmem) + wave * L::WAVE_BYTES;
 
   // ---- this workgroup's run of blocks
   int b, unit, lo, left, blocks;
@@ -101,15 +106,16 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void paged_token8_kernel(
   const float grow_thr = kRescaleLog2 / c;
   const uint32_t flip = scale < 0.f ? 0x80008000u : 0u;
   const uint32_t krow = (uint32_t)args.p.ks_s, vrow = (uint32_t)args.p.vs_s;
+  const bool one_page = args.page16 % 2 == 0;  // both halves of a tile lie in the same one
   uint32_t k_voff[2][L::LOADS], v_voff[2][L::LOADS];
 #pragma unroll
   for (int h = 0; h < 2; ++h)
 #pragma unroll
     for (int i = 0; i < L::LOADS; ++i) {
-      const int r = i * (1024 / L::ROW) + lane / (L::ROW / 16);
+      const int r = i * (1024 / L::ROW) + lane / (L::ROW / 16), from = one_page ? 16 * h + r : r;
       const int pg = lane % (L::ROW / 16);  // physical 16-byte group
-      k_voff[h][i] = r * krow + ((pg ^ k8_swz<D>(r)) << 4);
-      v_voff[h][i] = r * vrow + ((pg ^ v8_swz<D>(16 * h + r)) << 4);
+      k_voff[h][i] = from * krow + ((pg ^ k8_swz<D>(r)) << 4);
+      v_voff[h][i] = from * vrow + ((pg ^ v8_swz<D>(16 * h + r)) << 4);
     }
   uint32_t k_raddr[D / 64], v_raddr[D / 16];
 #pragma unroll
@@ -135,54 +141,77 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void paged_token8_kernel(
     const char* vh = (const char*)p.v + (int64_t)kvh * p.vs_h;
     const uint8_t* ksh = p.k_scales + (int64_t)kvh * p.kss_h;
     const uint8_t* vsh = p.v_scales + (int64_t)kvh * p.vss_h;
+    const uint32_t ks_p = in_sgpr((uint32_t)p.ks_p), vs_p = in_sgpr((uint32_t)p.vs_p), pages = in_sgpr((uint32_t)p.P);
+    const uint32_t kss_p = in_sgpr((uint32_t)p.kss_p), vss_p = in_sgpr((uint32_t)p.vss_p);
+    const uint32_t page16 = in_sgpr((uint32_t)t.page16), magic = in_sgpr(t.magic), ts_w = in_sgpr((uint32_t)p.ts_w);
 
-    // this wave's tiles: slots slot0, slot0 + BLK, ... below end, two halves each
-    auto page_of = [&](int slot) -> int {
-      const uint32_t u = (uint32_t)slot >> 4;
-      return (int)(t.page16 == 1 ? u : __umulhi(u, t.magic));
-    };
+    // this wave's tiles: slots slot0, slot0 + BLK, ... below end, two halves each; the places in their pages are
+    // known as soon as the pages' indices are asked for
     struct Ids {
       int64_t id[2];
+      uint32_t place[2];
     };
     auto ids_of = [&](int slot) -> Ids {
       Ids x;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int at = slot + 16 * h;
-        x.id[h] = at < cap ? table[(int64_t)page_of(at) * p.ts_w] : -1;
+        if (h == 1 && one_page) {
+          x.id[1] = x.id[0], x.place[1] = x.place[0] + 16;
+          break;
+        }
+        const uint32_t u = (uint32_t)(slot + 16 * h) >> 4, pg = page16 == 1 ? u : __umulhi(u, magic);
+        x.id[h] = slot + 16 * h < cap ? table[(uint64_t)pg * ts_w] : -1;
+        x.place[h] = (u - pg * page16) * 16;
       }
       return x;
     };
-    auto there = [&](int64_t id) { return id >= 0 && id < p.P; };
-    auto load_tile = [&](int slot0, const Ids& ids, int buf) {
-      char* dst = wb + buf * L::BUF_BYTES;
-      const uint8_t* sk[2];
-      const uint8_t* sv[2];
+    auto there = [&](int64_t id) { return (uint32_t)(id >> 32) == 0 && (uint32_t)id < pages; };
+    // Rows `rows` from a place of page `id` on: keys and values of one half or both (to LDS at lds), positions; what is
+    // behind the row's end, and of no page, reads 0.  (Strides fit 32 bits, so an address is two multiplications.)
+    struct Scales {
+      uint64_t k, v;
+    };
+    auto load_rows = [&](int64_t id, uint32_t place, int rows, uint32_t lds, auto first, auto halves) -> Scales {
+      constexpr int H0 = decltype(first)::value, HN = decltype(halves)::value;
+      const bool ok = there(id) && rows > 0;
+      const uint32_t at = ok ? (uint32_t)id : 0u, last = (uint32_t)(min(rows, 16 * HN) - 1);
+      if (!ok) place = 0;
+      const i32x4 krs = make_rsrc(kh + (uint64_t)at * ks_p + (uint64_t)place * krow, ok ? last * krow + L::ROW : 0u);
+      const i32x4 vrs = make_rsrc(vh + (uint64_t)at * vs_p + (uint64_t)place * vrow, ok ? last * vrow + L::ROW : 0u);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int slot = slot0 + 16 * h, rows = min(n - slot, 16);  // slots behind the row's end read 0
-        const bool ok = there(ids.id[h]) && rows > 0;
-        const int64_t at = ok ? ids.id[h] : 0;
-        const int place = ok ? slot - page_of(slot) * (t.page16 * 16) : 0;
-        const uint32_t kb = ok ? (uint32_t)(rows - 1) * krow + L::ROW : 0u, vb = ok ? (uint32_t)(rows - 1) * vrow + L::ROW : 0u;
-        const i32x4 krs = make_rsrc(kh + at * p.ks_p + (int64_t)place * p.ks_s, kb);
-        const i32x4 vrs = make_rsrc(vh + at * p.vs_p + (int64_t)place * p.vs_s, vb);
+      for (int h = H0; h < H0 + HN; ++h)
 #pragma unroll
-        for (int i = 0; i < L::LOADS; ++i) buffer_load_lds16_nt(krs, dst + h * L::HALF + i * 1024, k_voff[h][i]);
+        for (int i = 0; i < L::LOADS; ++i) buffer_load_lds16_nt_m0(krs, lds + h * L::HALF + i * 1024, k_voff[h][i]);
+#pragma unroll
+      for (int h = H0; h < H0 + HN; ++h)
 #pragma unroll
         for (int i = 0; i < L::LOADS; ++i)
-          buffer_load_lds16_nt(vrs, dst + L::TILE_BYTES + h * L::HALF + i * 1024, v_voff[h][i]);
-        // (the bytes of all 16 slots, which a page holds whatever the row's length; of no page, page 0's)
-        sk[h] = ksh + at * p.kss_p + place;
-        sv[h] = vsh + at * p.vss_p + place;
-        if constexpr (POS) {
-          const i32x4 prs = make_rsrc(p.pos + at * p.ps_p + place, ok ? rows * 8 : 0);
-          if (lane < 8) buffer_load_lds16(prs, dst + L::POS + h * 128, lane * 16);
-        }
+          buffer_load_lds16_nt_m0(vrs, lds + L::TILE_BYTES + h * L::HALF + i * 1024, v_voff[h][i]);
+      if constexpr (POS) {
+        const i32x4 prs = make_rsrc(p.pos + (int64_t)at * p.ps_p + place, ok ? (last + 1) * 8 : 0);
+        if (lane < 8 * HN) buffer_load_lds16_m0(prs, lds + L::POS + H0 * 128, lane * 16);
       }
-      if (lane < 4) global_load_lds16(lane == 0 ? sk[0] : lane == 1 ? sk[1] : lane == 2 ? sv[0] : sv[1], dst + L::SCALES);
+      // (the scale bytes of all slots, which a page holds whatever the row's length; of no page, page 0's)
+      return {(uint64_t)ksh + (uint64_t)at * kss_p + place, (uint64_t)vsh + (uint64_t)at * vss_p + place};
     };
-    constexpr int LPT = 4 * L::LOADS + 1 + (POS ? 2 : 0);
+    auto load_tile = [&](int slot, const Ids& ids, int buf) {
+      const uint32_t lds = wave_lds + buf * L::BUF_BYTES;
+      typedef std::integral_constant<int, 0> I0;
+      typedef std::integral_constant<int, 1> I1;
+      uint64_t from;  // lanes 0, 1: K's scales of the halves, 2, 3: V's
+      if (one_page) {
+        const Scales x = load_rows(ids.id[0], ids.place[0], n - slot, lds, I0(), std::integral_constant<int, 2>());
+        from = (lane & 2 ? x.v : x.k) + 16 * (lane & 1);
+      } else {
+        const Scales x = load_rows(ids.id[0], ids.place[0], n - slot, lds, I0(), I1());
+        const Scales y = load_rows(ids.id[1], ids.place[1], n - slot - 16, lds, I1(), I1());
+        const uint64_t k = lane & 1 ? y.k : x.k, v = lane & 1 ? y.v : x.v;
+        from = lane & 2 ? v : k;
+      }
+      if (lane < 4) global_load_lds16_m0(from, lds + L::SCALES);
+    };
+    // (with positions two of a page's halves come at once, or each by a load of its own)
+    constexpr int LPT = 4 * L::LOADS + 1 + (POS ? 1 : 0);
 
     // (the first two tiles are on their way before the queries' positions are known: they may be read
     // for nothing)
@@ -238,8 +267,9 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void paged_token8_kernel(
 
     int buf = 0;
     for (; s0 < end; s0 += BLK) {
-      if (s0 + BLK < end) wait_vmcnt<LPT>();  // this tile landed; the next may be in flight
-      else wait_vmcnt<0>();
+      if (s0 + BLK >= end) wait_vmcnt<0>();
+      else if (POS && !one_page) wait_vmcnt<LPT + 1>();
+      else wait_vmcnt<LPT>();  // this tile landed; the next may be in flight
       const char* tb = wb + buf * L::BUF_BYTES;
       u32x4 kr[2][D / 64];
       i32x2 vr[D / 16];
@@ -275,18 +305,20 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void paged_token8_kernel(
         whole = __ballot(row_real && vis != 255u) == 0;
       } else {
         whole = there(id0.id[0]) && there(id0.id[1]) && s0 + TK8 <= lim_all;
+        if (!whole) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int slot = s0 + 16 * h + grp * 4;
-          if constexpr (TREE) {
-            if (there(id0.id[h]) && row_sees) vis |= tree_window<4>(tree, slot) << (4 * h);
+          for (int h = 0; h < 2; ++h) {
+            const int slot = s0 + 16 * h + grp * 4;
+            if constexpr (TREE) {
+              if (there(id0.id[h]) && row_sees) vis |= tree_window<4>(tree, slot) << (4 * h);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (slot + i >= n) vis &= ~(1u << (4 * h + i));
-          } else {
+              for (int i = 0; i < 4; ++i)
+                if (slot + i >= n) vis &= ~(1u << (4 * h + i));
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (there(id0.id[h]) && slot + i < lim) vis |= 1u << (4 * h + i);
+              for (int i = 0; i < 4; ++i)
+                if (there(id0.id[h]) && slot + i < lim) vis |= 1u << (4 * h + i);
+            }
           }
         }
       }
@@ -325,7 +357,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void paged_token8_kernel(
           s[h] = Mfma16<T>::qk(widen8<T>(kr[h][ks][2], kr[h][ks][3], kscale[h]), qf[2 * ks + 1], s[h]);
         }
       }
-      if (!whole || nrows < ROWS) {
+      if (!whole) {  // (in whole tiles rows that are none hold scores of 0, which reach no other row)
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if (!((vis >> e) & 1u)) s[e >> 2][e & 3] = -__builtin_inff();
