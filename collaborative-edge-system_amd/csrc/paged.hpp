@@ -103,7 +103,10 @@ int launch_paged_token(const PagedParams& p, const HeadMap& map, void* ws, hipSt
 // Any number of new tokens per row.  Scratch: tile summaries with positions in the pool, and the partial
 // results of key splits.
 bool paged_chunk_supported(const PagedParams& p, const HeadMap& map);
-size_t paged_chunk_workspace_bytes(int64_t B, int64_t Sq, int64_t Hq, int group, int64_t D, int64_t slots, bool pos);
+// Forms whose rows are cut into runs that cross them, and not one by one.
+inline bool paged_chunk_runs(const PagedParams& p) { return p.kv_dtype == CEA_F8 || p.masks != nullptr; }
+size_t paged_chunk_workspace_bytes(int64_t B, int64_t Sq, int64_t Hq, int group, int64_t D, int64_t slots, bool pos,
+                                   bool runs);
 int launch_paged_chunk(const PagedParams& p, const HeadMap& map, void* ws, hipStream_t s);
 
 // f32, head size 64 or 128.  Scratch: the partial results of key splits.

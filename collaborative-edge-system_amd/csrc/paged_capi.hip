@@ -179,7 +179,7 @@ int prepare_attention(Attention& c, const AttentionArgs& a) {
       c.bytes = paged_token_workspace_bytes(B, Sq, Hq, Hkv, group, D, slots, bytes8);
     } else if (paged_chunk_supported(p, c.map)) {
       c.form = Form::chunk;
-      c.bytes = paged_chunk_workspace_bytes(B, Sq, Hq, group, D, slots, p.pos != nullptr);
+      c.bytes = paged_chunk_workspace_bytes(B, Sq, Hq, group, D, slots, p.pos != nullptr, paged_chunk_runs(p));
     }
   }
   if (c.form == Form::none && paged_f32_supported(p, c.map)) {
@@ -361,7 +361,7 @@ size_t cea_paged_attention_workspace_bytes(int64_t B, int64_t Sq, int64_t Hq, in
   for (const int group : {0, Hq % Hkv == 0 ? (int)(Hq / Hkv) : 0})
     if (in_dtype == CEA_F32) most = std::max(most, paged_f32_workspace_bytes(B, Sq, Hq, group, D, slots));
     else most = std::max({most, paged_token_workspace_bytes(B, Sq, Hq, Hkv, group, D, slots, false),
-                     paged_chunk_workspace_bytes(B, Sq, Hq, group, D, slots, true)});
+                     paged_chunk_workspace_bytes(B, Sq, Hq, group, D, slots, true, false)});
   return most;
 }
 

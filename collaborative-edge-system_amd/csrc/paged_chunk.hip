@@ -49,30 +49,38 @@ int heads_per_wg(int64_t Sq, int64_t group) {
 }
 
 struct ChunkPlan {
-  int hp, splits;
+  int hp, splits, runs;
   size_t tiles, pos32, part_out, part_lse;  // bytes: summaries, positions, the splits' partial results
 };
 
-ChunkPlan plan_chunk(int64_t B, int64_t Sq, int64_t Hq, int group, int64_t D, int64_t slots, bool pos) {
+ChunkPlan plan_chunk(int64_t B, int64_t Sq, int64_t Hq, int group, int64_t D, int64_t slots, bool pos, bool runs) {
   ChunkPlan r;
   r.hp = heads_per_wg(Sq, group);
   // Below two workgroups per compute unit the rows may be cut; their splits are at most the workgroups that the
   // tiles are dealt to, over those of a row's split, and one a row more for what does not divide.
   const int64_t per_row = (Sq + BM / r.hp - 1) / (BM / r.hp) * (Hq / r.hp), tiles = (slots + BN - 1) / BN;
-  r.splits = 0;
-  if (per_row * B < kSplitWgs && tiles >= 2 * kSplitTiles)
-    r.splits = (int)std::min<int64_t>(B * kMaxKeySplits, kSplitWgs / per_row + 1 + B);
+  r.splits = r.runs = 0;
+  const int64_t most = std::min<int64_t>(B * kMaxKeySplits, kSplitWgs / per_row + 1 + B);
+  if (runs) {
+    // (while all workgroups make less than four rounds: rows of uneven length leave the last ones to a few)
+    if (per_row < kSplitWgs && per_row * B < 4 * kSplitWgs && tiles >= kCutTiles)
+      r.splits = (int)most, r.runs = (int)(kSplitWgs / per_row);
+  } else if (per_row * B < kSplitWgs && tiles >= 2 * kSplitTiles) {
+    r.splits = (int)most;
+  }
   r.tiles = pos ? align256((size_t)B * ((slots + BN - 1) / BN) * sizeof(TileInfo)) : 0;
   r.pos32 = pos ? align256((size_t)B * ((slots + BN - 1) / BN) * 2 * BN * sizeof(int32_t)) : 0;
-  r.part_out = align256((size_t)r.splits * Sq * Hq * D * sizeof(float));
-  r.part_lse = align256((size_t)r.splits * Sq * Hq * sizeof(float));
+  const size_t parts = std::max<int64_t>(r.splits, r.runs > 0 ? r.runs + B : 0);
+  r.part_out = align256(parts * Sq * Hq * D * sizeof(float));
+  r.part_lse = align256(parts * Sq * Hq * sizeof(float));
   return r;
 }
 
 }  // namespace
 
-size_t paged_chunk_workspace_bytes(int64_t B, int64_t Sq, int64_t Hq, int group, int64_t D, int64_t slots, bool pos) {
-  const ChunkPlan r = plan_chunk(B, Sq, Hq, group, D, slots, pos);
+size_t paged_chunk_workspace_bytes(int64_t B, int64_t Sq, int64_t Hq, int group, int64_t D, int64_t slots, bool pos,
+                                   bool runs) {
+  const ChunkPlan r = plan_chunk(B, Sq, Hq, group, D, slots, pos, runs);
   return r.tiles + r.pos32 + r.part_out + r.part_lse;
 }
 
@@ -90,11 +98,12 @@ bool paged_chunk_supported(const PagedParams& p, const HeadMap& map) {
 int launch_paged_chunk(const PagedParams& params, const HeadMap& map, void* ws, hipStream_t st) {
   const int64_t slots = (int64_t)params.W * params.page;
   const PagedParams& o = params;
-  const ChunkPlan r = plan_chunk(o.B, o.Sq, o.Hq, map.group, o.D, slots, o.pos != nullptr);
+  const ChunkPlan r = plan_chunk(o.B, o.Sq, o.Hq, map.group, o.D, slots, o.pos != nullptr,
+                                 paged_chunk_runs(o));
   ChunkParams c;
   memset(&c, 0, sizeof(c));
   c.p = o;
-  c.hp = r.hp, c.splits = r.splits;
+  c.hp = r.hp, c.splits = r.splits, c.runs = r.runs;
   c.page16 = o.page / 16;
   c.magic = c.page16 > 1 ? (uint32_t)((((uint64_t)1 << 32) + c.page16 - 1) / c.page16) : 0;
   for (int h = 0; h < kPagedMapHeads && h < o.Hq && map.group <= 0; ++h) c.kv[h] = (uint8_t)map.kv[h];

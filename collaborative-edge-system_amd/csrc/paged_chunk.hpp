@@ -60,6 +60,7 @@ struct ChunkParams {
   int32_t ntiles;
   int32_t hp;                // query heads of a workgroup: 1, 2, 4
   int32_t splits;            // rows may be cut into key splits: at most so many splits in all (0: no)
+  int32_t runs;              // > 0: or the tiles of all rows into so many runs, as their number on the device says
   int32_t kv_units;          // units of query heads that share keys: KV heads (or all heads)
   float* part;               // partial results of the splits: [splits, Sq, Hq, D] and [splits, Hq, Sq]
   float* part_lse;
@@ -192,6 +193,9 @@ template <typename X> __device__ __forceinline__ X scalar(X v) {
 // four chunks of 300 over 700 to 4001 keys, 32/4 heads of 64, 54.6 / 52.4 / 56.7 / 56.2; 6 tokens of 8 rows of 100
 // to 4096, 32/8 heads of 128, - / 25.4 / - / 33.8; 128 tokens over 32768 - / 93.5 / - / 94.7)
 constexpr int kSplitWgs = 512, kSplitTiles = 4;
+// Trees and 8-bit pages are cut from tables of kCutTiles on (18 trees of 59 nodes after up to 457 slots, 8 tiles, 16.9 us
+// whole, 26.0 cut; one of 26 nodes after 777, 13 tiles, 18.7 and 15.0), and into runs where these have kRunTiles tiles.
+constexpr int kCutTiles = 12, kRunTiles = 16;
 struct Split {
   int b, split, first, count;  // a row, one of its splits, the place of its first one, how many it has
 };
@@ -206,16 +210,45 @@ __device__ __forceinline__ int scan64(int v) {  // inclusive prefix sum over the
   return v;
 }
 
+// Runs, for trees and 8-bit pages: the tiles of all rows are one line (a row without keys has one, for its result),
+// cut into equal runs, whatever the rows' lengths; a run may span several rows.  Part r + b of the partial results
+// is what run r has of row b.  Splits of rows one by one are as uneven as the rows, but none starts a second row,
+// which counts where they are short.  (us, splits / runs: 16 trees of 60 nodes after 500 to 8192 slots of 8 bits,
+// 32/8 heads of 128, 34 tiles a run, 144 / 125; 9 tokens of 5 rows of 13245, 16 tiles, 79 / 60; two trees of 90
+// after up to 9715, 14 tiles, 45.0 / 48.3; four of 51 after up to 3566, 4 tiles, 35 / 40.)
+struct Line {
+  int total, run, more;  // tiles, of a run, runs with one more
+  int mine, sums;        // this lane's row of the first 64: its tiles, and their prefix sum
+  __device__ __forceinline__ bool by_runs() const { return run >= kRunTiles; }  // (else by splits)
+  __device__ __forceinline__ int start(int r) const { return r * run + min(r, more); }
+  __device__ __forceinline__ int run_of(int at) const {
+    const int big = more * (run + 1);
+    return at < big ? at / (run + 1) : more + (at - big) / run;
+  }
+};
+__device__ __forceinline__ int row_tiles(const PagedParams& p, int b) {
+  return b < p.B ? ((int)paged_slots(p, b) + BN - 1) / BN : 0;
+}
+__device__ __forceinline__ int line_tiles(const PagedParams& p, int b) { return b < p.B ? max(1, row_tiles(p, b)) : 0; }
+__device__ __forceinline__ Line line_of(const ChunkParams& c_) {
+  const int lane = threadIdx.x & 63;
+  Line l;
+  l.mine = line_tiles(c_.p, lane);
+  l.sums = scan64(l.mine);
+  l.total = __builtin_amdgcn_readlane(l.sums, 63);
+  for (int b0 = 64; b0 < c_.p.B; b0 += 64) l.total += wave_sum_i32(line_tiles(c_.p, b0 + lane));
+  l.total = uniform(l.total);
+  l.run = uniform(l.total / max(1, c_.runs));
+  l.more = l.total - l.run * c_.runs;
+  return l;
+}
 // The split at place `at` (count 0 past the line's end), or with at < 0 row `b`'s.  per_row: workgroups of a
-// row's split.
-__device__ __forceinline__ Split find_split(const ChunkParams& c, int per_row, int at, int b) {
+// row's split; mine, total: the tiles of this lane's row of the first 64, and of all.
+__device__ __forceinline__ Split find_split(const ChunkParams& c, int per_row, int at, int b, int mine, int total) {
   const PagedParams& p = c.p;
   const int lane = threadIdx.x & 63;
-  auto tiles_of = [&](int row) { return row < p.B ? ((int)paged_slots(p, row) + BN - 1) / BN : 0; };
-  const int mine = tiles_of(lane);  // of the first 64 rows
-  int total = wave_sum_i32(mine);
-  for (int b0 = 64; b0 < p.B; b0 += 64) total += wave_sum_i32(tiles_of(b0 + lane));
-  const int per = (int)max(((int64_t)total * per_row + kSplitWgs - 1) / kSplitWgs, (int64_t)kSplitTiles);
+  auto tiles_of = [&](int row) { return row_tiles(p, row); };
+  int per = (int)max(((int64_t)total * per_row + kSplitWgs - 1) / kSplitWgs, (int64_t)kSplitTiles);
   Split r = {0, 0, 0, 0};
   int before = 0;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
@@ -249,30 +282,34 @@ template <int VIS> struct Shared {
   uint64_t words[VIS == kTree ? BM * kTreeWords : 1];  // the rows' masks
 };
 
-// PIECES: 16-bit numbers whose sum enters the value product for a probability: one for 16-bit results
-// (p rounded once, half a step of the type, as the result's own rounding is), three of bf16 or two of f16
-// for f32 results (p to 2^-23 and better).  2-norm errors against 64 bits and us, one piece / f32 results: 128 bf16
-// tokens over 32768 keys 2.3e-3, 91 / 6.8e-7, 136 (rounded to bf16 1.7e-3); two prompts of 2000 2.1e-3, 83 / 2.3e-7,
-// 125; four f16 chunks of 300 with positions 2.9e-4, 58 / 3.2e-7, 80.
-// AGAIN: over the tiles a second time, after values that are not finite.  Returns whether that is needed
-// (nothing has been written then).
-template <typename T, int D, int VIS, int PIECES, bool F8, bool AGAIN>
-__device__ __forceinline__ bool chunk_body(const ChunkParams& c_, char* smem, Shared<VIS>& sh) {
-  typedef Layout<D, VIS, F8> L;
-  constexpr bool POS = VIS == kPosition, TREE = VIS == kTree;
-  constexpr int kSize = F8 ? 1 : 2;  // bytes of an element of the pages
-  typedef typename Mfma<T>::frag frag;
-  const PagedParams& p = c_.p;
-  const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63;
-  const int r = lane & 31, g = lane >> 5;
+__device__ __forceinline__ Split find_split(const ChunkParams& c, int per_row, int at, int b) {
+  const int lane = threadIdx.x & 63, mine = row_tiles(c.p, lane);
+  int total = wave_sum_i32(mine);
+  for (int b0 = 64; b0 < c.p.B; b0 += 64) total += wave_sum_i32(row_tiles(c.p, b0 + lane));
+  return find_split(c, per_row, at, b, mine, total);
+}
 
-  // ---- work mapping over the 8 XCDs, as the prefill kernel's: KV heads are dealt to the XCDs in turn, an
-  // XCD takes as many query heads together as its L2 holds the keys of and starts the latest query
-  // blocks, which see the most, of all of them first; splits are slowest
-  const int hp_log2 = __builtin_ctz(c_.hp), hp = 1 << hp_log2;
-  const int rows_pb = BM >> hp_log2;
-  const int nqb = (p.Sq + rows_pb - 1) >> (__builtin_ctz(BM) - hp_log2);
-  const int ngroups = p.Hq >> hp_log2, units = ngroups * p.B, total = nqb * units;
+// What a workgroup does at a time: query block qb of head group hg of row b over a split of the row's tiles, or
+// over tiles [from, to).  Of a row that is cut the results go to part `place`.
+struct Job {
+  int qb, b, hg, split, nsplit, from, to, place;
+  bool cut;
+};
+struct Grid {
+  int nqb, ngroups;  // query blocks, head groups
+};
+__device__ __forceinline__ Grid grid_of(const ChunkParams& c_) {
+  const int hp_log2 = __builtin_ctz(c_.hp), rows_pb = BM >> hp_log2;
+  return {(c_.p.Sq + rows_pb - 1) >> (__builtin_ctz(BM) - hp_log2), c_.p.Hq >> hp_log2};
+}
+
+// The job of a workgroup over the 8 XCDs, as the prefill kernel's: KV heads are dealt to the XCDs in turn, an
+// XCD takes as many query heads together as its L2 holds the keys of and starts the latest query
+// blocks, which see the most, of all of them first; splits are slowest.  (nsplit 0: past the line of splits)
+template <bool LINE> __device__ __forceinline__ Job job_of(const ChunkParams& c_, const Line& line) {
+  const PagedParams& p = c_.p;
+  const Grid x = grid_of(c_);
+  const int nqb = x.nqb, ngroups = x.ngroups, units = ngroups * p.B;
   int blk = blockIdx.x, split = 0, nsplit = 1, place = 0, qb, b, hg;
   if (c_.splits > 0) {
     // (split, KV head) in turn over the XCDs, the workgroups that share its keys together
@@ -280,8 +317,9 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, char* smem, Sh
     const int i = blk >> 3, set = i / shared, in = i - set * shared;
     const int u = uniform(set * 8 + (blk & 7));
     place = u / c_.kv_units;
-    const Split x = find_split(c_, nqb * ngroups, place, 0);
-    if (x.count == 0) return false;
+    Split x;
+    if constexpr (LINE) x = find_split(c_, nqb * ngroups, place, 0, line.mine, line.total);
+    else x = find_split(c_, nqb * ngroups, place, 0);
     b = x.b, split = x.split, nsplit = x.count;
     qb = nqb - 1 - in / per_kv;
     hg = (u - place * c_.kv_units) * per_kv + in % per_kv;
@@ -315,7 +353,60 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, char* smem, Sh
     b = p.B == 1 ? 0 : unit / ngroups;
     hg = unit - b * ngroups;
   }
-  qb = uniform(qb), b = uniform(b), hg = uniform(hg), split = uniform(split);
+  Job job;
+  job.qb = uniform(qb), job.b = uniform(b), job.hg = uniform(hg), job.split = uniform(split);
+  job.nsplit = uniform(nsplit), job.place = uniform(place);
+  job.from = job.to = 0;
+  job.cut = nsplit > 1;
+  return job;
+}
+
+// The row that holds tile `at` of the line, or with at < 0 row b: its place, and its tiles.
+struct LineRow {
+  int b, first, tiles;
+};
+__device__ __forceinline__ LineRow line_row(const ChunkParams& c_, const Line& l, int at, int b) {
+  const int lane = threadIdx.x & 63;
+  LineRow r = {0, 0, 1};
+  int before = 0;
+  for (int b0 = 0; b0 < c_.p.B; b0 += 64) {
+    const int sums = b0 == 0 ? l.sums : scan64(line_tiles(c_.p, b0 + lane));
+    const uint64_t found = at >= 0 ? __ballot(before + sums > at) : (b - b0 < 64 ? 1ull << (b - b0) : 0ull);
+    if (found != 0) {
+      const int k = (int)__builtin_ctzll(found);
+      const int begin = k > 0 ? __builtin_amdgcn_readlane(sums, k - 1) : 0;
+      r = {b0 + k, before + begin, __builtin_amdgcn_readlane(sums, k) - begin};
+      break;
+    }
+    before += __builtin_amdgcn_readlane(sums, 63);
+  }
+  return r;
+}
+
+// PIECES: 16-bit numbers whose sum enters the value product for a probability: one for 16-bit results
+// (p rounded once, half a step of the type, as the result's own rounding is), three of bf16 or two of f16
+// for f32 results (p to 2^-23 and better).  2-norm errors against 64 bits and us, one piece / f32 results: 128 bf16
+// tokens over 32768 keys 2.3e-3, 91 / 6.8e-7, 136 (rounded to bf16 1.7e-3); two prompts of 2000 2.1e-3, 83 / 2.3e-7,
+// 125; four f16 chunks of 300 with positions 2.9e-4, 58 / 3.2e-7, 80.
+// AGAIN: over the tiles a second time, after values that are not finite.  Returns whether that is needed
+// (nothing has been written then).
+template <typename T, int D, int VIS, int PIECES, bool F8, bool AGAIN>
+__device__ __forceinline__ bool chunk_body(const ChunkParams& c_, const Job& job, char* smem, Shared<VIS>& sh) {
+  typedef Layout<D, VIS, F8> L;
+  constexpr bool POS = VIS == kPosition, TREE = VIS == kTree;
+  constexpr int kSize = F8 ? 1 : 2;  // bytes of an element of the pages
+  typedef typename Mfma<T>::frag frag;
+  const PagedParams& p = c_.p;
+  int tid = threadIdx.x;
+  // (what follows from the thread's number is computed again for every row of a run: kept across them it took 55
+  // registers too many)
+  if constexpr (TREE || F8) asm volatile("" : "+v"(tid));
+  const int wave = uniform(tid >> 6), lane = tid & 63;
+  const int r = lane & 31, g = lane >> 5;
+
+  const int hp_log2 = __builtin_ctz(c_.hp), hp = 1 << hp_log2;
+  const int rows_pb = BM >> hp_log2;
+  const int qb = job.qb, b = job.b, hg = job.hg;
   const int waves_log2 = __builtin_ctz(NWAVES) - hp_log2;  // waves of one head
   const int h = hg * hp + (wave >> waves_log2);
   const int kvh = p.group > 0 ? hg * hp / p.group : c_.kv[hg * hp];
@@ -341,11 +432,17 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, char* smem, Sh
     const uint32_t u = (uint32_t)slot >> 4;
     return (int)(page16 == 1 ? u : __umulhi(u, magic));
   };
-  // this split's run of the row's tiles (what its queries cannot see is left out below)
-  const int row_tiles = (n + BN - 1) / BN;
-  const int per_split = nsplit > 1 ? (row_tiles + nsplit - 1) / nsplit : row_tiles;
-  const int t_first = scalar(min(row_tiles, split * per_split));
-  int t_last = scalar(min(row_tiles, t_first + per_split));
+  // this job's part of the row's tiles (what its queries cannot see is left out below)
+  const int tiles_here = (n + BN - 1) / BN;
+  int t_first, t_last;
+  if (job.nsplit > 0) {
+    const int per_split = job.nsplit > 1 ? (tiles_here + job.nsplit - 1) / job.nsplit : tiles_here;
+    t_first = scalar(min(tiles_here, job.split * per_split));
+    t_last = scalar(min(tiles_here, t_first + per_split));
+  } else {
+    t_first = scalar(min(tiles_here, job.from));
+    t_last = scalar(min(tiles_here, job.to));
+  }
 
   // the page indices and summaries of a pass, from memory to registers and from there to LDS
   constexpr int kIdsPer = PASS * BN / 16 / NTHREADS;
@@ -433,6 +530,9 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, char* smem, Sh
   const char* vh = scalar((const char*)p.v + (int64_t)kvh * p.vs_h * kSize);
   const int64_t ks_p = scalar(p.ks_p * kSize), vs_p = scalar(p.vs_p * kSize);
   char* raw = smem + L::RAW + wave * L::RAW_WAVE;  // this wave's rows of 8-bit pages
+  const uint8_t* ksh = F8 ? scalar(p.k_scales + kvh * p.kss_h) : nullptr;
+  const uint8_t* vsh = F8 ? scalar(p.v_scales + kvh * p.vss_h) : nullptr;
+  const uint32_t kss_p = F8 ? scalar((uint32_t)p.kss_p) : 0, vss_p = F8 ? scalar((uint32_t)p.vss_p) : 0;
   const int32_t* pos32 = POS ? scalar(c_.pos32 + (int64_t)b * c_.ntiles * (2 * BN)) : nullptr;
 
   // the page index of this wave's rows of a tile (behind the row's end: the last one's)
@@ -443,8 +543,10 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, char* smem, Sh
     const bool ok = id >= 0 && rows > 0;
     const int at = ok ? id : 0;
     const int place = ok ? slot - page_of(slot) * (page16 * 16) : 0;
-    const i32x4 krs = make_rsrc(kh + at * ks_p + (int64_t)place * krow, ok ? (uint32_t)(rows - 1) * krow + L::SRC_ROW : 0u);
-    const i32x4 vrs = make_rsrc(vh + at * vs_p + (int64_t)place * vrow, ok ? (uint32_t)(rows - 1) * vrow + L::SRC_ROW : 0u);
+    const int64_t at_k = F8 ? (int64_t)((uint64_t)(uint32_t)at * (uint32_t)ks_p) : at * ks_p;
+    const int64_t at_v = F8 ? (int64_t)((uint64_t)(uint32_t)at * (uint32_t)vs_p) : at * vs_p;
+    const i32x4 krs = make_rsrc(kh + at_k + (int64_t)place * krow, ok ? (uint32_t)(rows - 1) * krow + L::SRC_ROW : 0u);
+    const i32x4 vrs = make_rsrc(vh + at_v + (int64_t)place * vrow, ok ? (uint32_t)(rows - 1) * vrow + L::SRC_ROW : 0u);
     const uint32_t st = F8 ? smem_lds + L::RAW + wave * L::RAW_WAVE : smem_lds + L::stage(stage) + wave_kv;
     constexpr int kVAt = F8 ? L::RAW_TILE : L::K_BYTES;
 #pragma unroll
@@ -452,12 +554,9 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, char* smem, Sh
 #pragma unroll
     for (int i = 0; i < L::KV_LOADS; ++i) buffer_load_lds16_m0(vrs, st + kVAt + i * 1024, v_voff[i]);
     if constexpr (F8) {  // (the scale bytes of all 16 slots, which their page holds whatever the row's length)
-      const i32x4 sk = make_rsrc(p.k_scales + at * p.kss_p + kvh * p.kss_h + place, ok ? 16u : 0u);
-      const i32x4 sv = make_rsrc(p.v_scales + at * p.vss_p + kvh * p.vss_h + place, ok ? 16u : 0u);
-      if (lane == 0) {
-        buffer_load_lds16_m0(sk, st + 2 * L::RAW_TILE, 0);
-        buffer_load_lds16_m0(sv, st + 2 * L::RAW_TILE + WROWS, 0);
-      }
+      const uint64_t sk = (uint64_t)ksh + (uint64_t)(uint32_t)at * kss_p + place;
+      const uint64_t sv = (uint64_t)vsh + (uint64_t)(uint32_t)at * vss_p + place;
+      if (lane < 2) global_load_lds16_m0(lane == 0 ? sk : sv, st + 2 * L::RAW_TILE);
     }
     if constexpr (POS) {
       if (wave == 0) {
@@ -909,14 +1008,14 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, char* smem, Sh
   asm volatile("" : "+v"(l_bits));  // (compared as a float, a NaN might be taken for 0 in this file)
   const bool empty = !sees || (l_bits << 1) == 0;
   const float inv = empty ? 0.f : 1.f / (l_tot * kPieceScale);
-  if ((p.lse || nsplit > 1) && g == 0) {
-    float* lp = nsplit > 1 ? c_.part_lse + ((int64_t)place * p.Hq + h) * p.Sq + row
+  if ((p.lse || job.cut) && g == 0) {
+    float* lp = job.cut ? c_.part_lse + ((int64_t)job.place * p.Hq + h) * p.Sq + row
                            : (float*)p.lse + b * p.ls_b + h * p.ls_h + (int64_t)row * p.ls_s;
     *lp = empty ? -__builtin_inff() : (m_run * fabsf(scale) + logf(l_tot)) - kExpShift * 0.69314718055994531f;
   }
-  const int64_t orow = nsplit > 1 ? (((int64_t)place * p.Sq + row) * p.Hq + h) * D
+  const int64_t orow = job.cut ? (((int64_t)job.place * p.Sq + row) * p.Hq + h) * D
                                   : b * p.os_b + (int64_t)row * p.os_s + h * p.os_h;
-  float* fout = nsplit > 1 ? c_.part : p.out_dtype == CEA_F32 ? (float*)p.out : nullptr;
+  float* fout = job.cut ? c_.part : p.out_dtype == CEA_F32 ? (float*)p.out : nullptr;
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
@@ -941,8 +1040,8 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, char* smem, Sh
 typedef const void __attribute__((address_space(4))) * kernel_args_ptr;
 typedef __attribute__((address_space(3))) char* lds_ptr;
 template <typename T, int D, int VIS, int PIECES, bool F8>
-__device__ __noinline__ void chunk_again(kernel_args_ptr args, lds_ptr smem, lds_ptr sh) {
-  chunk_body<T, D, VIS, PIECES, F8, true>(*(const ChunkParams*)args, (char*)smem, *(Shared<VIS>*)(char*)sh);
+__device__ __noinline__ void chunk_again(kernel_args_ptr args, Job job, lds_ptr smem, lds_ptr sh) {
+  chunk_body<T, D, VIS, PIECES, F8, true>(*(const ChunkParams*)args, job, (char*)smem, *(Shared<VIS>*)(char*)sh);
 }
 
 // Three waves a SIMD at D = 64 and one piece leave 168 registers, of which the form with positions spills 5 (four
@@ -951,9 +1050,56 @@ template <typename T, int D, int VIS, int PIECES, bool F8>
 __global__ __launch_bounds__(NTHREADS, D == 64 && PIECES == 1 ? 3 : 2) void paged_chunk_kernel(const ChunkParams c_) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ Shared<VIS> sh;
-  if (chunk_body<T, D, VIS, PIECES, F8, false>(c_, smem, sh))
-    chunk_again<T, D, VIS, PIECES, F8>((kernel_args_ptr)__builtin_amdgcn_kernarg_segment_ptr(), (lds_ptr)smem,
-                                       (lds_ptr)(char*)&sh);
+  auto work = [&](const ChunkParams& args, const Job& job) {
+    if (chunk_body<T, D, VIS, PIECES, F8, false>(args, job, smem, sh))
+      chunk_again<T, D, VIS, PIECES, F8>((kernel_args_ptr)__builtin_amdgcn_kernarg_segment_ptr(), job, (lds_ptr)smem,
+                                         (lds_ptr)(char*)&sh);
+  };
+  if constexpr (VIS != kTree && !F8) {
+    const Job job = job_of<false>(c_, Line());
+    if (job.nsplit > 0) work(c_, job);
+  } else {
+    Job job;
+    int left = 0, tiles = 0, run = 0;
+    Line line = {};
+    if (c_.runs > 0) line = line_of(c_);
+    const bool by_runs = uniform(line.by_runs() ? 1 : 0) != 0;
+    if (by_runs) {
+      // (run, KV head) in turn over the XCDs, the workgroups that share its keys together
+      const Grid x = grid_of(c_);
+      const int per_kv = x.ngroups / c_.kv_units, shared = per_kv * x.nqb;
+      const int i = blockIdx.x >> 3, set = i / shared, in = i - set * shared, u = set * 8 + (blockIdx.x & 7);
+      run = uniform(u / c_.kv_units);
+      if (run >= c_.runs) return;
+      const int at = line.start(run);
+      const LineRow r = line_row(c_, line, at, 0);
+      left = line.run + (run < line.more ? 1 : 0);
+      job.qb = uniform(x.nqb - 1 - in / per_kv);
+      job.hg = uniform((u - run * c_.kv_units) * per_kv + in % per_kv);
+      job.b = uniform(r.b), job.from = uniform(at - r.first), job.split = 0, job.nsplit = 0;
+      tiles = uniform(r.tiles), left = uniform(left);
+    } else {
+      job = job_of<true>(c_, line);
+      if (job.nsplit == 0) return;
+    }
+    while (true) {
+      if (by_runs) {
+        job.to = min(tiles, job.from + left);
+        job.cut = job.from > 0 || job.to < tiles;
+        job.place = run + job.b;
+      }
+      // (the arguments too are read again)
+      kernel_args_ptr args = (kernel_args_ptr)__builtin_amdgcn_kernarg_segment_ptr();
+      asm volatile("" : "+s"(args));
+      work(*(const ChunkParams*)args, job);
+      left -= job.to - job.from;
+      if (!by_runs || left <= 0) return;
+      __syncthreads();  // the next row's start writes what this one's end reads
+      ++job.b;
+      job.from = 0;
+      tiles = uniform(line_tiles(c_.p, job.b));
+    }
+  }
 }
 
 
@@ -963,34 +1109,52 @@ template <typename T, int D>
 __global__ __launch_bounds__(256) void paged_chunk_join_kernel(const ChunkParams c, int per_row) {
   const PagedParams& p = c.p;
   const int b = blockIdx.y;
-  const Split cut = find_split(c, per_row, -1, b);
-  const int n = uniform(cut.count);
+  int n, part;
+  Line line = {};
+  if (c.runs > 0) line = line_of(c);
+  if (line.by_runs()) {
+    const LineRow r = line_row(c, line, -1, b);
+    const int first = line.run_of(r.first);
+    n = uniform(line.run_of(r.first + r.tiles - 1) - first + 1);
+    part = uniform(first + b);
+  } else {
+    const Split cut = c.runs > 0 ? find_split(c, per_row, -1, b, line.mine, line.total) : find_split(c, per_row, -1, b);
+    n = uniform(cut.count);
+    part = uniform(cut.first);
+  }
   if (n == 1) return;  // written by its workgroups
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= (int64_t)p.Sq * p.Hq * (D / 4)) return;
   const int f = (int)(i % (D / 4)) * 4;
   const int h = (int)(i / (D / 4) % p.Hq), s = (int)(i / ((int64_t)(D / 4) * p.Hq));
   const int64_t o_split = (int64_t)p.Sq * p.Hq * D, l_split = (int64_t)p.Hq * p.Sq;
-  const float* o = c.part + cut.first * o_split + ((int64_t)s * p.Hq + h) * D + f;
-  const float* l = c.part_lse + cut.first * l_split + (int64_t)h * p.Sq + s;
-  float4 x[kMaxKeySplits];
-  float lse[kMaxKeySplits], m = -__builtin_inff();
-#pragma unroll
-  for (int k = 0; k < kMaxKeySplits; ++k)
-    if (k < n) lse[k] = l[k * l_split], x[k] = *(const float4*)(o + k * o_split);
-#pragma unroll
-  for (int k = 0; k < kMaxKeySplits; ++k)
-    if (k < n) m = fmaxf(m, lse[k]);
-  const float shift = m == -__builtin_inff() ? 0.f : m;
+  const float* o = c.part + part * o_split + ((int64_t)s * p.Hq + h) * D + f;
+  const float* l = c.part_lse + part * l_split + (int64_t)h * p.Sq + s;
+  float m = -__builtin_inff(), shift = 0.f, sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float sum = 0.f;
+  for (int k0 = 0; k0 < n; k0 += kMaxKeySplits) {  // (splits: one turn)
+    float4 x[kMaxKeySplits];
+    float lse[kMaxKeySplits], m_new = m;
 #pragma unroll
-  for (int k = 0; k < kMaxKeySplits; ++k)
-    if (k < n) {
-      const float w = expf(lse[k] - shift);  // 0 for a split that the row sees nothing of, whose output is 0
-      sum += w;
-      acc.x += x[k].x * w, acc.y += x[k].y * w, acc.z += x[k].z * w, acc.w += x[k].w * w;
+    for (int k = 0; k < kMaxKeySplits; ++k)
+      if (k0 + k < n) lse[k] = l[(k0 + k) * l_split], x[k] = *(const float4*)(o + (k0 + k) * o_split);
+#pragma unroll
+    for (int k = 0; k < kMaxKeySplits; ++k)
+      if (k0 + k < n) m_new = fmaxf(m_new, lse[k]);
+    shift = m_new == -__builtin_inff() ? 0.f : m_new;
+    if (k0 > 0) {
+      const float a = expf(m - shift);  // (0 while there was nothing)
+      sum *= a, acc.x *= a, acc.y *= a, acc.z *= a, acc.w *= a;
     }
+    m = m_new;
+#pragma unroll
+    for (int k = 0; k < kMaxKeySplits; ++k)
+      if (k0 + k < n) {
+        const float w = expf(lse[k] - shift);  // 0 for a split that the row sees nothing of, whose output is 0
+        sum += w;
+        acc.x += x[k].x * w, acc.y += x[k].y * w, acc.z += x[k].z * w, acc.w += x[k].w * w;
+      }
+  }
   uint32_t bits = __float_as_uint(sum);
   asm volatile("" : "+v"(bits));  // (the file is compiled as if no NaN occurred)
   const bool empty = bits == 0;
@@ -1015,14 +1179,15 @@ int launch_form(const ChunkParams& c, hipStream_t st) {
   const int nqb = (p.Sq + BM / c.hp - 1) / (BM / c.hp);
   const int64_t per_row = (int64_t)nqb * (p.Hq / c.hp);
   int64_t total = per_row * p.B;
-  if (c.splits > 0) total = ((int64_t)c.splits * c.kv_units + 7) / 8 * 8 * (per_row / c.kv_units);
+  const int cuts = std::max(c.splits, c.runs);
+  if (cuts > 0) total = ((int64_t)cuts * c.kv_units + 7) / 8 * 8 * (per_row / c.kv_units);
   constexpr int lds = Layout<D, VIS, F8>::LDS_BYTES;
   const hipError_t e = reserve_lds<paged_chunk_kernel<T, D, VIS, PIECES, F8>>(lds);
   CEA_REQUIRE(e == hipSuccess, CEA_ELAUNCH, "paged_attention: cannot reserve %d bytes of LDS: %s", lds,
               hipGetErrorString(e));
   hipLaunchKernelGGL((paged_chunk_kernel<T, D, VIS, PIECES, F8>), dim3((unsigned)total), dim3(NTHREADS), lds, st, c);
   CEA_CHECK_LAUNCH("paged_chunk");
-  if (c.splits > 0) {
+  if (cuts > 0) {
     const int64_t vectors = (int64_t)p.Sq * p.Hq * (D / 4);
     hipLaunchKernelGGL((paged_chunk_join_kernel<T, D>), dim3((unsigned)((vectors + 255) / 256), (unsigned)p.B), dim3(256),
                        0, st, c, (int)per_row);
