@@ -435,7 +435,7 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, const Job& job
   // this job's part of the row's tiles (what its queries cannot see is left out below)
   const int tiles_here = (n + BN - 1) / BN;
   int t_first, t_last;
-  if (job.nsplit > 0) {
+  if (!(TREE || F8) || job.nsplit > 0) {
     const int per_split = job.nsplit > 1 ? (tiles_here + job.nsplit - 1) / job.nsplit : tiles_here;
     t_first = scalar(min(tiles_here, job.split * per_split));
     t_last = scalar(min(tiles_here, t_first + per_split));
@@ -547,12 +547,14 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, const Job& job
     const int64_t at_v = F8 ? (int64_t)((uint64_t)(uint32_t)at * (uint32_t)vs_p) : at * vs_p;
     const i32x4 krs = make_rsrc(kh + at_k + (int64_t)place * krow, ok ? (uint32_t)(rows - 1) * krow + L::SRC_ROW : 0u);
     const i32x4 vrs = make_rsrc(vh + at_v + (int64_t)place * vrow, ok ? (uint32_t)(rows - 1) * vrow + L::SRC_ROW : 0u);
-    const uint32_t st = F8 ? smem_lds + L::RAW + wave * L::RAW_WAVE : smem_lds + L::stage(stage) + wave_kv;
+    const uint32_t stage_lds = smem_lds + L::stage(stage);
+    const uint32_t st = F8 ? smem_lds + L::RAW + wave * L::RAW_WAVE : stage_lds;
+    const uint32_t k_at = F8 ? 0 : wave_kv;
     constexpr int kVAt = F8 ? L::RAW_TILE : L::K_BYTES;
 #pragma unroll
-    for (int i = 0; i < L::KV_LOADS; ++i) buffer_load_lds16_m0(krs, st + i * 1024, k_voff[i]);
+    for (int i = 0; i < L::KV_LOADS; ++i) buffer_load_lds16_m0(krs, st + k_at + i * 1024, k_voff[i]);
 #pragma unroll
-    for (int i = 0; i < L::KV_LOADS; ++i) buffer_load_lds16_m0(vrs, st + kVAt + i * 1024, v_voff[i]);
+    for (int i = 0; i < L::KV_LOADS; ++i) buffer_load_lds16_m0(vrs, st + kVAt + k_at + i * 1024, v_voff[i]);
     if constexpr (F8) {  // (the scale bytes of all 16 slots, which their page holds whatever the row's length)
       const uint64_t sk = (uint64_t)ksh + (uint64_t)(uint32_t)at * kss_p + place;
       const uint64_t sv = (uint64_t)vsh + (uint64_t)(uint32_t)at * vss_p + place;
@@ -561,7 +563,7 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, const Job& job
     if constexpr (POS) {
       if (wave == 0) {
         const i32x4 prs = make_rsrc(pos32 + (int64_t)tile * (2 * BN), BN * 8);
-        if (lane < BN / 2) buffer_load_lds16_m0(prs, smem_lds + L::pos(stage), lane * 16);
+        if (lane < BN / 2) buffer_load_lds16_m0(prs, (F8 ? smem_lds + L::pos(stage) : stage_lds + L::pos(0)), lane * 16);
       }
     }
   };
@@ -653,7 +655,7 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, const Job& job
       for (int ks = 0; ks < D / 16; ++ks) kf[ks] = *(const frag*)(sb + kb * 32 * L::KROW + (k_read0 ^ (ks << 5)));
       f32x16 acc = {};
       if constexpr (POS) {  // 0, or -inf where no key
-        const char* start = smem + L::pos(stage) + BN * 4 + (kb * 32 + g * 4) * 4;
+        const char* start = (F8 ? smem + L::pos(stage) : sb + L::pos(0)) + BN * 4 + (kb * 32 + g * 4) * 4;
 #pragma unroll
         for (int i4 = 0; i4 < 4; ++i4) {
           const float4 x = *(const float4*)(start + i4 * 32);
@@ -675,7 +677,7 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, const Job& job
     if (mode == 1) return;
     if (mode == 2) {
       if constexpr (POS) {
-        const char* pl = smem + L::pos(stage);
+        const char* pl = F8 ? smem + L::pos(stage) : sb + L::pos(0);
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -1105,20 +1107,27 @@ __global__ __launch_bounds__(NTHREADS, D == 64 && PIECES == 1 ? 3 : 2) void page
 
 // Joins a row's key splits by their log-sum-exp, four features a thread; every read is under way before
 // the first weight is known.
-template <typename T, int D>
+// (RUNS: the parts of a row may be many, eight at a time; a row's splits are 16 at most)
+template <typename T, int D, bool RUNS>
 __global__ __launch_bounds__(256) void paged_chunk_join_kernel(const ChunkParams c, int per_row) {
+  constexpr int TURN = RUNS ? 8 : kMaxKeySplits;
   const PagedParams& p = c.p;
   const int b = blockIdx.y;
   int n, part;
-  Line line = {};
-  if (c.runs > 0) line = line_of(c);
-  if (line.by_runs()) {
-    const LineRow r = line_row(c, line, -1, b);
-    const int first = line.run_of(r.first);
-    n = uniform(line.run_of(r.first + r.tiles - 1) - first + 1);
-    part = uniform(first + b);
+  if constexpr (RUNS) {
+    const Line line = line_of(c);
+    if (line.by_runs()) {
+      const LineRow r = line_row(c, line, -1, b);
+      const int first = line.run_of(r.first);
+      n = uniform(line.run_of(r.first + r.tiles - 1) - first + 1);
+      part = uniform(first + b);
+    } else {
+      const Split cut = find_split(c, per_row, -1, b, line.mine, line.total);
+      n = uniform(cut.count);
+      part = uniform(cut.first);
+    }
   } else {
-    const Split cut = c.runs > 0 ? find_split(c, per_row, -1, b, line.mine, line.total) : find_split(c, per_row, -1, b);
+    const Split cut = find_split(c, per_row, -1, b);
     n = uniform(cut.count);
     part = uniform(cut.first);
   }
@@ -1132,28 +1141,29 @@ __global__ __launch_bounds__(256) void paged_chunk_join_kernel(const ChunkParams
   const float* l = c.part_lse + part * l_split + (int64_t)h * p.Sq + s;
   float m = -__builtin_inff(), shift = 0.f, sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int k0 = 0; k0 < n; k0 += kMaxKeySplits) {  // (splits: one turn)
-    float4 x[kMaxKeySplits];
-    float lse[kMaxKeySplits], m_new = m;
+  for (int k0 = 0; k0 < n; k0 += TURN) {
+    float4 x[TURN];
+    float lse[TURN], m_new = m;
 #pragma unroll
-    for (int k = 0; k < kMaxKeySplits; ++k)
+    for (int k = 0; k < TURN; ++k)
       if (k0 + k < n) lse[k] = l[(k0 + k) * l_split], x[k] = *(const float4*)(o + (k0 + k) * o_split);
 #pragma unroll
-    for (int k = 0; k < kMaxKeySplits; ++k)
+    for (int k = 0; k < TURN; ++k)
       if (k0 + k < n) m_new = fmaxf(m_new, lse[k]);
     shift = m_new == -__builtin_inff() ? 0.f : m_new;
-    if (k0 > 0) {
+    if (RUNS && k0 > 0) {
       const float a = expf(m - shift);  // (0 while there was nothing)
       sum *= a, acc.x *= a, acc.y *= a, acc.z *= a, acc.w *= a;
     }
     m = m_new;
 #pragma unroll
-    for (int k = 0; k < kMaxKeySplits; ++k)
+    for (int k = 0; k < TURN; ++k)
       if (k0 + k < n) {
         const float w = expf(lse[k] - shift);  // 0 for a split that the row sees nothing of, whose output is 0
         sum += w;
         acc.x += x[k].x * w, acc.y += x[k].y * w, acc.z += x[k].z * w, acc.w += x[k].w * w;
       }
+    if constexpr (!RUNS) break;
   }
   uint32_t bits = __float_as_uint(sum);
   asm volatile("" : "+v"(bits));  // (the file is compiled as if no NaN occurred)
@@ -1189,7 +1199,7 @@ int launch_form(const ChunkParams& c, hipStream_t st) {
   CEA_CHECK_LAUNCH("paged_chunk");
   if (cuts > 0) {
     const int64_t vectors = (int64_t)p.Sq * p.Hq * (D / 4);
-    hipLaunchKernelGGL((paged_chunk_join_kernel<T, D>), dim3((unsigned)((vectors + 255) / 256), (unsigned)p.B), dim3(256),
+    hipLaunchKernelGGL((paged_chunk_join_kernel<T, D, VIS == kTree || F8>), dim3((unsigned)((vectors + 255) / 256), (unsigned)p.B), dim3(256),
                        0, st, c, (int)per_row);
     CEA_CHECK_LAUNCH("paged_chunk_join");
   }
