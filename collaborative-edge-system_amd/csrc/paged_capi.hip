@@ -201,6 +201,24 @@ bool pages_apart(const cea_tensor& t) {
   return (t.size[near] <= 1 || t.stride[near] >= t.size[2]) && (t.size[far] <= 1 || t.stride[far] >= span);
 }
 
+// The elements of a pool are apart: in the order of the strides each dimension steps over all that the ones
+// before it span.  Views of a tensor that holds each element once are.
+bool elements_apart(const cea_tensor& t) {
+  int order[CEA_MAX_DIMS], n = 0;
+  for (int i = 0; i < t.ndim; ++i) {
+    if (t.size[i] == 0) return true;
+    if (t.size[i] > 1) order[n++] = i;
+  }
+  std::sort(order, order + n, [&](int a, int b) { return t.stride[a] < t.stride[b]; });
+  int64_t span = 1;
+  for (int i = 0; i < n; ++i) {
+    const int64_t stride = t.stride[order[i]], steps = t.size[order[i]] - 1;
+    if (stride < span || stride > (((int64_t)1 << 62) - span) / steps) return false;
+    span += stride * steps;
+  }
+  return true;
+}
+
 }  // namespace
 
 bool paged_tiles_supported(const PagedParams& p) {
@@ -479,6 +497,8 @@ int cea_paged_kv_keep(cea_tensor* kv, cea_tensor* scales, int32_t page, const ce
                     scales->size[3] == page,
                 CEA_EINVAL, "%s: scales must be [N, P, H, page]", what);
   }
+  // (a row that two of the pools hold would be moved by both)
+  CEA_REQUIRE(elements_apart(*kv) && (!scales || elements_apart(*scales)), CEA_EINVAL, "%s: pools overlap", what);
   if ((rc = check_tensor(path, "path", 2, CEA_I64, false))) return rc;
   if ((rc = check_rows(tables, offsets, "offsets", path->size[0], what))) return rc;
   if (counts && (rc = check_counts(counts, path->size[0], what))) return rc;

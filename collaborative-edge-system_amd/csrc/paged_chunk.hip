@@ -62,9 +62,14 @@ ChunkPlan plan_chunk(int64_t B, int64_t Sq, int64_t Hq, int group, int64_t D, in
   r.splits = r.runs = 0;
   const int64_t most = std::min<int64_t>(B * kMaxKeySplits, kSplitWgs / per_row + 1 + B);
   if (runs) {
-    // (while all workgroups make less than four rounds: rows of uneven length leave the last ones to a few)
-    if (per_row < kSplitWgs && per_row * B < 4 * kSplitWgs && tiles >= kCutTiles)
-      r.splits = (int)most, r.runs = (int)(kSplitWgs / per_row);
+    // Runs where a row's query blocks see about the same tiles (of a prompt the last blocks see the most, and would
+    // see the most of every row of a run), and up to four rounds of workgroups: rows of uneven length leave the last
+    // ones to a few.
+    const bool even = Sq <= BM / r.hp || Sq * 8 <= slots;
+    if (tiles >= kCutTiles && per_row < kSplitWgs && per_row * B < (even ? 4 : 1) * kSplitWgs) {
+      r.splits = (int)most;
+      r.runs = even ? (int)(kSplitWgs / per_row) : 0;
+    }
   } else if (per_row * B < kSplitWgs && tiles >= 2 * kSplitTiles) {
     r.splits = (int)most;
   }

@@ -238,7 +238,7 @@ __device__ __forceinline__ Line line_of(const ChunkParams& c_) {
   l.total = __builtin_amdgcn_readlane(l.sums, 63);
   for (int b0 = 64; b0 < c_.p.B; b0 += 64) l.total += wave_sum_i32(line_tiles(c_.p, b0 + lane));
   l.total = uniform(l.total);
-  l.run = uniform(l.total / max(1, c_.runs));
+  l.run = c_.runs > 0 ? uniform(l.total / c_.runs) : 0;
   l.more = l.total - l.run * c_.runs;
   return l;
 }
@@ -1064,7 +1064,7 @@ __global__ __launch_bounds__(NTHREADS, D == 64 && PIECES == 1 ? 3 : 2) void page
     Job job;
     int left = 0, tiles = 0, run = 0;
     Line line = {};
-    if (c_.runs > 0) line = line_of(c_);
+    if (c_.splits > 0) line = line_of(c_);
     const bool by_runs = uniform(line.by_runs() ? 1 : 0) != 0;
     if (by_runs) {
       // (run, KV head) in turn over the XCDs, the workgroups that share its keys together

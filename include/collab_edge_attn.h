@@ -494,7 +494,7 @@ int cea_tree_masks(const cea_tensor* parents, const cea_tensor* counts, cea_tens
  * offsets[b] + path[b, i] held before the call, in all N pools of kv [N,P,H,page*D] (the layers' keys and values;
  * any type, `page` slots of D contiguous elements) and, for 8-bit pages, scales [N,P,H,page] (else NULL).  path
  * [B,n] int64 on the device; entries below i (-1: none) move nothing, and nodes in order need no others, nor do
- * entries from counts[b] on (the row's nodes; NULL: any).
+ * entries from counts[b] on (the row's nodes; NULL: any).  No element of the pools may be another's too.
  */
 int cea_paged_kv_keep(cea_tensor* kv, cea_tensor* scales, int32_t page, const cea_tensor* tables,
                       const cea_tensor* offsets, const cea_tensor* counts, const cea_tensor* path, void* stream);

@@ -395,3 +395,100 @@ def test_other_stream(cea, dev):
         got = D.call(cea, c, dev)
     s.synchronize()
     assert torch.equal(got, want)
+
+
+# ---------------------------------------------------------------------------------------
+# rows cut into runs that cross them, and many rows
+# ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("bits,dtype", [(16, BF16), (8, BF16), (8, F16)])
+def test_runs_across_rows(cea, dev, bits, dtype):
+    """Long uneven rows of many heads: a workgroup's run of tiles ends one row and starts the next."""
+    T = 18
+    c = D.make_tree(T, (4000, 0, 300, 5003, 18), counts=(T, 0, 7, T, T), bits=bits, Hq=64, Hkv=64, D=64, page=16, dtype=dtype)
+    D.check(cea, dev, c)
+
+
+@pytest.mark.parametrize("explicit", [False, True])
+def test_runs_of_8_bit_chunks(cea, dev, explicit):
+    c = D.pool8(P.make(B=4, n=18, Hq=64, Hkv=64, D=64, page=32, lengths=(5000, 40, 0, 4100), explicit=explicit,
+                       pad_rows=[(0, 17), (1, 0)]), 3)
+    D.check(cea, dev, c)
+
+
+def test_runs_with_values_that_are_not_finite(cea, dev):
+    """The second time over a row's tiles, between the rows of a run."""
+    T = 18
+    seen = torch.ones(3, T, T).tril().bool()
+    c = D.make_tree(T, (4000, 300, 5003), seen=seen, Hq=64, Hkv=64, D=64, page=16)
+    want = D.call(cea, c, dev).cpu()
+    for b, at in ((0, 4000 - 1), (1, 299), (2, 5002)):
+        c.v_pages[c.tables[b, at // 16], 5, at % 16, 3] = math.inf
+    out = D.call(cea, c, dev).cpu()
+    last = torch.zeros_like(out, dtype=torch.bool)
+    last[:, T - 1, 5, 3] = True
+    assert bool((out[last] == math.inf).all())
+    half = P.half_step(BF16)
+    assert bool(((out - want).abs()[~last].double() <= 4 * half * want.abs()[~last].double() + 1e-6).all())
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_many_rows(cea, dev, bits):
+    """More rows than a wave has lanes, in runs, in splits and in the token form's."""
+    lengths = [900 if i % 3 == 0 else 17 + i % 40 for i in range(70)]
+    D.check(cea, dev, D.make_tree(17, lengths, bits=bits, Hq=4, Hkv=4, D=64))
+    D.check(cea, dev, D.make_tree(17, [x * 2 for x in lengths[:66]], bits=bits, Hq=16, Hkv=16, D=64))
+    D.check(cea, dev, D.make_tree(2, [x + 300 * (i == 9) for i, x in enumerate(lengths)], bits=bits, Hq=4, Hkv=1, D=64))
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_sweep(cea, dev, seed):
+    """Random calls of the documented ranges."""
+    import random
+
+    r = random.Random(seed)
+    T = r.choice([1, 2, r.randint(3, 16), r.randint(17, 70), r.randint(17, 70), r.randint(71, 140)])
+    bits, dtype = r.choice([(8, BF16), (8, F16), (16, BF16), (16, F16), (32, F32), (8, F32)])
+    Hkv = r.choice([1, 2, 3])
+    Hq = Hkv * r.choice([1, 2, 4, 5, 7])
+    B = r.randint(1, 4)
+    lengths = [r.randint(0, r.choice([40, 300, 1200])) + T for _ in range(B)]
+    counts = [r.choice([T, r.randint(0, T)]) for _ in range(B)]
+    kw = dict(Hq=Hq, Hkv=Hkv, D=r.choice([64, 64, 128, 128, 96]), page=r.choice([16, 16, 32, 48, 64, 10]), dtype=dtype)
+    D.check(cea, dev, D.make_tree(T, lengths, counts=counts, bits=bits, seed=seed, **kw))
+    n = r.choice([1, 1, r.randint(2, 12), r.randint(17, 90)])
+    c = P.make(B=B, n=n, lengths=[max(x, n) for x in lengths], seed=seed, explicit=r.random() < 0.4, causal=r.random() < 0.8,
+               **{**kw, "dtype": r.choice([BF16, F16])})
+    D.check(cea, dev, D.pool8(c, seed))
+
+
+def test_pools_beyond_4_gib(cea, dev):
+    """Pages whose offsets pass 32 bits, in every operator on 8-bit pools."""
+    P_, H, page, d, n = 72000, 8, 64, 128, 40  # 4.7 GB each
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB of device memory")
+    kv = torch.empty(2, P_, H, page, d, dtype=torch.uint8, device=dev)
+    sc = torch.empty(2, P_, H, page, dtype=torch.uint8, device=dev)
+    g = torch.Generator().manual_seed(2)
+    tables = torch.tensor([[P_ - 1, 3, P_ - 7], [P_ - 2, 70001, 65600]])
+    lengths, counts = torch.tensor([150, 130]), torch.tensor([n, n])
+    small = torch.arange(6).view(2, 3)
+    for t in (tables, small):  # the same contents in far pages, and in the first pages of a small pool
+        pools = (kv, sc) if t is tables else (torch.empty(2, 6, H, page, d, dtype=torch.uint8, device=dev),
+                                              torch.empty(2, 6, H, page, dtype=torch.uint8, device=dev))
+        a, s = pools
+        gg = torch.Generator().manual_seed(5)
+        rand = lambda *x: torch.randn(*x, generator=gg).to(dev, BF16)
+        k, v, q = rand(2, 150, H, d), rand(2, 150, H, d), rand(2, n, 32, d)
+        td, z = t.to(dev), torch.zeros(2, dtype=torch.int64, device=dev)
+        kw = {"k_scales": s[0], "v_scales": s[1]}
+        cea.paged_kv_append(a[0].view(F8), a[1].view(F8), td, z, k, v, counts=lengths.to(dev), **kw)
+        masks, _ = cea.tree_masks(D.parents(2, n, 3).to(dev))
+        got = [cea.paged_tree_attention(q, a[0].view(F8), a[1].view(F8), td, lengths.to(dev), counts.to(dev), masks, **kw),
+               cea.paged_attention(q[:, :1], a[0].view(F8), a[1].view(F8), td, lengths.to(dev), lengths.view(2, 1).to(dev) - 1, **kw)]
+        path = torch.tensor([[1, 5, 39], [0, 2, 3]], device=dev)
+        cea.paged_kv_keep(a.view(F8), td, (lengths - n).to(dev), path, scales=s)
+        got += cea.paged_kv_read(a[0].view(F8), a[1].view(F8), td, z, 150, counts=lengths.to(dev), **kw)
+        if t is tables:
+            want = got
+    for x, y in zip(want, got):
+        assert torch.equal(x, y)
