@@ -52,7 +52,6 @@ FILE_FLAGS = {
     "attn_prefill.hip": ["-fno-honor-nans", "-Wno-inline-asm"],
     "attn_decode.hip": ["-fno-honor-nans", "-Wno-inline-asm"],
     "paged_chunk.hip": ["-fno-honor-nans", "-Wno-inline-asm"],
-    "paged_chunk8.hip": ["-fno-honor-nans", "-Wno-inline-asm"],
     "paged_token.hip": ["-Wno-inline-asm"],
     "paged_token8.hip": ["-Wno-inline-asm"],
     # the layer ops round every product to the tensor dtype before the next add, as the
@@ -107,7 +106,7 @@ def build(jobs: int | None = None, verbose: bool = False) -> Path:
     """Compiles all kernels and links the kernel library, then the PyTorch operator library
     on top of it; returns the kernel library's path."""
     OBJ_DIR.mkdir(parents=True, exist_ok=True)
-    sources = sorted(CSRC.glob("*.hip"))
+    sources = sorted(CSRC.glob("*.hip"), key=lambda f: (-f.stat().st_size, f.name))  # the longest first
     if not sources:
         raise RuntimeError(f"no HIP sources under {CSRC}")
     inc, libdirs, abi = _torch_flags()

@@ -20,6 +20,8 @@
 //     unnormalised (o, m, l) go to the workspace, and a second launch joins the parts of the
 //     units that were cut.  Short tables (kTokenWhole) take one workgroup of 4 to 16 waves per
 //     unit and one launch.
+//   * The nodes of a tree see slots by a window of their mask's word (16 nodes at most, so one) in the tiles that
+//     reach into the tree; before it nothing changes.
 //   * Measured: 32 rows of 1024 to 32768 keys, 32/8 heads of 128, bf16: 358 us for 2.2 GB, 6.2 TB/s (reads
 //     reach 6.3 here, a copy 4.9), 364 with f32 results; 8 rows of 100 to 4096 keys in f16 22.6 us, 18 of them
 //     the stream and 4.5 the join; one row of 777 keys, 32/4 heads of 64, 10.7 us, a chain of dependent trips to memory (length,

@@ -14,9 +14,14 @@
 //     bf16 as they are (4 significant bits); their scales are the keys', so the probabilities take them, in f32, before
 //     they are cut into bf16 pieces (two leave 2^-16 of one, three for f32 results less than 2^-23), whose range f32's
 //     exponents fit.  The keys of a lane are those whose scores it holds, the order within a tile being free;
+//   * positions and masks are the 16-bit form's;
 //   * a number that is not finite can only be NaN.  In a tile that all rows see it makes the NaN that the
 //     definition makes.  In others (the last ones of a unit) what no row sees is taken as 0, and a NaN that some rows
 //     see sums its tile's products one by one.
+//   * Measured: 32 rows of 1024 to 32768 keys, 32/8 heads of 128, bf16: 196 us for 1.12 GB, 5.7 TB/s (the 16-bit form
+//     6.2 over twice the bytes), 188 of them the stream and 8 the join.  A byte carries twice the 16-bit form's work:
+//     250 vector and 150 scalar instructions a tile (330 and 330, 223 us, with 64-bit addresses for each half and
+//     every tile's visibility key by key).
 #include <type_traits>
 
 #include "paged_token.hpp"
