@@ -36,7 +36,7 @@
 //   * drafts: the queries are nodes of a tree in the row's last slots.  The slots before them are tiles that
 //     every row sees whole; in the last tiles a query row's 64 keys are a window of its mask's words, which wait in
 //     LDS, so a tile costs a shift and a test of a bit per score (16 trees of 60 nodes after 500 to 8192 slots of
-//     8 bits, 32/8 heads of 128: 122 us, 560 TFLOP/s, 110 of them tiles; 26 nodes after 777, 32/4 heads of 64, 15.5);
+//     8 bits, 32/8 heads of 128: 122 us, 550 TFLOP/s, 110 of them tiles; 26 nodes after 777, 32/4 heads of 64, 15.5);
 //   * pages of 8 bits: a wave's 16 rows of a tile land in LDS as they are, and the wave itself turns them into
 //     16-bit rows in the one tile that is computed (v_cvt_scalef32_pk, exact: 4 significant bits and a power of
 //     two), a second barrier before the products.  The products are those of the 16-bit form.  128 tokens over
