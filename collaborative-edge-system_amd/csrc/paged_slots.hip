@@ -4,7 +4,7 @@
 // stream of calls on new data (a 1 GB copy moves 5.1 TB/s):
 //   * append: 2 x 4096 tokens of 8 heads of 128 from f16 (55 MB) 13.9, 3.9 TB/s; 32 single tokens 9.0, the call's own
 //     cost, 3.8 on the GPU;
-//   * read: 30000 slots of 8 heads of 128 into bf16 (185 MB) 52, 3.6 TB/s, and 33 where the Infinity Cache holds it;
+//   * read: 30000 slots of 8 heads of 128 into bf16 (185 MB) 33, 5.6 TB/s;
 //     8 rows of 350 to 700, 4 heads of 64, 11.0, 7.6 on the GPU, a chain of offsets, tables and rows;
 //   * moves: up to 9 nodes of 32 rows in 64 pools of 8 heads of 128 (28 MB) 11.1, 2.6 TB/s, four dependent trips to
 //     memory; 4 nodes of one row in 44 pools 8.0, 4.3 on the GPU;
@@ -27,12 +27,13 @@ template <typename V, typename T> __device__ __forceinline__ void load_bytes(con
   for (size_t i = 0; i < sizeof(T) / sizeof(V); ++i) raw[i] = ((const V*)p)[i];
   __builtin_memcpy(&x, raw, sizeof(T));
 }
+// (past the caches)
 template <typename V, typename T> __device__ __forceinline__ void store_bytes(void* p, const T& x) {
   static_assert(sizeof(T) % sizeof(V) == 0, "whole vectors");
   V raw[sizeof(T) / sizeof(V)];
   __builtin_memcpy(raw, &x, sizeof(T));
 #pragma unroll
-  for (size_t i = 0; i < sizeof(T) / sizeof(V); ++i) ((V*)p)[i] = raw[i];
+  for (size_t i = 0; i < sizeof(T) / sizeof(V); ++i) __builtin_nontemporal_store(raw[i], (V*)p + i);
 }
 
 // Where slot j of row b is: its page, or -1, and its place there.
@@ -382,7 +383,8 @@ template <typename I, typename O, int VEC> __device__ __forceinline__ void conve
 
 // A wave owns kReadSlots slots of a row and takes the tokens' vectors 64 at a time: where the slots are is known
 // once for all of them, and keys and values of all its slots are under way together.  (A vector a thread, each
-// with its own way to its slot: 30000 slots of 8 heads of 128 77 us, so 52.)
+// with its own way to its slot: 30000 slots of 8 heads of 128 77 us, so 52; with the rows written past the caches, where
+// they pushed the pages out, 33.)
 constexpr int kReadSlots = 4;
 template <typename I, typename O, int VEC>
 __global__ __launch_bounds__(256) void paged_read_kernel(const ReadParams p) {
