@@ -1125,7 +1125,7 @@ __global__ __launch_bounds__(NTHREADS, D == 64 && PIECES == 1 ? 3 : 2) void page
       asm volatile("" : "+s"(args));
       work(*(const ChunkParams*)args, job);
       left -= job.to - job.from;
-      if (!by_runs || left <= 0) return;
+      if (!by_runs || left <= 0 || job.b + 1 >= c_.p.B) return;
       __syncthreads();  // the next row's start writes what this one's end reads
       ++job.b;
       job.from = 0;

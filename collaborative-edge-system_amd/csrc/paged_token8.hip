@@ -436,7 +436,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void paged_token8_kernel(
     lo = 0;
     if (++unit == t.units) {
       unit = 0;
-      ++b;
+      if (++b >= p.B) return;
       const int n = slots_of(p, b);
       blocks = n > 0 ? (n + BLK - 1) / BLK : 1;
     }
