@@ -302,3 +302,49 @@ def test_repeats_itself(cea, dev, n):
     for _ in range(5):
         again = D.call(cea, c, dev, with_lse=True)
         assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+def _any_bytes_where_unused(c, seed):
+    """Numbers and scale bytes of every value in the slots that no row has, as in memory that nothing was written to."""
+    g = torch.Generator().manual_seed(seed)
+    used = torch.zeros(c.P, c.page, dtype=torch.bool)
+    for b in range(c.B):
+        for j in range(int(c.lengths[b])):
+            used[c.tables[b, j // c.page], j % c.page] = True
+    for which in "kv":
+        q, s = getattr(c, which + "_codes"), getattr(c, which + "_scales")
+        rq = torch.randint(0, 256, q.shape, generator=g, dtype=torch.uint8)
+        rs = torch.randint(0, 256, s.shape, generator=g, dtype=torch.uint8)
+        keep = used[:, None, :].expand(s.shape)
+        setattr(c, which + "_codes", torch.where(keep.unsqueeze(-1), q, rq))
+        setattr(c, which + "_scales", torch.where(keep, s, rs))
+    return c
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 64), (128, 48), (80, 16)])
+def test_unused_slots_hold_anything(cea, dev, dtype, d, page):
+    for n in (1, 4, 40):
+        for explicit in (False, True):
+            c = _case(B=3, n=n, Hq=4, Hkv=2, D=d, page=page, lengths=(203, n, 81), dtype=dtype, explicit=explicit, seed=n)
+            D.check(cea, dev, _any_bytes_where_unused(c, n))
+    for T in (5, 50):
+        c = D.make_tree(T, (203, T, 81), counts=(T, T, 3), bits=8, Hq=4, Hkv=2, D=d, page=page, dtype=dtype, seed=T)
+        D.check(cea, dev, _any_bytes_where_unused(c, T))
+
+
+def test_two_streams_at_once(cea, dev):
+    """Calls with scratch of their own, overlapping on two streams."""
+    cases = [_case(B=2, n=n, Hq=8, Hkv=2, D=128, page=64, lengths=(6000, 3000), seed=n) for n in (1, 40)]
+    cases += [D.make_tree(30, (5000, 2000), bits=8, Hq=8, Hkv=2, D=64, seed=3)]
+    want = [D.call(cea, c, dev) for c in cases]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for turn in range(6):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append([D.call(cea, c, dev) for c in cases])
+    torch.cuda.synchronize()
+    for x in got:
+        assert all(torch.equal(a, b) for a, b in zip(x, want))
