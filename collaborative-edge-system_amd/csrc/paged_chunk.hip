@@ -625,10 +625,12 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, const Job& job
   };
 
   // f16 takes 2^7 p, so small probabilities stay normal numbers: with one piece through the exponent (l
-  // holds the factor too), with two as a product, which costs small scores no bits
+  // holds the factor too), with two as a product, which costs small scores no bits.  bf16 takes 2^-8 p over pages of
+  // 8 bits, whose values reach 2^128: p is up to 2^8 before the maximum follows.
   constexpr bool kF16 = std::is_same<T, f16>::value;
-  constexpr float kExpShift = kF16 && PIECES == 1 ? 7.f : 0.f;
-  constexpr float kPieceScale = kF16 && PIECES > 1 ? 128.f : 1.f;
+  constexpr float kShift = kF16 ? 7.f : F8 ? -kRescaleLog2 : 0.f;
+  constexpr float kExpShift = PIECES == 1 ? kShift : 0.f;
+  constexpr float kPieceScale = PIECES == 1 ? 1.f : kF16 ? 128.f : F8 ? 1.f / 256 : 1.f;
   frag qf[D / 16];
   f32x16 oacc[D / 32];
   float m_run = -__builtin_inff(), m_use = -kExpShift, l_run = 0.f;

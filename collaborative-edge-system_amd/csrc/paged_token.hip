@@ -321,7 +321,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void paged_token_kernel(c
       buf ^= 1;
     }
 
-    finish_unit<T, D, NW, !SPLIT>(t, o, m_run, l_run, red_ml, dsmem, L::WAVE_BYTES, b, unit, lo == 0, hi == blocks,
+    finish_unit<T, D, NW, !SPLIT, 0>(t, o, m_run, l_run, red_ml, dsmem, L::WAVE_BYTES, b, unit, lo == 0, hi == blocks,
                                   1.f / kPScale);
     if constexpr (!SPLIT) return;
     left -= hi - lo;

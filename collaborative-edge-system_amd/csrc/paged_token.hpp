@@ -144,8 +144,10 @@ template <typename T> __device__ __forceinline__ void write_row(const PagedParam
 }
 
 // Joins the waves' sums of a unit in LDS and writes its rows, or (the unit is cut: not from its first block to its
-// last) its part.  `wave_bytes`: a wave's own share of `dsmem`, whose tiles are no longer read.
-template <typename T, int D, int NW, bool WHOLE>
+// last) its part.  `wave_bytes`: a wave's own share of `dsmem`, whose tiles are no longer read.  The sums o hold
+// 1 / unscale of the products' weights (undone before they are divided), and 2^kHeldLog2 of them beside that, which the
+// division undoes: a part of such sums has 2^kHeldLog2 of its weights' sum and a maximum that is as much higher.
+template <typename T, int D, int NW, bool WHOLE, int kHeldLog2>
 __device__ __forceinline__ void finish_unit(const TokenParams& t, const f32x4 (&o)[D / 16], float m_run, float l_run,
                                             float2 (&red_ml)[ROWS][NW], char* dsmem, int wave_bytes, int b, int unit,
                                             bool first, bool last, float unscale) {
@@ -154,6 +156,7 @@ __device__ __forceinline__ void finish_unit(const TokenParams& t, const f32x4 (&
   const int nrows = p.Sq * t.G;
   const float scale = (float)p.scale;
   const float c = fabsf(scale) * 1.4426950408889634f;  // exp2 units
+  const float held = __builtin_amdgcn_ldexpf(1.f, kHeldLog2);
       // A row's sum is 0 exactly where it saw no key (a NaN is kept).
       const float l_row = sum_halves(sum_rows16(l_run));
       if (grp == 0) red_ml[row][wave] = make_float2(m_run, l_row);
@@ -189,7 +192,7 @@ __device__ __forceinline__ void finish_unit(const TokenParams& t, const f32x4 (&
         M *= fabsf(scale);
         if (WHOLE || (first && last)) {
           const int s = r / t.G, h = unit * t.G + r - s * t.G;
-          write_row<T>(p, b, s, h, d, sum == 0.f ? 0.f : acc / sum);
+          write_row<T>(p, b, s, h, d, sum == 0.f ? 0.f : acc / (sum * held));
           if (p.lse && d == 0)
             ((float*)p.lse)[b * p.ls_b + h * p.ls_h + s * p.ls_s] =
                 sum == 0.f ? -__builtin_inff() : (M == -__builtin_inff() ? 0.f : M) + logf(sum);
@@ -197,8 +200,8 @@ __device__ __forceinline__ void finish_unit(const TokenParams& t, const f32x4 (&
           // non-temporal: written back past the caches, they disturb the reads of other workgroups least
           __builtin_nontemporal_store(acc, part + r * (D + 2) + d);
           if (d == 0) {
-            __builtin_nontemporal_store(M, part + r * (D + 2) + D);
-            __builtin_nontemporal_store(sum, part + r * (D + 2) + D + 1);
+            __builtin_nontemporal_store(M - kHeldLog2 * 0.69314718055994531f, part + r * (D + 2) + D);
+            __builtin_nontemporal_store(sum * held, part + r * (D + 2) + D + 1);
           }
         }
       }

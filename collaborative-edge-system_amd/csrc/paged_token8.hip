@@ -12,8 +12,11 @@
 //     order) and turns them into the queries' type with the key's scale, two an instruction, exactly;
 //   * O^T += V^T.P^T with v_mfma_f32_16x16x32_bf16: ds_read_b64_tr_b8 gives a lane 8 keys of one feature, which become
 //     bf16 as they are (4 significant bits); their scales are the keys', so the probabilities take them, in f32, before
-//     they are cut into bf16 pieces (two leave 2^-16 of one, three for f32 results less than 2^-23), whose range f32's
-//     exponents fit.  The keys of a lane are those whose scores it holds, the order within a tile being free;
+//     they are cut into bf16 pieces (two leave 2^-16 of one, three for f32 results less than 2^-23).  A weight is up to
+//     2^8 before the maximum follows, and a scale up to 2^127, so the sums are held at 2^-8 of theirs: no product
+//     passes f32 unless the result's own sum does.  At the other end a piece below bf16's normal numbers loses up
+//     to 2^-134: 2^-117 of a result's key, where its values are below 2^-92 (scale bytes below 26).  The keys of a
+//     lane are those whose scores it holds, the order within a tile being free;
 //   * positions and masks are the 16-bit form's;
 //   * a number that is not finite can only be NaN.  In a tile that all rows see it makes the NaN that the
 //     definition makes.  In others (the last ones of a unit) what no row sees is taken as 0, and a NaN that some rows
@@ -31,6 +34,10 @@ namespace {
 
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) i32x2* lds_i32x2_ptr;
+
+// What the sums hold of the products' weights, as a power of two: the reference maximum's lag.
+constexpr int kHeldLog2 = -8;
+static_assert(kHeldLog2 == -(int)kRescaleLog2, "the largest weight times the largest scale");
 
 template <int D> struct T8Layout {
   static constexpr int ROW = D;                // bytes
@@ -386,7 +393,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void paged_token8_kernel(
       l_run += ((pv[0] + pv[1]) + (pv[2] + pv[3])) + ((pv[4] + pv[5]) + (pv[6] + pv[7]));
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        pv[e] = __builtin_amdgcn_ldexpf(pv[e], (int)((vscale[e >> 2] >> (8 * (e & 3))) & 255u) - 127);
+        pv[e] = __builtin_amdgcn_ldexpf(pv[e], (int)((vscale[e >> 2] >> (8 * (e & 3))) & 255u) - 127 + kHeldLog2);
       if (!odd) {
         bf16x8 pf[PC];
 #pragma unroll
@@ -428,7 +435,8 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void paged_token8_kernel(
       buf ^= 1;
     }
 
-    finish_unit<T, D, NW, !SPLIT>(t, o, m_run, l_run, red_ml, dsmem, L::WAVE_BYTES, b, unit, lo == 0, hi == blocks, 1.f);
+    finish_unit<T, D, NW, !SPLIT, kHeldLog2>(t, o, m_run, l_run, red_ml, dsmem, L::WAVE_BYTES, b, unit, lo == 0, hi == blocks,
+                                             1.f);
     if constexpr (!SPLIT) return;
     left -= hi - lo;
     if (left == 0) return;

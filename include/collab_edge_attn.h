@@ -430,7 +430,8 @@ int cea_paged_attention(const cea_tensor* q, const cea_tensor* k_pages, const ce
  * type count as its largest, and a row whose q would read back beyond the type is cut at q = 240.
  *
  * cea_paged_attention8 is cea_paged_attention over such pages, q bf16, f16 or f32.  f16 queries meet values
- * that f16 holds: pages that f16 rows were appended to have no others.
+ * that f16 holds: pages that f16 rows were appended to have no others.  Weighted sums are f32: what passes it is
+ * infinite, and a key whose values are below 2^-92 may lose 2^-117 of its part.
  */
 int cea_paged_kv_append8(const cea_tensor* k, const cea_tensor* v, const cea_tensor* pos,
                          const cea_tensor* cos, const cea_tensor* sin, const cea_tensor* tables,
