@@ -324,16 +324,12 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void paged_token_kernel(c
     finish_unit<T, D, NW, !SPLIT, 0>(t, o, m_run, l_run, red_ml, dsmem, L::WAVE_BYTES, b, unit, lo == 0, hi == blocks,
                                   1.f / kPScale);
     if constexpr (!SPLIT) return;
-    left -= hi - lo;
-    if (left == 0) return;
+    const auto blocks_in = [&](int row) {
+      const int n = slots_of(p, row);
+      return n > 0 ? (n + BLK - 1) / BLK : 1;
+    };
+    if (!next_unit(b, unit, lo, left, blocks, hi - lo, t.units, p.B, blocks_in)) return;
     __syncthreads();  // the next unit's tiles overwrite the waves' sums
-    lo = 0;
-    if (++unit == t.units) {
-      unit = 0;
-      ++b;
-      const int n = slots_of(p, b);
-      blocks = n > 0 ? (n + BLK - 1) / BLK : 1;
-    }
   }
 }
 

@@ -133,6 +133,22 @@ __device__ __forceinline__ Runs runs_of(const TokenParams& t, int total) {
   return r;
 }
 
+// The unit of a run behind the one that `taken` blocks of it were of: false where the run ends.  The run was measured on
+// an earlier read of the lengths than blocks_in's, so it ends at the last row too, whatever they hold by now.
+template <typename BlocksIn>
+__host__ __device__ __forceinline__ bool next_unit(int& b, int& unit, int& lo, int& left, int& blocks, int taken,
+                                                   int units, int rows, BlocksIn blocks_in) {
+  left -= taken;
+  if (left <= 0) return false;
+  lo = 0;
+  if (++unit == units) {
+    unit = 0;
+    if (++b >= rows) return false;
+    blocks = blocks_in(b);
+  }
+  return true;
+}
+
 template <typename O> __device__ __forceinline__ void write_out(const PagedParams& p, int b, int s, int h, int d,
                                                                 float x) {
   ((O*)p.out)[b * p.os_b + s * p.os_s + h * p.os_h + d] = (O)x;

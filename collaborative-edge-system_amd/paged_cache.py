@@ -16,7 +16,8 @@ of row ``b`` is place ``j % page`` of page ``tables[b, j // page]``.  The operat
 * :func:`copy_pages` - copies of whole pages through all layers' pools,
 
 read tables and lengths on the device, so nothing waits for the host and a captured graph follows
-what its tensors hold.  A page index outside the pool is a page that holds nothing.
+what its tensors hold.  A page index outside the pool is a page that holds nothing.  The kernels read them
+more than once, so nothing may write to them (from another stream, say) before the call's work is done.
 
 Pages of ``torch.float8_e4m3fn`` take half the memory, and half the reads of a decode step.  With them go
 ``k_scales`` / ``v_scales`` ``[P, H, page]`` (uint8): the numbers ``q`` of a slot and head stand for

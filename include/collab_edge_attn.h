@@ -379,7 +379,7 @@ int cea_linear_gated_ws(const cea_tensor* x, const cea_tensor* w_gate, const cea
  * lengths, offsets and counts [B] are int64 device tensors that only the device reads: a page index
  * outside [0, P) is a page that holds nothing (no key there, and what would be written there is
  * dropped), lengths count up to W * page slots, and nothing outside the pools is touched whatever
- * they hold.
+ * they hold.  The kernels read them more than once: they stay as they are until the call's work is done.
  *
  * Append: token s < counts[b] (all of them with counts NULL) of row b goes to slot offsets[b] + s: k
  * [B,n,H,D], rotated with cos/sin [B,n,D] (both or neither; batch may be 1) in f32 (f64 for f64) and
