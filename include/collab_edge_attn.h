@@ -403,7 +403,8 @@ int cea_paged_kv_append(const cea_tensor* k, const cea_tensor* v, const cea_tens
  *   workspace: device memory (16-byte aligned, contents need no initialisation), not shared with a call
  *   that may run at the same time, of what cea_paged_attention_workspace() gives for the same arguments
  *   (no data is read), or of cea_paged_attention_workspace_bytes() bytes: enough for any layout and head
- *   map of these sizes, with positions in the pool, which take 8.5 bytes per slot of the tables.
+ *   map of these sizes, with positions in the pool, which take 8.5 bytes per slot of the tables (for this call, not
+ *   for those over 8-bit pages or of trees).
  */
 size_t cea_paged_attention_workspace_bytes(int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int64_t D,
                                            int64_t W, int64_t page, int32_t in_dtype);
@@ -430,7 +431,8 @@ int cea_paged_attention(const cea_tensor* q, const cea_tensor* k_pages, const ce
  * type count as its largest, and a row whose q would read back beyond the type is cut at q = 240.
  *
  * cea_paged_attention8 is cea_paged_attention over such pages, q bf16, f16 or f32.  f16 queries meet values
- * that f16 holds: pages that f16 rows were appended to have no others.  Weighted sums are f32: what passes it is
+ * that f16 holds: pages that f16 rows were appended to have no others.  Its workspace is of the size that
+ * cea_paged_attention8_workspace() gives (cea_paged_attention_workspace_bytes() does not bound it).  Weighted sums are f32: what passes it is
  * infinite, and a key whose values are below 2^-92 may lose 2^-117 of its part.
  */
 int cea_paged_kv_append8(const cea_tensor* k, const cea_tensor* v, const cea_tensor* pos,
@@ -466,8 +468,9 @@ int cea_paged_kv_read(const cea_tensor* k_pages, const cea_tensor* v_pages, cons
  * lengths[b] - counts[b] + i; node i sees every slot before them, and the slot of node j where bit j % 64 of
  * masks[b, i, j / 64] is set, masks int64 [B,T,ceil(T/64)] (any strides, any bits: those of its ancestors and
  * itself make a tree).  Nodes from counts[b] on are padding: their results are those of a row without keys.
- * Pages of any type, 8 bits with their scales (else NULL); T up to CEA_MAX_TREE; out, lse and the workspace as
- * cea_paged_attention's.
+ * Pages of any type, 8 bits with their scales (else NULL); T up to CEA_MAX_TREE; out and lse as
+ * cea_paged_attention's, and a workspace of the size that cea_paged_tree_attention_workspace() gives: trees cut their
+ * rows in other ways, and cea_paged_attention_workspace_bytes() does not bound it.
  */
 int cea_paged_tree_attention_workspace(const cea_tensor* q, const cea_tensor* k_pages, const cea_tensor* v_pages,
                                        const cea_tensor* k_scales, const cea_tensor* v_scales,
