@@ -36,12 +36,13 @@
 //   * drafts: the queries are nodes of a tree in the row's last slots.  The slots before them are tiles that
 //     every row sees whole; in the last tiles a query row's 64 keys are a window of its mask's words, which wait in
 //     LDS, so a tile costs a shift and a test of a bit per score (16 trees of 60 nodes after 500 to 8192 slots of
-//     8 bits, 32/8 heads of 128: 122 us, 550 TFLOP/s, 110 of them tiles; 26 nodes after 777, 32/4 heads of 64, 15.5);
+//     8 bits, 32/8 heads of 128: 124 us, 545 TFLOP/s, 112 of them tiles; 26 nodes after 777, 32/4 heads of 64, 15.5);
 //   * pages of 8 bits: a wave's 16 rows of a tile land in LDS as they are, and the wave itself turns them into
 //     16-bit rows in the one tile that is computed (v_cvt_scalef32_pk, exact: 4 significant bits and a power of
 //     two), a second barrier before the products.  The products are those of the 16-bit form.  128 tokens over
-//     32768 keys, 32/8 heads of 128: 96.5 us, 88 of them tiles and 9 the join, against 92 from 16 bits (83 and 9):
-//     the tiles are not bound by memory, and the conversion costs more than half the bytes save.
+//     32768 keys, 32/8 heads of 128: 97 us, 88 of them tiles and 9 the join, against 92 from 16 bits (83 and 9):
+//     the tiles are not bound by memory, the conversion and the products take turns within a workgroup, and each of a
+//     KV head's workgroups (four here, two of a tree of 60 nodes) converts every tile for itself.
 #include <math.h>
 #include <string.h>
 
@@ -192,6 +193,9 @@ template <typename X> __device__ __forceinline__ X scalar(X v) {
 constexpr int kSplitWgs = 512, kSplitTiles = 4;
 // Trees and 8-bit pages are cut from tables of kCutTiles on (18 trees of 59 nodes after up to 457 slots, 8 tiles, 16.9 us
 // whole, 26.0 cut; one of 26 nodes after 777, 13 tiles, 18.7 and 15.0), and into runs where these have kRunTiles tiles.
+// kCutTiles is compared with the table's width, which the host knows: short rows in a wide table are cut (18 trees of 59
+// after up to 457 slots of 8 bits, 32/8 heads of 128: 31 us in a table of 9 tiles, 46 in one of 128).  Both constants lie
+// between the few calls that are named here, not on a law.
 constexpr int kCutTiles = 12, kRunTiles = 16;
 struct Split {
   int b, split, first, count;  // a row, one of its splits, the place of its first one, how many it has
@@ -415,7 +419,7 @@ __device__ __forceinline__ LineRow line_row(const ChunkParams& c_, const Line& l
 
 // PIECES: 16-bit numbers whose sum enters the value product for a probability: one for 16-bit results
 // (p rounded once, half a step of the type, as the result's own rounding is), three of bf16 or two of f16
-// for f32 results (p to 2^-23 and better).  2-norm errors against 64 bits and us, one piece / f32 results: 128 bf16
+// for f32 results (p to 2^-23 and better; f16's to 2^-32 where p is below 2^-9).  2-norm errors against 64 bits and us, one piece / f32 results: 128 bf16
 // tokens over 32768 keys 2.3e-3, 91 / 6.8e-7, 136 (rounded to bf16 1.7e-3); two prompts of 2000 2.1e-3, 83 / 2.3e-7,
 // 125; four f16 chunks of 300 with positions 2.9e-4, 58 / 3.2e-7, 80.
 // AGAIN: over the tiles a second time, after values that are not finite.  Returns whether that is needed
@@ -635,8 +639,6 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, const Job& job
   f32x16 oacc[D / 32];
   float m_run = -__builtin_inff(), m_use = -kExpShift, l_run = 0.f;
 
-  // Which of this lane's keys its row does not see, bit by bit, looked up one by one (rare: the pool's positions
-  // are read in place, which waits for every load).
   // the 64 keys from slot0 on that this lane's row sees, by its mask
   auto window = [&](int slot0) -> uint64_t {
     const int off = slot0 - base, words = (p.Sq + 63) >> 6;
@@ -653,6 +655,8 @@ __device__ __forceinline__ bool chunk_body(const ChunkParams& c_, const Job& job
     if (left < 64) x &= ((uint64_t)1 << left) - 1;
     return sees ? x : 0;
   };
+  // Which of this lane's keys its row does not see, bit by bit, looked up one by one (rare: the pool's positions
+  // are read in place, which waits for every load).
   auto hidden = [&](int slot0) -> uint32_t {
     uint32_t hide = 0;
     uint64_t mask = 0;
@@ -1079,7 +1083,9 @@ __device__ __noinline__ void chunk_again(kernel_args_ptr args, Job job, lds_ptr 
 }
 
 // Three waves a SIMD at D = 64 and one piece leave 168 registers, of which the form with positions spills 5 (four
-// chunks of 300 over 700 to 4001 slots: 60.6 us so, 70.7 with two waves and none).
+// chunks of 300 over 700 to 4001 slots: 60.6 us so, 70.7 with two waves and none), over pages of 8 bits 14; other forms
+// spill up to 6 (positions, 8 bits, D = 128) and mostly 0 or 1.  Scalar registers that go to vector ones: none in 16-bit
+// sequences, 10 to 13 in their trees; over 8 bits 15 to 27 in trees, 44 to 52 by number, 78 to 82 with positions.
 template <typename T, int D, int VIS, int PIECES, bool F8>
 __global__ __launch_bounds__(NTHREADS, D == 64 && PIECES == 1 ? 3 : 2) void paged_chunk_kernel(const ChunkParams c_) {
   extern __shared__ __attribute__((aligned(16))) char smem[];

@@ -5,9 +5,11 @@
 //   * append: 2 x 4096 tokens of 8 heads of 128 from f16 (55 MB) 13.9, 3.9 TB/s; 32 single tokens 9.0, the call's own
 //     cost, 3.8 on the GPU;
 //   * read: 30000 slots of 8 heads of 128 into bf16 (185 MB) 33, 5.6 TB/s;
-//     8 rows of 350 to 700, 4 heads of 64, 11.0, 7.6 on the GPU, a chain of offsets, tables and rows;
-//   * moves: up to 9 nodes of 32 rows in 64 pools of 8 heads of 128 (28 MB) 11.1, 2.6 TB/s, four dependent trips to
-//     memory; 4 nodes of one row in 44 pools 8.0, 4.3 on the GPU;
+//     8 rows of 350 to 700, 4 heads of 64, 11.0, 7.5 on the GPU: a chain of offsets, tables and rows, in waves of which a
+//     token's 32 vectors fill half;
+//   * moves: up to 9 nodes of 32 rows in 64 pools of 8 heads of 128 (28 MB) 11.1, 2.6 TB/s: three dependent trips to
+//     memory (path and offsets, tables, rows), and behind the first 64 vectors' stores a second turn of up to 8, behind
+//     that one's the scale bytes; 4 nodes of one row in 44 pools 8.0, 4.3 on the GPU;
 //   * masks: 64 trees of 250 nodes 9.4 (5.6 on the GPU), one of 26 9.3 (1.8): the call's own cost.
 #include <algorithm>
 #include <type_traits>

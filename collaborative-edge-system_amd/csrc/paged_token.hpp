@@ -173,54 +173,54 @@ __device__ __forceinline__ void finish_unit(const TokenParams& t, const f32x4 (&
   const float scale = (float)p.scale;
   const float c = fabsf(scale) * 1.4426950408889634f;  // exp2 units
   const float held = __builtin_amdgcn_ldexpf(1.f, kHeldLog2);
-      // A row's sum is 0 exactly where it saw no key (a NaN is kept).
-      const float l_row = sum_halves(sum_rows16(l_run));
-      if (grp == 0) red_ml[row][wave] = make_float2(m_run, l_row);
-      float* red_o = (float*)(dsmem + wave * wave_bytes);
-      if (row < nrows) {
-  #pragma unroll
-        for (int dt = 0; dt < D / 16; ++dt) *(f32x4*)(red_o + row * D + dt * 16 + grp * 4) = o[dt];
+  // A row's sum is 0 exactly where it saw no key (a NaN is kept).
+  const float l_row = sum_halves(sum_rows16(l_run));
+  if (grp == 0) red_ml[row][wave] = make_float2(m_run, l_row);
+  float* red_o = (float*)(dsmem + wave * wave_bytes);
+  if (row < nrows) {
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) *(f32x4*)(red_o + row * D + dt * 16 + grp * 4) = o[dt];
+  }
+  __syncthreads();
+  float* part = t.partial + ((int64_t)blockIdx.x * 2 + (first ? 1 : 0)) * nrows * (D + 2);
+  for (int i = tid; i < nrows * D; i += NW * 64) {
+    const int r = i / D, d = i % D;
+    float2 ml[NW];
+    float x[NW];
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      ml[w] = red_ml[r][w];
+      x[w] = ((const float*)(dsmem + w * wave_bytes))[i];
+    }
+    float M = -__builtin_inff();  // of the raw scores
+#pragma unroll
+    for (int w = 0; w < NW; ++w) M = fmaxf(M, ml[w].x);
+    const float shift = M == -__builtin_inff() ? 0.f : M;
+    float acc = 0.f, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      // (a wave that saw nothing has zeros; one whose scores are all NaN keeps its NaN)
+      const float wt = ml[w].x == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f((ml[w].x - shift) * c);
+      acc = __builtin_fmaf(x[w], wt, acc);
+      sum = __builtin_fmaf(ml[w].y, wt, sum);
+    }
+    acc *= unscale;
+    M *= fabsf(scale);
+    if (WHOLE || (first && last)) {
+      const int s = r / t.G, h = unit * t.G + r - s * t.G;
+      write_row<T>(p, b, s, h, d, sum == 0.f ? 0.f : acc / (sum * held));
+      if (p.lse && d == 0)
+        ((float*)p.lse)[b * p.ls_b + h * p.ls_h + s * p.ls_s] =
+            sum == 0.f ? -__builtin_inff() : (M == -__builtin_inff() ? 0.f : M) + logf(sum);
+    } else {
+      // non-temporal: written back past the caches, they disturb the reads of other workgroups least
+      __builtin_nontemporal_store(acc, part + r * (D + 2) + d);
+      if (d == 0) {
+        __builtin_nontemporal_store(M - kHeldLog2 * 0.69314718055994531f, part + r * (D + 2) + D);
+        __builtin_nontemporal_store(sum * held, part + r * (D + 2) + D + 1);
       }
-      __syncthreads();
-      float* part = t.partial + ((int64_t)blockIdx.x * 2 + (first ? 1 : 0)) * nrows * (D + 2);
-      for (int i = tid; i < nrows * D; i += NW * 64) {
-        const int r = i / D, d = i % D;
-        float2 ml[NW];
-        float x[NW];
-  #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-          ml[w] = red_ml[r][w];
-          x[w] = ((const float*)(dsmem + w * wave_bytes))[i];
-        }
-        float M = -__builtin_inff();  // of the raw scores
-  #pragma unroll
-        for (int w = 0; w < NW; ++w) M = fmaxf(M, ml[w].x);
-        const float shift = M == -__builtin_inff() ? 0.f : M;
-        float acc = 0.f, sum = 0.f;
-  #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-          // (a wave that saw nothing has zeros; one whose scores are all NaN keeps its NaN)
-          const float wt = ml[w].x == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f((ml[w].x - shift) * c);
-          acc = __builtin_fmaf(x[w], wt, acc);
-          sum = __builtin_fmaf(ml[w].y, wt, sum);
-        }
-        acc *= unscale;
-        M *= fabsf(scale);
-        if (WHOLE || (first && last)) {
-          const int s = r / t.G, h = unit * t.G + r - s * t.G;
-          write_row<T>(p, b, s, h, d, sum == 0.f ? 0.f : acc / (sum * held));
-          if (p.lse && d == 0)
-            ((float*)p.lse)[b * p.ls_b + h * p.ls_h + s * p.ls_s] =
-                sum == 0.f ? -__builtin_inff() : (M == -__builtin_inff() ? 0.f : M) + logf(sum);
-        } else {
-          // non-temporal: written back past the caches, they disturb the reads of other workgroups least
-          __builtin_nontemporal_store(acc, part + r * (D + 2) + d);
-          if (d == 0) {
-            __builtin_nontemporal_store(M - kHeldLog2 * 0.69314718055994531f, part + r * (D + 2) + D);
-            __builtin_nontemporal_store(sum * held, part + r * (D + 2) + D + 1);
-          }
-        }
-      }
+    }
+  }
 }
 
 // What the tree's mask lets a query row see of the `NK` keys from slot0 on, up to 16 nodes.

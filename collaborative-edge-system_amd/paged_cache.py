@@ -198,8 +198,9 @@ def paged_kv_keep(kv: torch.Tensor, tables: torch.Tensor, offsets: torch.Tensor,
                   counts: Optional[torch.Tensor] = None, scales: Optional[torch.Tensor] = None) -> None:
     """Moves the accepted nodes of a tree into line, in place: slot ``offsets[b] + i`` of row ``b`` takes
     what slot ``offsets[b] + path[b, i]`` held, in every pool of ``kv`` ``[..., P, H, page, D]`` (all
-    layers' keys and values; what precedes the pages collapses into one dimension) and of ``scales`` ``[...,
-    P, H, page]``, which 8-bit pages have.
+    layers' keys and values; what precedes the pages collapses into one dimension, and a head's slots of a page are
+    contiguous, so pools of ``[P, page, H, D]`` seen as these are refused) and of ``scales`` ``[..., P, H, page]``,
+    which 8-bit pages have.
 
     ``path`` ``[B, n]`` names the accepted nodes in order, on the device, padded with -1.  A node is never
     before its place in line, so entries below their index move nothing, nor do those from ``counts[b]`` on,
